@@ -83,6 +83,13 @@ SIGNATURES: dict[str, list] = {
     "fns_hip_moe_layer_from_gguf": [_P, _I, _P, _P],
     "fns_hip_moe_resident_free": [_P],
     "fns_hip_add": [_P, _P, _P, _I64, _P],
+    "fns_hip_add_rms_norm_q8_1": [_P, _P, _P, _P, _P, _P, _I, _F, _I, _P],
+    "fns_hip_dequantize_q8_1": [_P, _I, _P, _P, _I64, _I64, _P],
+    "fns_hip_kv_page_bytes": [_I, _I, _I],
+    "fns_hip_kv_append": [_P, _P, _P, _P],
+    "fns_hip_kv_read": [_P, _P, _P, _P, _P],
+    "fns_hip_attn_workspace": [_P, _P, _P, _P],
+    "fns_hip_attn": [_P, _P, _P, _P, _P, _P, _SZ, _P],
     "fns_hip_dense_ffn_workspace": [_P, _I64, _P],
     "fns_hip_dense_ffn": [_P, _P, _P, _I64, _P, _SZ, _P],
     "fns_hip_dense_ffn_prefill": [_P, _P, _P, _I64, _P, _SZ, _P],
@@ -93,6 +100,7 @@ _RESTYPE = {
     "fns_hip_last_error": ctypes.c_char_p,
     "fns_hip_q8_1_row_bytes": _SZ,
     "fns_hip_mmq_q8_1_bytes": _SZ,
+    "fns_hip_kv_page_bytes": _SZ,
     "fns_hip_mmq_bounds_bytes": _SZ,
     "fns_hip_moe_noalloc_max_bytes": _SZ,
     "fns_hip_gguf_close": None,

@@ -231,6 +231,36 @@ int fns_hip_dense_ffn_prefill(const FnsDenseFfn *ffn, const float *x, float *out
     return impl::dense_ffn(ffn, x, out, n_tok, workspace, workspace_bytes, true, S(stream));
 }
 
+int fns_hip_add_rms_norm_q8_1(const float *x, const float *y, const float *w, float *sum, float *out, void *xq, int n,
+                              float eps, int rows, void *stream) {
+    return impl::add_rms_norm_q8_1(x, y, w, sum, out, xq, n, eps, rows, S(stream));
+}
+
+int fns_hip_dequantize_q8_1(const void *xq, int dtype, void *x, void *sums, int64_t ncols, int64_t nrows, void *stream) {
+    return impl::dequantize_q8_1(xq, dtype, x, sums, ncols, nrows, S(stream));
+}
+
+size_t fns_hip_kv_page_bytes(int n_head_kv, int head_dim, int page_size) {
+    return impl::kv_page_bytes(n_head_kv, head_dim, page_size);
+}
+
+int fns_hip_kv_append(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvAppend *x, void *stream) {
+    return impl::kv_append(cache, batch, x, S(stream));
+}
+
+int fns_hip_kv_read(const FnsKvCache *cache, const FnsKvBatch *batch, float *k, float *v, void *stream) {
+    return impl::kv_read(cache, batch, k, v, S(stream));
+}
+
+int fns_hip_attn_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, size_t *bytes) {
+    return impl::attn_workspace(cache, batch, x, bytes);
+}
+
+int fns_hip_attn(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const void *q, void *out,
+                 void *workspace, size_t workspace_bytes, void *stream) {
+    return impl::attn(cache, batch, x, q, out, workspace, workspace_bytes, S(stream));
+}
+
 int fns_hip_moe_prefill_image(const FnsMoeLayer *layer, int section, int *form, size_t *row_stride) {
     return impl::moe_prefill_image(layer, section, form, row_stride);
 }

@@ -106,6 +106,16 @@ int dense_ffn_workspace(const FnsDenseFfn *D, int64_t n_tok, size_t *total);
 int dense_ffn(const FnsDenseFfn *D, const float *x, float *out, int64_t n_tok, void *ws, size_t ws_bytes, bool prefill,
               hipStream_t st);
 
+int add_rms_norm_q8_1(const float *x, const float *y, const float *w, float *sum, float *out, void *xq, int n, float eps,
+                      int rows, hipStream_t st);
+int dequantize_q8_1(const void *xq, int dtype, void *x, void *sums, int64_t ncols, int64_t nrows, hipStream_t st);
+size_t kv_page_bytes(int n_head_kv, int head_dim, int page_size);
+int kv_append(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, hipStream_t st);
+int kv_read(const FnsKvCache *c, const FnsKvBatch *b, float *k, float *v, hipStream_t st);
+int attn_workspace(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, size_t *bytes);
+int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void *q, void *out, void *ws, size_t ws_bytes,
+         hipStream_t st);
+
 int fill_normal(float *out, int64_t n, uint64_t seed, uint64_t offset, float mean, float std, hipStream_t st);
 int quantize_weights(int type, const float *x, void *out, int64_t nrows, int64_t ncols, hipStream_t st);
 

@@ -1,0 +1,327 @@
+// kv_cache.hip - filling and reading back the paged 4-bit key/value cache (fns_kv.hpp), for MI355X gfx950.
+//
+// Append. A token of a batch brings k and v of every kv head (and its queries); its position is the sequence's length
+// less the tokens after it. With a rotation, a pair of channels (a, b) of k and q becomes
+//   (a cos t - b sin t, a sin t + b cos t),  t = position * inv_freq[i],
+// and k and v go into the cache in 4 bits, k from the rotated value before any rounding. The rotation and the block
+// arithmetic are done in 64 bits: an f32 angle of a far position is off by its spacing (4e-3 at position 65536), and a
+// 4-bit code next to a border would depend on the last bit of a 32-bit rotation. The pass moves the bytes of q, k and
+// v and is bound by them (and by its launch for a few tokens), not by this arithmetic.
+#include "fns_kv.hpp"
+
+#include "fns/kernels.h"
+#include "fns_common.hpp"
+#include "fns_host.hpp"
+#include "fns_internal.hpp"
+
+namespace fns {
+
+using namespace fns::dev;
+
+namespace {
+
+constexpr int kGroup = 16;  // positions of a workgroup: the V bytes of one column and one 16-position group are 16 bytes
+
+struct AppendArgs {
+    KvView c;
+    BatchView b;
+    const void *k, *v, *q;
+    void *q_out;
+    const float *inv_freq;
+    int64_t k_stride, v_stride, q_stride, qo_stride;
+    int rope_dim, n_group;  // n_group: query heads of a kv head (0: no queries)
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(uint16_t x) { return __builtin_bit_cast(float, (uint32_t) x << 16); }
+
+// Eight consecutive elements at any alignment of an element.
+template <class T> __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+    T t[8];
+    __builtin_memcpy(t, p, sizeof t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(t[i]);
+}
+__device__ __forceinline__ uint16_t to_bf16(float x) {  // nearest, ties to even; NaN stays NaN
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t) ((u >> 16) | 0x40u);
+    return (uint16_t) ((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+__device__ __forceinline__ void store8(float *p, const double (&v)[8]) {
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = (float) v[i];
+    __builtin_memcpy(p, t, sizeof t);
+}
+__device__ __forceinline__ void store8(uint16_t *p, const double (&v)[8]) {
+    uint16_t t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = to_bf16((float) v[i]);
+    __builtin_memcpy(p, t, sizeof t);
+}
+
+// Channels ch .. ch + 7 of a head's row after the rotation. cs: the token's (cos, sin) of every pair.
+template <int ROPE, class T>
+__device__ __forceinline__ void rotated8(const T *row, int ch, int rope_dim, const double2 *cs, double (&o)[8]) {
+    float x[8];
+    load8(row + ch, x);
+    if (ROPE == FNS_ROPE_NONE || ch >= rope_dim) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = x[i];
+        if (ROPE == FNS_ROPE_NONE || ch >= rope_dim) return;
+    }
+    if constexpr (ROPE == FNS_ROPE_PAIRS) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const double2 t = cs[(ch + i) / 2];
+            o[i] = x[i] * t.x - x[i + 1] * t.y;
+            o[i + 1] = x[i] * t.y + x[i + 1] * t.x;
+        }
+    } else if constexpr (ROPE == FNS_ROPE_HALVES) {
+        const int half = rope_dim / 2;
+        const bool second = ch >= half;
+        float y[8];
+        load8(row + (second ? ch - half : ch + half), y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double2 t = cs[ch + i - (second ? half : 0)];
+            o[i] = second ? y[i] * t.y + x[i] * t.x : x[i] * t.x - y[i] * t.y;
+        }
+    }
+}
+
+// Codes of the eight values of a lane (four lanes of a quad hold a block), 4 bits each; e: the block's scale byte.
+__device__ __forceinline__ uint32_t hold8(const double (&v)[8], int &e) {
+    double amax = 0.0;
+    int bad = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double a = fabs(v[i]);
+        bad |= !(a <= 1.7976931348623157e308);
+        amax = a > amax ? a : amax;
+    }
+    auto other = [](double x, auto lane) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        constexpr int O = decltype(lane)::value;
+        const uint32_t lo = (uint32_t) xor_lane_i<O>((int) (uint32_t) u), hi = (uint32_t) xor_lane_i<O>((int) (uint32_t) (u >> 32));
+        return __builtin_bit_cast(double, ((uint64_t) hi << 32) | lo);
+    };
+    amax = fmax(amax, other(amax, std::integral_constant<int, 1>{}));
+    amax = fmax(amax, other(amax, std::integral_constant<int, 2>{}));
+    bad |= xor_lane_i<1>(bad);
+    bad |= xor_lane_i<2>(bad);
+    e = bad ? 255 : kv_scale_of(amax);
+    if (bad) return 0;
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w |= kv_code(v[i], ldexp(fabs(v[i]), 127 - e)) << (4 * i);
+    return w;
+}
+
+// One workgroup: the new tokens among 16 aligned positions of one sequence, one kv head and its query heads.
+// Rows of 8 channels a thread: 2 D threads hold the 16 rows of a head.
+template <int D, int ROPE, class T>
+__global__ __launch_bounds__(2 * D) void k_kv_append(AppendArgs a) {
+    constexpr int NT = 2 * D;
+    __shared__ double2 cs[ROPE == FNS_ROPE_NONE ? 1 : kGroup * (D / 2)];
+    __shared__ __align__(16) uint8_t code[D][kGroup];
+    const int s = blockIdx.y / a.c.n_kv, head = blockIdx.y % a.c.n_kv, tid = threadIdx.x;
+    const SeqRange r = seq_range(a.b, s);
+    const int first = r.len - r.n;                                  // position of the first new token
+    const int64_t start = (int64_t) (first & ~(kGroup - 1)) + (int64_t) blockIdx.x * kGroup;
+    if (r.n == 0 || start >= r.len) return;
+    const int base = (int) start;
+    const int lo = max(first, base), hi = r.len - base < kGroup ? r.len : base + kGroup;  // [lo, hi): the tokens of this workgroup
+    if constexpr (ROPE != FNS_ROPE_NONE) {
+        const int half = a.rope_dim / 2;
+        for (int i = tid; i < kGroup * half; i += NT) {
+            const int p = base + i / half, c = i % half;
+            if (p < lo || p >= hi) continue;
+            // in turns: the product is exact to 53 bits, its whole part leaves no error
+            double turns = (double) p * (double) a.inv_freq[c] * 0.15915494309189533577;
+            turns -= rint(turns);
+            double sn, cn;
+            sincospi(2.0 * turns, &sn, &cn);
+            cs[i / half * (D / 2) + c] = make_double2(cn, sn);
+        }
+        __syncthreads();
+    }
+    const int row = tid / (D / 8), ch = tid % (D / 8) * 8, pos = base + row;
+    const bool have = pos >= lo && pos < hi;
+    const int64_t tok = r.q0 + (pos - first);
+    const double2 *mine = cs + (ROPE == FNS_ROPE_NONE ? 0 : row * (D / 2));
+    const int page = page_of(a.c, a.b, s, base);  // 16 aligned positions lie in one page
+    const int P = 1 << a.c.shift;
+    uint8_t *dst = a.c.pages + (int64_t) max(page, 0) * a.c.page_bytes + head * kv_head_bytes(D, P);
+    using L = KvParts<D>;
+    double v[8] = {};
+    int e;
+    if (have) rotated8<ROPE>((const T *) a.k + tok * a.k_stride + head * D, ch, a.rope_dim, mine, v);
+    uint32_t w = hold8(v, e);
+    if (have && page >= 0 && pos >= 0) {
+        *(uint32_t *) (dst + L::k_row(P, pos & (P - 1)) + ch / 2) = w;
+        if (ch % 32 == 0) dst[L::k_scale(P, pos & (P - 1)) + ch / 32] = (uint8_t) e;
+    }
+    if (have) rotated8<FNS_ROPE_NONE>((const T *) a.v + tok * a.v_stride + head * D, ch, 0, mine, v);
+    w = hold8(v, e);
+    if (have && page >= 0 && pos >= 0 && ch % 32 == 0) dst[L::v_scale(P, pos & (P - 1)) + ch / 32] = (uint8_t) e;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code[ch + i][row] = (uint8_t) ((w >> (4 * i)) & 15u);
+    __syncthreads();
+    if (page >= 0 && base >= 0) {  // byte column tid / 4, positions 4 (tid % 4) .. + 3
+        const int j = tid / 4, p4 = base + tid % 4 * 4;
+        const int c0 = j / 16 * 32 + j % 16;
+        const uint32_t b = *(const uint32_t *) &code[c0][tid % 4 * 4] | (*(const uint32_t *) &code[c0 + 16][tid % 4 * 4] << 4);
+        uint8_t *o = dst + L::v_col(P, j) + (p4 & (P - 1));
+        if (p4 >= lo && p4 + 4 <= hi) {
+            *(uint32_t *) o = b;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (p4 + i >= lo && p4 + i < hi) o[i] = (uint8_t) (b >> (8 * i));
+        }
+    }
+    if (have)
+        for (int g = 0; g < a.n_group; ++g) {
+            const int64_t h = (int64_t) (head * a.n_group + g) * D;
+            // in place too: the threads of a row are lanes of one wave, whose loads all precede the stores they feed
+            rotated8<ROPE>((const T *) a.q + tok * a.q_stride + h, ch, a.rope_dim, mine, v);
+            store8((T *) a.q_out + tok * a.qo_stride + h + ch, v);
+        }
+}
+
+// Values of the batch's tokens as the cache holds them; NaN where a position has no page.
+template <int D>
+__global__ __launch_bounds__(256) void k_kv_read(KvView c, BatchView b, float *k, float *v) {
+    const int s = blockIdx.y / c.n_kv, head = blockIdx.y % c.n_kv;
+    const SeqRange r = seq_range(b, s);
+    const int P = 1 << c.shift;
+    using L = KvParts<D>;
+    const int i = blockIdx.x * (256 / (D / 4)) + threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4) * 4;
+    if (i >= r.n) return;
+    const int pos = r.len - r.n + i, page = page_of(c, b, s, pos);
+    float kv[4], vv[4];
+    if (page >= 0) {
+        const int row = pos & (P - 1);
+        const uint8_t *src = c.pages + (int64_t) page * c.page_bytes + head * kv_head_bytes(D, P);
+        const int ke = src[L::k_scale(P, row) + ch / 32], ve = src[L::v_scale(P, row) + ch / 32];
+        const int kw = src[L::k_row(P, row) + ch / 2] | (src[L::k_row(P, row) + ch / 2 + 1] << 8);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            kv[t] = kv_value((kw >> (4 * t)) & 15, ke);
+            const int x = ch % 32 + t;
+            vv[t] = kv_value((src[L::v_col(P, ch / 32 * 16 + x % 16) + row] >> (x / 16 * 4)) & 15, ve);
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) kv[t] = vv[t] = __builtin_nanf("");
+    }
+    const int64_t o = ((r.q0 + i) * c.n_kv + head) * D + ch;
+    __builtin_memcpy(k + o, kv, sizeof kv);
+    __builtin_memcpy(v + o, vv, sizeof vv);
+}
+
+}  // namespace
+
+namespace host {
+
+int kv_check(const FnsKvCache *c, const FnsKvBatch *b, const char *what) {
+    if (!c || !b) return set_error(ERR_SHAPE, "%s: null cache or batch", what);
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return set_error(ERR_SHAPE, "%s: head_dim must be 64, 128 or 256 (%d)", what, c->head_dim);
+    if (c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
+        return set_error(ERR_SHAPE, "%s: page_size must be a power of two from 16 to 4096 (%d)", what, c->page_size);
+    if (c->n_head_kv <= 0 || c->n_head_kv > 1024 || c->n_pages <= 0 || c->n_pages > INT32_MAX)
+        return set_error(ERR_SHAPE, "%s: n_head_kv must be 1..1024 and n_pages 1..2^31-1 (%d, %lld)", what, c->n_head_kv,
+                         (long long) c->n_pages);
+    if (!c->pages || ((uintptr_t) c->pages & 15)) return set_error(ERR_SHAPE, "%s: pages must be 16-byte aligned device memory", what);
+    if (b->n_seq < 0 || b->n_tok < 0 || b->max_q < 0 || b->max_kv < 0 || b->table_stride < 0 || b->n_tok > INT32_MAX ||
+        b->max_kv > INT32_MAX || b->table_stride > INT32_MAX)
+        return set_error(ERR_SHAPE, "%s: negative or too large batch numbers (n_seq %d n_tok %lld max_q %d)", what, b->n_seq,
+                         (long long) b->n_tok, b->max_q);
+    if ((int64_t) b->n_seq * c->n_head_kv > 65535)
+        return set_error(ERR_SHAPE, "%s: n_seq * n_head_kv must be at most 65535 (%d * %d)", what, b->n_seq, c->n_head_kv);
+    if (b->n_seq > 0 && (!b->q_start || !b->kv_len || !b->page_table)) return set_error(ERR_SHAPE, "%s: null batch array", what);
+    return OK;
+}
+
+}  // namespace host
+
+namespace impl {
+
+size_t kv_page_bytes(int n_head_kv, int head_dim, int page_size) {
+    FnsKvCache c{n_head_kv, head_dim, page_size, 1, (void *) 16};
+    FnsKvBatch b{};
+    if (host::kv_check(&c, &b, "kv_page_bytes") != host::OK) return 0;
+    return (size_t) n_head_kv * dev::kv_head_bytes(head_dim, page_size);
+}
+
+int kv_append(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, hipStream_t st) {
+    FNS_TRY(host::kv_check(c, b, "kv_append"));
+    if (!x) return host::set_error(host::ERR_SHAPE, "kv_append: null arguments");
+    if (x->dtype != FNS_TYPE_F32 && x->dtype != FNS_TYPE_BF16)
+        return host::set_error(host::ERR_TYPE, "kv_append: type %d is not supported (0 f32, 30 bf16)", x->dtype);
+    if (x->rope != FNS_ROPE_NONE && x->rope != FNS_ROPE_HALVES && x->rope != FNS_ROPE_PAIRS)
+        return host::set_error(host::ERR_SHAPE, "kv_append: unknown rotation %d", x->rope);
+    const int D = c->head_dim;
+    // a thread rotates 8 channels, and a half's partner channels have to be 8 of the other half
+    if (x->rope != FNS_ROPE_NONE && (!x->inv_freq || x->rope_dim <= 0 || x->rope_dim > D || x->rope_dim % 16))
+        return host::set_error(host::ERR_SHAPE, "kv_append: a rotation needs inv_freq and a rope_dim that is a multiple of 16 up to head_dim (%d)",
+                               x->rope_dim);
+    if (x->n_head < 0 || x->n_head % c->n_head_kv)
+        return host::set_error(host::ERR_SHAPE, "kv_append: n_head %d is no multiple of n_head_kv %d", x->n_head, c->n_head_kv);
+    if (b->n_seq == 0 || b->n_tok == 0 || b->max_q == 0) return host::OK;
+    if (!x->k || !x->v || (x->n_head > 0 && (!x->q || !x->q_out))) return host::set_error(host::ERR_SHAPE, "kv_append: null argument");
+    const int64_t kvw = (int64_t) c->n_head_kv * D, qw = (int64_t) x->n_head * D;
+    if (x->k_stride < kvw || x->v_stride < kvw || (x->n_head > 0 && (x->q_stride < qw || x->q_out_stride < qw)))
+        return host::set_error(host::ERR_SHAPE, "kv_append: a token stride is shorter than a token's heads");
+    if (x->n_head > 0 && x->q == x->q_out && x->q_stride != x->q_out_stride)
+        return host::set_error(host::ERR_SHAPE, "kv_append: queries rotated in place keep their stride");
+    AppendArgs a{host::kv_view(c), host::kv_batch(b), x->k, x->v, x->q, x->q_out, x->inv_freq, x->k_stride, x->v_stride,
+                 x->q_stride, x->q_out_stride, x->rope_dim, x->n_head / c->n_head_kv};
+    // new tokens of a sequence start anywhere in a group
+    const dim3 grid((unsigned) ((b->max_q + kGroup - 2) / kGroup + 1), (unsigned) (b->n_seq * c->n_head_kv));
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(2 * D), 0, st, a); };
+    auto by_type = [&](auto dim, auto rope) {
+        constexpr int DD = decltype(dim)::value, R = decltype(rope)::value;
+        if (x->dtype == FNS_TYPE_F32) go(k_kv_append<DD, R, float>);
+        else go(k_kv_append<DD, R, uint16_t>);
+    };
+    auto by_rope = [&](auto dim) {
+        if (x->rope == FNS_ROPE_NONE) by_type(dim, std::integral_constant<int, FNS_ROPE_NONE>{});
+        else if (x->rope == FNS_ROPE_HALVES) by_type(dim, std::integral_constant<int, FNS_ROPE_HALVES>{});
+        else by_type(dim, std::integral_constant<int, FNS_ROPE_PAIRS>{});
+    };
+    if (D == 64) by_rope(std::integral_constant<int, 64>{});
+    else if (D == 128) by_rope(std::integral_constant<int, 128>{});
+    else by_rope(std::integral_constant<int, 256>{});
+    return host::check_launch("kv_append");
+}
+
+int kv_read(const FnsKvCache *c, const FnsKvBatch *b, float *k, float *v, hipStream_t st) {
+    FNS_TRY(host::kv_check(c, b, "kv_read"));
+    if (b->n_seq == 0 || b->n_tok == 0 || b->max_q == 0) return host::OK;
+    if (!k || !v) return host::set_error(host::ERR_SHAPE, "kv_read: null output");
+    const int rows = 256 / (c->head_dim / 4);
+    const dim3 grid((unsigned) ((b->max_q + rows - 1) / rows), (unsigned) (b->n_seq * c->n_head_kv));
+    auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, host::kv_view(c), host::kv_batch(b), k, v);
+    };
+    if (c->head_dim == 64) go(k_kv_read<64>);
+    else if (c->head_dim == 128) go(k_kv_read<128>);
+    else go(k_kv_read<256>);
+    return host::check_launch("kv_read");
+}
+
+}  // namespace impl
+
+namespace k {
+void kv_append(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsKvAppend &x, hipStream_t st) {
+    host::abort_on_error(impl::kv_append(&cache, &batch, &x, st), "kv_append");
+}
+void kv_read(const FnsKvCache &cache, const FnsKvBatch &batch, float *k, float *v, hipStream_t st) {
+    host::abort_on_error(impl::kv_read(&cache, &batch, k, v, st), "kv_read");
+}
+}  // namespace k
+
+}  // namespace fns

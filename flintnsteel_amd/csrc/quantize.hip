@@ -71,6 +71,117 @@ __global__ __launch_bounds__(256) void k_rms_norm_q8_1(const float *__restrict__
     }
 }
 
+// The residual add in front of the same: s = x + y, then the RMSNorm row and its Q8_1 of s, so that the residual stream
+// goes through once (s, its norm and the blocks: 16 + 9/8 bytes a value instead of the 24 + 9/8 of add and
+// rms_norm_q8_1). The order of every sum is theirs: the same bits. sum may be x or y: a row is whole in registers (or
+// read and written by the same thread) before it is overwritten. out may be null.
+template <int C>
+__global__ __launch_bounds__(256) void k_add_rms_norm_q8_1_rows(const float *x, const float *y, const float *__restrict__ w,
+                                                                float *sum, float *__restrict__ out,
+                                                                uint8_t *__restrict__ xq, int n, float eps, int64_t row_bytes) {
+    __shared__ __align__(16) float xs[2048 * C];
+    __shared__ float red[4];
+    const int tid = threadIdx.x;
+    const size_t r = (size_t) blockIdx.x * n;
+    float v[C][8], wv[C][8];
+    const auto load = [](const float *p, float (&o)[8]) {
+        const float4 a = *(const float4 *) p, b = *(const float4 *) (p + 4);
+        o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
+    };
+    const auto store = [](float *p, const float (&o)[8]) {
+        *(float4 *) p = make_float4(o[0], o[1], o[2], o[3]);
+        *(float4 *) (p + 4) = make_float4(o[4], o[5], o[6], o[7]);
+    };
+    float yv[C][8];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {  // clamped, unconditional loads: all in flight together
+        const int col = min((256 * c + tid) * 8, n - 8);
+        load(x + r + col, v[c]);
+        load(y + r + col, yv[c]);
+        load(w + col, wv[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int col = (256 * c + tid) * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[c][k] = col < n ? v[c][k] + yv[c][k] : 0.0f;
+        store(xs + col, v[c]);
+    }
+    __syncthreads();
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8 * C; ++j) {
+        const float a = xs[tid + 256 * j];
+        s += a * a;
+    }
+    s = lanes_sum<64>(s);
+    if (tid % 64 == 0) red[tid / 64] = s;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int col = (256 * c + tid) * 8;
+        if (col < n) store(sum + r + col, v[c]);
+    }
+    __syncthreads();
+    s = (red[0] + red[1]) + (red[2] + red[3]);
+    const float scale = 1.0f / sqrtf(s / n + eps);
+    const int npad = (n + 511) / 512 * 512;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int col = (256 * c + tid) * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[c][k] = col < n ? scale * v[c][k] * wv[c][k] : 0.0f;
+        if (col < n && out) store(out + r + col, v[c]);
+        const Q8x8 q = q8_1_x8(v[c]);
+        if (col < npad) q8_1_store_x8(q, xq + blockIdx.x * row_bytes, col);
+    }
+}
+
+// Any n that is a multiple of 32, any alignment.
+__global__ __launch_bounds__(256) void k_add_rms_norm_q8_1(const float *x, const float *y, const float *__restrict__ w,
+                                                           float *sum, float *__restrict__ out, uint8_t *__restrict__ xq,
+                                                           int n, float eps, int64_t row_bytes) {
+    __shared__ float red[4];
+    const size_t r = (size_t) blockIdx.x * n;
+    float s = 0.0f;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const float a = x[r + i] + y[r + i];
+        sum[r + i] = a;
+        s += a * a;
+    }
+    s = lanes_sum<64>(s);
+    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = s;
+    __syncthreads();
+    s = (red[0] + red[1]) + (red[2] + red[3]);
+    const float scale = 1.0f / sqrtf(s / n + eps);
+    const int npad = (n + 511) / 512 * 512;
+    for (int i = threadIdx.x; i < npad; i += 256) {
+        float xi = 0.0f;
+        if (i < n) {
+            xi = scale * sum[r + i] * w[i];  // (each thread reads back what it wrote)
+            if (out) out[r + i] = xi;
+        }
+        q8_1_store(xi, xq + (size_t) blockIdx.x * row_bytes, i / 32, i % 32);
+    }
+}
+
+// What Q8_1 rows stand for: values q * d, and the blocks' sums. Four values a thread.
+template <class T>
+__global__ __launch_bounds__(256) void k_dequantize_q8_1(const uint8_t *__restrict__ xq, T *x, T *sums, int n, int64_t total4,
+                                                         int64_t row_bytes) {
+    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (i >= total4) return;
+    const int64_t r = i / (n / 4);
+    const int col = (int) (i % (n / 4)) * 4;
+    const uint8_t *b = xq + r * row_bytes + (size_t) (col / 32) * 36;
+    const uint32_t ds = *(const uint32_t *) b, q = *(const uint32_t *) (b + 4 + col % 32);
+    const float d = half_to_float(ds & 0xffffu);
+    T o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = (T) ((float) (int) (int8_t) ((q >> (8 * k)) & 0xffu) * d);
+    __builtin_memcpy(x + r * n + col, o, sizeof o);
+    if (sums && col % 32 == 0) sums[r * (n / 32) + col / 32] = (T) half_to_float(ds >> 16);
+}
+
 __device__ __forceinline__ float block_max256(float m, float *red) {
     m = lanes_max<64>(m);
     __syncthreads();
@@ -209,6 +320,45 @@ int rms_norm_q8_1(const float *x, const float *w, float *out, void *xq, int n, f
     return host::check_launch("rms_norm_q8_1");
 }
 
+int add_rms_norm_q8_1(const float *x, const float *y, const float *w, float *sum, float *out, void *xq, int n, float eps,
+                      int rows, hipStream_t st) {
+    if (n <= 0 || n % 32 || rows < 0)
+        return host::set_error(host::ERR_SHAPE, "add_rms_norm_q8_1: n must be a positive multiple of 32, rows not negative");
+    if (rows == 0) return host::OK;
+    if (!x || !y || !w || !sum || !xq) return host::set_error(host::ERR_SHAPE, "add_rms_norm_q8_1: null argument");
+    if ((uintptr_t) xq & 3) return host::set_error(host::ERR_SHAPE, "add_rms_norm_q8_1: xq must be 4-byte aligned");
+    // as rms_norm_q8_1
+    const bool vec = n <= 8192 && (((uintptr_t) x | (uintptr_t) y | (uintptr_t) w | (uintptr_t) sum | (uintptr_t) out) & 15) == 0;
+    auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, dim3((unsigned) rows), dim3(256), 0, st, x, y, w, sum, out, (uint8_t *) xq, n, eps,
+                           host::q8_1_row_bytes(n));
+    };
+    if (!vec) go(k_add_rms_norm_q8_1);
+    else if (n <= 2048) go(k_add_rms_norm_q8_1_rows<1>);
+    else if (n <= 4096) go(k_add_rms_norm_q8_1_rows<2>);
+    else go(k_add_rms_norm_q8_1_rows<4>);
+    return host::check_launch("add_rms_norm_q8_1");
+}
+
+int dequantize_q8_1(const void *xq, int dtype, void *x, void *sums, int64_t ncols, int64_t nrows, hipStream_t st) {
+    if (dtype != FNS_TYPE_F32 && dtype != FNS_TYPE_F16)
+        return host::set_error(host::ERR_TYPE, "dequantize_q8_1: type %d is not supported (0 f32, 1 f16)", dtype);
+    if (ncols <= 0 || ncols % 32 || ncols > INT32_MAX || nrows < 0 || nrows > INT32_MAX)
+        return host::set_error(host::ERR_SHAPE, "dequantize_q8_1: bad arguments (ncols %lld nrows %lld)", (long long) ncols,
+                               (long long) nrows);
+    if (nrows == 0) return host::OK;
+    if (!xq || !x || ((uintptr_t) xq & 3)) return host::set_error(host::ERR_SHAPE, "dequantize_q8_1: null or misaligned argument");
+    const int64_t total4 = nrows * (ncols / 4), grid = (total4 + 255) / 256;
+    if (grid > INT32_MAX) return host::set_error(host::ERR_SHAPE, "dequantize_q8_1: too many values");
+    if (dtype == FNS_TYPE_F32)
+        hipLaunchKernelGGL(k_dequantize_q8_1<float>, dim3((unsigned) grid), dim3(256), 0, st, (const uint8_t *) xq, (float *) x,
+                           (float *) sums, (int) ncols, total4, host::q8_1_row_bytes(ncols));
+    else
+        hipLaunchKernelGGL(k_dequantize_q8_1<_Float16>, dim3((unsigned) grid), dim3(256), 0, st, (const uint8_t *) xq,
+                           (_Float16 *) x, (_Float16 *) sums, (int) ncols, total4, host::q8_1_row_bytes(ncols));
+    return host::check_launch("dequantize_q8_1");
+}
+
 int amax_guard(float *act, float *escale, int n, int rows, hipStream_t st) {
     if (!act || !escale || n <= 0 || rows < 0) return host::set_error(host::ERR_SHAPE, "amax_guard: bad arguments");
     if (rows == 0) return host::OK;
@@ -277,6 +427,10 @@ void quantize_q8_1(const float *x, void *xq, int64_t ncols, int64_t nrows, hipSt
 namespace k {
 void rms_norm_q8_1(const float *x, const float *w, float *out, void *xq, int n, float eps, int rows, hipStream_t st) {
     host::abort_on_error(impl::rms_norm_q8_1(x, w, out, xq, n, eps, rows, st), "rms_norm_q8_1");
+}
+void add_rms_norm_q8_1(const float *x, const float *y, const float *w, float *sum, float *out, void *xq, int n, float eps,
+                       int rows, hipStream_t st) {
+    host::abort_on_error(impl::add_rms_norm_q8_1(x, y, w, sum, out, xq, n, eps, rows, st), "add_rms_norm_q8_1");
 }
 void amax_guard(float *act, float *escale, int n, int rows, hipStream_t st) {
     host::abort_on_error(impl::amax_guard(act, escale, n, rows, st), "amax_guard");

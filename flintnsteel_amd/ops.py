@@ -14,8 +14,9 @@ from ._lib import call, lib
 
 Q8_0, Q8_1, Q3_K, Q4_K, Q5_K, Q6_K = 8, 9, 11, 12, 13, 14
 IQ3_XXS, IQ3_S, IQ2_S, IQ4_XS = 18, 21, 22, 23
-F32, BF16 = 0, 30
+F32, F16, BF16 = 0, 1, 30
 GATING_SOFTMAX, GATING_SIGMOID = 0, 1
+ROPE_NONE, ROPE_HALVES, ROPE_PAIRS = 0, 1, 2
 STATUS_EXCHANGE_TIMEOUT = 1  # FNS_STATUS_EXCHANGE_TIMEOUT
 # bytes per 256 values of a row (a K-quant block; 8 Q8_0 blocks)
 BLOCK_BYTES = {Q8_0: 272, Q3_K: 110, Q4_K: 144, Q5_K: 176, Q6_K: 210, IQ3_XXS: 98, IQ3_S: 110, IQ2_S: 82, IQ4_XS: 136}
@@ -541,6 +542,237 @@ def add(x: torch.Tensor, y: torch.Tensor, out: torch.Tensor | None = None) -> to
     """out = x + y (reference add_inplace, src/kernels.cuh:119); out may be x."""
     out = torch.empty_like(x) if out is None else out
     call("fns_hip_add", _p(x), _p(y), _p(out), x.numel(), _s())
+    return out
+
+
+def _rows_f32(what: str, *ts: torch.Tensor) -> None:
+    """Every tensor f32, contiguous, on the current device and of the first one's shape."""
+    for t in ts:
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != ts[0].shape:
+            raise ValueError(f"{what}: expected contiguous f32 tensors of one shape")
+    _on_device(what, *ts)
+
+
+def _on_device(what: str, *ts: torch.Tensor | None) -> None:
+    """The launch goes to the current device's current stream: every tensor has to be there."""
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
+            raise ValueError(f"{what}: expected tensors on the current device")
+
+
+def add_rms_norm_q8_1(x: torch.Tensor, y: torch.Tensor, w: torch.Tensor, eps: float, sum_out: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None, xq: torch.Tensor | None = None):
+    """-> (sum, out, xq): sum = x + y, out = RMSNorm(sum) * w, xq its Q8_1 rows. sum_out may be x or y (in place)."""
+    n = x.shape[-1]
+    rows = x.numel() // max(n, 1)
+    sum_out = torch.empty_like(x, memory_format=torch.contiguous_format) if sum_out is None else sum_out
+    out = torch.empty_like(sum_out) if out is None else out
+    _rows_f32("add_rms_norm_q8_1", x, y, sum_out, out)
+    _rows_f32("add_rms_norm_q8_1", w)
+    if w.numel() != n:
+        raise ValueError(f"add_rms_norm_q8_1: {w.numel()} weights for rows of {n}")
+    if xq is None:
+        xq = torch.empty(rows, q8_1_row_bytes(n), dtype=torch.uint8, device=x.device)
+    if xq.dtype != torch.uint8 or not xq.is_contiguous() or xq.numel() != rows * q8_1_row_bytes(n):
+        raise ValueError("add_rms_norm_q8_1: xq must be uint8 [rows][q8_1_row_bytes(n)]")
+    _on_device("add_rms_norm_q8_1", xq)
+    call("fns_hip_add_rms_norm_q8_1", _p(x), _p(y), _p(w), _p(sum_out), _p(out), _p(xq), n, ctypes.c_float(eps), rows, _s())
+    return sum_out, out, xq
+
+
+def dequantize_q8_1(xq: torch.Tensor, ncols: int, dtype: torch.dtype = torch.float32):
+    """-> (values [nrows][ncols], block sums [nrows][ncols / 32]) that Q8_1 rows stand for, in f32 or f16."""
+    if dtype not in (torch.float32, torch.float16):
+        raise ValueError(f"dequantize_q8_1: {dtype} not supported")
+    if xq.dtype != torch.uint8 or not xq.is_contiguous() or ncols <= 0 or xq.numel() % q8_1_row_bytes(ncols):
+        raise ValueError("dequantize_q8_1: xq must be uint8 [nrows][q8_1_row_bytes(ncols)]")
+    _on_device("dequantize_q8_1", xq)
+    nrows = xq.numel() // q8_1_row_bytes(ncols)
+    x = torch.empty(nrows, ncols, dtype=dtype, device=xq.device)
+    sums = torch.empty(nrows, ncols // 32, dtype=dtype, device=xq.device)
+    call("fns_hip_dequantize_q8_1", _p(xq), F32 if dtype == torch.float32 else F16, _p(x), _p(sums), ncols, nrows, _s())
+    return x, sums
+
+
+class KvCacheDesc(ctypes.Structure):
+    """Mirror of FnsKvCache (include/fns_hip.h)."""
+    _fields_ = [("n_head_kv", ctypes.c_int), ("head_dim", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("n_pages", ctypes.c_int64), ("pages", ctypes.c_void_p)]
+
+
+class KvBatchDesc(ctypes.Structure):
+    """Mirror of FnsKvBatch."""
+    _fields_ = [("n_seq", ctypes.c_int), ("max_q", ctypes.c_int), ("n_tok", ctypes.c_int64), ("max_kv", ctypes.c_int64),
+                ("table_stride", ctypes.c_int64), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("page_table", ctypes.c_void_p)]
+
+
+class KvAppendDesc(ctypes.Structure):
+    """Mirror of FnsKvAppend."""
+    _fields_ = [("dtype", ctypes.c_int), ("rope", ctypes.c_int), ("rope_dim", ctypes.c_int), ("n_head", ctypes.c_int),
+                ("inv_freq", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q", ctypes.c_void_p),
+                ("q_out", ctypes.c_void_p), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+                ("q_stride", ctypes.c_int64), ("q_out_stride", ctypes.c_int64)]
+
+
+class AttnDesc(ctypes.Structure):
+    """Mirror of FnsAttn."""
+    _fields_ = [("dtype", ctypes.c_int), ("n_head", ctypes.c_int), ("window", ctypes.c_int), ("scale", ctypes.c_float),
+                ("sinks", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64)]
+
+
+class KvCache:
+    """A paged key/value cache held in 4 bits (FnsKvCache): n_pages pages of page_size positions of every kv head, one
+    layer's. pages: uint8 device memory of an earlier cache of this shape, or None: zeroed."""
+
+    def __init__(self, n_pages: int, page_size: int, n_head_kv: int, head_dim: int, pages: torch.Tensor | None = None):
+        self.page_bytes = int(lib().fns_hip_kv_page_bytes(n_head_kv, head_dim, page_size))
+        if not self.page_bytes or n_pages <= 0:
+            raise ValueError(f"KvCache: unsupported shape (n_pages {n_pages}, page_size {page_size}, n_head_kv {n_head_kv}, "
+                             f"head_dim {head_dim})")
+        if pages is None:
+            pages = torch.zeros(n_pages, self.page_bytes, dtype=torch.uint8, device="cuda")
+        if pages.dtype != torch.uint8 or not pages.is_contiguous() or pages.numel() != n_pages * self.page_bytes:
+            raise ValueError(f"KvCache: pages must be contiguous uint8 of {n_pages} * {self.page_bytes} bytes")
+        _on_device("KvCache", pages)
+        self.pages, self.n_head_kv, self.head_dim, self.page_size = pages, n_head_kv, head_dim, page_size
+        self.desc = KvCacheDesc(n_head_kv, head_dim, page_size, n_pages, pages.data_ptr())
+
+
+class KvBatch:
+    """New tokens of some sequences over a KvCache (FnsKvBatch): q_start [n_seq + 1], kv_len [n_seq] and page_table
+    [n_seq][pages of a sequence] int32 device tensors, whose values a captured graph takes anew at each replay; n_tok rows of
+    the token arrays, max_q at least the new tokens of any sequence, max_kv about the longest sequence (None: what the table
+    has room for)."""
+
+    def __init__(self, q_start: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, n_tok: int, max_q: int,
+                 max_kv: int | None = None):
+        n_seq = kv_len.numel()
+        for t in (q_start, kv_len, page_table):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError("KvBatch: expected contiguous int32 tensors")
+        if q_start.numel() != n_seq + 1 or page_table.dim() != 2 or page_table.shape[0] != n_seq:
+            raise ValueError("KvBatch: expected q_start [n_seq + 1], kv_len [n_seq] and page_table [n_seq][pages]")
+        _on_device("KvBatch", q_start, kv_len, page_table)
+        self.q_start, self.kv_len, self.page_table, self.n_tok = q_start, kv_len, page_table, n_tok
+        self._open = max_kv is None
+        self.desc = KvBatchDesc(n_seq, max_q, n_tok, max_kv or 0, page_table.shape[1], q_start.data_ptr(), kv_len.data_ptr(),
+                                page_table.data_ptr())
+
+    def _for(self, cache: KvCache) -> KvBatchDesc:
+        if self._open:
+            self.desc.max_kv = min(self.desc.table_stride * cache.page_size, 2 ** 31 - 1)
+        return self.desc
+
+    @classmethod
+    def from_lists(cls, q_lens, kv_lens, pages, n_tok: int | None = None) -> "KvBatch":
+        """From host lists: new tokens and lengths (with them) of every sequence, and its pages in order."""
+        start = [0]
+        for q in q_lens:
+            start.append(start[-1] + q)
+        width = max([len(p) for p in pages] + [1])
+        table = [list(p) + [-1] * (width - len(p)) for p in pages]
+        dev = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+        return cls(dev(start), dev(list(kv_lens)), dev(table).view(len(table), width), start[-1] if n_tok is None else n_tok,
+                   max([*q_lens, 0]), max([*kv_lens, 0]))
+
+
+def rope_freqs(rope_dim: int, base: float = 10000.0, factors=None) -> torch.Tensor:
+    """inv_freq of kv_append: base^(-2 i / rope_dim), divided by factors[i] if given; f32 on the current device."""
+    f = float(base) ** (-torch.arange(0, rope_dim, 2, dtype=torch.float64) / rope_dim)
+    if factors is not None:
+        f = f / torch.as_tensor(factors, dtype=torch.float64, device="cpu")
+    return f.float().cuda()
+
+
+def _heads(what: str, t: torch.Tensor, n_tok: int, dim: int, dtype: torch.dtype) -> int:
+    """Token stride of t [n_tok][heads][dim], heads contiguous within a token (a slice of a fused projection is)."""
+    if t.dim() != 3 or t.shape[0] != n_tok or t.shape[2] != dim:
+        raise ValueError(f"{what}: expected [{n_tok}][heads][{dim}], got {list(t.shape)}")
+    if t.dtype != dtype or dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{what}: expected one type of f32 and bf16, got {t.dtype}")
+    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim)):
+        raise ValueError(f"{what}: the heads of a token must be contiguous")
+    _on_device(what, t)
+    width = t.shape[1] * dim
+    if n_tok > 1 and t.stride(0) < width:
+        raise ValueError(f"{what}: tokens overlap")
+    return t.stride(0) if n_tok > 1 else width
+
+
+def kv_append(cache: KvCache, batch: KvBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
+              rope: int = ROPE_NONE, inv_freq: torch.Tensor | None = None, q_out: torch.Tensor | None = None):
+    """k, v [n_tok][n_head_kv][head_dim] into the cache, k (and q) rotated by position * inv_freq over the first
+    2 * len(inv_freq) channels. -> the rotated q (in q_out, which may be q; None without q)."""
+    D, Hk = cache.head_dim, cache.n_head_kv
+    ks, vs = _heads("kv_append", k, batch.n_tok, D, k.dtype), _heads("kv_append", v, batch.n_tok, D, k.dtype)
+    if k.shape[1] != Hk or v.shape[1] != Hk:
+        raise ValueError(f"kv_append: expected {Hk} kv heads, got {k.shape[1]} and {v.shape[1]}")
+    qs = qos = 0
+    if q is not None:
+        qs = _heads("kv_append", q, batch.n_tok, D, k.dtype)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+        qos = _heads("kv_append", q_out, batch.n_tok, D, k.dtype)
+        if q_out.shape != q.shape:
+            raise ValueError("kv_append: q_out is not of q's shape")
+    elif q_out is not None:
+        raise ValueError("kv_append: q_out without q")
+    dim = 0
+    if rope != ROPE_NONE:
+        if inv_freq is None or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or inv_freq.dim() != 1:
+            raise ValueError("kv_append: a rotation needs inv_freq, a contiguous f32 vector")
+        _on_device("kv_append", inv_freq)
+        dim = 2 * inv_freq.numel()
+    x = KvAppendDesc(_dtype_code(k), rope, dim, 0 if q is None else q.shape[1], inv_freq.data_ptr() if dim else None,
+                     k.data_ptr(), v.data_ptr(), None if q is None else q.data_ptr(),
+                     None if q is None else q_out.data_ptr(), ks, vs, qs, qos)
+    call("fns_hip_kv_append", ctypes.byref(cache.desc), ctypes.byref(batch._for(cache)), ctypes.byref(x), _s())
+    return q_out
+
+
+def kv_read(cache: KvCache, batch: KvBatch):
+    """-> (k, v) f32 [n_tok][n_head_kv][head_dim]: what the cache holds of the batch's tokens."""
+    k = torch.empty(batch.n_tok, cache.n_head_kv, cache.head_dim, dtype=torch.float32, device=cache.pages.device)
+    v = torch.empty_like(k)
+    call("fns_hip_kv_read", ctypes.byref(cache.desc), ctypes.byref(batch._for(cache)), _p(k), _p(v), _s())
+    return k, v
+
+
+def _attn_desc(cache: KvCache, batch: KvBatch, q: torch.Tensor, out: torch.Tensor | None, scale: float, window: int,
+               sinks: torch.Tensor | None) -> AttnDesc:
+    qs = _heads("attn", q, batch.n_tok, cache.head_dim, q.dtype)
+    os_ = q.shape[1] * cache.head_dim
+    if out is not None:
+        os_ = _heads("attn", out, batch.n_tok, cache.head_dim, q.dtype)
+        if out.shape != q.shape:
+            raise ValueError("attn: out is not of q's shape")
+    if sinks is not None and (sinks.dtype != torch.float32 or not sinks.is_contiguous() or sinks.numel() != q.shape[1]):
+        raise ValueError("attn: sinks must be a contiguous f32 vector, one a query head")
+    _on_device("attn", sinks)
+    return AttnDesc(_dtype_code(q), q.shape[1], window, scale, None if sinks is None else sinks.data_ptr(), qs, os_)
+
+
+def attn_workspace(cache: KvCache, batch: KvBatch, q: torch.Tensor) -> torch.Tensor:
+    """A workspace of attn for this batch's numbers and q's heads; it may serve every layer of a step in turn."""
+    size = ctypes.c_size_t()
+    desc = _attn_desc(cache, batch, q, None, 1.0, 0, None)
+    call("fns_hip_attn_workspace", ctypes.byref(cache.desc), ctypes.byref(batch._for(cache)), ctypes.byref(desc),
+         ctypes.byref(size))
+    return torch.empty(size.value, dtype=torch.uint8, device=q.device)
+
+
+def attn(cache: KvCache, batch: KvBatch, q: torch.Tensor, scale: float | None = None, window: int = 0,
+         sinks: torch.Tensor | None = None, out: torch.Tensor | None = None, ws: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of q [n_tok][n_head][head_dim] over the cache -> out (rows of no sequence are left as they were). scale
+    None: head_dim^-0.5; window > 0: the last `window` positions only; sinks f32 [n_head] join the denominator."""
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    desc = _attn_desc(cache, batch, q, out, cache.head_dim ** -0.5 if scale is None else scale, window, sinks)
+    if ws is None:
+        ws = attn_workspace(cache, batch, q)
+    _on_device("attn", ws)
+    call("fns_hip_attn", ctypes.byref(cache.desc), ctypes.byref(batch._for(cache)), ctypes.byref(desc), _p(q), _p(out),
+         _p(ws), ws.numel() * ws.element_size(), _s())
     return out
 
 

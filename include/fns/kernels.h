@@ -10,6 +10,7 @@
 #include <cstdint>
 
 #include "fns/ggml_kernels.h"
+#include "fns_hip.h"
 
 namespace fns::k {
 
@@ -18,6 +19,11 @@ enum Gating : int { GATING_SOFTMAX = 0, GATING_SIGMOID = 1 };
 // rms_norm of `rows` rows of n, times w, then quantize_q8_1 of each output row into xq (rows of q8_1_row_bytes(n)).
 // Reference: src/kernels.cuh:29-32, src/kernels.cu:128-161 (n = 2048 there; any multiple of 32 here).
 void rms_norm_q8_1(const float *x, const float *w, float *out, void *xq, int n, float eps, int rows, hipStream_t st);
+
+// sum = x + y, then rms_norm_q8_1 of it (the same bits); sum may be x or y, out may be null. No counterpart in the
+// reference, whose engine adds and normalises in two launches.
+void add_rms_norm_q8_1(const float *x, const float *y, const float *w, float *sum, float *out, void *xq, int n, float eps,
+                       int rows, hipStream_t st);
 
 // y[c][r] = sum_i W[r][i] x[c][i] in fp32, c < cols (1..8). Reference: src/kernels.cuh:90-91, src/kernels.cu:452-482.
 void gemv_bf16(const void *w, const float *x, float *y, int ncols, int nrows, int cols, hipStream_t st);
@@ -62,5 +68,12 @@ void moe_combine_batch(const float *dexp, const float *escale, const float *w, c
 void gemm_bf16_batch(void *handle, const void *w, const float *x, void *xb, float *y, int ncols, int nrows, int n_tok,
                      hipStream_t st);
 void gemm_f32_batch(const float *w, const float *x, float *y, int ncols, int nrows, int n_tok, hipStream_t st);
+
+// The paged 4-bit key/value cache and attention over it; the descriptors and rules are those of fns_hip.h. In the place of
+// the reference's attention over a 16-bit cache (src/kernels.cu:230-450).
+void kv_append(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsKvAppend &x, hipStream_t st);
+void kv_read(const FnsKvCache &cache, const FnsKvBatch &batch, float *k, float *v, hipStream_t st);
+void attn(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsAttn &x, const void *q, void *out, void *workspace,
+          size_t workspace_bytes, hipStream_t st);
 
 }  // namespace fns::k

@@ -27,6 +27,7 @@ extern "C" {
 
 /* ggml type ids accepted by the quantized entry points (ggml.h numbering); router dtypes: 0 = f32, 30 = bf16. */
 #define FNS_TYPE_F32 0
+#define FNS_TYPE_F16 1
 #define FNS_TYPE_Q8_1 9
 #define FNS_TYPE_Q3_K 11
 #define FNS_TYPE_Q4_K 12
@@ -288,6 +289,95 @@ int fns_hip_dense_ffn_prefill(const FnsDenseFfn *ffn, const float *x, float *out
                               size_t workspace_bytes, void *stream);
 /* src/kernels.cuh:119 add_inplace, out-of-place: out[i] = x[i] + y[i]; out may alias x. */
 int fns_hip_add(const float *x, const float *y, float *out, int64_t n, void *stream);
+
+/* --- the attention half of a decoder block ---
+ * What an engine runs between the projections (fns_hip_mmvq / fns_hip_mmq of the quantised rows) and the FFN calls above:
+ *   Q8_1 rows -> mmvq (q, k, v) -> fns_hip_kv_append -> fns_hip_attn -> quantize_q8_1, mmvq (output projection)
+ *   -> fns_hip_add_rms_norm_q8_1 -> gemv_router, mmvq_experts_swiglu ...
+ * The reference's counterparts (src/kernels.cuh k::attention*, src/kernels.cu:230-450, flash_attn_prefill of
+ * include/fns/ggml_kernels.h:71-77) read a 16-bit cache of one sequence; this cache is paged, holds many sequences and
+ * takes 4.25 bits a value. */
+
+/* sum = x + y; out = sum * w / sqrt(mean(sum^2) + eps) per row; xq = Q8_1 blocks of out (rows of
+ * fns_hip_q8_1_row_bytes(n), padded with zeros as rms_norm_q8_1's). All f32 [rows][n], n a multiple of 32, w [n]. The bits
+ * of fns_hip_add followed by fns_hip_rms_norm_q8_1. sum may be x or y (otherwise no overlaps); out may be NULL. */
+int fns_hip_add_rms_norm_q8_1(const float *x, const float *y, const float *w, float *sum, float *out, void *xq, int n,
+                              float eps, int rows, void *stream);
+/* What Q8_1 rows (fns_hip_q8_1_row_bytes(ncols) apart, ncols a multiple of 32) stand for: x [nrows][ncols] = q * d and,
+ * unless NULL, sums [nrows][ncols / 32], the blocks' held sums; both of `dtype` FNS_TYPE_F32 or FNS_TYPE_F16. */
+int fns_hip_dequantize_q8_1(const void *xq, int dtype, void *x, void *sums, int64_t ncols, int64_t nrows, void *stream);
+
+/* A paged key/value cache held in 4 bits: blocks of 32 channels of one token and kv head, e2m1 codes (0, .5, 1, 1.5, 2, 3,
+ * 4, 6 and their negatives) times 2^(e - 127), one byte e a block, the least with max |block| <= 7 * 2^(e - 127); codes to
+ * nearest, ties to even. A block with a NaN or infinity stands for NaNs. `pages`: n_pages * fns_hip_kv_page_bytes bytes,
+ * 16-byte aligned; what is never read need not be initialised. */
+typedef struct FnsKvCache {
+    int n_head_kv;  /* 1..1024 */
+    int head_dim;   /* 64, 128 or 256 */
+    int page_size;  /* positions of a page: a power of two, 16..4096 */
+    int64_t n_pages;
+    void *pages;
+} FnsKvCache;
+/* Bytes of a page; 0 for an unsupported shape. */
+size_t fns_hip_kv_page_bytes(int n_head_kv, int head_dim, int page_size);
+/* New tokens of n_seq sequences. Tokens q_start[s] .. q_start[s + 1] - 1 are sequence s's last ones: kv_len[s] is its length
+ * with them, so token i of n has position kv_len[s] - n + i. Position p lies in page page_table[s * table_stride +
+ * p / page_size]; an entry that no position of a call needs may be anything. q_start, kv_len and page_table are device
+ * memory (a captured graph takes their values at each replay); the numbers below are the host's:
+ *   n_tok   rows of the token arrays: tokens from q_start[n_seq] on are padding and left alone
+ *   max_q   at least the new tokens of any sequence (more than this many are not handled)
+ *   max_kv  about the longest kv_len: work is split by it, results hold for any
+ * A q_start range outside 0..n_tok or descending is a sequence without tokens. A position whose table entry is outside the
+ * table or the cache's pages is never read or written: append leaves it out, attention sees no key there, kv_read gives NaN. */
+typedef struct FnsKvBatch {
+    int n_seq, max_q;
+    int64_t n_tok, max_kv, table_stride;
+    const int32_t *q_start;     /* [n_seq + 1] */
+    const int32_t *kv_len;      /* [n_seq] */
+    const int32_t *page_table;  /* [n_seq][table_stride] */
+} FnsKvBatch;
+
+#define FNS_ROPE_NONE 0
+#define FNS_ROPE_HALVES 1 /* channel i turns with i + rope_dim / 2 */
+#define FNS_ROPE_PAIRS 2  /* channel 2 i turns with 2 i + 1 */
+/* k, v [n_tok][n_head_kv][head_dim] (tokens k_stride / v_stride elements apart) into the cache; the first rope_dim channels
+ * of k and of q are turned by position * inv_freq[i] on the way (in 64 bits; k is held from the unrounded result). q
+ * [n_tok][n_head][head_dim] -> q_out of the same type, n_head a multiple of n_head_kv, or n_head = 0: no queries. q_out may
+ * be q (with its stride). Heads are contiguous within a token; no alignment beyond an element's is needed. Positions that
+ * two sequences share (a common page) must not be appended by both in one call. */
+typedef struct FnsKvAppend {
+    int dtype; /* of k, v, q and q_out: FNS_TYPE_F32 or FNS_TYPE_BF16 */
+    int rope;  /* FNS_ROPE_* */
+    int rope_dim; /* a multiple of 16 up to head_dim (ignored without a rotation) */
+    int n_head;
+    const float *inv_freq; /* f32 [rope_dim / 2] */
+    const void *k, *v, *q;
+    void *q_out;
+    int64_t k_stride, v_stride, q_stride, q_out_stride;
+} FnsKvAppend;
+int fns_hip_kv_append(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvAppend *x, void *stream);
+/* k, v f32 [n_tok][n_head_kv][head_dim]: what the cache holds of the batch's tokens. */
+int fns_hip_kv_read(const FnsKvCache *cache, const FnsKvBatch *batch, float *k, float *v, void *stream);
+
+/* Attention of the batch's tokens over the cache (their own keys included: append first). Query head h reads kv head
+ * h / (n_head / n_head_kv). The token at position p sees positions 0..p, with window > 0 the last `window` of them.
+ *   out = sum_j p_j V_j, p = softmax over the seen positions of scale * q . K_j; with sinks, exp(sinks[h]) joins the
+ *   softmax's denominator. A row that sees nothing is zero; one that sees a token whose K or V holds a NaN block is NaN.
+ * q and out [n_tok][n_head][head_dim], heads contiguous within a token, no overlap, any element alignment. With FNS_TYPE_F32
+ * products carry 22 bits of q and of p; with FNS_TYPE_BF16, q is exact and p has 11 bits. Softmax statistics and sums are
+ * f32. workspace: fns_hip_attn_workspace bytes (it grows with n_tok, n_seq, max_q, max_kv and n_head only), 16-byte aligned,
+ * no initialisation; calls that overlap in time need one each. */
+typedef struct FnsAttn {
+    int dtype; /* of q and out: FNS_TYPE_F32 or FNS_TYPE_BF16 */
+    int n_head;
+    int window; /* 0: none */
+    float scale;
+    const float *sinks; /* NULL or f32 [n_head] */
+    int64_t q_stride, out_stride; /* elements between tokens */
+} FnsAttn;
+int fns_hip_attn_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, size_t *bytes);
+int fns_hip_attn(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const void *q, void *out,
+                 void *workspace, size_t workspace_bytes, void *stream);
 
 /* --- GGUF checkpoints: reader and fully resident MoE layers ---
  * Replaces the reference's loader (src/model.cpp:30-136: gguf header and tensor table, the file mapped without copying)
