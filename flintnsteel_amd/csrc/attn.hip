@@ -23,7 +23,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;     // keys of a step
 constexpr int kHead = 12;     // K and V expand to f16 with their tile's largest block scale at 2^12 (codes to 6: 24576)
 constexpr int kBias = 127 + kHead;
-constexpr float kPShift = 10.0f;  // p is carried times 2^10: its low half stays clear of f16's subnormals
+// p is carried times 2^8: its low half stays clear of f16's subnormals. Sums are rescaled only where a row's maximum has
+// grown by more than 2^7 since the last time, so p stays below 2^15.
+constexpr float kPShift = 8.0f, kLazy = 7.0f;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -81,24 +83,19 @@ __device__ __forceinline__ int split_chunk(const AttnArgs &a, const RowTiles &t)
     return max(a.chunk, (t.t1 - t.t0 + a.splits - 1) / a.splits);
 }
 
-// The scale bytes of one position's K and V, NB of each.
-template <int NB> struct ScaleWords {
-    static constexpr int W = (NB + 3) / 4;
-    uint32_t k[W], v[W];
-};
-template <int D> __device__ __forceinline__ ScaleWords<D / 32> load_scales(const uint8_t *base, int P, int row) {
-    using L = KvParts<D>;
-    constexpr int NB = D / 32;
-    ScaleWords<NB> w = {};
-    __builtin_memcpy(w.k, __builtin_assume_aligned(base + L::k_scale(P, row), NB), NB);
-    __builtin_memcpy(w.v, __builtin_assume_aligned(base + L::v_scale(P, row), NB), NB);
-    return w;
-}
-
 // What a wave knows of a tile, a key a lane: which keys are there, which of them hold NaNs, the largest scale bytes.
 struct TileInfo {
     uint64_t there, nan;
     int ek, ev;
+};
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_max(uint32_t x, uint32_t y) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, x), __builtin_bit_cast(us2, y)));
+}
+// The scale bytes of one position's K and V, NB of each.
+template <int NB> struct ScaleWords {
+    static constexpr int W = (NB + 3) / 4;
+    uint32_t k[W], v[W];
 };
 // ... and the block scales as the f32 operands of the expansion, in the wave's LDS: K [64 in the order of the products'
 // rows][NB], V [NB][64 keys]. A block's operand is 2^(e - E + 12) for the tile's (K) or the largest so far (V) scale E; what
@@ -106,41 +103,53 @@ struct TileInfo {
 __device__ __forceinline__ int row_of_key(int key) { return (key >> 2 & 3) * 16 + (key >> 4) * 4 + (key & 3); }
 template <int NB>
 __device__ __forceinline__ TileInfo tile_scales(ScaleWords<NB> w, bool there, int ev_before, float *ksc, float *vsc) {
+    constexpr int W = ScaleWords<NB>::W;
+    constexpr uint32_t kEven = 0x00ff00ffu;
     const int lane = threadIdx.x % 64;
-    int e[2][NB], top[2] = {0, 0};
-    bool nan = false;
+    uint32_t e[2][W][2], top[2];  // bytes 0 and 2, 1 and 3 of every word, in halves
+    const auto split = [&](int s) {
+        top[s] = 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        e[0][b] = there ? (w.k[b / 4] >> (b % 4 * 8)) & 255 : 0;
-        e[1][b] = there ? (w.v[b / 4] >> (b % 4 * 8)) & 255 : 0;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            nan |= e[s][b] == 255;
-            e[s][b] = e[s][b] == 255 ? 0 : e[s][b];
-            top[s] = max(top[s], e[s][b]);
+        for (int i = 0; i < W; ++i) {
+            const uint32_t x = s ? w.v[i] : w.k[i];
+            e[s][i][0] = x & kEven, e[s][i][1] = x >> 8 & kEven;
+            top[s] = pk_max(top[s], pk_max(e[s][i][0], e[s][i][1]));
         }
-    }
+        top[s] = max(top[s] & 0xffffu, top[s] >> 16);
+    };
+#pragma unroll
+    for (int i = 0; i < W; ++i) w.k[i] = there ? w.k[i] : 0, w.v[i] = there ? w.v[i] : 0;
+    split(0), split(1);
     TileInfo t;
     t.there = __ballot(there);
-    t.nan = __ballot(nan);
-    int both = top[0] << 16 | top[1];
-    const auto pkmax = [](int x, int y) {
-        typedef uint16_t us2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(int, __builtin_elementwise_max(__builtin_bit_cast(us2, x), __builtin_bit_cast(us2, y)));
-    };
-    both = pkmax(both, xor_lane_i<1>(both));
-    both = pkmax(both, xor_lane_i<2>(both));
-    both = pkmax(both, xor_lane_i<4>(both));
-    both = pkmax(both, xor_lane_i<8>(both));
-    both = pkmax(both, xor_lane_i<16>(both));
-    both = pkmax(both, xor_lane_i<32>(both));
+    t.nan = __ballot(max(top[0], top[1]) == 255u);
+    if (t.nan) {  // rare: their blocks count as zeros, the rows that see them are made NaN
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t m = 255u << (8 * b);
+                w.k[i] = (w.k[i] & m) == m ? w.k[i] & ~m : w.k[i];
+                w.v[i] = (w.v[i] & m) == m ? w.v[i] & ~m : w.v[i];
+            }
+        split(0), split(1);
+    }
+    uint32_t both = top[0] << 16 | top[1];
+    both = pk_max(both, xor_lane_i<1>(both));
+    both = pk_max(both, xor_lane_i<2>(both));
+    both = pk_max(both, xor_lane_i<4>(both));
+    both = pk_max(both, xor_lane_i<8>(both));
+    both = pk_max(both, xor_lane_i<16>(both));
+    both = pk_max(both, xor_lane_i<32>(both));
     both = __builtin_amdgcn_readfirstlane(both);
     t.ek = both >> 16;
-    t.ev = max(both & 0xffff, ev_before);
+    t.ev = max((int) (both & 0xffffu), ev_before);
+    const auto field = [](uint32_t e, int top) { return __builtin_bit_cast(float, max((int) e + kBias - top, 0) << 23); };
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        ksc[row_of_key(lane) * NB + b] = __builtin_bit_cast(float, max(e[0][b] + kBias - t.ek, 0) << 23);
-        vsc[b * 64 + lane] = __builtin_bit_cast(float, max(e[1][b] + kBias - t.ev, 0) << 23);
+        const int i = b / 4, odd = b % 2, sh = b % 4 / 2 * 16;
+        ksc[row_of_key(lane) * NB + b] = field(e[0][i][odd] >> sh & 0xffu, t.ek);
+        vsc[b * 64 + lane] = field(e[1][i][odd] >> sh & 0xffu, t.ev);
     }
     return t;
 }
@@ -170,13 +179,9 @@ __device__ __forceinline__ void expand_v(uint32_t w0, uint32_t w1, const float *
 
 // The queries of one column tile (16 rows) as operands of the products: lane (row r = lane % 16, g = lane / 16) holds the
 // channels g NB 8 + 8 u .. + 7 of step u, in one (bf16: exact) or two (f32: 22 bits) f16 parts, the row scaled by a power
-// of two to a largest magnitude in [2^10, 2^11). mul turns a product (of K at its tile's 2^12) into log2 units.
-template <int NB, int SPLIT> struct Queries {
-    h8 part[SPLIT][NB];
-    float mul;
-};
+// of two to a largest magnitude in [2^10, 2^11). Returns what turns a product (of K at its tile's 2^12) into log2 units.
 template <int NB, int SPLIT, class T>
-__device__ __forceinline__ void load_queries(Queries<NB, SPLIT> &o, const T *row, bool there, float scale) {
+__device__ __forceinline__ float load_queries(h8 (&part)[SPLIT][NB], const T *row, bool there, float scale) {
     const int g = threadIdx.x % 64 / 16;
     float v[NB][8], amax = 0.0f;
     bool bad = false;
@@ -199,20 +204,20 @@ __device__ __forceinline__ void load_queries(Queries<NB, SPLIT> &o, const T *row
     if (amax > 0.0f && !bad) k = ilogbf(amax) + 1;
     k = max(k, -100);
     const float f = bad ? __builtin_nanf("") : ldexpf(scale < 0.0f ? -1.0f : 1.0f, 11 - k);
-    o.mul = fabsf(scale) * kLog2e * ldexpf(1.0f, k - 11);
 #pragma unroll
     for (int u = 0; u < NB; ++u)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float x = v[u][i] * f;
             const _Float16 hi = (_Float16) x;
-            o.part[0][u][i] = hi;
-            if constexpr (SPLIT == 2) o.part[1][u][i] = (_Float16) (x - (float) hi);
+            part[0][u][i] = hi;
+            if constexpr (SPLIT == 2) part[1][u][i] = (_Float16) (x - (float) hi);
         }
+    return fabsf(scale) * kLog2e * ldexpf(1.0f, k - 11);
 }
 
 // A lane's state of one column tile: row r = lane % 16; a lane sums the keys 16 g .. 16 g + 15 of every tile, and holds
-// channels 16 dt + 4 g + i of its row in o[dt][i] (in units of 2^(ev - 139)).
+// channels 16 dt + 4 g + i of its row in o[dt][i] (in units of 2^(ev - 139)). m: the maximum that p and the sums refer to.
 template <int NB> struct RowState {
     f4 o[2 * NB];
     float m, l;
@@ -229,38 +234,54 @@ __device__ __forceinline__ float softmax_step(f4 (&s)[4], float mul, uint32_t se
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[t][i] = see >> (4 * t + i) & 1 ? s[t][i] : -INFINITY;
     }
-    float top = s[0][0];
+    float top = fmaxf(s[0][0], s[0][1]);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][i]);
+    for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[i / 4][i % 4]), s[i / 4][i % 4 + 1]);
     top = fmaxf(top, xor_lane<16>(top));
     top = fmaxf(top, xor_lane<32>(top));
-    const float now = fmaxf(m, top == -INFINITY ? top : top * mul);
-    const float off = now == -INFINITY ? 0.0f : now;  // nothing seen so far: no difference of infinities
-    const float keep = __builtin_amdgcn_exp2f(m - off);
-    m = now;
+    const float now = top == -INFINITY ? top : top * mul;
+    float keep = 1.0f;
+    if (__any(now > m + kLazy)) {
+        const float to = fmaxf(m, now);
+        keep = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));  // (nothing seen so far: no difference of infinities)
+        m = to;
+    }
+    const float add = kPShift - (m == -INFINITY ? 0.0f : m);
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], mul, kPShift - off));
-            if (!all) x = see >> (4 * t + i) & 1 ? x : 0.0f;
-            if (nan) x = see >> (4 * t + i) & nan >> (4 * t + i) & 1 ? __builtin_nanf("") : x;
-            sum += x;
-            s[t][i] = x;
-        }
+        for (int i = 0; i < 4; ++i) s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], mul, add));
+    if (!all)  // (a scale of zero times -infinity)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][i] = see >> (4 * t + i) & 1 ? s[t][i] : 0.0f;
+    if (nan)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][i] = see >> (4 * t + i) & nan >> (4 * t + i) & 1 ? __builtin_nanf("") : s[t][i];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) sum += (s[t][0] + s[t][1]) + (s[t][2] + s[t][3]);
     l = l * keep + sum;
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
+    for (int v = 0; v < 2; ++v) {
+        u4 w[SPLIT];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = s[2 * v + i / 4][i % 4];
-            const _Float16 hi = (_Float16) x;
-            p[0][v][i] = hi;
-            if constexpr (SPLIT == 2) p[1][v][i] = (_Float16) (x - (float) hi);
+        for (int i = 0; i < 4; ++i) {
+            const float x = s[2 * v + i / 2][i % 2 * 2], y = s[2 * v + i / 2][i % 2 * 2 + 1];
+            if constexpr (SPLIT == 2) {  // toward zero: the second part has the rest
+                const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+                w[0][i] = __builtin_bit_cast(uint32_t, hi);
+                w[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - (float) hi[0], y - (float) hi[1]));
+            } else {
+                w[0][i] = __builtin_bit_cast(uint32_t, h2{(_Float16) x, (_Float16) y});
+            }
         }
+#pragma unroll
+        for (int h = 0; h < SPLIT; ++h) p[h][v] = __builtin_bit_cast(h8, w[h]);
+    }
     return keep;
 }
 
@@ -283,20 +304,65 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t tok, int h,
     else store4((T *) a.out + tok * a.out_stride + (int64_t) h * D + ch, v);
 }
 
+// Where a tile's bytes are. With pages of 64 positions or more a tile lies in one page: every address is the tile's (in
+// scalar registers) plus an offset that a lane keeps; smaller pages (SMALL) are looked up for every 16 positions.
+template <int D, bool SMALL> struct TileReader {
+    static constexpr int NB = D / 32, KC = NB * 4;  // KC: code bytes of a lane's channels of one key
+    using L = KvParts<D>;
+    int P, lane, r, g;
+    int64_t head_off;
+    const uint8_t *bk, *bv;  // of the lane's K rows (keys 16 (r / 4) ..), and of its own key and V columns (16 g ..)
+    int row;                 // of the tile's first position in its page
+    bool there;
+    __device__ __forceinline__ void page(const AttnArgs &a, int s, int tile, bool in) {
+        const int base = tile * kTile;
+        row = base & (P - 1);
+        if constexpr (SMALL) {
+            const int pk = in ? page_of(a.c, a.b, s, base + 16 * (r / 4)) : -1, pv = in ? page_of(a.c, a.b, s, base + 16 * g) : -1;
+            bk = a.c.pages + max(pk, 0) * a.c.page_bytes + head_off;
+            bv = a.c.pages + max(pv, 0) * a.c.page_bytes + head_off;
+            there = pv >= 0;
+        } else {
+            const int p = in ? __builtin_amdgcn_readfirstlane(page_of(a.c, a.b, s, base)) : -1;
+            bk = bv = a.c.pages + max(p, 0) * a.c.page_bytes + head_off;
+            there = p >= 0;
+        }
+    }
+    __device__ __forceinline__ void scales(ScaleWords<NB> &w) const {
+        const int at = (SMALL ? (row + lane) & (P - 1) : row + lane);
+        w = {};
+        __builtin_memcpy(w.k, __builtin_assume_aligned(bv + L::k_scale(P, at), NB), NB);
+        __builtin_memcpy(w.v, __builtin_assume_aligned(bv + L::v_scale(P, at), NB), NB);
+    }
+    __device__ __forceinline__ void k(uint32_t (&x)[4][NB]) const {
+        const int at = SMALL ? (row + 16 * (r / 4)) & (P - 1) : row + 16 * (r / 4);
+        const uint8_t *p = bk + (uint32_t) ((at + r % 4) * (D / 2) + g * KC);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) __builtin_memcpy(x[t], __builtin_assume_aligned(p + 4 * t * (D / 2), KC < 16 ? KC : 16), KC);
+    }
+    __device__ __forceinline__ void v(u4 (&x)[NB]) const {
+        const int at = SMALL ? (row + 16 * g) & (P - 1) : row + 16 * g;
+        const uint8_t *p = bv + (uint32_t) (P * (D / 2) + r * P + at);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) x[j] = *(const u4 *) (p + (uint32_t) (16 * j * P));
+    }
+};
+
 // Few rows (decode, verify): the workgroup's waves take tiles of keys in turn and are joined at the end. A wave's tile goes
 // from the pages to registers and stays there: S^T = K Q^T with K's rows in an order that leaves every lane with the 16
 // consecutive keys 16 g .. 16 g + 15 of its query row, which is where the second product, O^T = V^T P^T, wants P, and where
 // V's bytes (16 consecutive positions of a channel pair) are. Bound by the cache's bytes for long contexts and by a few
-// dependent loads for short ones: each wave asks for its next tile before it works on this one.
-template <int D, int CT, class T>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_few(AttnArgs a) {
+// dependent loads for short ones. One wave issues a vector instruction about every 5 cycles where the SIMD takes one every
+// 2: what pays is waves, so the queries lie in LDS and the next tile's K is asked for when this one's is used up.
+template <int D, int CT, bool SMALL, class T>
+__global__ __launch_bounds__(256, D == 256 || CT == 2 ? 2 : 4) void k_attn_few(AttnArgs a) {
     constexpr int NB = D / 32, SPLIT = sizeof(T) == 4 ? 2 : 1, NW = 4;
-    constexpr int KC = NB * 4;  // code bytes of a lane's channels of one key
-    constexpr int kScale = 2 * 64 * NB;
-    __shared__ __align__(16) float lds[NW * kScale > NW / 2 * CT * 2 * NB * 256 ? NW * kScale : NW / 2 * CT * 2 * NB * 256];
-    __shared__ float join[NW][3][CT * 16];
+    constexpr int kScale = 2 * 64 * NB, kJoin = NW / 2 * CT * 2 * NB * 256;
+    __shared__ __align__(16) float lds[NW * kScale > kJoin ? NW * kScale : kJoin];
+    __shared__ __align__(16) h8 qs[CT][SPLIT][NB][64];
+    __shared__ float join[NW][2][CT * 16], qmul[CT][16];
     const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, row0 = blockIdx.y * 16 * CT, split = blockIdx.z;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     const SeqRange sr = seq_range(a.b, s);
     const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) INT32_MAX);
     if (row0 >= rows) return;
@@ -305,11 +371,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_few(AttnArgs a) 
     const int t0 = (int) min((int64_t) rt.t0 + (int64_t) split * chunk, (int64_t) rt.t1);
     const int t1 = min(t0 + chunk, rt.t1);
     if (split > 0 && t0 >= t1) return;  // (split 0 of an empty range writes the zeros)
-    const int P = 1 << a.c.shift, pmask = P - 1;
-    using L = KvParts<D>;
-    const int64_t head_off = head * kv_head_bytes(D, P);
+    const int P = 1 << a.c.shift;
 
-    Queries<NB, SPLIT> q[CT];
+    TileReader<D, SMALL> rd;
+    rd.P = P, rd.lane = lane, rd.r = r, rd.g = g, rd.head_off = head * kv_head_bytes(D, P);
+    uint32_t kraw[4][NB];
+    u4 vraw[NB];
+    ScaleWords<NB> sw = {};
+    int tile = t0 + wave;
+    rd.page(a, s, tile, tile < t1);
+    if (tile < t1) rd.scales(sw), rd.k(kraw), rd.v(vraw);
+
     RowState<NB> st[CT];
     int pos[CT];
 #pragma unroll
@@ -317,65 +389,62 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_few(AttnArgs a) 
         const int row = row0 + 16 * c + r, i = row / a.group;
         const bool there = row < rows;
         pos[c] = there ? sr.len - sr.n + i : -1;
-        load_queries(q[c], (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D, there, a.scale);
+        if (wave == c) {
+            h8 part[SPLIT][NB];
+            const float mul = load_queries(part, (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D,
+                                           there, a.scale);
+#pragma unroll
+            for (int h = 0; h < SPLIT; ++h)
+#pragma unroll
+                for (int u = 0; u < NB; ++u) qs[c][h][u][lane] = part[h][u];
+            if (g == 0) qmul[c][r] = mul;
+        }
         st[c].m = -INFINITY, st[c].l = 0.0f;
 #pragma unroll
         for (int d = 0; d < 2 * NB; ++d) st[c].o[d] = f4{0, 0, 0, 0};
     }
+    __syncthreads();
+    float mul[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) mul[c] = qmul[c][r];
 
-    struct Raw {
-        uint32_t k[4][NB];
-        u4 v[NB];
-        ScaleWords<NB> sc;
-        bool there;
-    } cur, nxt;
-    // pages of the lane's K rows (keys 16 (r / 4) ..) and of its own key and V columns (16 g ..)
-    const auto pages_of = [&](int tile, int &pk, int &pv) {
-        pk = tile < t1 ? page_of(a.c, a.b, s, tile * kTile + 16 * (r / 4)) : -1;
-        pv = tile < t1 ? page_of(a.c, a.b, s, tile * kTile + 16 * g) : -1;
-    };
-    const auto load = [&](Raw &x, int tile, int pk, int pv) {
-        const int base = tile * kTile, key = base + lane;
-        const uint8_t *bk = a.c.pages + max(pk, 0) * a.c.page_bytes + head_off;
-        const uint8_t *bv = a.c.pages + max(pv, 0) * a.c.page_bytes + head_off;
-        x.there = pv >= 0 && key >= rt.lo && key < rt.hi;
-        x.sc = load_scales<D>(bv, P, key & pmask);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int krow = (base + 16 * (r / 4) + 4 * t + r % 4) & pmask;
-            __builtin_memcpy(x.k[t], __builtin_assume_aligned(bk + L::k_row(P, krow) + g * KC, KC < 16 ? KC : 16), KC);
-        }
-#pragma unroll
-        for (int j = 0; j < NB; ++j) x.v[j] = *(const u4 *) (bv + L::v_col(P, 16 * j + r) + ((base + 16 * g) & pmask));
-    };
     float *ksc = lds + wave * kScale, *vsc = ksc + 64 * NB;
-    int ev = 1, pk, pv;
-    int tile = t0 + wave;
-    pages_of(tile, pk, pv);
-    if (tile < t1) load(cur, tile, pk, pv);
-    pages_of(tile + NW, pk, pv);
+    int ev = 1;
     for (; tile < t1; tile += NW) {
-        if (tile + NW < t1) load(nxt, tile + NW, pk, pv);
-        pages_of(tile + 2 * NW, pk, pv);
-        const int base = tile * kTile;
-        const TileInfo ti = tile_scales<NB>(cur.sc, cur.there, ev, ksc, vsc);
+        const int base = tile * kTile, key = base + lane;
+        const TileInfo ti = tile_scales<NB>(sw, rd.there && key >= rt.lo && key < rt.hi, ev, ksc, vsc);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         f4 sc[CT][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int c = 0; c < CT; ++c)
 #pragma unroll
-            for (int c = 0; c < CT; ++c) sc[c][t] = f4{0, 0, 0, 0};
+            for (int t = 0; t < 4; ++t) sc[c][t] = f4{0, 0, 0, 0};
+        float ks[4][(NB + 3) / 4];
 #pragma unroll
-            for (int u = 0; u < NB; ++u) {
-                const h8 k = expand_k(cur.k[t][u], ksc[(16 * t + r) * NB + (g * NB + u) / 4]);
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int u = 0; u < (NB + 3) / 4; ++u) ks[t][u] = ksc[(16 * t + r) * NB + (g * NB + 4 * u) / 4];
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+            h8 q[CT][SPLIT];
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int h = 0; h < SPLIT; ++h) q[c][h] = qs[c][h][u][lane];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const h8 k = expand_k(kraw[t][u], ks[t][u / 4]);
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
                     for (int h = SPLIT - 1; h >= 0; --h)
-                        sc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[c].part[h][u], sc[c][t], 0, 0, 0);
+                        sc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[c][h], sc[c][t], 0, 0, 0);
             }
         }
+        const bool more = tile + NW < t1;
+        rd.page(a, s, tile + NW, more);
+        if (more) rd.scales(sw), rd.k(kraw);
         const float back = ldexpf(1.0f, ti.ek - kBias), vkeep = ldexpf(1.0f, max(ev - ti.ev, -126));
         ev = ti.ev;
         h8 p[CT][SPLIT][2];
@@ -383,7 +452,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_few(AttnArgs a) 
         for (int c = 0; c < CT; ++c) {
             const uint32_t see = seen(pos[c], a.window, base, ti.there);
             const uint32_t nan = ti.nan ? (uint32_t) (ti.nan >> (16 * g)) & 0xffffu : 0u;
-            const float keep = softmax_step<SPLIT>(sc[c], q[c].mul * back, see, nan, st[c].m, st[c].l, p[c]) * vkeep;
+            const float keep = softmax_step<SPLIT>(sc[c], mul[c] * back, see, nan, st[c].m, st[c].l, p[c]) * vkeep;
             if (__any(keep != 1.0f))
 #pragma unroll
                 for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= keep;
@@ -396,7 +465,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_few(AttnArgs a) 
                 float w[8];
                 *(f4 *) w = *(const f4 *) (vsc + j * 64 + 16 * g + 8 * v);
                 *(f4 *) (w + 4) = *(const f4 *) (vsc + j * 64 + 16 * g + 8 * v + 4);
-                expand_v(cur.v[j][2 * v], cur.v[j][2 * v + 1], w, lo, hi);
+                expand_v(vraw[j][2 * v], vraw[j][2 * v + 1], w, lo, hi);
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -405,9 +474,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_few(AttnArgs a) 
                         st[c].o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, p[c][h][v], st[c].o[2 * j + 1], 0, 0, 0);
                     }
             }
+        if (more) rd.v(vraw);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        cur = nxt;
     }
 
     // join the waves: the common maximum and sum of every row, then the sums in a tree over registers of equal layout
@@ -449,7 +518,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_few(AttnArgs a) 
             for (int c = 0; c < CT; ++c)
 #pragma unroll
                 for (int d = 0; d < 2 * NB; ++d) st[c].o[d] += x[(c * 2 * NB + d) * 64];
-        __syncthreads();
+        if (half > 1) __syncthreads();
     }
     if (wave != 0) return;
 #pragma unroll
@@ -464,44 +533,48 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_few(AttnArgs a) 
     }
 }
 
-// The splits of a row into its result: a wave a row.
+// The splits of a row into its result: a workgroup a row, its waves the splits in turn (at most 64: one a lane for their
+// weights), a lane D / 64 channels.
 template <int D, class T>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int rows_per_wg) {
-    const int s = blockIdx.y, lane = threadIdx.x % 64;
+    constexpr int C = D / 64, NW = 4;
+    __shared__ float part[NW][D], weight[64];
+    const int s = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const SeqRange sr = seq_range(a.b, s);
-    const int64_t w = (int64_t) blockIdx.x * 4 + threadIdx.x / 64;
-    const int i = (int) (w / a.n_head), h = (int) (w % a.n_head);
+    const int i = blockIdx.x / a.n_head, h = blockIdx.x % a.n_head;
     if (i >= sr.n) return;
     const int64_t tok = sr.q0 + i, first = tok * a.n_head + h, step = a.b.n_tok * a.n_head;
     const int row = i * a.group + h % a.group, row0 = row / rows_per_wg * rows_per_wg;
     const RowTiles rt = row_tiles(a, sr, row0, rows_per_wg);
     const int chunk = split_chunk(a, rt);
-    const int n = max(1, (rt.t1 - rt.t0 + chunk - 1) / chunk);  // splits that have tiles (the first one in any case)
+    const int n = max(1, (rt.t1 - rt.t0 + chunk - 1) / max(chunk, 1));  // splits that have tiles (the first one in any case)
     const float sk = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-    float top = sk;
-    for (int k = lane; k < n; k += 64) top = fmaxf(top, a.part_ml[k * step + first].x);
-    top = lanes_max<64>(top);
+    const float2 ml = lane < n ? a.part_ml[lane * step + first] : make_float2(-INFINITY, 0.0f);
+    const float top = fmaxf(lanes_max<64>(ml.x), sk);
     const float off = top == -INFINITY ? 0.0f : top;
-    float sum = a.sinks ? __builtin_amdgcn_exp2f(sk - off + kPShift) : 0.0f;
-    constexpr int C = D / 64;
+    const float f = ml.y == 0.0f ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - off);
+    const float sum = lanes_sum<64>(f) + (a.sinks ? __builtin_amdgcn_exp2f(sk - off + kPShift) : 0.0f);
+    if (wave == 0) weight[lane] = sum == 0.0f ? 0.0f : f / sum;
+    __syncthreads();
     float o[C] = {};
-    for (int k = 0; k < n; ++k) {
-        const float2 ml = a.part_ml[k * step + first];
-        const float f = ml.y == 0.0f ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - off);
-        sum += f;
+    const float *src = a.part + first * D + lane * C;
+#pragma unroll 8
+    for (int k = wave; k < n; k += NW) {
+        const float wk = weight[k];
         float v[C];
-        __builtin_memcpy(v, __builtin_assume_aligned(a.part + (k * step + first) * D + lane * C, 4 * C), sizeof v);
+        __builtin_memcpy(v, __builtin_assume_aligned(src + k * step * D, 4 * C), sizeof v);
 #pragma unroll
-        for (int c = 0; c < C; ++c) o[c] += f == 0.0f ? 0.0f : f * v[c];
+        for (int c = 0; c < C; ++c) o[c] += wk == 0.0f ? 0.0f : wk * v[c];
     }
-    T t[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const float x = sum == 0.0f ? 0.0f : o[c] / sum;
-        if constexpr (sizeof(T) == 4) t[c] = x;
-        else t[c] = to_bf16(x);
+    for (int c = 0; c < C; ++c) part[wave][lane * C + c] = o[c];
+    __syncthreads();
+    T *out = (T *) a.out + tok * a.out_stride + (int64_t) h * D;
+    for (int d = threadIdx.x; d < D; d += 256) {
+        const float x = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
+        if constexpr (sizeof(T) == 4) out[d] = x;
+        else out[d] = to_bf16(x);
     }
-    __builtin_memcpy((T *) a.out + tok * a.out_stride + (int64_t) h * D + lane * C, t, sizeof t);
 }
 
 }  // namespace
@@ -571,12 +644,15 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
     a.n_head = x->n_head, a.group = x->n_head / c->n_head_kv, a.window = x->window;
     a.splits = p.splits, a.chunk = p.chunk, a.scale = x->scale;
     const dim3 grid((unsigned) (b->n_seq * c->n_head_kv), (unsigned) p.row_tiles, (unsigned) p.splits);
+    const bool small = c->page_size < kTile;
     auto few = [&](auto dim, auto ct, auto type) {
-        hipLaunchKernelGGL((k_attn_few<decltype(dim)::value, decltype(ct)::value, decltype(type)>), grid, dim3(256), 0, st, a);
+        constexpr int D = decltype(dim)::value, CT = decltype(ct)::value;
+        if (small) hipLaunchKernelGGL((k_attn_few<D, CT, true, decltype(type)>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_attn_few<D, CT, false, decltype(type)>), grid, dim3(256), 0, st, a);
     };
     auto join = [&](auto dim, auto type) {
         const int64_t rows = (int64_t) b->max_q * x->n_head;
-        hipLaunchKernelGGL((k_attn_join<decltype(dim)::value, decltype(type)>), dim3((unsigned) ((rows + 3) / 4), (unsigned) b->n_seq),
+        hipLaunchKernelGGL((k_attn_join<decltype(dim)::value, decltype(type)>), dim3((unsigned) rows, (unsigned) b->n_seq),
                            dim3(256), 0, st, a, p.rows);
     };
     auto by_type = [&](auto dim, auto type) {

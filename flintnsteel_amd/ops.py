@@ -545,52 +545,60 @@ def add(x: torch.Tensor, y: torch.Tensor, out: torch.Tensor | None = None) -> to
     return out
 
 
-def _rows_f32(what: str, *ts: torch.Tensor) -> None:
-    """Every tensor f32, contiguous, on the current device and of the first one's shape."""
-    for t in ts:
-        if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != ts[0].shape:
-            raise ValueError(f"{what}: expected contiguous f32 tensors of one shape")
-    _on_device(what, *ts)
+# The stream of a device as an integer, without the object that torch.cuda.current_stream() makes: a decode step's calls
+# are a few microseconds each, and so is what surrounds them here.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _on_device(what: str, *ts: torch.Tensor | None) -> None:
-    """The launch goes to the current device's current stream: every tensor has to be there."""
+def _here(what: str, *ts: torch.Tensor | None) -> int:
+    """The launch goes to the current device's current stream: every tensor has to be there. -> that stream."""
+    dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"{what}: expected tensors on the current device")
+    return _raw_stream(dev)
 
 
 def add_rms_norm_q8_1(x: torch.Tensor, y: torch.Tensor, w: torch.Tensor, eps: float, sum_out: torch.Tensor | None = None,
                       out: torch.Tensor | None = None, xq: torch.Tensor | None = None):
     """-> (sum, out, xq): sum = x + y, out = RMSNorm(sum) * w, xq its Q8_1 rows. sum_out may be x or y (in place)."""
-    n = x.shape[-1]
+    shape = x.shape
+    n = shape[-1]
     rows = x.numel() // max(n, 1)
-    sum_out = torch.empty_like(x, memory_format=torch.contiguous_format) if sum_out is None else sum_out
-    out = torch.empty_like(sum_out) if out is None else out
-    _rows_f32("add_rms_norm_q8_1", x, y, sum_out, out)
-    _rows_f32("add_rms_norm_q8_1", w)
-    if w.numel() != n:
-        raise ValueError(f"add_rms_norm_q8_1: {w.numel()} weights for rows of {n}")
+    row_bytes_ = (n + 511) // 512 * 576  # q8_1_row_bytes
+    if sum_out is None:
+        sum_out = torch.empty_like(x)
+    if out is None:
+        out = torch.empty_like(x)
     if xq is None:
-        xq = torch.empty(rows, q8_1_row_bytes(n), dtype=torch.uint8, device=x.device)
-    if xq.dtype != torch.uint8 or not xq.is_contiguous() or xq.numel() != rows * q8_1_row_bytes(n):
+        xq = torch.empty((rows, row_bytes_), dtype=torch.uint8, device=x.device)
+    for t in (x, y, sum_out, out):
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != shape:
+            raise ValueError("add_rms_norm_q8_1: expected contiguous f32 tensors of one shape")
+    if w.dtype != torch.float32 or not w.is_contiguous() or w.numel() != n:
+        raise ValueError(f"add_rms_norm_q8_1: expected {n} contiguous f32 weights, got {w.numel()} {w.dtype}")
+    if xq.dtype != torch.uint8 or not xq.is_contiguous() or xq.numel() != rows * row_bytes_:
         raise ValueError("add_rms_norm_q8_1: xq must be uint8 [rows][q8_1_row_bytes(n)]")
-    _on_device("add_rms_norm_q8_1", xq)
-    call("fns_hip_add_rms_norm_q8_1", _p(x), _p(y), _p(w), _p(sum_out), _p(out), _p(xq), n, ctypes.c_float(eps), rows, _s())
+    st = _here("add_rms_norm_q8_1", x, y, w, sum_out, out, xq)
+    call("fns_hip_add_rms_norm_q8_1", x.data_ptr(), y.data_ptr(), w.data_ptr(), sum_out.data_ptr(), out.data_ptr(),
+         xq.data_ptr(), n, eps, rows, st)
     return sum_out, out, xq
 
 
 def dequantize_q8_1(xq: torch.Tensor, ncols: int, dtype: torch.dtype = torch.float32):
     """-> (values [nrows][ncols], block sums [nrows][ncols / 32]) that Q8_1 rows stand for, in f32 or f16."""
-    if dtype not in (torch.float32, torch.float16):
+    if dtype is not torch.float32 and dtype is not torch.float16:
         raise ValueError(f"dequantize_q8_1: {dtype} not supported")
-    if xq.dtype != torch.uint8 or not xq.is_contiguous() or ncols <= 0 or xq.numel() % q8_1_row_bytes(ncols):
+    row_bytes_ = (ncols + 511) // 512 * 576  # q8_1_row_bytes
+    if xq.dtype != torch.uint8 or not xq.is_contiguous() or ncols <= 0 or xq.numel() % row_bytes_:
         raise ValueError("dequantize_q8_1: xq must be uint8 [nrows][q8_1_row_bytes(ncols)]")
-    _on_device("dequantize_q8_1", xq)
-    nrows = xq.numel() // q8_1_row_bytes(ncols)
-    x = torch.empty(nrows, ncols, dtype=dtype, device=xq.device)
-    sums = torch.empty(nrows, ncols // 32, dtype=dtype, device=xq.device)
-    call("fns_hip_dequantize_q8_1", _p(xq), F32 if dtype == torch.float32 else F16, _p(x), _p(sums), ncols, nrows, _s())
+    st = _here("dequantize_q8_1", xq)
+    nrows = xq.numel() // row_bytes_
+    x = torch.empty((nrows, ncols), dtype=dtype, device=xq.device)
+    sums = torch.empty((nrows, ncols // 32), dtype=dtype, device=xq.device)
+    call("fns_hip_dequantize_q8_1", xq.data_ptr(), F32 if dtype is torch.float32 else F16, x.data_ptr(), sums.data_ptr(),
+         ncols, nrows, st)
     return x, sums
 
 
@@ -634,9 +642,10 @@ class KvCache:
             pages = torch.zeros(n_pages, self.page_bytes, dtype=torch.uint8, device="cuda")
         if pages.dtype != torch.uint8 or not pages.is_contiguous() or pages.numel() != n_pages * self.page_bytes:
             raise ValueError(f"KvCache: pages must be contiguous uint8 of {n_pages} * {self.page_bytes} bytes")
-        _on_device("KvCache", pages)
+        _here("KvCache", pages)
         self.pages, self.n_head_kv, self.head_dim, self.page_size = pages, n_head_kv, head_dim, page_size
         self.desc = KvCacheDesc(n_head_kv, head_dim, page_size, n_pages, pages.data_ptr())
+        self.ref = ctypes.byref(self.desc)
 
 
 class KvBatch:
@@ -653,16 +662,17 @@ class KvBatch:
                 raise ValueError("KvBatch: expected contiguous int32 tensors")
         if q_start.numel() != n_seq + 1 or page_table.dim() != 2 or page_table.shape[0] != n_seq:
             raise ValueError("KvBatch: expected q_start [n_seq + 1], kv_len [n_seq] and page_table [n_seq][pages]")
-        _on_device("KvBatch", q_start, kv_len, page_table)
+        _here("KvBatch", q_start, kv_len, page_table)
         self.q_start, self.kv_len, self.page_table, self.n_tok = q_start, kv_len, page_table, n_tok
-        self._open = max_kv is None
+        self._open = max_kv is None  # the table's room, which depends on the cache's page size
         self.desc = KvBatchDesc(n_seq, max_q, n_tok, max_kv or 0, page_table.shape[1], q_start.data_ptr(), kv_len.data_ptr(),
                                 page_table.data_ptr())
+        self.ref = ctypes.byref(self.desc)
 
-    def _for(self, cache: KvCache) -> KvBatchDesc:
+    def _for(self, cache: KvCache):
         if self._open:
             self.desc.max_kv = min(self.desc.table_stride * cache.page_size, 2 ** 31 - 1)
-        return self.desc
+        return self.ref
 
     @classmethod
     def from_lists(cls, q_lens, kv_lens, pages, n_tok: int | None = None) -> "KvBatch":
@@ -687,77 +697,71 @@ def rope_freqs(rope_dim: int, base: float = 10000.0, factors=None) -> torch.Tens
 
 def _heads(what: str, t: torch.Tensor, n_tok: int, dim: int, dtype: torch.dtype) -> int:
     """Token stride of t [n_tok][heads][dim], heads contiguous within a token (a slice of a fused projection is)."""
-    if t.dim() != 3 or t.shape[0] != n_tok or t.shape[2] != dim:
-        raise ValueError(f"{what}: expected [{n_tok}][heads][{dim}], got {list(t.shape)}")
-    if t.dtype != dtype or dtype not in (torch.float32, torch.bfloat16):
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != n_tok or shape[2] != dim:
+        raise ValueError(f"{what}: expected [{n_tok}][heads][{dim}], got {list(shape)}")
+    if t.dtype is not dtype or (dtype is not torch.float32 and dtype is not torch.bfloat16):
         raise ValueError(f"{what}: expected one type of f32 and bf16, got {t.dtype}")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim)):
+    width = shape[1] * dim
+    if t.is_contiguous():
+        return width
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (shape[1] > 1 and s1 != dim):
         raise ValueError(f"{what}: the heads of a token must be contiguous")
-    _on_device(what, t)
-    width = t.shape[1] * dim
-    if n_tok > 1 and t.stride(0) < width:
+    if n_tok <= 1:
+        return width
+    if s0 < width:
         raise ValueError(f"{what}: tokens overlap")
-    return t.stride(0) if n_tok > 1 else width
+    return s0
 
 
 def kv_append(cache: KvCache, batch: KvBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
               rope: int = ROPE_NONE, inv_freq: torch.Tensor | None = None, q_out: torch.Tensor | None = None):
     """k, v [n_tok][n_head_kv][head_dim] into the cache, k (and q) rotated by position * inv_freq over the first
     2 * len(inv_freq) channels. -> the rotated q (in q_out, which may be q; None without q)."""
-    D, Hk = cache.head_dim, cache.n_head_kv
-    ks, vs = _heads("kv_append", k, batch.n_tok, D, k.dtype), _heads("kv_append", v, batch.n_tok, D, k.dtype)
+    D, Hk, n_tok, dt = cache.head_dim, cache.n_head_kv, batch.n_tok, k.dtype
+    x = KvAppendDesc()
+    x.k_stride, x.v_stride = _heads("kv_append", k, n_tok, D, dt), _heads("kv_append", v, n_tok, D, dt)
     if k.shape[1] != Hk or v.shape[1] != Hk:
         raise ValueError(f"kv_append: expected {Hk} kv heads, got {k.shape[1]} and {v.shape[1]}")
-    qs = qos = 0
     if q is not None:
-        qs = _heads("kv_append", q, batch.n_tok, D, k.dtype)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-        qos = _heads("kv_append", q_out, batch.n_tok, D, k.dtype)
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+        x.q_stride = _heads("kv_append", q, n_tok, D, dt)
+        x.q_out_stride = _heads("kv_append", q_out, n_tok, D, dt)
         if q_out.shape != q.shape:
             raise ValueError("kv_append: q_out is not of q's shape")
+        x.n_head, x.q, x.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("kv_append: q_out without q")
-    dim = 0
     if rope != ROPE_NONE:
         if inv_freq is None or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or inv_freq.dim() != 1:
             raise ValueError("kv_append: a rotation needs inv_freq, a contiguous f32 vector")
-        _on_device("kv_append", inv_freq)
-        dim = 2 * inv_freq.numel()
-    x = KvAppendDesc(_dtype_code(k), rope, dim, 0 if q is None else q.shape[1], inv_freq.data_ptr() if dim else None,
-                     k.data_ptr(), v.data_ptr(), None if q is None else q.data_ptr(),
-                     None if q is None else q_out.data_ptr(), ks, vs, qs, qos)
-    call("fns_hip_kv_append", ctypes.byref(cache.desc), ctypes.byref(batch._for(cache)), ctypes.byref(x), _s())
+        x.rope, x.rope_dim, x.inv_freq = rope, 2 * inv_freq.numel(), inv_freq.data_ptr()
+    else:
+        inv_freq = None
+    x.dtype, x.k, x.v = F32 if dt is torch.float32 else BF16, k.data_ptr(), v.data_ptr()
+    st = _here("kv_append", cache.pages, batch.kv_len, k, v, q, q_out, inv_freq)
+    call("fns_hip_kv_append", cache.ref, batch._for(cache), ctypes.byref(x), st)
     return q_out
 
 
 def kv_read(cache: KvCache, batch: KvBatch):
     """-> (k, v) f32 [n_tok][n_head_kv][head_dim]: what the cache holds of the batch's tokens."""
-    k = torch.empty(batch.n_tok, cache.n_head_kv, cache.head_dim, dtype=torch.float32, device=cache.pages.device)
-    v = torch.empty_like(k)
-    call("fns_hip_kv_read", ctypes.byref(cache.desc), ctypes.byref(batch._for(cache)), _p(k), _p(v), _s())
+    st = _here("kv_read", cache.pages, batch.kv_len)
+    shape = (batch.n_tok, cache.n_head_kv, cache.head_dim)
+    k = torch.empty(shape, dtype=torch.float32, device=cache.pages.device)
+    v = torch.empty(shape, dtype=torch.float32, device=cache.pages.device)
+    call("fns_hip_kv_read", cache.ref, batch._for(cache), k.data_ptr(), v.data_ptr(), st)
     return k, v
-
-
-def _attn_desc(cache: KvCache, batch: KvBatch, q: torch.Tensor, out: torch.Tensor | None, scale: float, window: int,
-               sinks: torch.Tensor | None) -> AttnDesc:
-    qs = _heads("attn", q, batch.n_tok, cache.head_dim, q.dtype)
-    os_ = q.shape[1] * cache.head_dim
-    if out is not None:
-        os_ = _heads("attn", out, batch.n_tok, cache.head_dim, q.dtype)
-        if out.shape != q.shape:
-            raise ValueError("attn: out is not of q's shape")
-    if sinks is not None and (sinks.dtype != torch.float32 or not sinks.is_contiguous() or sinks.numel() != q.shape[1]):
-        raise ValueError("attn: sinks must be a contiguous f32 vector, one a query head")
-    _on_device("attn", sinks)
-    return AttnDesc(_dtype_code(q), q.shape[1], window, scale, None if sinks is None else sinks.data_ptr(), qs, os_)
 
 
 def attn_workspace(cache: KvCache, batch: KvBatch, q: torch.Tensor) -> torch.Tensor:
     """A workspace of attn for this batch's numbers and q's heads; it may serve every layer of a step in turn."""
+    width = _heads("attn", q, batch.n_tok, cache.head_dim, q.dtype)
+    desc = AttnDesc(_dtype_code(q), q.shape[1], 0, 1.0, None, width, q.shape[1] * cache.head_dim)
     size = ctypes.c_size_t()
-    desc = _attn_desc(cache, batch, q, None, 1.0, 0, None)
-    call("fns_hip_attn_workspace", ctypes.byref(cache.desc), ctypes.byref(batch._for(cache)), ctypes.byref(desc),
-         ctypes.byref(size))
+    call("fns_hip_attn_workspace", cache.ref, batch._for(cache), ctypes.byref(desc), ctypes.byref(size))
     return torch.empty(size.value, dtype=torch.uint8, device=q.device)
 
 
@@ -765,14 +769,24 @@ def attn(cache: KvCache, batch: KvBatch, q: torch.Tensor, scale: float | None = 
          sinks: torch.Tensor | None = None, out: torch.Tensor | None = None, ws: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [n_tok][n_head][head_dim] over the cache -> out (rows of no sequence are left as they were). scale
     None: head_dim^-0.5; window > 0: the last `window` positions only; sinks f32 [n_head] join the denominator."""
+    D, dt = cache.head_dim, q.dtype
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    desc = _attn_desc(cache, batch, q, out, cache.head_dim ** -0.5 if scale is None else scale, window, sinks)
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
+    desc = AttnDesc()
+    desc.q_stride, desc.out_stride = _heads("attn", q, batch.n_tok, D, dt), _heads("attn", out, batch.n_tok, D, dt)
+    if out.shape != q.shape:
+        raise ValueError("attn: out is not of q's shape")
+    if sinks is not None:
+        if sinks.dtype != torch.float32 or not sinks.is_contiguous() or sinks.numel() != q.shape[1]:
+            raise ValueError("attn: sinks must be a contiguous f32 vector, one a query head")
+        desc.sinks = sinks.data_ptr()
+    desc.dtype, desc.n_head, desc.window = F32 if dt is torch.float32 else BF16, q.shape[1], window
+    desc.scale = D ** -0.5 if scale is None else scale
     if ws is None:
         ws = attn_workspace(cache, batch, q)
-    _on_device("attn", ws)
-    call("fns_hip_attn", ctypes.byref(cache.desc), ctypes.byref(batch._for(cache)), ctypes.byref(desc), _p(q), _p(out),
-         _p(ws), ws.numel() * ws.element_size(), _s())
+    st = _here("attn", cache.pages, batch.kv_len, q, out, sinks, ws)
+    call("fns_hip_attn", cache.ref, batch._for(cache), ctypes.byref(desc), q.data_ptr(), out.data_ptr(), ws.data_ptr(),
+         ws.numel() * ws.element_size(), st)
     return out
 
 
