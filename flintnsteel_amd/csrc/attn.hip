@@ -21,7 +21,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;     // keys of a step
-constexpr int kHead = 12;     // K and V expand to f16 with their tile's largest block scale at 2^12 (codes to 6: 24576)
+constexpr int kFewRows = 32, kManyRows = 128;  // rows of the few-row form at most, of a workgroup of the other
+constexpr int kFewWaves = 4;  // waves of a workgroup of few rows
+constexpr int kHead = 12;     // V expands to f16 with the largest block scale so far at 2^12 (codes to 6: 24576)
 constexpr int kBias = 127 + kHead;
 // p is carried times 2^8: its low half stays clear of f16's subnormals. Sums are rescaled only where a row's maximum has
 // grown by more than 2^7 since the last time, so p stays below 2^15.
@@ -31,6 +33,7 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef int i8v __attribute__((ext_vector_type(8)));
 
 struct AttnArgs {
     KvView c;
@@ -78,88 +81,73 @@ __device__ __forceinline__ RowTiles row_tiles(const AttnArgs &a, const SeqRange 
     t.t1 = t.hi > t.lo ? t.hi / kTile + (t.hi % kTile > 0) : t.t0;
     return t;
 }
-// Tiles of one split: a chunk that the host chose from max_kv, more where the sequence is longer than that.
+// Tiles of one split: as many splits as chunks (the host's number, from max_kv) are needed, of equal lengths; longer ones
+// where the sequence is longer than max_kv.
 __device__ __forceinline__ int split_chunk(const AttnArgs &a, const RowTiles &t) {
-    return max(a.chunk, (t.t1 - t.t0 + a.splits - 1) / a.splits);
+    const int tiles = t.t1 - t.t0;
+    const int n = min(max((tiles + a.chunk - 1) / a.chunk, 1), a.splits);
+    return max(((tiles + n - 1) / n + kFewWaves - 1) / kFewWaves * kFewWaves, 1);
 }
 
-// What a wave knows of a tile, a key a lane: which keys are there, which of them hold NaNs, the largest scale bytes.
-struct TileInfo {
-    uint64_t there, nan;
-    int ek, ev;
-};
+// What a wave knows of a tile, a key a lane: which keys are there, which of them hold NaNs in V; and the wave's V scale.
 typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pk_max(uint32_t x, uint32_t y) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, x), __builtin_bit_cast(us2, y)));
 }
-// The scale bytes of one position's K and V, NB of each.
-template <int NB> struct ScaleWords {
-    static constexpr int W = (NB + 3) / 4;
-    uint32_t k[W], v[W];
+struct TileInfo {
+    uint64_t there, nan;
+    int ev;
 };
-// ... and the block scales as the f32 operands of the expansion, in the wave's LDS: K [64 in the order of the products'
-// rows][NB], V [NB][64 keys]. A block's operand is 2^(e - E + 12) for the tile's (K) or the largest so far (V) scale E; what
-// lies 2^36 below that is dropped, which is less than the last bit of any sum it could join.
-__device__ __forceinline__ int row_of_key(int key) { return (key >> 2 & 3) * 16 + (key >> 4) * 4 + (key & 3); }
-template <int NB>
-__device__ __forceinline__ TileInfo tile_scales(ScaleWords<NB> w, bool there, int ev_before, float *ksc, float *vsc) {
-    constexpr int W = ScaleWords<NB>::W;
+// The block scales of V as the f32 operands of the expansion, in the wave's LDS, [NB][64 keys]: 2^(e - E + 12), E at least
+// every scale so far; what lies 2^36 below that is dropped, which is less than the last bit of any sum it could join. w: the
+// scale bytes of the lane's key.
+template <int NB> struct ScaleBytes {
+    std::conditional_t<NB == 2, uint16_t, uint32_t> w[(NB + 3) / 4];
+};
+// STEP, first: the blocks first, first + STEP ... only, in rows of their own.
+template <int NB, int STEP = 1>
+__device__ __forceinline__ TileInfo v_scales(const ScaleBytes<NB> &bytes, bool there, int ev, float *vsc, int first = 0) {
+    constexpr int W = (NB + 3) / 4;
     constexpr uint32_t kEven = 0x00ff00ffu;
     const int lane = threadIdx.x % 64;
-    uint32_t e[2][W][2], top[2];  // bytes 0 and 2, 1 and 3 of every word, in halves
-    const auto split = [&](int s) {
-        top[s] = 0;
+    uint32_t w[W], top = 0;
+    const auto largest = [&] {
+        top = 0;
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            const uint32_t x = s ? w.v[i] : w.k[i];
-            e[s][i][0] = x & kEven, e[s][i][1] = x >> 8 & kEven;
-            top[s] = pk_max(top[s], pk_max(e[s][i][0], e[s][i][1]));
-        }
-        top[s] = max(top[s] & 0xffffu, top[s] >> 16);
+        for (int i = 0; i < W; ++i) top = pk_max(top, pk_max(w[i] & kEven, w[i] >> 8 & kEven));
+        top = max(top & 0xffffu, top >> 16);
     };
 #pragma unroll
-    for (int i = 0; i < W; ++i) w.k[i] = there ? w.k[i] : 0, w.v[i] = there ? w.v[i] : 0;
-    split(0), split(1);
+    for (int i = 0; i < W; ++i) w[i] = there ? bytes.w[i] : 0;
+    largest();
     TileInfo t;
     t.there = __ballot(there);
-    t.nan = __ballot(max(top[0], top[1]) == 255u);
-    if (t.nan) {  // rare: their blocks count as zeros, the rows that see them are made NaN
+    t.nan = 0;
+    t.ev = ev;
+    if (__any((int) top > ev)) {
+        t.nan = __ballot(top == 255u);
+        if (t.nan) {  // rare: their blocks count as zeros, the rows that see them are made NaN
 #pragma unroll
-        for (int i = 0; i < W; ++i)
+            for (int i = 0; i < W; ++i)
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const uint32_t m = 255u << (8 * b);
-                w.k[i] = (w.k[i] & m) == m ? w.k[i] & ~m : w.k[i];
-                w.v[i] = (w.v[i] & m) == m ? w.v[i] & ~m : w.v[i];
-            }
-        split(0), split(1);
+                for (int b = 0; b < 4; ++b) w[i] = (w[i] >> (8 * b) & 255u) == 255u ? w[i] & ~(255u << (8 * b)) : w[i];
+            largest();
+        }
+        top = max(top, (uint32_t) xor_lane_i<1>(top));
+        top = max(top, (uint32_t) xor_lane_i<2>(top));
+        top = max(top, (uint32_t) xor_lane_i<4>(top));
+        top = max(top, (uint32_t) xor_lane_i<8>(top));
+        top = max(top, (uint32_t) xor_lane_i<16>(top));
+        top = max(top, (uint32_t) xor_lane_i<32>(top));
+        t.ev = max(ev, __builtin_amdgcn_readfirstlane(top));
     }
-    uint32_t both = top[0] << 16 | top[1];
-    both = pk_max(both, xor_lane_i<1>(both));
-    both = pk_max(both, xor_lane_i<2>(both));
-    both = pk_max(both, xor_lane_i<4>(both));
-    both = pk_max(both, xor_lane_i<8>(both));
-    both = pk_max(both, xor_lane_i<16>(both));
-    both = pk_max(both, xor_lane_i<32>(both));
-    both = __builtin_amdgcn_readfirstlane(both);
-    t.ek = both >> 16;
-    t.ev = max((int) (both & 0xffffu), ev_before);
-    const auto field = [](uint32_t e, int top) { return __builtin_bit_cast(float, max((int) e + kBias - top, 0) << 23); };
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int i = b / 4, odd = b % 2, sh = b % 4 / 2 * 16;
-        ksc[row_of_key(lane) * NB + b] = field(e[0][i][odd] >> sh & 0xffu, t.ek);
-        vsc[b * 64 + lane] = field(e[1][i][odd] >> sh & 0xffu, t.ev);
-    }
+    for (int b = 0; b < NB; ++b)
+        if (STEP == 1 || b % STEP == first)
+            vsc[b / STEP * 64 + lane] = __builtin_bit_cast(float, max((int) (w[b / 4] >> (b % 4 * 8) & 0xffu) + (kBias - t.ev), 0) << 23);
     return t;
 }
 
-// Eight consecutive channels of K from their four bytes.
-__device__ __forceinline__ h8 expand_k(uint32_t w, float sc) {
-    const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 1);
-    const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, 3);
-    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 // Eight consecutive positions of V from their eight bytes: two channels 16 apart (low and high halves).
 __device__ __forceinline__ void expand_v(uint32_t w0, uint32_t w1, const float *sc, h8 &lo, h8 &hi) {
     h2 p[8];
@@ -177,58 +165,104 @@ __device__ __forceinline__ void expand_v(uint32_t w0, uint32_t w1, const float *
     lo = __builtin_bit_cast(h8, l), hi = __builtin_bit_cast(h8, h);
 }
 
-// The queries of one column tile (16 rows) as operands of the products: lane (row r = lane % 16, g = lane / 16) holds the
-// channels g NB 8 + 8 u .. + 7 of step u, in one (bf16: exact) or two (f32: 22 bits) f16 parts, the row scaled by a power
-// of two to a largest magnitude in [2^10, 2^11). Returns what turns a product (of K at its tile's 2^12) into log2 units.
-template <int NB, int SPLIT, class T>
-__device__ __forceinline__ float load_queries(h8 (&part)[SPLIT][NB], const T *row, bool there, float scale) {
+// The first product takes K as it is held, e2m1 codes and block scales, from the cache to the matrix pipe. Its other operand,
+// the queries, is a sum of digits: a row is scaled by a power of two to a largest magnitude in [2, 4) and written as
+// d_0 + d_1 + d_2 ..., each the nearest 6-bit e2m3 number, in units of 32^-j, to what the ones before it left (e2m3 has steps
+// of at most 1/4 below 4: an eighth is left, 4 units of the next): 5 digits leave 2^-24 of the row's largest element (f32),
+// 3 leave 2^-14 (bf16). A product is exact and its sum f32. Operand lane (row r = lane % 16, g = lane / 16) holds the 32
+// channels of block g of step u; a head of 64 channels has two blocks, and its lanes g = 2, 3 take the next digit.
+template <int D, class T> struct QueryShape {
+    static constexpr int kDigits = sizeof(T) == 4 ? 5 : 3;
+    static constexpr int kPerStep = D == 64 ? 2 : 1;  // digits of one product
+    static constexpr int kSteps = D == 256 ? 2 : 1;   // products of one digit
+    static constexpr int N = (kDigits + kPerStep - 1) / kPerStep;
+};
+typedef uint32_t u6 __attribute__((ext_vector_type(6)));
+template <int D, class T> using Digits = u6[QueryShape<D, T>::N][QueryShape<D, T>::kSteps];
+// Returns what turns a product into log2 units.
+template <int D, class T>
+__device__ __forceinline__ float query_digits(Digits<D, T> &w, const T *row, bool there, float scale) {
+    typedef float v16 __attribute__((ext_vector_type(16)));
+    typedef float v32 __attribute__((ext_vector_type(32)));
+    using Q = QueryShape<D, T>;
     const int g = threadIdx.x % 64 / 16;
-    float v[NB][8], amax = 0.0f;
-    bool bad = false;
+    v16 even[Q::kSteps], odd[Q::kSteps];
+    float amax = 0.0f;
+    int bad = 0;
 #pragma unroll
-    for (int u = 0; u < NB; ++u) {
-        T t[8] = {};
-        if (there) __builtin_memcpy(t, row + g * NB * 8 + u * 8, sizeof t);
+    for (int u = 0; u < Q::kSteps; ++u) {
+        T t[32] = {};
+        if (there) __builtin_memcpy(t, row + ((D == 64 ? g & 1 : g) + 4 * u) * 32, sizeof t);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[u][i] = to_f32(t[i]);
-            bad |= !(fabsf(v[u][i]) <= 3.4028234663852886e38f);
-            amax = fmaxf(amax, fabsf(v[u][i]));
+        for (int i = 0; i < 16; ++i) even[u][i] = to_f32(t[2 * i]), odd[u][i] = to_f32(t[2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            amax = fmaxf(fmaxf(amax, fabsf(even[u][i])), fabsf(odd[u][i]));
+            bad |= !(fmaxf(fabsf(even[u][i]), fabsf(odd[u][i])) < INFINITY) || even[u][i] != even[u][i] || odd[u][i] != odd[u][i];
         }
     }
+    amax = bad ? INFINITY : amax;
     amax = fmaxf(amax, xor_lane<16>(amax));
     amax = fmaxf(amax, xor_lane<32>(amax));
-    bad |= xor_lane_i<16>(bad);
-    bad |= xor_lane_i<32>(bad);
-    int k = 0;
-    if (amax > 0.0f && !bad) k = ilogbf(amax) + 1;
-    k = max(k, -100);
-    const float f = bad ? __builtin_nanf("") : ldexpf(scale < 0.0f ? -1.0f : 1.0f, 11 - k);
+    // (below 2^-100 the row is smaller than any difference that a score can show)
+    const int k = amax < 7.8886090522101181e-31f ? -100 : (int) (__builtin_bit_cast(uint32_t, amax) >> 23) - 126;  // amax < 2^k
+    const float f = amax == INFINITY ? 0.0f : ldexpf(scale < 0.0f ? -1.0f : 1.0f, 2 - k);
 #pragma unroll
-    for (int u = 0; u < NB; ++u)
+    for (int u = 0; u < Q::kSteps; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = v[u][i] * f;
-            const _Float16 hi = (_Float16) x;
-            part[0][u][i] = hi;
-            if constexpr (SPLIT == 2) part[1][u][i] = (_Float16) (x - (float) hi);
+        for (int i = 0; i < 16; ++i) even[u][i] = bad ? 0.0f : even[u][i] * f, odd[u][i] = bad ? 0.0f : odd[u][i] * f;
+#pragma unroll
+    for (int d = 0; d < Q::N * Q::kPerStep; ++d)
+#pragma unroll
+        for (int u = 0; u < Q::kSteps; ++u) {
+            const float unit = __builtin_bit_cast(float, (uint32_t) (127 - 5 * d) << 23);
+            u6 code;
+            v32 back;
+            // (as assembly for its "&": the conversion writes its result while it still reads its operands, and the builtin
+            // lets them share registers)
+            asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3" : "=&v"(code) : "v"(even[u]), "v"(odd[u]), "v"(unit));
+            asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2" : "=&v"(back) : "v"(code), "v"(unit));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) even[u][i] -= back[2 * i], odd[u][i] -= back[2 * i + 1];
+            if constexpr (D == 64) {
+                if (d % 2 == 0) w[d / 2][0] = code;
+                else
+#pragma unroll
+                    for (int i = 0; i < 6; ++i) w[d / 2][0][i] = g >= 2 ? code[i] : w[d / 2][0][i];
+            } else {
+                w[d][u] = code;
+            }
         }
-    return fabsf(scale) * kLog2e * ldexpf(1.0f, k - 11);
+    return amax == INFINITY ? __builtin_nanf("") : fabsf(scale) * kLog2e * ldexpf(1.0f, k - 2);
 }
 
-// A lane's state of one column tile: row r = lane % 16; a lane sums the keys 16 g .. 16 g + 15 of every tile, and holds
-// channels 16 dt + 4 g + i of its row in o[dt][i] (in units of 2^(ev - 139)). m: the maximum that p and the sums refer to.
+// S^T of 16 keys and 16 query rows: the products of digit (pair) n with every 128 channels.
+template <int D> constexpr int kKPieces = D == 256 ? 2 : 1;  // 16-byte pieces of a key that a lane holds
+template <int D, class T>
+__device__ __forceinline__ f4 scores(const u4 (&k)[kKPieces<D>], const int (&ksc)[kKPieces<D>], const u6 (&q)[QueryShape<D, T>::kSteps], int n, f4 acc) {
+    const int qsc = 127 - 5 * (n * QueryShape<D, T>::kPerStep) - (D == 64 && threadIdx.x % 64 >= 32 ? 5 : 0);
+#pragma unroll
+    for (int u = 0; u < QueryShape<D, T>::kSteps; ++u) {
+        const i8v a = {(int) k[u][0], (int) k[u][1], (int) k[u][2], (int) k[u][3], 0, 0, 0, 0};
+        const i8v b = {(int) q[u][0], (int) q[u][1], (int) q[u][2], (int) q[u][3], (int) q[u][4], (int) q[u][5], 0, 0};
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 2, 0, ksc[u], 0, qsc);
+    }
+    return acc;
+}
+
+// A lane's state of one column tile: row r = lane % 16; a lane holds channels 16 dt + 4 g + i of its row in o[dt][i] (in
+// units of 2^(ev - 139)). m: the maximum that p and the sums refer to; l: the sum of p, four times the same (a product with
+// ones: the matrix pipe has time for it, the vector pipe has none, and p counts as it was rounded).
 template <int NB> struct RowState {
-    f4 o[2 * NB];
-    float m, l;
+    f4 o[2 * NB], l;
+    float m;
 };
 
-// One tile's softmax of a column tile: s (product units) of the lane's 16 keys -> p as operand parts, m and l updated;
-// returns what earlier sums have to be multiplied by. see: the lane's keys that its row sees.
-template <int SPLIT>
-__device__ __forceinline__ float softmax_step(f4 (&s)[4], float mul, uint32_t see, uint32_t nan, float &m, float &l, h8 (&p)[SPLIT][2]) {
-    const bool all = __all(see == 0xffffu);
-    if (!all) {
+// One tile's softmax of a column tile: s (product units) of the lane's 16 keys -> p as operand parts, m updated; returns
+// what earlier sums have to be multiplied by. MASKED: only the keys of `see` count, those of `nan` make the row NaN.
+template <int SPLIT, bool MASKED>
+__device__ __forceinline__ float softmax_step(f4 (&s)[4], float mul, uint32_t see, uint32_t nan, float &m, h8 (&p)[SPLIT][2]) {
+    if constexpr (MASKED) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -247,24 +281,16 @@ __device__ __forceinline__ float softmax_step(f4 (&s)[4], float mul, uint32_t se
         m = to;
     }
     const float add = kPShift - (m == -INFINITY ? 0.0f : m);
-    float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], mul, add));
-    if (!all)  // (a scale of zero times -infinity)
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][i] = see >> (4 * t + i) & 1 ? s[t][i] : 0.0f;
-    if (nan)
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][i] = see >> (4 * t + i) & nan >> (4 * t + i) & 1 ? __builtin_nanf("") : s[t][i];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) sum += (s[t][0] + s[t][1]) + (s[t][2] + s[t][3]);
-    l = l * keep + sum;
+        for (int i = 0; i < 4; ++i) {
+            s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], mul, add));
+            if constexpr (MASKED) {  // (a scale of zero times -infinity)
+                s[t][i] = see >> (4 * t + i) & 1 ? s[t][i] : 0.0f;
+                s[t][i] = see >> (4 * t + i) & nan >> (4 * t + i) & 1 ? __builtin_nanf("") : s[t][i];
+            }
+        }
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
         u4 w[SPLIT];
@@ -274,7 +300,8 @@ __device__ __forceinline__ float softmax_step(f4 (&s)[4], float mul, uint32_t se
             if constexpr (SPLIT == 2) {  // toward zero: the second part has the rest
                 const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
                 w[0][i] = __builtin_bit_cast(uint32_t, hi);
-                w[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - (float) hi[0], y - (float) hi[1]));
+                w[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float) hi[0], -1.0f, x),
+                                                                                  __builtin_fmaf((float) hi[1], -1.0f, y)));
             } else {
                 w[0][i] = __builtin_bit_cast(uint32_t, h2{(_Float16) x, (_Float16) y});
             }
@@ -307,38 +334,55 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t tok, int h,
 // Where a tile's bytes are. With pages of 64 positions or more a tile lies in one page: every address is the tile's (in
 // scalar registers) plus an offset that a lane keeps; smaller pages (SMALL) are looked up for every 16 positions.
 template <int D, bool SMALL> struct TileReader {
-    static constexpr int NB = D / 32, KC = NB * 4;  // KC: code bytes of a lane's channels of one key
+    static constexpr int NB = D / 32;
     using L = KvParts<D>;
-    int P, lane, r, g;
+    int P, lane, r, g, last;  // last: the table's last entry
     int64_t head_off;
     const uint8_t *bk, *bv;  // of the lane's K rows (keys 16 (r / 4) ..), and of its own key and V columns (16 g ..)
     int row;                 // of the tile's first position in its page
     bool there;
-    __device__ __forceinline__ void page(const AttnArgs &a, int s, int tile, bool in) {
-        const int base = tile * kTile;
-        row = base & (P - 1);
+    int pk, pv;              // table entries of the tile that take() goes to (one of them without SMALL)
+    // Asks for a tile's table entries (a tile of the table); take() moves there a step later. Nothing here waits for a load
+    // or skips one: a wait would be for every load before it, the next tile's among them.
+    __device__ __forceinline__ void ask(const AttnArgs &a, const int32_t *table, int tile) {
+        const int at = (tile * kTile) >> a.c.shift;
         if constexpr (SMALL) {
-            const int pk = in ? page_of(a.c, a.b, s, base + 16 * (r / 4)) : -1, pv = in ? page_of(a.c, a.b, s, base + 16 * g) : -1;
-            bk = a.c.pages + max(pk, 0) * a.c.page_bytes + head_off;
-            bv = a.c.pages + max(pv, 0) * a.c.page_bytes + head_off;
-            there = pv >= 0;
+            pk = table[min(at + ((16 * (r / 4)) >> a.c.shift), last)];
+            pv = table[min(at + ((16 * g) >> a.c.shift), last)];
         } else {
-            const int p = in ? __builtin_amdgcn_readfirstlane(page_of(a.c, a.b, s, base)) : -1;
-            bk = bv = a.c.pages + max(p, 0) * a.c.page_bytes + head_off;
-            there = p >= 0;
+            pk = pv = table[at];
         }
     }
-    __device__ __forceinline__ void scales(ScaleWords<NB> &w) const {
-        const int at = (SMALL ? (row + lane) & (P - 1) : row + lane);
-        w = {};
-        __builtin_memcpy(w.k, __builtin_assume_aligned(bv + L::k_scale(P, at), NB), NB);
-        __builtin_memcpy(w.v, __builtin_assume_aligned(bv + L::v_scale(P, at), NB), NB);
+    __device__ __forceinline__ void take(const AttnArgs &a, int tile) {
+        row = (tile * kTile) & (P - 1);
+        const auto in = [&](int p) { return p >= 0 && p < a.c.n_pages; };
+        if constexpr (SMALL) {
+            bk = a.c.pages + (in(pk) ? pk : 0) * a.c.page_bytes + head_off;
+            bv = a.c.pages + (in(pv) ? pv : 0) * a.c.page_bytes + head_off;
+            there = in(pv);
+        } else {
+            const int p = __builtin_amdgcn_readfirstlane(pv);
+            there = in(p);
+            bk = bv = a.c.pages + (there ? p : 0) * a.c.page_bytes + head_off;
+        }
     }
-    __device__ __forceinline__ void k(uint32_t (&x)[4][NB]) const {
-        const int at = SMALL ? (row + 16 * (r / 4)) & (P - 1) : row + 16 * (r / 4);
-        const uint8_t *p = bk + (uint32_t) ((at + r % 4) * (D / 2) + g * KC);
+    __device__ __forceinline__ void scales(ScaleBytes<NB> &k, ScaleBytes<NB> &v) const {
+        const int at = SMALL ? (row + lane) & (P - 1) : row + lane;
+        __builtin_memcpy(&k, __builtin_assume_aligned(bv + L::k_scale(P, at), NB), NB);
+        __builtin_memcpy(&v, __builtin_assume_aligned(bv + L::v_scale(P, at), NB), NB);
+    }
+    __device__ __forceinline__ void k(u4 (&x)[4][kKPieces<D>]) const {
+        const int at = (SMALL ? (row + 16 * (r / 4)) & (P - 1) : row + 16 * (r / 4)) + r % 4;
+        const int block = D == 64 ? g & 1 : g;
+        const uint8_t *p = bk + (uint32_t) (at * (D / 2) + block * 16);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) __builtin_memcpy(x[t], __builtin_assume_aligned(p + 4 * t * (D / 2), KC < 16 ? KC : 16), KC);
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int u = 0; u < kKPieces<D>; ++u) x[t][u] = *(const u4 *) (p + 4 * t * (D / 2) + u * 64);
+    }
+    __device__ __forceinline__ u4 v_block(int j) const {
+        const int at = SMALL ? (row + 16 * g) & (P - 1) : row + 16 * g;
+        return *(const u4 *) (bv + (uint32_t) (P * (D / 2) + r * P + at) + (uint32_t) (16 * j * P));
     }
     __device__ __forceinline__ void v(u4 (&x)[NB]) const {
         const int at = SMALL ? (row + 16 * g) & (P - 1) : row + 16 * g;
@@ -355,12 +399,14 @@ template <int D, bool SMALL> struct TileReader {
 // dependent loads for short ones. One wave issues a vector instruction about every 5 cycles where the SIMD takes one every
 // 2: what pays is waves, so the queries lie in LDS and the next tile's K is asked for when this one's is used up.
 template <int D, int CT, bool SMALL, class T>
-__global__ __launch_bounds__(256, D == 256 || CT == 2 ? 2 : 4) void k_attn_few(AttnArgs a) {
-    constexpr int NB = D / 32, SPLIT = sizeof(T) == 4 ? 2 : 1, NW = 4;
-    constexpr int kScale = 2 * 64 * NB, kJoin = NW / 2 * CT * 2 * NB * 256;
+__global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k_attn_few(AttnArgs a) {
+    constexpr int NB = D / 32, SPLIT = sizeof(T) == 4 ? 2 : 1, NW = kFewWaves;
+    constexpr int kScale = 64 * NB + 16 * NB, kJoin = NW / 2 * CT * 2 * NB * 256;
     __shared__ __align__(16) float lds[NW * kScale > kJoin ? NW * kScale : kJoin];
-    __shared__ __align__(16) h8 qs[CT][SPLIT][NB][64];
-    __shared__ float join[NW][2][CT * 16], qmul[CT][16];
+    using Q = QueryShape<D, T>;
+    __shared__ __align__(16) uint2 qs[CT][Q::N][Q::kSteps][64][3];
+    __shared__ float qmul[CT][16];
+    __shared__ float join[NW][2][CT * 16];
     const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, row0 = blockIdx.y * 16 * CT, split = blockIdx.z;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     const SeqRange sr = seq_range(a.b, s);
@@ -375,31 +421,38 @@ __global__ __launch_bounds__(256, D == 256 || CT == 2 ? 2 : 4) void k_attn_few(A
 
     TileReader<D, SMALL> rd;
     rd.P = P, rd.lane = lane, rd.r = r, rd.g = g, rd.head_off = head * kv_head_bytes(D, P);
-    uint32_t kraw[4][NB];
-    u4 vraw[NB];
-    ScaleWords<NB> sw = {};
+    u4 kraw[4][kKPieces<D>], vraw[NB];
+    ScaleBytes<NB> swk, swv;  // the scale bytes of the lane's key
     int tile = t0 + wave;
-    rd.page(a, s, tile, tile < t1);
-    if (tile < t1) rd.scales(sw), rd.k(kraw), rd.v(vraw);
+    const int32_t *table = a.b.table + s * a.b.table_stride;
+    rd.last = (int) a.b.table_stride - 1;
+    if (tile < t1) {
+        rd.ask(a, table, tile);
+        rd.take(a, tile);
+        rd.ask(a, table, min(tile + NW, t1 - 1));
+        rd.scales(swk, swv), rd.k(kraw), rd.v(vraw);
+    }
 
+    if (wave < CT) {  // a wave a column tile
+        const int row = row0 + 16 * wave + r, i = row / a.group;
+        Digits<D, T> w;
+        const float mul = query_digits<D, T>(w, (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D,
+                                             row < rows, a.scale);
+#pragma unroll
+        for (int n = 0; n < Q::N; ++n)
+#pragma unroll
+            for (int u = 0; u < Q::kSteps; ++u)
+#pragma unroll
+                for (int i2 = 0; i2 < 3; ++i2) qs[wave][n][u][lane][i2] = make_uint2(w[n][u][2 * i2], w[n][u][2 * i2 + 1]);
+        if (g == 0) qmul[wave][r] = mul;
+    }
     RowState<NB> st[CT];
     int pos[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-        const int row = row0 + 16 * c + r, i = row / a.group;
-        const bool there = row < rows;
-        pos[c] = there ? sr.len - sr.n + i : -1;
-        if (wave == c) {
-            h8 part[SPLIT][NB];
-            const float mul = load_queries(part, (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D,
-                                           there, a.scale);
-#pragma unroll
-            for (int h = 0; h < SPLIT; ++h)
-#pragma unroll
-                for (int u = 0; u < NB; ++u) qs[c][h][u][lane] = part[h][u];
-            if (g == 0) qmul[c][r] = mul;
-        }
-        st[c].m = -INFINITY, st[c].l = 0.0f;
+        const int row = row0 + 16 * c + r;
+        pos[c] = row < rows ? sr.len - sr.n + row / a.group : -1;
+        st[c].m = -INFINITY, st[c].l = f4{0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < 2 * NB; ++d) st[c].o[d] = f4{0, 0, 0, 0};
     }
@@ -408,54 +461,75 @@ __global__ __launch_bounds__(256, D == 256 || CT == 2 ? 2 : 4) void k_attn_few(A
 #pragma unroll
     for (int c = 0; c < CT; ++c) mul[c] = qmul[c][r];
 
-    float *ksc = lds + wave * kScale, *vsc = ksc + 64 * NB;
+    float *vsc = lds + wave * kScale;
+    uint8_t *ksb = (uint8_t *) (vsc + 64 * NB);  // K's scale bytes, [64 keys][NB]
+    h8 ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = (_Float16) 1.0f;
     int ev = 1;
     for (; tile < t1; tile += NW) {
         const int base = tile * kTile, key = base + lane;
-        const TileInfo ti = tile_scales<NB>(sw, rd.there && key >= rt.lo && key < rt.hi, ev, ksc, vsc);
+        *(ScaleBytes<NB> *) (ksb + lane * NB) = swk;
+        const TileInfo ti = v_scales<NB>(swv, rd.there && key >= rt.lo && key < rt.hi, ev, vsc);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        int ksc[4][kKPieces<D>];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int u = 0; u < kKPieces<D>; ++u) ksc[t][u] = ksb[(16 * (r / 4) + 4 * t + r % 4) * NB + (D == 64 ? g & 1 : g) + 4 * u];
         f4 sc[CT][4];
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
             for (int t = 0; t < 4; ++t) sc[c][t] = f4{0, 0, 0, 0};
-        float ks[4][(NB + 3) / 4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int n = Q::N - 1; n >= 0; --n)
 #pragma unroll
-            for (int u = 0; u < (NB + 3) / 4; ++u) ks[t][u] = ksc[(16 * t + r) * NB + (g * NB + 4 * u) / 4];
+            for (int c = 0; c < CT; ++c) {
+                u6 q[Q::kSteps];
 #pragma unroll
-        for (int u = 0; u < NB; ++u) {
-            h8 q[CT][SPLIT];
+                for (int u = 0; u < Q::kSteps; ++u)
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
+                    for (int i = 0; i < 3; ++i) {
+                        const uint2 w = qs[c][n][u][lane][i];
+                        q[u][2 * i] = w.x, q[u][2 * i + 1] = w.y;
+                    }
 #pragma unroll
-                for (int h = 0; h < SPLIT; ++h) q[c][h] = qs[c][h][u][lane];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const h8 k = expand_k(kraw[t][u], ks[t][u / 4]);
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-#pragma unroll
-                    for (int h = SPLIT - 1; h >= 0; --h)
-                        sc[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[c][h], sc[c][t], 0, 0, 0);
+                for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q, n, sc[c][t]);
             }
-        }
-        const bool more = tile + NW < t1;
-        rd.page(a, s, tile + NW, more);
-        if (more) rd.scales(sw), rd.k(kraw);
-        const float back = ldexpf(1.0f, ti.ek - kBias), vkeep = ldexpf(1.0f, max(ev - ti.ev, -126));
+        // K is used up here, before the next tile's is asked for: the products may not sink below the loads, which would
+        // keep both tiles' registers
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(sc[c][t]));
+        __builtin_amdgcn_sched_barrier(0);
+        // (the last tile is asked for once more behind the end: it is in the cache, and the loop has no branch)
+        rd.take(a, min(tile + NW, t1 - 1));
+        rd.ask(a, table, min(tile + 2 * NW, t1 - 1));
+        rd.scales(swk, swv), rd.k(kraw);
+        const float vkeep = ldexpf(1.0f, max(ev - ti.ev, -126));
         ev = ti.ev;
         h8 p[CT][SPLIT][2];
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
             const uint32_t see = seen(pos[c], a.window, base, ti.there);
-            const uint32_t nan = ti.nan ? (uint32_t) (ti.nan >> (16 * g)) & 0xffffu : 0u;
-            const float keep = softmax_step<SPLIT>(sc[c], mul[c] * back, see, nan, st[c].m, st[c].l, p[c]) * vkeep;
-            if (__any(keep != 1.0f))
+            float keep;
+            if (ti.nan == 0 && __all(see == 0xffffu))
+                keep = softmax_step<SPLIT, false>(sc[c], mul[c], 0, 0, st[c].m, p[c]);
+            else
+                keep = softmax_step<SPLIT, true>(sc[c], mul[c], see, (uint32_t) (ti.nan >> (16 * g)) & 0xffffu, st[c].m, p[c]);
+            if (__any(keep != 1.0f) || vkeep != 1.0f) {
+                st[c].l *= keep;
 #pragma unroll
-                for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= keep;
+                for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= keep * vkeep;
+            }
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int h = SPLIT - 1; h >= 0; --h) st[c].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[c][h][v], st[c].l, 0, 0, 0);
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j)
@@ -473,8 +547,13 @@ __global__ __launch_bounds__(256, D == 256 || CT == 2 ? 2 : 4) void k_attn_few(A
                         st[c].o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, p[c][h][v], st[c].o[2 * j], 0, 0, 0);
                         st[c].o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, p[c][h][v], st[c].o[2 * j + 1], 0, 0, 0);
                     }
+                __builtin_amdgcn_sched_barrier(0);  // (one step's operands at a time: the registers are counted)
             }
-        if (more) rd.v(vraw);
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int d = 0; d < 2 * NB; ++d) asm volatile("" : "+v"(st[c].o[d]));  // (and V likewise)
+        rd.v(vraw);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -482,16 +561,16 @@ __global__ __launch_bounds__(256, D == 256 || CT == 2 ? 2 : 4) void k_attn_few(A
     // join the waves: the common maximum and sum of every row, then the sums in a tree over registers of equal layout
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-        st[c].l += xor_lane<16>(st[c].l);
-        st[c].l += xor_lane<32>(st[c].l);
-        if (g == 0) join[wave][0][16 * c + r] = st[c].m, join[wave][1][16 * c + r] = st[c].l;
+        if (g == 0) join[wave][0][16 * c + r] = st[c].m, join[wave][1][16 * c + r] = st[c].l[0];
     }
     __syncthreads();
     float top[CT], sum[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         const int row = 16 * c + r;
-        top[c] = fmaxf(fmaxf(join[0][0][row], join[1][0][row]), fmaxf(join[2][0][row], join[3][0][row]));
+        top[c] = join[0][0][row];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) top[c] = fmaxf(top[c], join[w][0][row]);
         const int h = head * a.group + (row0 + row) % a.group;
         const bool sink = a.splits == 1 && a.sinks && row0 + row < rows;
         const float sk = sink ? a.sinks[h] * kLog2e : -INFINITY;
@@ -530,6 +609,211 @@ __global__ __launch_bounds__(256, D == 256 || CT == 2 ? 2 : 4) void k_attn_few(A
 #pragma unroll
         for (int d = 0; d < 2 * NB; ++d) store_row<D, T>(a, tok, h, split, 16 * d + 4 * g, st[c].o[d]);
         if (a.splits > 1 && g == 0) a.part_ml[(split * a.b.n_tok + tok) * a.n_head + h] = make_float2(top[c], sum[c]);
+    }
+}
+
+// Many rows (prompts): a workgroup takes 128 rows, 32 a wave, and walks over the keys; its waves expand a tile's V together,
+// a tile ahead, into LDS as the second product wants it, [channel][64 keys] (rows 16 bytes apart in banks: a lane's 16-byte
+// reads of 16 channels touch every bank once). K needs no expansion: each wave reads its codes, which the workgroup's first
+// reader brings into L1, and keeps them in registers with the digits of its queries. Bound by the vector pipe's work on the
+// scores, about 6 instructions each where the two products take as long for bf16.
+__device__ __forceinline__ void tile_barrier() {
+    // LDS only: the tiles asked for stay in flight
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+template <int D, bool SMALL, class T>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a) {
+    constexpr int NB = D / 32, SPLIT = sizeof(T) == 4 ? 2 : 1, NW = 4, CT = 2;
+    constexpr int VS = 64 + 8;             // f16 values between V rows
+    constexpr int MB = (NB + NW - 1) / NW; // blocks that a wave expands: wave, wave + 4
+    using Q = QueryShape<D, T>;
+    __shared__ __align__(16) _Float16 vt[2][D * VS];
+    __shared__ __align__(16) float vsc_all[NW][MB * 64];
+    __shared__ __align__(16) uint8_t ksb_all[NW][64 * NB];
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, split = blockIdx.z;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+    const SeqRange sr = seq_range(a.b, s);
+    const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) INT32_MAX);
+    // the last rows, which see the most keys, first
+    const int row0 = ((int) gridDim.y - 1 - (int) blockIdx.y) * kManyRows;
+    if (row0 >= rows) return;
+    const RowTiles rt = row_tiles(a, sr, row0, kManyRows);
+    const int chunk = split_chunk(a, rt);
+    const int t0 = (int) min((int64_t) rt.t0 + (int64_t) split * chunk, (int64_t) rt.t1);
+    const int t1 = min(t0 + chunk, rt.t1);
+    if (split > 0 && t0 >= t1) return;  // (split 0 of an empty range writes the zeros)
+    const int P = 1 << a.c.shift, first = sr.len - sr.n;
+    float *vsc = vsc_all[wave];
+    uint8_t *ksb = ksb_all[wave];
+
+    Digits<D, T> q[CT];
+    RowState<NB> st[CT];
+    int pos[CT];
+    float mul[CT];
+    const int w0 = row0 + wave * 32;  // the wave's rows, and the positions that they see at most and at least
+    const int most = w0 < rows ? first + min(w0 + 31, rows - 1) / a.group : -1;
+    const int least = a.window ? first + w0 / a.group - a.window + 1 : 0;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        const int row = w0 + 16 * c + r, i = row / a.group;
+        const bool there = row < rows;
+        pos[c] = there ? first + i : -1;
+        mul[c] = query_digits<D, T>(q[c], (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D, there, a.scale);
+        st[c].m = -INFINITY, st[c].l = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int d = 0; d < 2 * NB; ++d) st[c].o[d] = f4{0, 0, 0, 0};
+    }
+    h8 ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = (_Float16) 1.0f;
+
+    TileReader<D, SMALL> rk, rv;  // K of the next tile, V of the one after it
+    rk.P = rv.P = P, rk.lane = rv.lane = lane, rk.r = rv.r = r, rk.g = rv.g = g;
+    rk.head_off = rv.head_off = head * kv_head_bytes(D, P);
+    rk.last = rv.last = (int) a.b.table_stride - 1;
+    const int32_t *table = a.b.table + s * a.b.table_stride;
+    u4 kraw[4][kKPieces<D>], vraw[MB];
+    ScaleBytes<NB> swk, swv, unused;
+    const auto load_v = [&] {  // the wave's blocks; a wave without one asks for another's
+#pragma unroll
+        for (int m = 0; m < MB; ++m) vraw[m] = rv.v_block((wave + NW * m) % NB);
+    };
+    const auto expand = [&](int buf) {
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            const int j = wave + NW * m;
+            if (j >= NB) break;
+            h8 lo[2], hi[2];
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                float w[8];
+                *(f4 *) w = *(const f4 *) (vsc + m * 64 + 16 * g + 8 * v);
+                *(f4 *) (w + 4) = *(const f4 *) (vsc + m * 64 + 16 * g + 8 * v + 4);
+                expand_v(vraw[m][2 * v], vraw[m][2 * v + 1], w, lo[v], hi[v]);
+            }
+            h8 *at = (h8 *) (vt[buf] + (32 * j + r) * VS + 16 * g);
+            at[0] = lo[0], at[1] = lo[1];
+            at += 16 * VS / 8;
+            at[0] = hi[0], at[1] = hi[1];
+        }
+    };
+    const auto wave_sync = [] {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    int ev = 1;
+    TileInfo ti{}, next{};
+    if (t0 < t1) {
+        rv.ask(a, table, t0), rk.ask(a, table, t0);
+        rv.take(a, t0), rk.take(a, t0);
+        rk.scales(swk, swv), rk.k(kraw), load_v();
+        rv.ask(a, table, min(t0 + 1, t1 - 1)), rk.ask(a, table, min(t0 + 1, t1 - 1));
+        const int key = t0 * kTile + lane;
+        ti = v_scales<NB, NW>(swv, rv.there && key >= rt.lo && key < rt.hi, ev, vsc, wave);
+        wave_sync();
+        expand(0);
+        wave_sync();
+        rv.take(a, min(t0 + 1, t1 - 1));
+        rv.scales(unused, swv), load_v();
+        rv.ask(a, table, min(t0 + 2, t1 - 1));
+        tile_barrier();
+    }
+    for (int tile = t0; tile < t1; ++tile) {
+        const int base = tile * kTile, buf = (tile - t0) & 1;
+        const bool active = base <= most && base + kTile > least;
+        f4 sc[CT][4];
+        if (active) {
+            *(ScaleBytes<NB> *) (ksb + lane * NB) = swk;
+            wave_sync();
+            int ksc[4][kKPieces<D>];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int u = 0; u < kKPieces<D>; ++u) ksc[t][u] = ksb[(16 * (r / 4) + 4 * t + r % 4) * NB + (D == 64 ? g & 1 : g) + 4 * u];
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) sc[c][t] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int n = Q::N - 1; n >= 0; --n)
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q[c][n], n, sc[c][t]);
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(sc[c][t]));  // (K is used up before the next one is asked for)
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        rk.take(a, min(tile + 1, t1 - 1));
+        rk.ask(a, table, min(tile + 2, t1 - 1));
+        rk.scales(swk, unused), rk.k(kraw);
+        if (active) {
+            const float vkeep = ldexpf(1.0f, max(ev - ti.ev, -126));
+            ev = ti.ev;
+            h8 p[CT][SPLIT][2];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                const uint32_t see = seen(pos[c], a.window, base, ti.there);
+                float keep;
+                if (ti.nan == 0 && __all(see == 0xffffu))
+                    keep = softmax_step<SPLIT, false>(sc[c], mul[c], 0, 0, st[c].m, p[c]);
+                else
+                    keep = softmax_step<SPLIT, true>(sc[c], mul[c], see, (uint32_t) (ti.nan >> (16 * g)) & 0xffffu, st[c].m, p[c]);
+                if (__any(keep != 1.0f) || vkeep != 1.0f) {
+                    st[c].l *= keep;
+#pragma unroll
+                    for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= keep * vkeep;
+                }
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int h = SPLIT - 1; h >= 0; --h) st[c].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[c][h][v], st[c].l, 0, 0, 0);
+            }
+            const h8 *at = (const h8 *) (vt[buf] + r * VS + 16 * g);
+#pragma unroll
+            for (int d = 0; d < 2 * NB; ++d)
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const h8 x = at[d * 16 * VS / 8 + v];
+#pragma unroll
+                    for (int c = 0; c < CT; ++c)
+#pragma unroll
+                        for (int h = SPLIT - 1; h >= 0; --h) st[c].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[c][h][v], st[c].o[d], 0, 0, 0);
+                }
+        }
+        const int after = min(tile + 1, t1 - 1), key = after * kTile + lane;
+        next = v_scales<NB, NW>(swv, rv.there && key >= rt.lo && key < rt.hi, ti.ev, vsc, wave);
+        wave_sync();
+        if (tile + 1 < t1) expand(buf ^ 1);
+        wave_sync();
+        rv.take(a, min(tile + 2, t1 - 1));
+        rv.scales(unused, swv), load_v();
+        rv.ask(a, table, min(tile + 3, t1 - 1));
+        ti = next;
+        tile_barrier();
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        const int row = w0 + 16 * c + r;
+        if (row >= rows) continue;
+        const int64_t tok = sr.q0 + row / a.group;
+        const int h = head * a.group + row % a.group;
+        float sum = st[c].l[0], off = st[c].m;
+        if (a.splits == 1 && a.sinks) {
+            const float sk = a.sinks[h] * kLog2e;
+            off = fmaxf(off, sk);
+            const float o = off == -INFINITY ? 0.0f : off;
+            sum = sum * __builtin_amdgcn_exp2f(st[c].m - o) + __builtin_amdgcn_exp2f(sk - o + kPShift);
+        }
+        const float o = off == -INFINITY ? 0.0f : off;
+        const float f = sum == 0.0f ? 0.0f : ldexpf(__builtin_amdgcn_exp2f(st[c].m - o) / sum, ev - kBias);
+#pragma unroll
+        for (int d = 0; d < 2 * NB; ++d) store_row<D, T>(a, tok, h, split, 16 * d + 4 * g, st[c].o[d] * f);
+        if (a.splits > 1 && g == 0) a.part_ml[(split * a.b.n_tok + tok) * a.n_head + h] = make_float2(st[c].m, sum);
     }
 }
 
@@ -604,13 +888,20 @@ struct Plan {
 Plan attn_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
     Plan p{};
     const int64_t rows = (int64_t) b->max_q * (x->n_head / c->n_head_kv);
-    p.rows = rows <= 16 || c->head_dim == 256 ? 16 : 32;
+    p.rows = rows > kFewRows ? kManyRows : rows <= 16 || c->head_dim == 256 ? 16 : 32;
     p.row_tiles = (int) ((rows + p.rows - 1) / p.rows);
     const int64_t wgs = std::max<int64_t>(1, (int64_t) b->n_seq * c->n_head_kv * p.row_tiles);
     const int64_t tiles = std::max<int64_t>(1, (b->max_kv + kTile - 1) / kTile);
-    const int64_t want = (2048 + wgs - 1) / wgs, most = (tiles + 3) / 4;
-    p.splits = (int) std::max<int64_t>(1, std::min({want, most, (int64_t) 64}));
-    p.chunk = (int) ((tiles + p.splits - 1) / p.splits);
+    const auto per = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
+    int64_t splits = 1;
+    if (p.rows == kManyRows) {
+        splits = std::min(per(512, wgs), tiles / 8);
+    } else if (tiles > 12) {
+        splits = std::max(per(p.rows == 16 && c->head_dim <= 128 ? 768 : 512, wgs), std::min(per(tiles, 40), per(2304, wgs)));
+        splits = std::min(splits, per(tiles, kFewWaves));
+    }
+    p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(splits, 64));
+    p.chunk = (int) per(tiles, p.splits);
     if (p.splits > 1) {
         const size_t n = (size_t) p.splits * b->n_tok * x->n_head;
         p.ml_off = n * c->head_dim * 4;
@@ -647,8 +938,8 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
     const bool small = c->page_size < kTile;
     auto few = [&](auto dim, auto ct, auto type) {
         constexpr int D = decltype(dim)::value, CT = decltype(ct)::value;
-        if (small) hipLaunchKernelGGL((k_attn_few<D, CT, true, decltype(type)>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_attn_few<D, CT, false, decltype(type)>), grid, dim3(256), 0, st, a);
+        if (small) hipLaunchKernelGGL((k_attn_few<D, CT, true, decltype(type)>), grid, dim3(64 * kFewWaves), 0, st, a);
+        else hipLaunchKernelGGL((k_attn_few<D, CT, false, decltype(type)>), grid, dim3(64 * kFewWaves), 0, st, a);
     };
     auto join = [&](auto dim, auto type) {
         const int64_t rows = (int64_t) b->max_q * x->n_head;
@@ -657,7 +948,10 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
     };
     auto by_type = [&](auto dim, auto type) {
         constexpr int D = decltype(dim)::value;
-        if constexpr (D == 256) few(dim, std::integral_constant<int, 1>{}, type);
+        if (p.rows == kManyRows) {
+            if (small) hipLaunchKernelGGL((k_attn_many<D, true, decltype(type)>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((k_attn_many<D, false, decltype(type)>), grid, dim3(256), 0, st, a);
+        } else if constexpr (D == 256) few(dim, std::integral_constant<int, 1>{}, type);
         else if (p.rows == 16) few(dim, std::integral_constant<int, 1>{}, type);
         else few(dim, std::integral_constant<int, 2>{}, type);
         FNS_TRY(host::check_launch("attn"));
