@@ -179,9 +179,10 @@ template <int D, class T> struct QueryShape {
 };
 typedef uint32_t u6 __attribute__((ext_vector_type(6)));
 template <int D, class T> using Digits = u6[QueryShape<D, T>::N][QueryShape<D, T>::kSteps];
-// Returns what turns a product into log2 units.
+// The row is first multiplied by scale * log2(e): scores are log2 units. Returns the block scale of digit 0 (255: the row has a
+// NaN or an infinity, and every score is NaN).
 template <int D, class T>
-__device__ __forceinline__ float query_digits(Digits<D, T> &w, const T *row, bool there, float scale) {
+__device__ __forceinline__ int query_digits(Digits<D, T> &w, const T *row, bool there, float scale) {
     typedef float v16 __attribute__((ext_vector_type(16)));
     typedef float v32 __attribute__((ext_vector_type(32)));
     using Q = QueryShape<D, T>;
@@ -189,12 +190,13 @@ __device__ __forceinline__ float query_digits(Digits<D, T> &w, const T *row, boo
     v16 even[Q::kSteps], odd[Q::kSteps];
     float amax = 0.0f;
     int bad = 0;
+    const float in_log2 = scale * kLog2e;
 #pragma unroll
     for (int u = 0; u < Q::kSteps; ++u) {
         T t[32] = {};
         if (there) __builtin_memcpy(t, row + ((D == 64 ? g & 1 : g) + 4 * u) * 32, sizeof t);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) even[u][i] = to_f32(t[2 * i]), odd[u][i] = to_f32(t[2 * i + 1]);
+        for (int i = 0; i < 16; ++i) even[u][i] = to_f32(t[2 * i]) * in_log2, odd[u][i] = to_f32(t[2 * i + 1]) * in_log2;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             amax = fmaxf(fmaxf(amax, fabsf(even[u][i])), fabsf(odd[u][i]));
@@ -206,7 +208,7 @@ __device__ __forceinline__ float query_digits(Digits<D, T> &w, const T *row, boo
     amax = fmaxf(amax, xor_lane<32>(amax));
     // (below 2^-100 the row is smaller than any difference that a score can show)
     const int k = amax < 7.8886090522101181e-31f ? -100 : (int) (__builtin_bit_cast(uint32_t, amax) >> 23) - 126;  // amax < 2^k
-    const float f = amax == INFINITY ? 0.0f : ldexpf(scale < 0.0f ? -1.0f : 1.0f, 2 - k);
+    const float f = amax == INFINITY ? 0.0f : ldexpf(1.0f, 2 - k);
 #pragma unroll
     for (int u = 0; u < Q::kSteps; ++u)
 #pragma unroll
@@ -233,14 +235,17 @@ __device__ __forceinline__ float query_digits(Digits<D, T> &w, const T *row, boo
                 w[d][u] = code;
             }
         }
-    return amax == INFINITY ? __builtin_nanf("") : fabsf(scale) * kLog2e * ldexpf(1.0f, k - 2);
+    return amax == INFINITY ? 255 : 127 + k - 2;
 }
 
-// S^T of 16 keys and 16 query rows: the products of digit (pair) n with every 128 channels.
+// S^T of 16 keys and 16 query rows: the products of one digit (or pair), of block scale qsc, with every 128 channels.
 template <int D> constexpr int kKPieces = D == 256 ? 2 : 1;  // 16-byte pieces of a key that a lane holds
+template <int D, class T> __device__ __forceinline__ int digit_scale(int qsc0, int n) {
+    const int qsc = qsc0 - 5 * (n * QueryShape<D, T>::kPerStep) - (D == 64 && threadIdx.x % 64 >= 32 ? 5 : 0);
+    return qsc0 == 255 ? 255 : max(qsc, 0);
+}
 template <int D, class T>
-__device__ __forceinline__ f4 scores(const u4 (&k)[kKPieces<D>], const int (&ksc)[kKPieces<D>], const u6 (&q)[QueryShape<D, T>::kSteps], int n, f4 acc) {
-    const int qsc = 127 - 5 * (n * QueryShape<D, T>::kPerStep) - (D == 64 && threadIdx.x % 64 >= 32 ? 5 : 0);
+__device__ __forceinline__ f4 scores(const u4 (&k)[kKPieces<D>], const int (&ksc)[kKPieces<D>], const u6 (&q)[QueryShape<D, T>::kSteps], int qsc, f4 acc) {
 #pragma unroll
     for (int u = 0; u < QueryShape<D, T>::kSteps; ++u) {
         const i8v a = {(int) k[u][0], (int) k[u][1], (int) k[u][2], (int) k[u][3], 0, 0, 0, 0};
@@ -258,59 +263,8 @@ template <int NB> struct RowState {
     float m;
 };
 
-// One tile's softmax of a column tile: s (product units) of the lane's 16 keys -> p as operand parts, m updated; returns
-// what earlier sums have to be multiplied by. MASKED: only the keys of `see` count, those of `nan` make the row NaN.
-template <int SPLIT, bool MASKED>
-__device__ __forceinline__ float softmax_step(f4 (&s)[4], float mul, uint32_t see, uint32_t nan, float &m, h8 (&p)[SPLIT][2]) {
-    if constexpr (MASKED) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[t][i] = see >> (4 * t + i) & 1 ? s[t][i] : -INFINITY;
-    }
-    float top = fmaxf(s[0][0], s[0][1]);
-#pragma unroll
-    for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, s[i / 4][i % 4]), s[i / 4][i % 4 + 1]);
-    top = fmaxf(top, xor_lane<16>(top));
-    top = fmaxf(top, xor_lane<32>(top));
-    const float now = top == -INFINITY ? top : top * mul;
-    float keep = 1.0f;
-    if (__any(now > m + kLazy)) {
-        const float to = fmaxf(m, now);
-        keep = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));  // (nothing seen so far: no difference of infinities)
-        m = to;
-    }
-    const float add = kPShift - (m == -INFINITY ? 0.0f : m);
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], mul, add));
-            if constexpr (MASKED) {  // (a scale of zero times -infinity)
-                s[t][i] = see >> (4 * t + i) & 1 ? s[t][i] : 0.0f;
-                s[t][i] = see >> (4 * t + i) & nan >> (4 * t + i) & 1 ? __builtin_nanf("") : s[t][i];
-            }
-        }
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
-        u4 w[SPLIT];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = s[2 * v + i / 2][i % 2 * 2], y = s[2 * v + i / 2][i % 2 * 2 + 1];
-            if constexpr (SPLIT == 2) {  // toward zero: the second part has the rest
-                const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
-                w[0][i] = __builtin_bit_cast(uint32_t, hi);
-                w[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float) hi[0], -1.0f, x),
-                                                                                  __builtin_fmaf((float) hi[1], -1.0f, y)));
-            } else {
-                w[0][i] = __builtin_bit_cast(uint32_t, h2{(_Float16) x, (_Float16) y});
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < SPLIT; ++h) p[h][v] = __builtin_bit_cast(h8, w[h]);
-    }
-    return keep;
-}
+// What a tile's scores of a row start from, so that they come as the exponents of p: the row's maximum so far, 2^8 down.
+__device__ __forceinline__ float score_origin(float m) { return kPShift - (m == -INFINITY ? 0.0f : m); }
 
 // Bits of the lane's 16 keys (base + 16 g ..) that a row at position pos sees; there: the tile's keys that exist.
 __device__ __forceinline__ uint32_t seen(int pos, int window, int base, uint64_t there) {
@@ -322,6 +276,78 @@ __device__ __forceinline__ uint32_t seen(int pos, int window, int base, uint64_t
         bits = dn <= 0 ? bits : dn > 15 ? 0u : bits & (0xffffu << dn);
     }
     return bits & (uint32_t) (there >> (16 * g));
+}
+
+// One tile's softmax: s (from score_origin) of the lane's 16 keys and CT rows -> p as operand parts, and its sums. Rows that do
+// not see every key, a maximum that has grown, a NaN in V or a larger V scale (vkeep) are seen to first, in place: keys that
+// a row does not see become -infinity, m moves and what refers to it follows.
+template <int NB, int CT, int SPLIT>
+__device__ __forceinline__ void softmax_tile(f4 (&s)[CT][4], const int (&pos)[CT], int window, int base, const TileInfo &ti, float vkeep,
+                                             RowState<NB> (&st)[CT], h8 (&p)[CT][SPLIT][2]) {
+    const int g = threadIdx.x % 64 / 16;
+    const auto largest = [](const f4 (&x)[4]) {
+        float top = fmaxf(x[0][0], x[0][1]);
+#pragma unroll
+        for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, x[i / 4][i % 4]), x[i / 4][i % 4 + 1]);
+        return top;
+    };
+    bool plain = ti.nan == 0 && vkeep == 1.0f;
+#pragma unroll
+    for (int c = 0; c < CT; ++c)  // (a lane's own keys will do: one that exceeds the row's bound is found by its lane)
+        plain = plain && largest(s[c]) <= (st[c].m == -INFINITY ? -INFINITY : kPShift + kLazy) &&
+                seen(pos[c], window, base, ti.there) == 0xffffu;
+    if (!__all(plain)) {
+        const uint32_t nan = (uint32_t) (ti.nan >> (16 * g)) & 0xffffu;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const uint32_t see = seen(pos[c], window, base, ti.there);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[c][t][i] = see >> (4 * t + i) & 1 ? s[c][t][i] : -INFINITY;
+            float top = largest(s[c]);
+            top = fmaxf(top, xor_lane<16>(top));
+            top = fmaxf(top, xor_lane<32>(top));
+            const float off = st[c].m == -INFINITY ? 0.0f : st[c].m;  // (nothing seen so far: no difference of infinities)
+            const float to = fmaxf(st[c].m, top + (off - kPShift)), now = to == -INFINITY ? 0.0f : to;
+            const float keep = __builtin_amdgcn_exp2f(st[c].m - now);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[c][t][i] = see & nan & 1u << (4 * t + i) ? __builtin_nanf("") : s[c][t][i] - (now - off);
+            st[c].m = to;
+            st[c].l *= keep;
+#pragma unroll
+            for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= keep * vkeep;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            u4 w[SPLIT];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = __builtin_amdgcn_exp2f(s[c][2 * v + i / 2][i % 2 * 2]), y = __builtin_amdgcn_exp2f(s[c][2 * v + i / 2][i % 2 * 2 + 1]);
+                // toward zero: a second part has the rest, and without one the sum of p counts the same values
+                const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
+                w[0][i] = __builtin_bit_cast(uint32_t, hi);
+                if constexpr (SPLIT == 2)
+                    w[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float) hi[0], -1.0f, x),
+                                                                                      __builtin_fmaf((float) hi[1], -1.0f, y)));
+            }
+#pragma unroll
+            for (int h = 0; h < SPLIT; ++h) p[c][h][v] = __builtin_bit_cast(h8, w[h]);
+        }
+    h8 ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = (_Float16) 1.0f;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int h = SPLIT - 1; h >= 0; --h) st[c].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[c][h][v], st[c].l, 0, 0, 0);
 }
 
 // Result of one row's 4 channels or, with splits, its partial.
@@ -405,7 +431,7 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
     __shared__ __align__(16) float lds[NW * kScale > kJoin ? NW * kScale : kJoin];
     using Q = QueryShape<D, T>;
     __shared__ __align__(16) uint2 qs[CT][Q::N][Q::kSteps][64][3];
-    __shared__ float qmul[CT][16];
+    __shared__ int qscale[CT][16];
     __shared__ float join[NW][2][CT * 16];
     const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, row0 = blockIdx.y * 16 * CT, split = blockIdx.z;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
@@ -436,7 +462,7 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
     if (wave < CT) {  // a wave a column tile
         const int row = row0 + 16 * wave + r, i = row / a.group;
         Digits<D, T> w;
-        const float mul = query_digits<D, T>(w, (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D,
+        const int scale = query_digits<D, T>(w, (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D,
                                              row < rows, a.scale);
 #pragma unroll
         for (int n = 0; n < Q::N; ++n)
@@ -444,7 +470,7 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
             for (int u = 0; u < Q::kSteps; ++u)
 #pragma unroll
                 for (int i2 = 0; i2 < 3; ++i2) qs[wave][n][u][lane][i2] = make_uint2(w[n][u][2 * i2], w[n][u][2 * i2 + 1]);
-        if (g == 0) qmul[wave][r] = mul;
+        if (g == 0) qscale[wave][r] = scale;
     }
     RowState<NB> st[CT];
     int pos[CT];
@@ -457,15 +483,12 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
         for (int d = 0; d < 2 * NB; ++d) st[c].o[d] = f4{0, 0, 0, 0};
     }
     __syncthreads();
-    float mul[CT];
+    int qsc[CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) mul[c] = qmul[c][r];
+    for (int c = 0; c < CT; ++c) qsc[c] = qscale[c][r];
 
     float *vsc = lds + wave * kScale;
     uint8_t *ksb = (uint8_t *) (vsc + 64 * NB);  // K's scale bytes, [64 keys][NB]
-    h8 ones;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ones[i] = (_Float16) 1.0f;
     int ev = 1;
     for (; tile < t1; tile += NW) {
         const int base = tile * kTile, key = base + lane;
@@ -483,9 +506,9 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) sc[c][t] = f4{0, 0, 0, 0};
+            for (int t = 0; t < 4; ++t) sc[c][t] = f4{1, 1, 1, 1} * score_origin(st[c].m);
 #pragma unroll
-        for (int n = Q::N - 1; n >= 0; --n)
+        for (int n = 0; n < Q::N; ++n)  // the largest digit first: the rest adds to small numbers
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 u6 q[Q::kSteps];
@@ -497,7 +520,7 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
                         q[u][2 * i] = w.x, q[u][2 * i + 1] = w.y;
                     }
 #pragma unroll
-                for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q, n, sc[c][t]);
+                for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q, digit_scale<D, T>(qsc[c], n), sc[c][t]);
             }
         // K is used up here, before the next tile's is asked for: the products may not sink below the loads, which would
         // keep both tiles' registers
@@ -513,24 +536,7 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
         const float vkeep = ldexpf(1.0f, max(ev - ti.ev, -126));
         ev = ti.ev;
         h8 p[CT][SPLIT][2];
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            const uint32_t see = seen(pos[c], a.window, base, ti.there);
-            float keep;
-            if (ti.nan == 0 && __all(see == 0xffffu))
-                keep = softmax_step<SPLIT, false>(sc[c], mul[c], 0, 0, st[c].m, p[c]);
-            else
-                keep = softmax_step<SPLIT, true>(sc[c], mul[c], see, (uint32_t) (ti.nan >> (16 * g)) & 0xffffu, st[c].m, p[c]);
-            if (__any(keep != 1.0f) || vkeep != 1.0f) {
-                st[c].l *= keep;
-#pragma unroll
-                for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= keep * vkeep;
-            }
-#pragma unroll
-            for (int v = 0; v < 2; ++v)
-#pragma unroll
-                for (int h = SPLIT - 1; h >= 0; --h) st[c].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[c][h][v], st[c].l, 0, 0, 0);
-        }
+        softmax_tile<NB, CT, SPLIT>(sc, pos, a.window, base, ti, vkeep, st, p);
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -648,27 +654,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     float *vsc = vsc_all[wave];
     uint8_t *ksb = ksb_all[wave];
 
-    Digits<D, T> q[CT];
-    RowState<NB> st[CT];
-    int pos[CT];
-    float mul[CT];
-    const int w0 = row0 + wave * 32;  // the wave's rows, and the positions that they see at most and at least
-    const int most = w0 < rows ? first + min(w0 + 31, rows - 1) / a.group : -1;
-    const int least = a.window ? first + w0 / a.group - a.window + 1 : 0;
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-        const int row = w0 + 16 * c + r, i = row / a.group;
-        const bool there = row < rows;
-        pos[c] = there ? first + i : -1;
-        mul[c] = query_digits<D, T>(q[c], (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D, there, a.scale);
-        st[c].m = -INFINITY, st[c].l = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int d = 0; d < 2 * NB; ++d) st[c].o[d] = f4{0, 0, 0, 0};
-    }
-    h8 ones;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ones[i] = (_Float16) 1.0f;
-
     TileReader<D, SMALL> rk, rv;  // K of the next tile, V of the one after it
     rk.P = rv.P = P, rk.lane = rv.lane = lane, rk.r = rv.r = r, rk.g = rv.g = g;
     rk.head_off = rv.head_off = head * kv_head_bytes(D, P);
@@ -710,6 +695,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         rv.take(a, t0), rk.take(a, t0);
         rk.scales(swk, swv), rk.k(kraw), load_v();
         rv.ask(a, table, min(t0 + 1, t1 - 1)), rk.ask(a, table, min(t0 + 1, t1 - 1));
+    }
+    Digits<D, T> q[CT];
+    RowState<NB> st[CT];
+    int pos[CT];
+    int qsc[CT];
+    const int w0 = row0 + wave * 32;  // the wave's rows, and the positions that they see at most and at least
+    const int most = w0 < rows ? first + min(w0 + 31, rows - 1) / a.group : -1;
+    const int least = a.window ? first + w0 / a.group - a.window + 1 : 0;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        const int row = w0 + 16 * c + r, i = row / a.group;
+        const bool there = row < rows;
+        pos[c] = there ? first + i : -1;
+        qsc[c] = query_digits<D, T>(q[c], (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D, there, a.scale);
+        st[c].m = -INFINITY, st[c].l = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int d = 0; d < 2 * NB; ++d) st[c].o[d] = f4{0, 0, 0, 0};
+    }
+    if (t0 < t1) {
         const int key = t0 * kTile + lane;
         ti = v_scales<NB, NW>(swv, rv.there && key >= rt.lo && key < rt.hi, ev, vsc, wave);
         wave_sync();
@@ -735,13 +739,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) sc[c][t] = f4{0, 0, 0, 0};
+                for (int t = 0; t < 4; ++t) sc[c][t] = f4{1, 1, 1, 1} * score_origin(st[c].m);
 #pragma unroll
-            for (int n = Q::N - 1; n >= 0; --n)
+            for (int n = 0; n < Q::N; ++n)  // the largest digit first: the rest adds to small numbers
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q[c][n], n, sc[c][t]);
+                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q[c][n], digit_scale<D, T>(qsc[c], n), sc[c][t]);
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -755,24 +759,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
             const float vkeep = ldexpf(1.0f, max(ev - ti.ev, -126));
             ev = ti.ev;
             h8 p[CT][SPLIT][2];
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                const uint32_t see = seen(pos[c], a.window, base, ti.there);
-                float keep;
-                if (ti.nan == 0 && __all(see == 0xffffu))
-                    keep = softmax_step<SPLIT, false>(sc[c], mul[c], 0, 0, st[c].m, p[c]);
-                else
-                    keep = softmax_step<SPLIT, true>(sc[c], mul[c], see, (uint32_t) (ti.nan >> (16 * g)) & 0xffffu, st[c].m, p[c]);
-                if (__any(keep != 1.0f) || vkeep != 1.0f) {
-                    st[c].l *= keep;
-#pragma unroll
-                    for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= keep * vkeep;
-                }
-#pragma unroll
-                for (int v = 0; v < 2; ++v)
-#pragma unroll
-                    for (int h = SPLIT - 1; h >= 0; --h) st[c].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[c][h][v], st[c].l, 0, 0, 0);
-            }
+            softmax_tile<NB, CT, SPLIT>(sc, pos, a.window, base, ti, vkeep, st, p);
             const h8 *at = (const h8 *) (vt[buf] + r * VS + 16 * g);
 #pragma unroll
             for (int d = 0; d < 2 * NB; ++d)
@@ -783,6 +770,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
                     for (int c = 0; c < CT; ++c)
 #pragma unroll
                         for (int h = SPLIT - 1; h >= 0; --h) st[c].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[c][h][v], st[c].o[d], 0, 0, 0);
+                    if (SPLIT == 2 && v == 1) __builtin_amdgcn_sched_barrier(0);  // (the registers are counted: no more reads ahead)
                 }
         }
         const int after = min(tile + 1, t1 - 1), key = after * kTile + lane;
@@ -817,48 +805,55 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     }
 }
 
-// The splits of a row into its result: a workgroup a row, its waves the splits in turn (at most 64: one a lane for their
-// weights), a lane D / 64 channels.
-template <int D, class T>
+// The splits of a row into its result, a lane D / 64 channels: few rows a workgroup each, whose waves take the splits in turn;
+// many rows a wave each (WAVE_ROW). At most 64 splits: one a lane for their weights.
+template <int D, bool WAVE_ROW, class T>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int rows_per_wg) {
     constexpr int C = D / 64, NW = 4;
-    __shared__ float part[NW][D], weight[64];
+    __shared__ float part[WAVE_ROW ? 1 : NW][D], weight[NW][64];
     const int s = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const SeqRange sr = seq_range(a.b, s);
-    const int i = blockIdx.x / a.n_head, h = blockIdx.x % a.n_head;
-    if (i >= sr.n) return;
+    const int at = WAVE_ROW ? blockIdx.x * NW + wave : blockIdx.x, i = at / a.n_head, h = at % a.n_head;
+    if (i >= sr.n) return;  // (the whole workgroup, or a wave that shares nothing)
     const int64_t tok = sr.q0 + i, first = tok * a.n_head + h, step = a.b.n_tok * a.n_head;
     const int row = i * a.group + h % a.group, row0 = row / rows_per_wg * rows_per_wg;
     const RowTiles rt = row_tiles(a, sr, row0, rows_per_wg);
     const int chunk = split_chunk(a, rt);
-    const int n = max(1, (rt.t1 - rt.t0 + chunk - 1) / max(chunk, 1));  // splits that have tiles (the first one in any case)
+    const int n = max(1, (rt.t1 - rt.t0 + chunk - 1) / chunk);  // splits that have tiles (the first one in any case)
     const float sk = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
     const float2 ml = lane < n ? a.part_ml[lane * step + first] : make_float2(-INFINITY, 0.0f);
     const float top = fmaxf(lanes_max<64>(ml.x), sk);
     const float off = top == -INFINITY ? 0.0f : top;
     const float f = ml.y == 0.0f ? 0.0f : ml.y * __builtin_amdgcn_exp2f(ml.x - off);
     const float sum = lanes_sum<64>(f) + (a.sinks ? __builtin_amdgcn_exp2f(sk - off + kPShift) : 0.0f);
-    if (wave == 0) weight[lane] = sum == 0.0f ? 0.0f : f / sum;
-    __syncthreads();
+    weight[wave][lane] = sum == 0.0f ? 0.0f : f / sum;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     float o[C] = {};
     const float *src = a.part + first * D + lane * C;
 #pragma unroll 8
-    for (int k = wave; k < n; k += NW) {
-        const float wk = weight[k];
+    for (int k = WAVE_ROW ? 0 : wave; k < n; k += WAVE_ROW ? 1 : NW) {
+        const float wk = weight[wave][k];
         float v[C];
         __builtin_memcpy(v, __builtin_assume_aligned(src + k * step * D, 4 * C), sizeof v);
 #pragma unroll
         for (int c = 0; c < C; ++c) o[c] += wk == 0.0f ? 0.0f : wk * v[c];
     }
+    if constexpr (!WAVE_ROW) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) part[wave][lane * C + c] = o[c];
-    __syncthreads();
-    T *out = (T *) a.out + tok * a.out_stride + (int64_t) h * D;
-    for (int d = threadIdx.x; d < D; d += 256) {
-        const float x = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
-        if constexpr (sizeof(T) == 4) out[d] = x;
-        else out[d] = to_bf16(x);
+        for (int c = 0; c < C; ++c) part[wave][lane * C + c] = o[c];
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] = (part[0][lane * C + c] + part[1][lane * C + c]) + (part[2][lane * C + c] + part[3][lane * C + c]);
     }
+    T t[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if constexpr (sizeof(T) == 4) t[c] = o[c];
+        else t[c] = to_bf16(o[c]);
+    }
+    __builtin_memcpy((T *) a.out + tok * a.out_stride + (int64_t) h * D + lane * C, t, sizeof t);
 }
 
 }  // namespace
@@ -942,9 +937,13 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
         else hipLaunchKernelGGL((k_attn_few<D, CT, false, decltype(type)>), grid, dim3(64 * kFewWaves), 0, st, a);
     };
     auto join = [&](auto dim, auto type) {
+        constexpr int D = decltype(dim)::value;
         const int64_t rows = (int64_t) b->max_q * x->n_head;
-        hipLaunchKernelGGL((k_attn_join<decltype(dim)::value, decltype(type)>), dim3((unsigned) rows, (unsigned) b->n_seq),
-                           dim3(256), 0, st, a, p.rows);
+        // a workgroup a row as long as all of them are resident at once
+        if (rows * b->n_seq <= 2048)
+            hipLaunchKernelGGL((k_attn_join<D, false, decltype(type)>), dim3((unsigned) rows, (unsigned) b->n_seq), dim3(256), 0, st, a, p.rows);
+        else
+            hipLaunchKernelGGL((k_attn_join<D, true, decltype(type)>), dim3((unsigned) ((rows + 3) / 4), (unsigned) b->n_seq), dim3(256), 0, st, a, p.rows);
     };
     auto by_type = [&](auto dim, auto type) {
         constexpr int D = decltype(dim)::value;
