@@ -188,42 +188,39 @@ __device__ __forceinline__ int query_digits(Digits<D, T> &w, const T *row, bool 
     using Q = QueryShape<D, T>;
     const int g = threadIdx.x % 64 / 16;
     v16 even[Q::kSteps], odd[Q::kSteps];
-    float amax = 0.0f;
-    int bad = 0;
-    const float in_log2 = scale * kLog2e;
+    int top = 0;  // bits of the largest magnitude: a NaN's are the largest
 #pragma unroll
     for (int u = 0; u < Q::kSteps; ++u) {
         T t[32] = {};
         if (there) __builtin_memcpy(t, row + ((D == 64 ? g & 1 : g) + 4 * u) * 32, sizeof t);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) even[u][i] = to_f32(t[2 * i]) * in_log2, odd[u][i] = to_f32(t[2 * i + 1]) * in_log2;
-#pragma unroll
         for (int i = 0; i < 16; ++i) {
-            amax = fmaxf(fmaxf(amax, fabsf(even[u][i])), fabsf(odd[u][i]));
-            bad |= !(fmaxf(fabsf(even[u][i]), fabsf(odd[u][i])) < INFINITY) || even[u][i] != even[u][i] || odd[u][i] != odd[u][i];
+            const float x = to_f32(t[2 * i]), y = to_f32(t[2 * i + 1]);
+            top = max(max(top, __builtin_bit_cast(int, x) & 0x7fffffff), __builtin_bit_cast(int, y) & 0x7fffffff);
+            even[u][i] = x, odd[u][i] = y;
         }
     }
-    amax = bad ? INFINITY : amax;
-    amax = fmaxf(amax, xor_lane<16>(amax));
-    amax = fmaxf(amax, xor_lane<32>(amax));
+    top = max(top, xor_lane_i<16>(top));
+    top = max(top, xor_lane_i<32>(top));
+    const float in_log2 = scale * kLog2e, amax = __builtin_bit_cast(float, top) * fabsf(in_log2);
+    const bool bad = !(amax < INFINITY);
     // (below 2^-100 the row is smaller than any difference that a score can show)
     const int k = amax < 7.8886090522101181e-31f ? -100 : (int) (__builtin_bit_cast(uint32_t, amax) >> 23) - 126;  // amax < 2^k
-    const float f = amax == INFINITY ? 0.0f : ldexpf(1.0f, 2 - k);
+    const float f = in_log2 * ldexpf(1.0f, 2 - k);
 #pragma unroll
     for (int u = 0; u < Q::kSteps; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) even[u][i] = bad ? 0.0f : even[u][i] * f, odd[u][i] = bad ? 0.0f : odd[u][i] * f;
+        for (int i = 0; i < 16; ++i) even[u][i] *= f, odd[u][i] *= f;
 #pragma unroll
     for (int d = 0; d < Q::N * Q::kPerStep; ++d)
 #pragma unroll
         for (int u = 0; u < Q::kSteps; ++u) {
             const float unit = __builtin_bit_cast(float, (uint32_t) (127 - 5 * d) << 23);
-            u6 code;
-            v32 back;
-            // (as assembly for its "&": the conversion writes its result while it still reads its operands, and the builtin
-            // lets them share registers)
-            asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3" : "=&v"(code) : "v"(even[u]), "v"(odd[u]), "v"(unit));
-            asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2" : "=&v"(back) : "v"(code), "v"(unit));
+            u6 code = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even[u], odd[u], unit);
+            // (the conversion writes its result while it still reads its operands, and the compiler lets a result have the
+            // registers of operands that end there: these end here)
+            asm volatile("" : "+v"(code) : "v"(even[u]), "v"(odd[u]));
+            const v32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(code, unit);
 #pragma unroll
             for (int i = 0; i < 16; ++i) even[u][i] -= back[2 * i], odd[u][i] -= back[2 * i + 1];
             if constexpr (D == 64) {
@@ -235,7 +232,7 @@ __device__ __forceinline__ int query_digits(Digits<D, T> &w, const T *row, bool 
                 w[d][u] = code;
             }
         }
-    return amax == INFINITY ? 255 : 127 + k - 2;
+    return bad ? 255 : 127 + k - 2;
 }
 
 // S^T of 16 keys and 16 query rows: the products of one digit (or pair), of block scale qsc, with every 128 channels.
