@@ -21,10 +21,11 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;     // keys of a step
-constexpr int kFewRows = 32, kManyRows = 128;  // rows of the few-row form at most, of a workgroup of the other
+constexpr int kFewRows = 64, kManyRows = 128;  // rows that always take the few-row form; rows of a workgroup of the other
 constexpr int kFewWaves = 4;  // waves of a workgroup of few rows
 constexpr int kHead = 12;     // V expands to f16 with the largest block scale so far at 2^12 (codes to 6: 24576)
 constexpr int kBias = 127 + kHead;
+constexpr int kBand = 36;     // block scales from E down that f16 holds exactly
 // p is carried times 2^8: its low half stays clear of f16's subnormals. Sums are rescaled only where a row's maximum has
 // grown by more than 2^7 since the last time, so p stays below 2^15.
 constexpr float kPShift = 8.0f, kLazy = 7.0f;
@@ -46,6 +47,7 @@ struct AttnArgs {
     int64_t q_stride, out_stride;
     int n_head, group, window, splits, chunk;
     float scale;
+    uint8_t *redo;  // many rows: [n_seq * n_kv][row tiles][4 waves], whether low blocks were left out
 };
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
@@ -94,13 +96,19 @@ typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pk_max(uint32_t x, uint32_t y) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, x), __builtin_bit_cast(us2, y)));
 }
+// Not zero in the halves of x that are from 1 to bound.
+__device__ __forceinline__ uint32_t pk_below(uint32_t x, uint32_t bound) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(us2, bound), (us2) (__builtin_bit_cast(us2, x) - (us2) {1, 1})));
+}
 struct TileInfo {
     uint64_t there, nan;
     int ev;
+    bool low;  // there are blocks (of those that the wave expands) that f16 cannot hold beside the largest
 };
 // The block scales of V as the f32 operands of the expansion, in the wave's LDS, [NB][64 keys]: 2^(e - E + 12), E at least
-// every scale so far; what lies 2^36 below that is dropped, which is less than the last bit of any sum it could join. w: the
-// scale bytes of the lane's key.
+// every scale so far. Half of 2^(12 - kBand) is the last bit of f16: blocks of E - kBand and below become zeros here and are
+// low_blocks' work (they are nothing beside the largest, but there may be rows that do not see the largest). w: the scale
+// bytes of the lane's key.
 template <int NB> struct ScaleBytes {
     std::conditional_t<NB == 2, uint16_t, uint32_t> w[(NB + 3) / 4];
 };
@@ -140,6 +148,24 @@ __device__ __forceinline__ TileInfo v_scales(const ScaleBytes<NB> &bytes, bool t
         top = max(top, (uint32_t) xor_lane_i<16>(top));
         top = max(top, (uint32_t) xor_lane_i<32>(top));
         t.ev = max(ev, __builtin_amdgcn_readfirstlane(top));
+    }
+    const uint32_t bound = (uint32_t) max(t.ev - kBand, 0);
+    uint32_t low = 0;
+    if constexpr (STEP == 1) {
+#pragma unroll
+        for (int i = 0; i < W; ++i)  // scales 1 .. bound: less 1, a scale of 0 is the largest
+            low |= pk_below(w[i] & kEven, bound * 0x10001u) | pk_below(w[i] >> 8 & kEven, bound * 0x10001u);
+    } else {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            if (b % STEP == first) low |= (w[b / 4] >> (b % 4 * 8) & 0xffu) - 1u < bound;
+    }
+    t.low = __ballot(low != 0) != 0;
+    if (t.low) {  // rare
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) w[i] = (w[i] >> (8 * b) & 255u) <= bound ? w[i] & ~(255u << (8 * b)) : w[i];
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -237,17 +263,35 @@ __device__ __forceinline__ int query_digits(Digits<D, T> &w, const T *row, bool 
 
 // S^T of 16 keys and 16 query rows: the products of one digit (or pair), of block scale qsc, with every 128 channels.
 template <int D> constexpr int kKPieces = D == 256 ? 2 : 1;  // 16-byte pieces of a key that a lane holds
-template <int D, class T> __device__ __forceinline__ int digit_scale(int qsc0, int n) {
-    const int qsc = qsc0 - 5 * (n * QueryShape<D, T>::kPerStep) - (D == 64 && threadIdx.x % 64 >= 32 ? 5 : 0);
-    return qsc0 == 255 ? 255 : max(qsc, 0);
+// The digits' block scales, a byte each (the instruction picks one): of the row whose digit 0 has scale qsc0.
+template <int D, class T> struct DigitScales {
+    static constexpr int W = (QueryShape<D, T>::N + 3) / 4;
+    int w[W];
+    __device__ __forceinline__ void set(int qsc0) {
+        const int first = D == 64 && threadIdx.x % 64 >= 32 ? qsc0 - 5 : qsc0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            w[i] = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                if (4 * i + b < QueryShape<D, T>::N)
+                    w[i] |= (qsc0 == 255 ? 255 : max(first - 5 * QueryShape<D, T>::kPerStep * (4 * i + b), 0)) << (8 * b);
+        }
+    }
+};
+template <int SEL> __device__ __forceinline__ f4 score_mfma(i8v a, i8v b, f4 acc, int ksc, int qsc) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 2, 0, ksc, SEL, qsc);
 }
 template <int D, class T>
-__device__ __forceinline__ f4 scores(const u4 (&k)[kKPieces<D>], const int (&ksc)[kKPieces<D>], const u6 (&q)[QueryShape<D, T>::kSteps], int qsc, f4 acc) {
+__device__ __forceinline__ f4 scores(const u4 (&k)[kKPieces<D>], const int (&ksc)[kKPieces<D>], const u6 (&q)[QueryShape<D, T>::kSteps],
+                                     const DigitScales<D, T> &qsc, int n, f4 acc) {
 #pragma unroll
     for (int u = 0; u < QueryShape<D, T>::kSteps; ++u) {
         const i8v a = {(int) k[u][0], (int) k[u][1], (int) k[u][2], (int) k[u][3], 0, 0, 0, 0};
         const i8v b = {(int) q[u][0], (int) q[u][1], (int) q[u][2], (int) q[u][3], (int) q[u][4], (int) q[u][5], 0, 0};
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 2, 0, ksc[u], 0, qsc);
+        const int w = qsc.w[n / 4];
+        acc = n % 4 == 0 ? score_mfma<0>(a, b, acc, ksc[u], w) : n % 4 == 1 ? score_mfma<1>(a, b, acc, ksc[u], w) :
+              n % 4 == 2 ? score_mfma<2>(a, b, acc, ksc[u], w) : score_mfma<3>(a, b, acc, ksc[u], w);
     }
     return acc;
 }
@@ -258,20 +302,30 @@ __device__ __forceinline__ f4 scores(const u4 (&k)[kKPieces<D>], const int (&ksc
 template <int NB> struct RowState {
     f4 o[2 * NB], l;
     float m;
+    __device__ __forceinline__ void reset() {
+        m = -INFINITY, l = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int d = 0; d < 2 * NB; ++d) o[d] = f4{0, 0, 0, 0};
+    }
 };
 
 // What a tile's scores of a row start from, so that they come as the exponents of p: the row's maximum so far, 2^8 down.
 __device__ __forceinline__ float score_origin(float m) { return kPShift - (m == -INFINITY ? 0.0f : m); }
 
-// Bits of the lane's 16 keys (base + 16 g ..) that a row at position pos sees; there: the tile's keys that exist.
-__device__ __forceinline__ uint32_t seen(int pos, int window, int base, uint64_t there) {
-    const int g = threadIdx.x % 64 / 16;
-    const int up = pos - (base + 16 * g);  // the last one
+// The positions (from, to] that a row sees; of a row that is not there (its queries are zeros and nothing of it is stored)
+// all, so that it never asks for the masked path.
+struct Sight {
+    int from, to;
+};
+__device__ __forceinline__ Sight sight(bool there, int pos, int window) {
+    return {there && window ? max(pos - window, -1) : -1, there ? pos : INT32_MAX};
+}
+// Bits of the lane's 16 keys (base + 16 g ..) that a row sees; there: the tile's keys that exist.
+__device__ __forceinline__ uint32_t seen(const Sight &w, int base, uint64_t there) {
+    const int g = threadIdx.x % 64 / 16, at = base + 16 * g;
+    const int up = w.to - at, dn = w.from + 1 - at;  // the last one, the first one
     uint32_t bits = up < 0 ? 0u : up >= 15 ? 0xffffu : (2u << up) - 1u;
-    if (window) {
-        const int dn = up - window + 1;  // the first one
-        bits = dn <= 0 ? bits : dn > 15 ? 0u : bits & (0xffffu << dn);
-    }
+    bits = dn <= 0 ? bits : dn > 15 ? 0u : bits & (0xffffu << dn);
     return bits & (uint32_t) (there >> (16 * g));
 }
 
@@ -279,7 +333,7 @@ __device__ __forceinline__ uint32_t seen(int pos, int window, int base, uint64_t
 // not see every key, a maximum that has grown, a NaN in V or a larger V scale (vkeep) are seen to first, in place: keys that
 // a row does not see become -infinity, m moves and what refers to it follows.
 template <int NB, int CT, int SPLIT>
-__device__ __forceinline__ void softmax_tile(f4 (&s)[CT][4], const int (&pos)[CT], int window, int base, const TileInfo &ti, float vkeep,
+__device__ __forceinline__ void softmax_tile(f4 (&s)[CT][4], const Sight (&see)[CT], int base, const TileInfo &ti, float vkeep,
                                              RowState<NB> (&st)[CT], h8 (&p)[CT][SPLIT][2]) {
     const int g = threadIdx.x % 64 / 16;
     const auto largest = [](const f4 (&x)[4]) {
@@ -288,20 +342,20 @@ __device__ __forceinline__ void softmax_tile(f4 (&s)[CT][4], const int (&pos)[CT
         for (int i = 2; i < 16; i += 2) top = fmaxf(fmaxf(top, x[i / 4][i % 4]), x[i / 4][i % 4 + 1]);
         return top;
     };
-    bool plain = ti.nan == 0 && vkeep == 1.0f;
+    bool plain = ti.nan == 0 && ti.there == ~0ull && vkeep == 1.0f;
 #pragma unroll
     for (int c = 0; c < CT; ++c)  // (a lane's own keys will do: one that exceeds the row's bound is found by its lane)
-        plain = plain && largest(s[c]) <= (st[c].m == -INFINITY ? -INFINITY : kPShift + kLazy) &&
-                seen(pos[c], window, base, ti.there) == 0xffffu;
+        plain = plain & (largest(s[c]) <= (st[c].m == -INFINITY ? -INFINITY : kPShift + kLazy)) & (see[c].from < base) &
+                (see[c].to >= base + kTile - 1);
     if (!__all(plain)) {
         const uint32_t nan = (uint32_t) (ti.nan >> (16 * g)) & 0xffffu;
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            const uint32_t see = seen(pos[c], window, base, ti.there);
+            const uint32_t bits = seen(see[c], base, ti.there);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[c][t][i] = see >> (4 * t + i) & 1 ? s[c][t][i] : -INFINITY;
+                for (int i = 0; i < 4; ++i) s[c][t][i] = bits >> (4 * t + i) & 1 ? s[c][t][i] : -INFINITY;
             float top = largest(s[c]);
             top = fmaxf(top, xor_lane<16>(top));
             top = fmaxf(top, xor_lane<32>(top));
@@ -311,7 +365,7 @@ __device__ __forceinline__ void softmax_tile(f4 (&s)[CT][4], const int (&pos)[CT
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[c][t][i] = see & nan & 1u << (4 * t + i) ? __builtin_nanf("") : s[c][t][i] - (now - off);
+                for (int i = 0; i < 4; ++i) s[c][t][i] = bits & nan & 1u << (4 * t + i) ? __builtin_nanf("") : s[c][t][i] - (now - off);
             st[c].m = to;
             st[c].l *= keep;
 #pragma unroll
@@ -347,7 +401,7 @@ __device__ __forceinline__ void softmax_tile(f4 (&s)[CT][4], const int (&pos)[CT
             for (int h = SPLIT - 1; h >= 0; --h) st[c].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[c][h][v], st[c].l, 0, 0, 0);
 }
 
-// Result of one row's 4 channels or, with splits, its partial.
+// Result of few rows: 4 channels of one or, with splits, their partial.
 template <int D, class T>
 __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t tok, int h, int split, int ch, f4 v) {
     if (a.splits > 1) *(f4 *) (a.part + ((split * a.b.n_tok + tok) * a.n_head + h) * D + ch) = v;
@@ -415,14 +469,56 @@ template <int D, bool SMALL> struct TileReader {
     }
 };
 
+// The second product of a tile's low blocks, in bands of kBand scales, each at a scale of its own and straight from the cache.
+template <int D, bool SMALL, int CT, int SPLIT>
+__device__ __forceinline__ void low_blocks(const AttnArgs &a, TileReader<D, SMALL> rd, const int32_t *table, int tile, const RowTiles &rt, int ev,
+                                           const h8 (&p)[CT][SPLIT][2], RowState<D / 32> (&st)[CT]) {
+    rd.ask(a, table, tile);
+    rd.take(a, tile);
+    const int at = SMALL ? (rd.row + 16 * rd.g) & (rd.P - 1) : rd.row + 16 * rd.g, key = tile * kTile + 16 * rd.g;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+        const u4 codes = rd.v_block(j);
+        const uint8_t *scale = rd.bv + KvParts<D>::v_scale(rd.P, at) + j;
+#pragma unroll 1
+        for (int top = ev - kBand; top > 0 && ev - top < 4 * kBand; top -= kBand) {  // (below: nothing that f32 sums hold)
+            f4 lo[CT], hi[CT];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) lo[c] = hi[c] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = key + 8 * v + i, e = rd.there && k >= rt.lo && k < rt.hi ? scale[(8 * v + i) * (D / 32)] : 0;
+                    w[i] = e <= top && e > max(top - kBand, 0) ? __builtin_bit_cast(float, (uint32_t) (e - top + kBias) << 23) : 0.0f;
+                }
+                h8 x, y;
+                expand_v(codes[2 * v], codes[2 * v + 1], w, x, y);
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int h = SPLIT - 1; h >= 0; --h) {
+                        lo[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, p[c][h][v], lo[c], 0, 0, 0);
+                        hi[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, p[c][h][v], hi[c], 0, 0, 0);
+                    }
+            }
+            const float unit = ldexpf(1.0f, top - ev);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) st[c].o[2 * j] += lo[c] * unit, st[c].o[2 * j + 1] += hi[c] * unit;
+        }
+    }
+}
+
 // Few rows (decode, verify): the workgroup's waves take tiles of keys in turn and are joined at the end. A wave's tile goes
 // from the pages to registers and stays there: S^T = K Q^T with K's rows in an order that leaves every lane with the 16
 // consecutive keys 16 g .. 16 g + 15 of its query row, which is where the second product, O^T = V^T P^T, wants P, and where
 // V's bytes (16 consecutive positions of a channel pair) are. Bound by the cache's bytes for long contexts and by a few
 // dependent loads for short ones. One wave issues a vector instruction about every 5 cycles where the SIMD takes one every
 // 2: what pays is waves, so the queries lie in LDS and the next tile's K is asked for when this one's is used up.
-template <int D, int CT, bool SMALL, class T>
-__global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k_attn_few(AttnArgs a) {
+// REDO: low blocks are known to be there.
+template <int D, int CT, bool SMALL, bool REDO, class T>
+__device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split) {
     constexpr int NB = D / 32, SPLIT = sizeof(T) == 4 ? 2 : 1, NW = kFewWaves;
     constexpr int kScale = 64 * NB + 16 * NB, kJoin = NW / 2 * CT * 2 * NB * 256;
     __shared__ __align__(16) float lds[NW * kScale > kJoin ? NW * kScale : kJoin];
@@ -430,8 +526,9 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
     __shared__ __align__(16) uint2 qs[CT][Q::N][Q::kSteps][64][3];
     __shared__ int qscale[CT][16];
     __shared__ float join[NW][2][CT * 16];
-    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, row0 = blockIdx.y * 16 * CT, split = blockIdx.z;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     const SeqRange sr = seq_range(a.b, s);
     const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) INT32_MAX);
     if (row0 >= rows) return;
@@ -446,15 +543,17 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
     rd.P = P, rd.lane = lane, rd.r = r, rd.g = g, rd.head_off = head * kv_head_bytes(D, P);
     u4 kraw[4][kKPieces<D>], vraw[NB];
     ScaleBytes<NB> swk, swv;  // the scale bytes of the lane's key
-    int tile = t0 + wave;
     const int32_t *table = a.b.table + s * a.b.table_stride;
     rd.last = (int) a.b.table_stride - 1;
-    if (tile < t1) {
+    const auto begin = [&] {
+        const int tile = t0 + wave;
+        if (tile >= t1) return;
         rd.ask(a, table, tile);
         rd.take(a, tile);
         rd.ask(a, table, min(tile + NW, t1 - 1));
         rd.scales(swk, swv), rd.k(kraw), rd.v(vraw);
-    }
+    };
+    begin();
 
     if (wave < CT) {  // a wave a column tile
         const int row = row0 + 16 * wave + r, i = row / a.group;
@@ -470,95 +569,114 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
         if (g == 0) qscale[wave][r] = scale;
     }
     RowState<NB> st[CT];
-    int pos[CT];
+    Sight see[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         const int row = row0 + 16 * c + r;
-        pos[c] = row < rows ? sr.len - sr.n + row / a.group : -1;
-        st[c].m = -INFINITY, st[c].l = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int d = 0; d < 2 * NB; ++d) st[c].o[d] = f4{0, 0, 0, 0};
+        see[c] = sight(row < rows, sr.len - sr.n + row / a.group, a.window);
     }
     __syncthreads();
-    int qsc[CT];
+    DigitScales<D, T> qsc[CT];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) qsc[c] = qscale[c][r];
+    for (int c = 0; c < CT; ++c) qsc[c].set(qscale[c][r]);
 
     float *vsc = lds + wave * kScale;
     uint8_t *ksb = (uint8_t *) (vsc + 64 * NB);  // K's scale bytes, [64 keys][NB]
     int ev = 1;
-    for (; tile < t1; tile += NW) {
-        const int base = tile * kTile, key = base + lane;
-        *(ScaleBytes<NB> *) (ksb + lane * NB) = swk;
-        const TileInfo ti = v_scales<NB>(swv, rd.there && key >= rt.lo && key < rt.hi, ev, vsc);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        int ksc[4][kKPieces<D>];
+    // Returns whether there were low blocks; with `all`, they are added.
+    const auto walk = [&](auto all) {
+        bool low = false;
+        ev = 1;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int c = 0; c < CT; ++c) st[c].reset();
+        for (int tile = t0 + wave; tile < t1; tile += NW) {
+            const int base = tile * kTile, key = base + lane;
+            *(ScaleBytes<NB> *) (ksb + lane * NB) = swk;
+            const TileInfo ti = v_scales<NB>(swv, rd.there && key >= rt.lo && key < rt.hi, ev, vsc);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            int ksc[4][kKPieces<D>];
 #pragma unroll
-            for (int u = 0; u < kKPieces<D>; ++u) ksc[t][u] = ksb[(16 * (r / 4) + 4 * t + r % 4) * NB + (D == 64 ? g & 1 : g) + 4 * u];
-        f4 sc[CT][4];
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+                for (int u = 0; u < kKPieces<D>; ++u) ksc[t][u] = ksb[(16 * (r / 4) + 4 * t + r % 4) * NB + (D == 64 ? g & 1 : g) + 4 * u];
+            f4 sc[CT][4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) sc[c][t] = f4{1, 1, 1, 1} * score_origin(st[c].m);
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int n = 0; n < Q::N; ++n)  // the largest digit first: the rest adds to small numbers
+                for (int t = 0; t < 4; ++t) sc[c][t] = f4{1, 1, 1, 1} * score_origin(st[c].m);
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                u6 q[Q::kSteps];
+            for (int n = 0; n < Q::N; ++n)  // the largest digit first: the rest adds to small numbers
 #pragma unroll
-                for (int u = 0; u < Q::kSteps; ++u)
+                for (int c = 0; c < CT; ++c) {
+                    u6 q[Q::kSteps];
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) {
-                        const uint2 w = qs[c][n][u][lane][i];
-                        q[u][2 * i] = w.x, q[u][2 * i + 1] = w.y;
-                    }
+                    for (int u = 0; u < Q::kSteps; ++u)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q, digit_scale<D, T>(qsc[c], n), sc[c][t]);
+                        for (int i = 0; i < 3; ++i) {
+                            const uint2 w = qs[c][n][u][lane][i];
+                            q[u][2 * i] = w.x, q[u][2 * i + 1] = w.y;
+                        }
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q, qsc[c], n, sc[c][t]);
+                }
+            // K is used up here, before the next tile's is asked for: the products may not sink below the loads, which would
+            // keep both tiles' registers
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(sc[c][t]));
+            __builtin_amdgcn_sched_barrier(0);
+            // (the last tile is asked for once more behind the end: it is in the cache, and the loop has no branch)
+            rd.take(a, min(tile + NW, t1 - 1));
+            rd.ask(a, table, min(tile + 2 * NW, t1 - 1));
+            rd.scales(swk, swv), rd.k(kraw);
+            const float vkeep = ldexpf(1.0f, ev - ti.ev);
+            ev = ti.ev;
+            h8 p[CT][SPLIT][2];
+            softmax_tile<NB, CT, SPLIT>(sc, see, base, ti, vkeep, st, p);
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    h8 lo, hi;
+                    float w[8];
+                    *(f4 *) w = *(const f4 *) (vsc + j * 64 + 16 * g + 8 * v);
+                    *(f4 *) (w + 4) = *(const f4 *) (vsc + j * 64 + 16 * g + 8 * v + 4);
+                    expand_v(vraw[j][2 * v], vraw[j][2 * v + 1], w, lo, hi);
+#pragma unroll
+                    for (int c = 0; c < CT; ++c)
+#pragma unroll
+                        for (int h = SPLIT - 1; h >= 0; --h) {
+                            st[c].o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, p[c][h][v], st[c].o[2 * j], 0, 0, 0);
+                            st[c].o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, p[c][h][v], st[c].o[2 * j + 1], 0, 0, 0);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);  // (one step's operands at a time: the registers are counted)
+                }
+            if constexpr (all) {
+                if (ti.low) low_blocks<D, SMALL>(a, rd, table, tile, rt, ev, p, st);
+            } else {
+                low |= ti.low;
             }
-        // K is used up here, before the next tile's is asked for: the products may not sink below the loads, which would
-        // keep both tiles' registers
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(sc[c][t]));
-        __builtin_amdgcn_sched_barrier(0);
-        // (the last tile is asked for once more behind the end: it is in the cache, and the loop has no branch)
-        rd.take(a, min(tile + NW, t1 - 1));
-        rd.ask(a, table, min(tile + 2 * NW, t1 - 1));
-        rd.scales(swk, swv), rd.k(kraw);
-        const float vkeep = ldexpf(1.0f, max(ev - ti.ev, -126));
-        ev = ti.ev;
-        h8 p[CT][SPLIT][2];
-        softmax_tile<NB, CT, SPLIT>(sc, pos, a.window, base, ti, vkeep, st, p);
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                h8 lo, hi;
-                float w[8];
-                *(f4 *) w = *(const f4 *) (vsc + j * 64 + 16 * g + 8 * v);
-                *(f4 *) (w + 4) = *(const f4 *) (vsc + j * 64 + 16 * g + 8 * v + 4);
-                expand_v(vraw[j][2 * v], vraw[j][2 * v + 1], w, lo, hi);
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-#pragma unroll
-                    for (int h = SPLIT - 1; h >= 0; --h) {
-                        st[c].o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, p[c][h][v], st[c].o[2 * j], 0, 0, 0);
-                        st[c].o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, p[c][h][v], st[c].o[2 * j + 1], 0, 0, 0);
-                    }
-                __builtin_amdgcn_sched_barrier(0);  // (one step's operands at a time: the registers are counted)
-            }
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int d = 0; d < 2 * NB; ++d) asm volatile("" : "+v"(st[c].o[d]));  // (and V likewise)
-        rd.v(vraw);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+                for (int d = 0; d < 2 * NB; ++d) asm volatile("" : "+v"(st[c].o[d]));  // (and V likewise)
+            rd.v(vraw);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+        return low;
+    };
+    if (REDO || walk(std::false_type{})) {
+        if (!REDO) {
+            // (so that nothing of its addresses is kept through the first walk)
+            asm volatile("" : "+v"(lane), "+v"(r), "+v"(g));
+            rd.lane = lane, rd.r = r, rd.g = g;
+            begin();
+        }
+        walk(std::true_type{});
     }
 
     // join the waves: the common maximum and sum of every row, then the sums in a tree over registers of equal layout
@@ -614,11 +732,29 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
         if (a.splits > 1 && g == 0) a.part_ml[(split * a.b.n_tok + tok) * a.n_head + h] = make_float2(top[c], sum[c]);
     }
 }
+template <int D, int CT, bool SMALL, class T>
+__global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k_attn_few(AttnArgs a) {
+    few_rows<D, CT, SMALL, false, T>(a, blockIdx.y * 16 * CT, blockIdx.z);
+}
+// The rows of k_attn_many's workgroups that met low blocks: none as a rule, which takes 4-5 us with the launch. In one
+// workgroup with the pass that found them, their scalars cost the f32 form's loop its registers (29 spilled instead of 9).
+template <int D, bool SMALL, class T>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void k_attn_redo(AttnArgs a, int row_tiles) {
+    for (int tile = blockIdx.y; tile < row_tiles; tile += gridDim.y) {
+        if (!((const uint32_t *) a.redo)[(int64_t) blockIdx.x * row_tiles + tile]) continue;
+        for (int sub = 0; sub < kManyRows / 16; ++sub) {
+            few_rows<D, 1, SMALL, true, T>(a, tile * kManyRows + 16 * sub, 0);
+            __syncthreads();
+        }
+    }
+}
 
 // Many rows (prompts): a workgroup takes 128 rows, 32 a wave, and walks over the keys; its waves expand a tile's V together,
 // a tile ahead, into LDS as the second product wants it, [channel][64 keys] (rows 16 bytes apart in banks: a lane's 16-byte
 // reads of 16 channels touch every bank once). K needs no expansion: each wave reads its codes, which the workgroup's first
-// reader brings into L1, and keeps them in registers with the digits of its queries. Bound by the vector pipe's work on the
+// reader brings into L1, and keeps them in registers with the digits of its queries. A workgroup that meets low blocks leaves
+// them out and says so: its rows are then done again by the form of few rows (with low blocks in this loop, 4096 tokens at
+// 4096 took 539 us instead of 423). Bound by the vector pipe's work on the
 // scores, about 6 instructions each where the two products take as long for bf16.
 __device__ __forceinline__ void tile_barrier() {
     // LDS only: the tiles asked for stay in flight
@@ -635,19 +771,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     __shared__ __align__(16) _Float16 vt[2][D * VS];
     __shared__ __align__(16) float vsc_all[NW][MB * 64];
     __shared__ __align__(16) uint8_t ksb_all[NW][64 * NB];
-    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, split = blockIdx.z;
+    __shared__ Sight sights[NW][CT][16];  // (the registers are counted)
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     const SeqRange sr = seq_range(a.b, s);
     const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) INT32_MAX);
     // the last rows, which see the most keys, first
     const int row0 = ((int) gridDim.y - 1 - (int) blockIdx.y) * kManyRows;
-    if (row0 >= rows) return;
+    uint8_t *redo = a.redo + ((int64_t) blockIdx.x * gridDim.y + row0 / kManyRows) * NW + wave;
+    if (row0 >= rows) {
+        if (lane == 0) *redo = 0;
+        return;
+    }
     const RowTiles rt = row_tiles(a, sr, row0, kManyRows);
-    const int chunk = split_chunk(a, rt);
-    const int t0 = (int) min((int64_t) rt.t0 + (int64_t) split * chunk, (int64_t) rt.t1);
-    const int t1 = min(t0 + chunk, rt.t1);
-    if (split > 0 && t0 >= t1) return;  // (split 0 of an empty range writes the zeros)
-    const int P = 1 << a.c.shift, first = sr.len - sr.n;
+    const int t0 = rt.t0, t1 = rt.t1, P = 1 << a.c.shift, first = sr.len - sr.n;
     float *vsc = vsc_all[wave];
     uint8_t *ksb = ksb_all[wave];
 
@@ -686,6 +823,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         __builtin_amdgcn_wave_barrier();
     };
     int ev = 1;
+    int low = 0;
     TileInfo ti{}, next{};
     if (t0 < t1) {
         rv.ask(a, table, t0), rk.ask(a, table, t0);
@@ -695,8 +833,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     }
     Digits<D, T> q[CT];
     RowState<NB> st[CT];
-    int pos[CT];
-    int qsc[CT];
+    DigitScales<D, T> qsc[CT];
     const int w0 = row0 + wave * 32;  // the wave's rows, and the positions that they see at most and at least
     const int most = w0 < rows ? first + min(w0 + 31, rows - 1) / a.group : -1;
     const int least = a.window ? first + w0 / a.group - a.window + 1 : 0;
@@ -704,11 +841,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     for (int c = 0; c < CT; ++c) {
         const int row = w0 + 16 * c + r, i = row / a.group;
         const bool there = row < rows;
-        pos[c] = there ? first + i : -1;
-        qsc[c] = query_digits<D, T>(q[c], (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D, there, a.scale);
-        st[c].m = -INFINITY, st[c].l = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int d = 0; d < 2 * NB; ++d) st[c].o[d] = f4{0, 0, 0, 0};
+        if (g == 0) sights[wave][c][r] = sight(there, first + i, a.window);
+        qsc[c].set(query_digits<D, T>(q[c], (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D, there, a.scale));
+        st[c].reset();
     }
     if (t0 < t1) {
         const int key = t0 * kTile + lane;
@@ -742,7 +877,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q[c][n], digit_scale<D, T>(qsc[c], n), sc[c][t]);
+                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q[c][n], qsc[c], n, sc[c][t]);
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -753,10 +888,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         rk.ask(a, table, min(tile + 2, t1 - 1));
         rk.scales(swk, unused), rk.k(kraw);
         if (active) {
-            const float vkeep = ldexpf(1.0f, max(ev - ti.ev, -126));
+            const float vkeep = ldexpf(1.0f, ev - ti.ev);
             ev = ti.ev;
             h8 p[CT][SPLIT][2];
-            softmax_tile<NB, CT, SPLIT>(sc, pos, a.window, base, ti, vkeep, st, p);
+            Sight see[CT];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) see[c] = sights[wave][c][r];
+            softmax_tile<NB, CT, SPLIT>(sc, see, base, ti, vkeep, st, p);
             const h8 *at = (const h8 *) (vt[buf] + r * VS + 16 * g);
 #pragma unroll
             for (int d = 0; d < 2 * NB; ++d)
@@ -778,9 +916,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         rv.take(a, min(tile + 2, t1 - 1));
         rv.scales(unused, swv), load_v();
         rv.ask(a, table, min(tile + 3, t1 - 1));
+        low |= (int) ti.low;
         ti = next;
         tile_barrier();
     }
+    if (lane == 0) *redo = low;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         const int row = w0 + 16 * c + r;
@@ -788,7 +928,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         const int64_t tok = sr.q0 + row / a.group;
         const int h = head * a.group + row % a.group;
         float sum = st[c].l[0], off = st[c].m;
-        if (a.splits == 1 && a.sinks) {
+        if (a.sinks) {
             const float sk = a.sinks[h] * kLog2e;
             off = fmaxf(off, sk);
             const float o = off == -INFINITY ? 0.0f : off;
@@ -797,8 +937,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         const float o = off == -INFINITY ? 0.0f : off;
         const float f = sum == 0.0f ? 0.0f : ldexpf(__builtin_amdgcn_exp2f(st[c].m - o) / sum, ev - kBias);
 #pragma unroll
-        for (int d = 0; d < 2 * NB; ++d) store_row<D, T>(a, tok, h, split, 16 * d + 4 * g, st[c].o[d] * f);
-        if (a.splits > 1 && g == 0) a.part_ml[(split * a.b.n_tok + tok) * a.n_head + h] = make_float2(st[c].m, sum);
+        for (int d = 0; d < 2 * NB; ++d) store4((T *) a.out + tok * a.out_stride + (int64_t) h * D + 16 * d + 4 * g, st[c].o[d] * f);
     }
 }
 
@@ -879,19 +1018,26 @@ struct Plan {
 };
 Plan attn_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
     Plan p{};
-    const int64_t rows = (int64_t) b->max_q * (x->n_head / c->n_head_kv);
-    p.rows = rows > kFewRows ? kManyRows : rows <= 16 || c->head_dim == 256 ? 16 : 32;
-    p.row_tiles = (int) ((rows + p.rows - 1) / p.rows);
-    const int64_t wgs = std::max<int64_t>(1, (int64_t) b->n_seq * c->n_head_kv * p.row_tiles);
-    const int64_t tiles = std::max<int64_t>(1, (b->max_kv + kTile - 1) / kTile);
+    const int64_t rows = std::min<int64_t>(b->max_q, b->n_tok) * (x->n_head / c->n_head_kv);  // of a sequence and kv head
     const auto per = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
+    // The form of few rows reads K and V once for 32 rows instead of 128, but has more workgroups. It is ahead up to 64 rows
+    // (64 sequences of 600 keys, 64 rows of 8 heads: 45 us against 51; 128 rows: 79 against 60), and wherever the other form
+    // leaves CUs idle: less than two workgroups a CU of it (256 tokens behind 1024 keys, 1024 rows of 8 heads: 26 us against
+    // 34 with 64 workgroups; 1024 tokens: 68 against 95 with 256; 2048 tokens: 145 against the few-row form's 168 with 512).
+    const int64_t heads = (int64_t) b->n_seq * c->n_head_kv;
+    const bool many = rows > kFewRows && heads * per(rows, kManyRows) >= 512;
+    p.rows = many ? kManyRows : rows <= 16 || c->head_dim == 256 ? 16 : 32;
+    p.row_tiles = (int) ((rows + p.rows - 1) / p.rows);
+    const int64_t wgs = std::max<int64_t>(1, heads * p.row_tiles);
+    const int64_t tiles = std::max<int64_t>(1, (b->max_kv + kTile - 1) / kTile);
+    // A split costs its join and a second start, 4-6 us; a workgroup alone on a CU is within a tenth of two or three on its
+    // rate. So: splits until 512 workgroups where there are fewer than 256 (131072 keys of 8 heads: 32 us with 512, 37 with
+    // 256; 64 sequences of 4096, 512 workgroups: 58 whole, 66 in two), of four tiles
+    // (one a wave) at least, and none at all below 13 tiles (500 keys: 9.2 whole, 10.9 in two). Beyond that, pieces of 40
+    // tiles, up to 2304, so that the longest of unequal sequences does not run on alone (48 of up to 16000
+    // keys: 74 us with 2304, 94 with 512).
     int64_t splits = 1;
-    if (p.rows == kManyRows) {
-        splits = std::min(per(512, wgs), tiles / 8);
-    } else if (tiles > 12) {
-        splits = std::max(per(p.rows == 16 && c->head_dim <= 128 ? 768 : 512, wgs), std::min(per(tiles, 40), per(2304, wgs)));
-        splits = std::min(splits, per(tiles, kFewWaves));
-    }
+    if (!many && tiles > 12) splits = std::max(wgs < 256 ? std::min(per(512, wgs), per(tiles, 4)) : 1, std::min(tiles / 40, per(2304, wgs)));
     p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(splits, 64));
     p.chunk = (int) per(tiles, p.splits);
     if (p.splits > 1) {
@@ -899,6 +1045,7 @@ Plan attn_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
         p.ml_off = n * c->head_dim * 4;
         p.bytes = p.ml_off + n * 8;
     }
+    if (many) p.bytes = (size_t) (heads * p.row_tiles) * 4;  // a byte a wave: whether the rows are to be done again
     return p;
 }
 
@@ -917,6 +1064,8 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
     if (b->n_seq == 0 || b->n_tok == 0 || b->max_q == 0) return host::OK;
     if (!q || !out) return host::set_error(host::ERR_SHAPE, "attn: null argument");
     const Plan p = attn_plan(c, b, x);
+    if (p.row_tiles > 65535)
+        return host::set_error(host::ERR_SHAPE, "attn: %lld tokens of a sequence in one call are too many", (long long) std::min<int64_t>(b->max_q, b->n_tok));
     if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t) ws & 15)))
         return host::set_error(host::ERR_NOMEM, "attn: workspace of %zu bytes, %zu needed (16-byte aligned)", ws ? ws_bytes : 0, p.bytes);
     AttnArgs a{};
@@ -926,7 +1075,8 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
     a.q_stride = x->q_stride, a.out_stride = x->out_stride;
     a.n_head = x->n_head, a.group = x->n_head / c->n_head_kv, a.window = x->window;
     a.splits = p.splits, a.chunk = p.chunk, a.scale = x->scale;
-    const dim3 grid((unsigned) (b->n_seq * c->n_head_kv), (unsigned) p.row_tiles, (unsigned) p.splits);
+    a.redo = (uint8_t *) ws;
+    const dim3 grid((unsigned) ((int64_t) b->n_seq * c->n_head_kv), (unsigned) p.row_tiles, (unsigned) p.splits);
     const bool small = c->page_size < kTile;
     auto few = [&](auto dim, auto ct, auto type) {
         constexpr int D = decltype(dim)::value, CT = decltype(ct)::value;
@@ -935,7 +1085,7 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
     };
     auto join = [&](auto dim, auto type) {
         constexpr int D = decltype(dim)::value;
-        const int64_t rows = (int64_t) b->max_q * x->n_head;
+        const int64_t rows = std::min<int64_t>(b->max_q, b->n_tok) * x->n_head;
         // a workgroup a row as long as all of them are resident at once
         if (rows * b->n_seq <= 2048)
             hipLaunchKernelGGL((k_attn_join<D, false, decltype(type)>), dim3((unsigned) rows, (unsigned) b->n_seq), dim3(256), 0, st, a, p.rows);
@@ -947,6 +1097,10 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
         if (p.rows == kManyRows) {
             if (small) hipLaunchKernelGGL((k_attn_many<D, true, decltype(type)>), grid, dim3(256), 0, st, a);
             else hipLaunchKernelGGL((k_attn_many<D, false, decltype(type)>), grid, dim3(256), 0, st, a);
+            FNS_TRY(host::check_launch("attn"));
+            const dim3 some(grid.x, std::min(grid.y, (512 + grid.x - 1) / grid.x));
+            if (small) hipLaunchKernelGGL((k_attn_redo<D, true, decltype(type)>), some, dim3(64 * kFewWaves), 0, st, a, p.row_tiles);
+            else hipLaunchKernelGGL((k_attn_redo<D, false, decltype(type)>), some, dim3(64 * kFewWaves), 0, st, a, p.row_tiles);
         } else if constexpr (D == 256) few(dim, std::integral_constant<int, 1>{}, type);
         else if (p.rows == 16) few(dim, std::integral_constant<int, 1>{}, type);
         else few(dim, std::integral_constant<int, 2>{}, type);

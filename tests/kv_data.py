@@ -95,11 +95,11 @@ class Pages:
 
 
 def attention(cache: Pages, table: np.ndarray, q_lens, kv_lens, q: np.ndarray, scale: float, window: int = 0, sinks=None):
-    """(out f64 [sum q][H][D], tol_x, vmax): the result, and for the tolerances per row scale * max_j sum_i |q_i K_ji| and
-    max |V| over what the row sees."""
+    """(out f64 [sum q][H][D], ax [sum q][H][2], vm): the result, and for the tolerances per row scale * max_j sum_i |q_i K_ji|
+    and scale * max_i |q_i| * max_j sum_i |K_ji|, and max |V|, over what the row sees."""
     H, D = q.shape[1], q.shape[2]
     G = H // cache.heads
-    out, ax, vm, t = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape[:2]), 0
+    out, ax, vm, t = np.zeros(q.shape), np.zeros((*q.shape[:2], 2)), np.zeros(q.shape[:2]), 0
     for s, (n, kv) in enumerate(zip(q_lens, kv_lens)):
         for h in range(cache.heads if n else 0):
             pos = np.arange(kv)
@@ -121,20 +121,25 @@ def attention(cache: Pages, table: np.ndarray, q_lens, kv_lens, q: np.ndarray, s
                     out[t + i, hh] = w @ v / (w.sum() + (np.exp(sinks[hh] - m) if sinks is not None else 0.0))
                     if np.isnan(k).any() or np.isnan(v).any():
                         out[t + i, hh] = np.nan
-                    ax[t + i, hh] = scale * (np.abs(k) @ np.abs(q[t + i, hh])).max()
+                    aq, ak = np.abs(q[t + i, hh]), np.abs(k)
+                    ax[t + i, hh] = scale * (ak @ aq).max(), scale * aq.max() * ak.sum(-1).max()
                     vm[t + i, hh] = np.abs(v).max()
         t += n
     return out, ax, vm
 
 
 def attn_tolerance(dtype: str, D: int, n: int, ref: np.ndarray, ax: np.ndarray, vm: np.ndarray) -> np.ndarray:
-    """What rounding allows, per element. A score's products carry q to 2^-21 (two 11-bit parts; bf16 q is exact) and their
-    f32 sum of D (+ 8 for scaling) terms at most D + 8 half steps, each relative to scale * sum |q_i K_i| = ax; exp2's
-    argument and result add 4 half steps of |x| <= ax and of 1. A probability that is off by the factor 1 + r moves the
-    output by at most 2 r vmax (numerator and denominator). p itself is carried to 2^-21 (f32) or 2^-11 (bf16), sums over n
-    keys by n half steps at worst; the result is rounded to its type."""
-    h = F32_STEP
-    x = ax * ((0 if dtype == "bf16" else 2.0 ** -21) + (D + 12) * h)
-    r = x + 4 * h + n * h + (2.0 ** -11 if dtype == "bf16" else 2.0 ** -21)
-    out = BF16_STEP if dtype == "bf16" else 4 * h
+    """What rounding allows, per element. A query row enters the products as a sum of 5 (f32) or 3 (bf16) e2m3 digits, each 32
+    times finer than the one before: with the largest element in [2, 4) the first digit leaves 1/8 (half of a step of 1/4),
+    each further one 1/32 of that, so 2^-3 2^-20 <= 2^-24 of the largest (2^-3 2^-10 <= 2^-14): a score is off by that times
+    scale * max |q_i| * sum |K_i| = ax[1]. Multiplying the row by scale * log2(e) costs two half steps, its products are exact,
+    and their f32 sums, one instruction a digit and 128 channels, are given D + 8 half steps of scale * sum |q_i K_i| = ax[0]
+    (which bounds the running maximum that they start from, too); exp2's argument and result add 4 half steps of |x| <= ax[0]
+    and of 1. A probability that is off by the factor 1 + r moves the output by at most 2 r vmax (numerator and denominator).
+    p itself is carried to 2^-21 (f32) or 2^-10 (bf16: 11 bits, toward zero; the sum of p counts the same values, which
+    leaves what differs from key to key), sums over n keys by n half steps at worst; the result is rounded to its type."""
+    h, bf16 = F32_STEP, dtype == "bf16"
+    x = ax[..., 0] * (D + 14) * h + ax[..., 1] * 2.0 ** (-14 if bf16 else -24)
+    r = x + 4 * h + n * h + 2.0 ** (-11 if bf16 else -21)
+    out = BF16_STEP if bf16 else 4 * h
     return 2 * (r * vm)[..., None] + np.abs(ref) * out + 1e-37

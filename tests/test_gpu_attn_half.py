@@ -268,8 +268,9 @@ def _check_attn(s: Setup, group: int, dtype: str, window: int = 0, sinks: bool =
     got = got[: s.tok]
     assert np.array_equal(np.isnan(got), np.isnan(ref))
     tol = kd.attn_tolerance(dtype, s.dim, max(s.kv_lens + [1]), ref, ax, vm)
-    fine = ~np.isnan(ref)
-    bad = fine & ~(np.abs(got - ref) <= tol)
+    far = np.abs(ref) >= 2.0 ** 128  # codes of scale 254 stand for up to 6 * 2^127, which f32 has as an infinity
+    assert np.array_equal(got[far], np.copysign(np.inf, ref[far]))
+    bad = ~np.isnan(ref) & ~far & ~(np.abs(got - ref) <= tol)
     assert not bad.any(), f"{bad.sum()} of {bad.size} off, worst {np.nanmax(np.abs(got - ref) / tol):.3g} of the tolerance"
     return q, out
 
@@ -304,6 +305,64 @@ def test_attn_decode_ragged(group, window, sinks, dtype):
 ])
 def test_attn_many_tokens(dim, page, heads_kv, group, q_lens, kv_lens, window, sinks, dtype):
     _check_attn(Setup(q_lens, kv_lens, page, heads_kv, dim, seed=dim + group, pad=1), group, dtype, window, sinks)
+
+
+MANY_ROWS = 65536  # rows a sequence at most, by the batch's numbers: what a prompt's workgroups are for
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,page,heads_kv,group,q_lens,kv_lens,window,sinks", [
+    (128, 16, 2, 4, [4, 2, 3], [4, 130, 67], 0, False),
+    (64, 32, 1, 8, [5, 8, 1, 0], [300, 8, 64, 20], 33, True),
+    (256, 64, 1, 3, [7, 60], [200, 60], 0, True),
+    (64, 64, 2, 8, [70], [70], 0, False),
+    (128, 64, 1, 4, [65, 1, 130], [65, 900, 401], 0, True),
+    (128, 16, 1, 7, [33, 90], [200, 90], 40, False),
+    (256, 32, 2, 2, [100], [333], 64, True),
+    (64, 16, 1, 1, [257], [300], 0, False),
+    (128, 256, 1, 40, [9], [77], 1, False),
+])
+def test_attn_in_a_prompts_workgroups(dim, page, heads_kv, group, q_lens, kv_lens, window, sinks, dtype):
+    """The same sequences in a batch that is padded to many rows."""
+    s = Setup(q_lens, kv_lens, page, heads_kv, dim, seed=dim + group, pad=MANY_ROWS // group)
+    s.batch.desc.max_q = s.n_tok
+    _check_attn(s, group, dtype, window, sinks)
+
+
+@pytest.mark.parametrize("q,many", [(4, False), (50, False), (50, True), (150, True)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attn_odd_places_in_a_prompts_workgroups(q, many, dtype):
+    """NaNs, missing pages and freed ones before a window, and scores of hundreds, in either form."""
+    s = Setup([q, 1], [400, 64], 16, 1, 64, seed=61, pad=MANY_ROWS // 4 if many else 0)
+    s.batch.desc.max_q = s.n_tok if many else q
+    h, first = s.host, 400 - q - 100 + 1
+    s.table[0, : first // 16] = np.array([-1, 1 << 30, h.n_pages] * 20)[: first // 16]
+    s.table[0, 20] = -1
+    for pos, off in ((399 - q // 2, 0), (399 - q // 3, 32), (first - 1, 0), (first - 1, 32)):
+        page = s.table[0, pos // 16]
+        if 0 <= page < h.n_pages:
+            h.raw[page, 16 * 64 + off + pos % 16 * 2] = 255
+    s.cache.pages.copy_(torch.from_numpy(h.raw.copy()).view(s.cache.pages.shape))
+    s.batch.page_table.copy_(torch.from_numpy(s.table))
+    _check_attn(s, 4, dtype, window=100, std=20.0)
+
+
+@pytest.mark.parametrize("scale", [160, 166, 200, 250, 254])
+@pytest.mark.parametrize("q,many", [(3, False), (50, False), (50, True), (140, True)])
+def test_attn_a_huge_block_of_v_is_nothing_to_rows_that_do_not_see_it(q, many, scale):
+    """V of two tokens in the middle far above everything else, and of one block far below: the rows before them, and with
+    the window those behind, keep the precision of what they see."""
+    s = Setup([q, q], [q + 30, q + 200], 32, 2, 64, seed=scale, pad=MANY_ROWS // 4 if many else 0)
+    s.batch.desc.max_q = s.n_tok if many else q
+    h = s.host
+    for seq in (0, 1):
+        for pos, block, e in ((s.kv_lens[seq] - 1 - q // 2, 0, scale), (s.kv_lens[seq] - 2 - q // 2, 1, scale - 20), (3, 1, 60)):
+            for head in (0, 1):
+                at = head * h.head_bytes + 32 * 64 + 32 * 2 + pos % 32 * 2 + block
+                h.raw[s.table[seq, pos // 32], at] = e
+    s.cache.pages.copy_(torch.from_numpy(h.raw.copy()).view(s.cache.pages.shape))
+    _check_attn(s, 4, "f32")
+    _check_attn(s, 4, "f32", window=q // 4 + 1)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
