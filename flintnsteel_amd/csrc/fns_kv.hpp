@@ -77,16 +77,17 @@ __device__ __forceinline__ float kv_value(int code, int e) {
 }
 
 // Scale byte of a block whose largest magnitude is amax (finite): the rule above.
-__device__ __forceinline__ int kv_scale_of(double amax) {
-    if (amax == 0.0) return 0;
+template <class F> __device__ __forceinline__ int kv_scale_of(F amax) {
+    if (amax == 0) return 0;
     int k;
-    const double m = frexp(amax, &k);  // amax = m 2^k, m in [.5, 1)
-    return min(max(k + 124 + (m > 0.875 ? 1 : 0), 1), 254);
+    const F m = frexp(amax, &k);  // amax = m 2^k, m in [.5, 1)
+    return min(max(k + 124 + (m > (F) 0.875 ? 1 : 0), 1), 254);
 }
 // Code of a value x, of which a = |x| in units of the block's scale.
-__device__ __forceinline__ uint32_t kv_code(double x, double a) {
-    const uint32_t c = (uint32_t) (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5.0);
-    return c | (x < 0.0 ? 8u : 0u);
+template <class F> __device__ __forceinline__ uint32_t kv_code(F x, F a) {
+    const uint32_t c = (uint32_t) (a > (F) 0.25) + (a >= (F) 0.75) + (a > (F) 1.25) + (a >= (F) 1.75) + (a > (F) 2.5) + (a >= (F) 3.5) +
+                       (a > (F) 5);
+    return c | (x < 0 ? 8u : 0u);
 }
 
 }  // namespace fns::dev

@@ -35,13 +35,6 @@ struct AppendArgs {
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(uint16_t x) { return __builtin_bit_cast(float, (uint32_t) x << 16); }
 
-// Eight consecutive elements at any alignment of an element.
-template <class T> __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-    T t[8];
-    __builtin_memcpy(t, p, sizeof t);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32(t[i]);
-}
 __device__ __forceinline__ uint16_t to_bf16(float x) {  // nearest, ties to even; NaN stays NaN
     const uint32_t u = __builtin_bit_cast(uint32_t, x);
     if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t) ((u >> 16) | 0x40u);
@@ -60,51 +53,66 @@ __device__ __forceinline__ void store8(uint16_t *p, const double (&v)[8]) {
     __builtin_memcpy(p, t, sizeof t);
 }
 
-// Channels ch .. ch + 7 of a head's row after the rotation. cs: the token's (cos, sin) of every pair.
+// Channels ch .. ch + 7 of a head's row, at any alignment of an element: asked for in one place and turned in another, with
+// the loads' latency between. Where halves turn against each other, the partners are another lane's of the same row.
+template <class T> struct Row8 {
+    T x[8];
+    __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(x, p, sizeof x); }
+};
+// After the rotation; cs: the token's (cos, sin) of every pair. All lanes of the row take part.
 template <int ROPE, class T>
-__device__ __forceinline__ void rotated8(const T *row, int ch, int rope_dim, const double2 *cs, double (&o)[8]) {
-    float x[8];
-    load8(row + ch, x);
-    if (ROPE == FNS_ROPE_NONE || ch >= rope_dim) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = x[i];
-        if (ROPE == FNS_ROPE_NONE || ch >= rope_dim) return;
-    }
+__device__ __forceinline__ void rotated(const Row8<T> &v, int ch, int rope_dim, const double2 *cs, double (&o)[8]) {
+    const bool turns = ch < rope_dim, second = ch >= rope_dim / 2;
     if constexpr (ROPE == FNS_ROPE_PAIRS) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-            const double2 t = cs[(ch + i) / 2];
-            o[i] = x[i] * t.x - x[i + 1] * t.y;
-            o[i + 1] = x[i] * t.y + x[i + 1] * t.x;
+            const double2 t = turns ? cs[(ch + i) / 2] : make_double2(1.0, 0.0);
+            const double a = to_f32(v.x[i]), b = to_f32(v.x[i + 1]);
+            o[i] = turns ? a * t.x - b * t.y : a;
+            o[i + 1] = turns ? a * t.y + b * t.x : b;
         }
     } else if constexpr (ROPE == FNS_ROPE_HALVES) {
-        const int half = rope_dim / 2;
-        const bool second = ch >= half;
-        float y[8];
-        load8(row + (second ? ch - half : ch + half), y);
+        const int lane = threadIdx.x % 64, other = 4 * (!turns ? lane : second ? lane - rope_dim / 16 : lane + rope_dim / 16);
+        constexpr int N = sizeof(v.x) / 4;
+        int w[N];
+        T y[8];
+        __builtin_memcpy(w, v.x, sizeof w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = __builtin_amdgcn_ds_bpermute(other, w[i]);
+        __builtin_memcpy(y, w, sizeof w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const double2 t = cs[ch + i - (second ? half : 0)];
-            o[i] = second ? y[i] * t.y + x[i] * t.x : x[i] * t.x - y[i] * t.y;
+            const double2 t = turns ? cs[ch + i - (second ? rope_dim / 2 : 0)] : make_double2(1.0, 0.0);
+            const double a = to_f32(v.x[i]), b = to_f32(y[i]);
+            o[i] = !turns ? a : second ? b * t.y + a * t.x : a * t.x - b * t.y;
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = to_f32(v.x[i]);
     }
 }
 
-// Codes of the eight values of a lane (four lanes of a quad hold a block), 4 bits each; e: the block's scale byte.
-__device__ __forceinline__ uint32_t hold8(const double (&v)[8], int &e) {
-    double amax = 0.0;
+// Codes of the eight values of a lane (four lanes of a quad hold a block), 4 bits each; e: the block's scale byte. F is f32
+// where the values are (its scaling and comparisons are exact: a magnitude in units of the scale that f32 would round is far
+// below the first border), else f64.
+template <class F> __device__ __forceinline__ uint32_t hold8(const F (&v)[8], int &e) {
+    F amax = 0;
     int bad = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const double a = fabs(v[i]);
-        bad |= !(a <= 1.7976931348623157e308);
+        const F a = fabs(v[i]);
+        bad |= !(a <= (sizeof(F) == 8 ? (F) 1.7976931348623157e308 : (F) 3.402823466e38f));
         amax = a > amax ? a : amax;
     }
-    auto other = [](double x, auto lane) {
-        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    auto other = [](F x, auto lane) {
         constexpr int O = decltype(lane)::value;
-        const uint32_t lo = (uint32_t) xor_lane_i<O>((int) (uint32_t) u), hi = (uint32_t) xor_lane_i<O>((int) (uint32_t) (u >> 32));
-        return __builtin_bit_cast(double, ((uint64_t) hi << 32) | lo);
+        if constexpr (sizeof(F) == 8) {
+            const uint64_t u = __builtin_bit_cast(uint64_t, x);
+            const uint32_t lo = (uint32_t) xor_lane_i<O>((int) (uint32_t) u), hi = (uint32_t) xor_lane_i<O>((int) (uint32_t) (u >> 32));
+            return __builtin_bit_cast(double, ((uint64_t) hi << 32) | lo);
+        } else {
+            return xor_lane<O>(x);
+        }
     };
     amax = fmax(amax, other(amax, std::integral_constant<int, 1>{}));
     amax = fmax(amax, other(amax, std::integral_constant<int, 2>{}));
@@ -114,15 +122,19 @@ __device__ __forceinline__ uint32_t hold8(const double (&v)[8], int &e) {
     if (bad) return 0;
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= kv_code(v[i], ldexp(fabs(v[i]), 127 - e)) << (4 * i);
+    for (int i = 0; i < 8; ++i) w |= kv_code(v[i], (F) ldexp(fabs(v[i]), 127 - e)) << (4 * i);
     return w;
 }
 
-// One workgroup: the new tokens among 16 aligned positions of one sequence, one kv head and its query heads.
-// Rows of 8 channels a thread: 2 D threads hold the 16 rows of a head.
+// One workgroup: the new tokens among 16 aligned positions of one sequence, one kv head and its query heads. Rows of 8
+// channels a thread: 2 D threads hold the 16 rows of a head. K and V are asked for before the angles are computed, a query
+// before the last one is stored, and the queries of the group's tokens are dealt to all threads: in turns by the threads of
+// their rows, one token's took as long as everything else (one token, 8 kv heads of 4 queries: 8.0 us, now 5.9; 61 sequences:
+// 10.0, now 5.9). For many tokens bound by the bytes: 4001 tokens, 168 MB in 34 us (a copy of them: 35); there it is waves
+// that pay, and a query's loads before the angles' arithmetic cost more registers than they hide (38 us).
 template <int D, int ROPE, class T>
-__global__ __launch_bounds__(2 * D) void k_kv_append(AppendArgs a) {
-    constexpr int NT = 2 * D;
+__global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_append(AppendArgs a) {
+    constexpr int NT = 2 * D, NR = D / 8;
     __shared__ double2 cs[ROPE == FNS_ROPE_NONE ? 1 : kGroup * (D / 2)];
     __shared__ __align__(16) uint8_t code[D][kGroup];
     const int s = blockIdx.y / a.c.n_kv, head = blockIdx.y % a.c.n_kv, tid = threadIdx.x;
@@ -132,39 +144,63 @@ __global__ __launch_bounds__(2 * D) void k_kv_append(AppendArgs a) {
     if (r.n == 0 || start >= r.len) return;
     const int base = (int) start;
     const int lo = max(first, base), hi = r.len - base < kGroup ? r.len : base + kGroup;  // [lo, hi): the tokens of this workgroup
+    const int row = tid / NR, ch = tid % NR * 8, pos = base + row;
+    const bool have = pos >= lo && pos < hi;
+    const int64_t tok = r.q0 + (pos - first);
+    const int page = page_of(a.c, a.b, s, base);  // 16 aligned positions lie in one page
+    Row8<T> k8 = {}, v8 = {}, q8 = {};
+    if (have) {
+        k8.load((const T *) a.k + tok * a.k_stride + head * D + ch);
+        v8.load((const T *) a.v + tok * a.v_stride + head * D + ch);
+    }
+    // Item i = row, row + 16, ... of the queries: token lo + i / n_group, head i % n_group of the group. In place too: the
+    // threads of a row are lanes of one wave, whose loads all precede the stores they feed.
+    const int n_group = a.n_group;
+    int qp = hi, qh = 0, dp = 0, dh = 0;
+    if (n_group) qp = lo + row / n_group, qh = row % n_group, dp = kGroup / n_group, dh = kGroup % n_group;
+    const auto ask = [&] {
+        if (qp < hi) q8.load((const T *) a.q + (r.q0 + (qp - first)) * a.q_stride + (int64_t) (head * n_group + qh) * D + ch);
+    };
     if constexpr (ROPE != FNS_ROPE_NONE) {
         const int half = a.rope_dim / 2;
-        for (int i = tid; i < kGroup * half; i += NT) {
-            const int p = base + i / half, c = i % half;
-            if (p < lo || p >= hi) continue;
+        for (int i = tid; i < (hi - lo) * half; i += NT) {
+            const int p = lo + i / half, c = i % half;
             // in turns: the product is exact to 53 bits, its whole part leaves no error
             double turns = (double) p * (double) a.inv_freq[c] * 0.15915494309189533577;
             turns -= rint(turns);
             double sn, cn;
             sincospi(2.0 * turns, &sn, &cn);
-            cs[i / half * (D / 2) + c] = make_double2(cn, sn);
+            cs[(p - base) * (D / 2) + c] = make_double2(cn, sn);
         }
         __syncthreads();
     }
-    const int row = tid / (D / 8), ch = tid % (D / 8) * 8, pos = base + row;
-    const bool have = pos >= lo && pos < hi;
-    const int64_t tok = r.q0 + (pos - first);
-    const double2 *mine = cs + (ROPE == FNS_ROPE_NONE ? 0 : row * (D / 2));
-    const int page = page_of(a.c, a.b, s, base);  // 16 aligned positions lie in one page
+    ask();
+    const auto angles = [&](int p) { return cs + (ROPE == FNS_ROPE_NONE ? 0 : (p - base) * (D / 2)); };
     const int P = 1 << a.c.shift;
     uint8_t *dst = a.c.pages + (int64_t) max(page, 0) * a.c.page_bytes + head * kv_head_bytes(D, P);
     using L = KvParts<D>;
-    double v[8] = {};
+    const bool put = have && page >= 0 && pos >= 0;
     int e;
-    if (have) rotated8<ROPE>((const T *) a.k + tok * a.k_stride + head * D, ch, a.rope_dim, mine, v);
-    uint32_t w = hold8(v, e);
-    if (have && page >= 0 && pos >= 0) {
+    uint32_t w;
+    if constexpr (ROPE == FNS_ROPE_NONE) {
+        float k[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = to_f32(k8.x[i]);
+        w = hold8(k, e);
+    } else {
+        double k[8] = {};
+        if (have) rotated<ROPE>(k8, ch, a.rope_dim, angles(pos), k);
+        w = hold8(k, e);
+    }
+    if (put) {
         *(uint32_t *) (dst + L::k_row(P, pos & (P - 1)) + ch / 2) = w;
         if (ch % 32 == 0) dst[L::k_scale(P, pos & (P - 1)) + ch / 32] = (uint8_t) e;
     }
-    if (have) rotated8<FNS_ROPE_NONE>((const T *) a.v + tok * a.v_stride + head * D, ch, 0, mine, v);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(v8.x[i]);
     w = hold8(v, e);
-    if (have && page >= 0 && pos >= 0 && ch % 32 == 0) dst[L::v_scale(P, pos & (P - 1)) + ch / 32] = (uint8_t) e;
+    if (put && ch % 32 == 0) dst[L::v_scale(P, pos & (P - 1)) + ch / 32] = (uint8_t) e;
 #pragma unroll
     for (int i = 0; i < 8; ++i) code[ch + i][row] = (uint8_t) ((w >> (4 * i)) & 15u);
     __syncthreads();
@@ -181,13 +217,15 @@ __global__ __launch_bounds__(2 * D) void k_kv_append(AppendArgs a) {
                 if (p4 + i >= lo && p4 + i < hi) o[i] = (uint8_t) (b >> (8 * i));
         }
     }
-    if (have)
-        for (int g = 0; g < a.n_group; ++g) {
-            const int64_t h = (int64_t) (head * a.n_group + g) * D;
-            // in place too: the threads of a row are lanes of one wave, whose loads all precede the stores they feed
-            rotated8<ROPE>((const T *) a.q + tok * a.q_stride + h, ch, a.rope_dim, mine, v);
-            store8((T *) a.q_out + tok * a.qo_stride + h + ch, v);
-        }
+    while (qp < hi) {
+        double q[8];
+        rotated<ROPE>(q8, ch, a.rope_dim, angles(qp), q);
+        T *out = (T *) a.q_out + (r.q0 + (qp - first)) * a.qo_stride + (int64_t) (head * n_group + qh) * D + ch;
+        qp += dp, qh += dh;
+        if (qh >= n_group) qh -= n_group, ++qp;
+        ask();
+        store8(out, q);
+    }
 }
 
 // Values of the batch's tokens as the cache holds them; NaN where a position has no page.
