@@ -941,8 +941,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     }
 }
 
-// The splits of a row into its result, a lane D / 64 channels: few rows a workgroup each, whose waves take the splits in turn;
-// many rows a wave each (WAVE_ROW). At most 64 splits: one a lane for their weights.
+// The splits of a row into its result, a lane D / 64 channels: a workgroup a row, whose waves take the splits in turn, or
+// (WAVE_ROW) a wave a row. At most 64 splits: one a lane for their weights.
 template <int D, bool WAVE_ROW, class T>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int rows_per_wg) {
     constexpr int C = D / 64, NW = 4;
@@ -1063,6 +1063,7 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
     FNS_TRY(attn_check(c, b, x));
     if (b->n_seq == 0 || b->n_tok == 0 || b->max_q == 0) return host::OK;
     if (!q || !out) return host::set_error(host::ERR_SHAPE, "attn: null argument");
+    if (q == out) return host::set_error(host::ERR_SHAPE, "attn: q and out must not overlap");
     const Plan p = attn_plan(c, b, x);
     if (p.row_tiles > 65535)
         return host::set_error(host::ERR_SHAPE, "attn: %lld tokens of a sequence in one call are too many", (long long) std::min<int64_t>(b->max_q, b->n_tok));
@@ -1086,8 +1087,9 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
     auto join = [&](auto dim, auto type) {
         constexpr int D = decltype(dim)::value;
         const int64_t rows = std::min<int64_t>(b->max_q, b->n_tok) * x->n_head;
-        // a workgroup a row as long as all of them are resident at once
-        if (rows * b->n_seq <= 2048)
+        // a workgroup a row where there are many splits and all of them are resident at once (64 splits of 32 rows: 5 us); with
+        // few splits its start outweighs them (8 of 2048 rows: 6.1 us, a wave each 3.6)
+        if (p.splits > 16 && rows * b->n_seq <= 2048)
             hipLaunchKernelGGL((k_attn_join<D, false, decltype(type)>), dim3((unsigned) rows, (unsigned) b->n_seq), dim3(256), 0, st, a, p.rows);
         else
             hipLaunchKernelGGL((k_attn_join<D, true, decltype(type)>), dim3((unsigned) ((rows + 3) / 4), (unsigned) b->n_seq), dim3(256), 0, st, a, p.rows);

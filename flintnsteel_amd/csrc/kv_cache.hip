@@ -9,6 +9,8 @@
 // v and is bound by them (and by its launch for a few tokens), not by this arithmetic.
 #include "fns_kv.hpp"
 
+#include <algorithm>
+
 #include "fns/kernels.h"
 #include "fns_common.hpp"
 #include "fns_host.hpp"
@@ -318,7 +320,8 @@ int kv_append(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, hi
     AppendArgs a{host::kv_view(c), host::kv_batch(b), x->k, x->v, x->q, x->q_out, x->inv_freq, x->k_stride, x->v_stride,
                  x->q_stride, x->q_out_stride, x->rope_dim, x->n_head / c->n_head_kv};
     // new tokens of a sequence start anywhere in a group
-    const dim3 grid((unsigned) ((b->max_q + kGroup - 2) / kGroup + 1), (unsigned) (b->n_seq * c->n_head_kv));
+    const int64_t most = std::min<int64_t>(b->max_q, b->n_tok);
+    const dim3 grid((unsigned) ((most + kGroup - 2) / kGroup + 1), (unsigned) (b->n_seq * c->n_head_kv));
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(2 * D), 0, st, a); };
     auto by_type = [&](auto dim, auto rope) {
         constexpr int DD = decltype(dim)::value, R = decltype(rope)::value;
@@ -340,8 +343,8 @@ int kv_read(const FnsKvCache *c, const FnsKvBatch *b, float *k, float *v, hipStr
     FNS_TRY(host::kv_check(c, b, "kv_read"));
     if (b->n_seq == 0 || b->n_tok == 0 || b->max_q == 0) return host::OK;
     if (!k || !v) return host::set_error(host::ERR_SHAPE, "kv_read: null output");
-    const int rows = 256 / (c->head_dim / 4);
-    const dim3 grid((unsigned) ((b->max_q + rows - 1) / rows), (unsigned) (b->n_seq * c->n_head_kv));
+    const int64_t rows = 256 / (c->head_dim / 4), most = std::min<int64_t>(b->max_q, b->n_tok);
+    const dim3 grid((unsigned) ((most + rows - 1) / rows), (unsigned) (b->n_seq * c->n_head_kv));
     auto go = [&](auto kern) {
         hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, host::kv_view(c), host::kv_batch(b), k, v);
     };

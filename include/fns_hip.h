@@ -363,10 +363,12 @@ int fns_hip_kv_read(const FnsKvCache *cache, const FnsKvBatch *batch, float *k, 
  * h / (n_head / n_head_kv). The token at position p sees positions 0..p, with window > 0 the last `window` of them.
  *   out = sum_j p_j V_j, p = softmax over the seen positions of scale * q . K_j; with sinks, exp(sinks[h]) joins the
  *   softmax's denominator. A row that sees nothing is zero; one that sees a token whose K or V holds a NaN block is NaN.
- * q and out [n_tok][n_head][head_dim], heads contiguous within a token, no overlap, any element alignment. With FNS_TYPE_F32
- * products carry 22 bits of q and of p; with FNS_TYPE_BF16, q is exact and p has 11 bits. Softmax statistics and sums are
- * f32. workspace: fns_hip_attn_workspace bytes (it grows with n_tok, n_seq, max_q, max_kv and n_head only), 16-byte aligned,
- * no initialisation; calls that overlap in time need one each. */
+ * A row of q that holds a NaN or an infinity gives NaN (where it sees anything).
+ * q and out [n_tok][n_head][head_dim], heads contiguous within a token, no overlap, any element alignment. What q enters the
+ * products with is within 2^-24 (FNS_TYPE_F32) or 2^-14 (FNS_TYPE_BF16) of its row's largest magnitude, p carries 22 or 11
+ * bits, and the sum of p counts the same values; softmax statistics and sums are f32. workspace: fns_hip_attn_workspace bytes
+ * (they depend on the numbers of the batch and on n_head, not on device memory; fewer tokens can need more), 16-byte
+ * aligned, no initialisation; calls that overlap in time need one each. */
 typedef struct FnsAttn {
     int dtype; /* of q and out: FNS_TYPE_F32 or FNS_TYPE_BF16 */
     int n_head;

@@ -37,7 +37,7 @@ def _append(c=None, b=None, x=None):
     return _lib.lib().fns_hip_kv_append(ctypes.byref(c), ctypes.byref(b), ctypes.byref(x), None)
 
 
-def _attn(c=None, b=None, x=None, q=BUF, out=BUF, ws=BUF, size=1 << 40):
+def _attn(c=None, b=None, x=None, q=BUF, out=2 * BUF, ws=BUF, size=1 << 40):
     c, b, x = c or cache(), b or batch(), x or att()
     return _lib.lib().fns_hip_attn(ctypes.byref(c), ctypes.byref(b), ctypes.byref(x), P(q), P(out), P(ws), size, None)
 
@@ -118,3 +118,26 @@ def test_page_bytes():
     assert L.fns_hip_kv_page_bytes(8, 128, 64) == 8 * 64 * (64 + 64 + 4 + 4)
     assert L.fns_hip_kv_page_bytes(1, 256, 16) == 16 * (128 + 128 + 8 + 8)
     assert L.fns_hip_kv_page_bytes(8, 100, 64) == 0 and L.fns_hip_kv_page_bytes(8, 128, 24) == 0
+
+
+def test_attn_overlap_workspace_and_limits():
+    L, r = _lib.lib(), ctypes.byref
+    assert _attn(out=BUF, q=BUF) == -2
+
+    def need(c, b, x):
+        size = ctypes.c_size_t()
+        assert L.fns_hip_attn_workspace(r(c), r(b), r(x), r(size)) == 0
+        return size.value
+
+    # one token over a long context is split; a long prompt leaves a note a wave of every 128 rows; short ones need nothing
+    long, prompt = batch(max_kv=100000, table_stride=2000), batch(n_tok=32768, max_q=32768, max_kv=32768, table_stride=512)
+    assert need(cache(), batch(), att()) == 0
+    assert need(cache(), prompt, att()) == 2 * (32768 * 2 // 128) * 4
+    for b in (long, prompt):
+        n = need(cache(), b, att())
+        assert n > 0
+        for ws, size in ((None, n), (BUF, n - 1), (BUF + 8, n), (BUF, 0)):
+            assert _attn(b=b, out=3 * BUF, ws=ws, size=size) == -4
+    # more row tiles than a grid has
+    assert _attn(c=cache(n_head_kv=1), b=batch(n_tok=1 << 30, max_q=1 << 30), x=att(n_head=16, q_stride=1 << 14, out_stride=1 << 14),
+                 out=3 * BUF) == -2

@@ -366,6 +366,61 @@ def test_attn_a_huge_block_of_v_is_nothing_to_rows_that_do_not_see_it(q, many, s
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,page,q,many", [(128, 64, 5, False), (128, 64, 90, True), (128, 16, 40, False), (256, 128, 6, False),
+                                             (256, 16, 70, True), (64, 256, 130, True)])
+def test_attn_huge_blocks_of_v_in_every_form(dim, page, q, many, dtype):
+    s = Setup([q, 2], [q + 100, 300], page, 1, dim, seed=67, pad=MANY_ROWS if many else 0)
+    s.batch.desc.max_q = s.n_tok if many else q
+    h = s.host
+    for seq, back, e in ((0, 1, 250), (0, q // 2, 200), (1, 1, 180)):
+        pos = s.kv_lens[seq] - back
+        at = page * dim + page * (dim // 32) + pos % page * (dim // 32) + back % (dim // 32)
+        h.raw[s.table[seq, pos // page], at] = e
+    s.cache.pages.copy_(torch.from_numpy(h.raw.copy()).view(s.cache.pages.shape))
+    _check_attn(s, 2, dtype)
+    _check_attn(s, 2, dtype, window=q // 3 + 1, sinks=True)
+
+
+@pytest.mark.parametrize("q,many", [(1, False), (20, False), (80, True)])
+def test_attn_odd_queries_scales_windows_and_sinks(q, many):
+    """Rows of q with NaNs and infinities are NaN, their neighbours are not; scales of zero and below; windows beyond any
+    length; sinks of either infinity."""
+    s = Setup([q], [q + 70], 64, 1, 64, seed=71, pad=MANY_ROWS if many else 0)
+    s.batch.desc.max_q = s.n_tok if many else q
+    x, xh = _rand(s.rng, (s.n_tok, 2, 64))
+    for scale, window in ((0.0, 0), (-0.3, 0), (0.2, 2 ** 31 - 1), (0.125, 2 ** 30)):
+        got = ops.attn(s.cache, s.batch, x, scale=scale, window=window)[: s.tok].double().cpu().numpy()
+        ref, ax, vm = kd.attention(s.host, s.table, s.q_lens, s.kv_lens, xh[: s.tok], scale, 0)
+        assert (np.abs(got - ref) <= kd.attn_tolerance("f32", 64, q + 70, ref, np.abs(ax), vm)).all()
+    good = ops.attn(s.cache, s.batch, x)[: s.tok]
+    low = ops.attn(s.cache, s.batch, x, sinks=torch.tensor([float("-inf"), 0.5], device="cuda"))[: s.tok]
+    assert torch.equal(low[:, 0], good[:, 0])
+    bad = x.clone()
+    bad[0, 0, 63], bad[q // 2, 1, 0] = float("nan"), float("-inf")
+    got = ops.attn(s.cache, s.batch, bad)[: s.tok]
+    assert torch.isnan(got[0, 0]).all() and torch.isnan(got[q // 2, 1]).all()
+    got[0, 0], got[q // 2, 1] = good[0, 0], good[q // 2, 1]
+    assert torch.equal(got, good)
+    tiny = ops.attn(s.cache, s.batch, x * 1e-36)[: s.tok]  # scores of nothing: the mean of V
+    assert torch.equal(tiny, ops.attn(s.cache, s.batch, x, scale=0.0)[: s.tok])
+
+
+def test_sequences_may_share_pages_and_workspaces_are_checked():
+    """A common prefix, in order and twice in one table; a workspace that is too small is refused before anything runs."""
+    s = Setup([1, 3], [2000, 2040], 64, 2, 128, seed=73)
+    s.table[1, :30] = s.table[0, :30]
+    s.table[0, 7] = s.table[0, 6]
+    s.batch.page_table.copy_(torch.from_numpy(s.table))
+    q, out = _check_attn(s, 4, "f32")
+    ws = ops.attn_workspace(s.cache, s.batch, q)
+    assert ws.numel() > 0
+    with pytest.raises(FnsError, match="workspace"):
+        ops.attn(s.cache, s.batch, q, out=out, ws=ws[:-16])
+    with pytest.raises(FnsError, match="overlap"):
+        ops.attn(s.cache, s.batch, q, out=q, ws=ws)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("q", [1, 3, 40])
 def test_attn_large_scores(q, dtype):
     """Scores of hundreds: a softmax that is nearly one-hot, its maximum moving from tile to tile."""
@@ -536,6 +591,33 @@ def test_graph_of_a_growing_sequence(q):
         step(b.cache, eager, want)
         assert torch.equal(got, want)
         assert torch.equal(a.cache.pages, b.cache.pages)
+
+
+def test_graphs_of_prompts_that_share_a_workspace():
+    """Two graphs of a prompt's workgroups over one workspace, replayed in turn while blocks that send rows to the second pass
+    come and go, eager calls between."""
+    s = Setup([70, 33], [70, 140], 64, 1, 128, seed=79, pad=MANY_ROWS)
+    s.batch.desc.max_q = s.n_tok
+    q = _rand(s.rng, (s.n_tok, 2, 128))[0]
+    ws, outs, graphs = ops.attn_workspace(s.cache, s.batch, q), [torch.zeros_like(q) for _ in range(2)], []
+    ops.attn(s.cache, s.batch, q, out=outs[0], ws=ws)
+    torch.cuda.synchronize()
+    for o in outs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.attn(s.cache, s.batch, q, out=o, ws=ws)
+        graphs.append(g)
+    page, row = int(s.table[0, 0]), 64 * 128 + 64 * 4 + 40 * 4
+    keep = s.cache.pages[page, row].clone()
+    for i in range(6):
+        s.cache.pages[page, row] = keep if i % 3 == 0 else torch.full_like(keep, 200 + i)
+        q.normal_()
+        graphs[i % 2].replay()
+        graphs[(i + 1) % 2].replay()
+        want = ops.attn(s.cache, s.batch, q)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0][: s.tok], want[: s.tok]) and torch.equal(outs[1][: s.tok], want[: s.tok])
+        assert torch.isfinite(want[:40]).all() and (want[:40].abs() < 100).all()
 
 
 def test_two_streams_with_workspaces_of_their_own():
