@@ -788,16 +788,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     float *vsc = vsc_all[wave];
     uint8_t *ksb = ksb_all[wave];
 
-    TileReader<D, SMALL> rk, rv;  // K of the next tile, V of the one after it
-    rk.P = rv.P = P, rk.lane = rv.lane = lane, rk.r = rv.r = r, rk.g = rv.g = g;
-    rk.head_off = rv.head_off = head * kv_head_bytes(D, P);
-    rk.last = rv.last = (int) a.b.table_stride - 1;
+    TileReader<D, SMALL> rd;  // at the next tile, when its K is asked for; then at the one after it, for V
+    rd.P = P, rd.lane = lane, rd.r = r, rd.g = g, rd.head_off = head * kv_head_bytes(D, P), rd.last = (int) a.b.table_stride - 1;
     const int32_t *table = a.b.table + s * a.b.table_stride;
     u4 kraw[4][kKPieces<D>], vraw[MB];
     ScaleBytes<NB> swk, swv, unused;
     const auto load_v = [&] {  // the wave's blocks; a wave without one asks for another's
 #pragma unroll
-        for (int m = 0; m < MB; ++m) vraw[m] = rv.v_block((wave + NW * m) % NB);
+        for (int m = 0; m < MB; ++m) vraw[m] = rd.v_block((wave + NW * m) % NB);
     };
     const auto expand = [&](int buf) {
 #pragma unroll
@@ -826,10 +824,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     int low = 0;
     TileInfo ti{}, next{};
     if (t0 < t1) {
-        rv.ask(a, table, t0), rk.ask(a, table, t0);
-        rv.take(a, t0), rk.take(a, t0);
-        rk.scales(swk, swv), rk.k(kraw), load_v();
-        rv.ask(a, table, min(t0 + 1, t1 - 1)), rk.ask(a, table, min(t0 + 1, t1 - 1));
+        rd.ask(a, table, t0);
+        rd.take(a, t0);
+        rd.scales(swk, swv), rd.k(kraw), load_v();
+        rd.ask(a, table, min(t0 + 1, t1 - 1));
     }
     Digits<D, T> q[CT];
     RowState<NB> st[CT];
@@ -847,13 +845,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     }
     if (t0 < t1) {
         const int key = t0 * kTile + lane;
-        ti = v_scales<NB, NW>(swv, rv.there && key >= rt.lo && key < rt.hi, ev, vsc, wave);
+        ti = v_scales<NB, NW>(swv, rd.there && key >= rt.lo && key < rt.hi, ev, vsc, wave);
         wave_sync();
         expand(0);
         wave_sync();
-        rv.take(a, min(t0 + 1, t1 - 1));
-        rv.scales(unused, swv), load_v();
-        rv.ask(a, table, min(t0 + 2, t1 - 1));
+        rd.take(a, min(t0 + 1, t1 - 1));
+        rd.scales(unused, swv), load_v();
+        rd.ask(a, table, min(t0 + 2, t1 - 1));
         tile_barrier();
     }
     for (int tile = t0; tile < t1; ++tile) {
@@ -872,6 +870,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
             for (int c = 0; c < CT; ++c)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) sc[c][t] = f4{1, 1, 1, 1} * score_origin(st[c].m);
+            __builtin_amdgcn_s_setprio(0);  // (matrix instructions wait for the pipe: the other waves' vector work goes first)
 #pragma unroll
             for (int n = 0; n < Q::N; ++n)  // the largest digit first: the rest adds to small numbers
 #pragma unroll
@@ -883,10 +882,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(sc[c][t]));  // (K is used up before the next one is asked for)
         }
+        __builtin_amdgcn_s_setprio(1);
         __builtin_amdgcn_sched_barrier(0);
-        rk.take(a, min(tile + 1, t1 - 1));
-        rk.ask(a, table, min(tile + 2, t1 - 1));
-        rk.scales(swk, unused), rk.k(kraw);
+        rd.scales(swk, unused), rd.k(kraw);
         if (active) {
             const float vkeep = ldexpf(1.0f, ev - ti.ev);
             ev = ti.ev;
@@ -895,6 +893,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
 #pragma unroll
             for (int c = 0; c < CT; ++c) see[c] = sights[wave][c][r];
             softmax_tile<NB, CT, SPLIT>(sc, see, base, ti, vkeep, st, p);
+            __builtin_amdgcn_s_setprio(0);
             const h8 *at = (const h8 *) (vt[buf] + r * VS + 16 * g);
 #pragma unroll
             for (int d = 0; d < 2 * NB; ++d)
@@ -908,14 +907,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
                     if (SPLIT == 2 && v == 1) __builtin_amdgcn_sched_barrier(0);  // (the registers are counted: no more reads ahead)
                 }
         }
+        __builtin_amdgcn_s_setprio(1);
         const int after = min(tile + 1, t1 - 1), key = after * kTile + lane;
-        next = v_scales<NB, NW>(swv, rv.there && key >= rt.lo && key < rt.hi, ti.ev, vsc, wave);
+        next = v_scales<NB, NW>(swv, rd.there && key >= rt.lo && key < rt.hi, ti.ev, vsc, wave);
         wave_sync();
         if (tile + 1 < t1) expand(buf ^ 1);
         wave_sync();
-        rv.take(a, min(tile + 2, t1 - 1));
-        rv.scales(unused, swv), load_v();
-        rv.ask(a, table, min(tile + 3, t1 - 1));
+        rd.take(a, min(tile + 2, t1 - 1));
+        rd.scales(unused, swv), load_v();
+        rd.ask(a, table, min(tile + 3, t1 - 1));
         low |= (int) ti.low;
         ti = next;
         tile_barrier();
