@@ -332,7 +332,7 @@ __device__ __forceinline__ uint32_t seen(const Sight &w, int base, uint64_t ther
 // One tile's softmax: s (from score_origin) of the lane's 16 keys and CT rows -> p as operand parts, and its sums. Where some
 // row does not see every key those become -infinity first; where the maximum has grown, or V's scale (vkeep), m moves and what
 // refers to it follows. The common path has one branch around both; inside it they are apart, as the last tile of a row and a
-// window's edge need the first alone (five prompts of 1021 tokens with a window of 256: 86 us with both always, 79 apart).
+// window's edge need the first alone (five prompts of 1021 tokens with a window of 513: 86 us with both always, 79 apart).
 template <int NB, int CT, int SPLIT>
 __device__ __forceinline__ void softmax_tile(f4 (&s)[CT][4], const Sight (&see)[CT], int base, const TileInfo &ti, float vkeep,
                                              RowState<NB> (&st)[CT], h8 (&p)[CT][SPLIT][2]) {
@@ -535,9 +535,12 @@ __device__ __forceinline__ void low_blocks(const AttnArgs &a, TileReader<D, SMAL
 // Few rows (decode, verify): the workgroup's waves take tiles of keys in turn and are joined at the end. A wave's tile goes
 // from the pages to registers and stays there: S^T = K Q^T with K's rows in an order that leaves every lane with the 16
 // consecutive keys 16 g .. 16 g + 15 of its query row, which is where the second product, O^T = V^T P^T, wants P, and where
-// V's bytes (16 consecutive positions of a channel pair) are. Bound by the cache's bytes for long contexts and by a few
-// dependent loads for short ones. One wave issues a vector instruction about every 5 cycles where the SIMD takes one every
-// 2: what pays is waves, so the queries lie in LDS and the next tile's K is asked for when this one's is used up.
+// V's bytes (16 consecutive positions of a channel pair) are. Bound by the cache's bytes for one long context (131072 keys of
+// 8 heads, bf16: 143 MB in 26 us, 5.5 TB/s; the pages' pattern of loads alone reaches 5.5), by the vector pipe's work on a
+// tile for f32 and many contexts (48 to 16000 keys: 272 MB in 60 us, 4.5 TB/s: 260 vector and 56 matrix instructions a tile
+// of 64 keys, at about 4.3 cycles a vector instruction with three waves a SIMD), by a few dependent loads for short ones (500
+// keys: 9 us). What pays is waves, so the queries lie in LDS and the next tile's K is asked for when this one's is used up;
+// workgroups of 8 waves, or four waves a SIMD at 128 registers, were slower (48 contexts: 84 and 76 us where this took 74).
 // REDO: low blocks are known to be there.
 template <int D, int CT, bool SMALL, bool REDO, class T>
 __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split) {
@@ -776,8 +779,11 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_attn_redo(AttnArgs a, int
 // reads of 16 channels touch every bank once). K needs no expansion: each wave reads its codes, which the workgroup's first
 // reader brings into L1, and keeps them in registers with the digits of its queries. A workgroup that meets low blocks leaves
 // them out and says so: its rows are then done again by the form of few rows (with low blocks in this loop, 4096 tokens at
-// 4096 took 539 us instead of 423). Bound by the vector pipe's work on the
-// scores, about 6 instructions each where the two products take as long for bf16.
+// 4096 took 539 us instead of 423).
+// 4096 tokens at 4096 keys, 32 heads over 8 of 128, bf16: 398 us, 1.04 PFLOP/s (a library product of 8192^3: 1.22). A tile
+// costs a wave 60 matrix instructions (about 970 cycles) and 147 vector instructions with 32 exponentials (about 890), of
+// which two waves a SIMD overlap little: the matrix pipe is busy 38% of the time. More waves do not fit the registers; the
+// expansion of V among the first product's instructions, which helps bf16 (by 3%), costs heads of 256 channels 6 to 18%.
 __device__ __forceinline__ void tile_barrier() {
     // LDS only: the tiles asked for stay in flight
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
