@@ -884,7 +884,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     }
     for (int tile = t0; tile < t1; ++tile) {
         const int base = tile * kTile, buf = (tile - t0) & 1;
-        const bool active = base <= most && base + kTile > least;
+        const bool active = base <= most && base + kTile - 1 >= least;
         f4 sc[CT][4];
         if (active) {
             *(ScaleBytes<NB> *) (ksb + lane * NB) = swk;

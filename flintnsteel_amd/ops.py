@@ -780,7 +780,7 @@ def attn(cache: KvCache, batch: KvBatch, q: torch.Tensor, scale: float | None = 
         if sinks.dtype != torch.float32 or not sinks.is_contiguous() or sinks.numel() != q.shape[1]:
             raise ValueError("attn: sinks must be a contiguous f32 vector, one a query head")
         desc.sinks = sinks.data_ptr()
-    desc.dtype, desc.n_head, desc.window = F32 if dt is torch.float32 else BF16, q.shape[1], window
+    desc.dtype, desc.n_head, desc.window = F32 if dt is torch.float32 else BF16, q.shape[1], min(window, 2 ** 31 - 1)
     desc.scale = D ** -0.5 if scale is None else scale
     if ws is None:
         ws = attn_workspace(cache, batch, q)
