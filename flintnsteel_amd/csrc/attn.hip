@@ -1058,14 +1058,14 @@ Plan attn_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
     p.row_tiles = (int) ((rows + p.rows - 1) / p.rows);
     const int64_t wgs = std::max<int64_t>(1, heads * p.row_tiles);
     const int64_t tiles = std::max<int64_t>(1, (b->max_kv + kTile - 1) / kTile);
-    // A split costs its join and a second start, 4-6 us; a workgroup alone on a CU is within a tenth of two or three on its
-    // rate. So: splits until 512 workgroups where there are fewer than 256 (131072 keys of 8 heads: 32 us with 512, 37 with
-    // 256; 64 sequences of 4096, 512 workgroups: 58 whole, 66 in two), of four tiles
-    // (one a wave) at least, and none at all below 13 tiles (500 keys: 9.2 whole, 10.9 in two). Beyond that, pieces of 40
-    // tiles, up to 2304, so that the longest of unequal sequences does not run on alone (48 of up to 16000
-    // keys: 74 us with 2304, 94 with 512).
+    // A split costs its join and a second start, 4-6 us, about what 11 tiles cost a workgroup; what it saves is the tiles' time
+    // on the CUs that have nothing. So, where that outweighs it, splits until 512 workgroups (131072 keys of 8 heads: 32 us
+    // with 512, 37 with 256), of four tiles (one a wave) at least: 24 sequences of 1500 keys, 8 heads: 20.5 us whole, 24.5 in
+    // three; 8 of 2048: 16.8 in eight, 21.6 whole; 500 keys: 9.2 whole, 10.9 in two. Beyond that, pieces of 40 tiles, up to
+    // 2304, so that the longest of unequal sequences does not run on alone (48 of up to 16000 keys: 74 us with 2304, 94 with
+    // 512).
     int64_t splits = 1;
-    if (!many && tiles > 12) splits = std::max(wgs < 256 ? std::min(per(512, wgs), per(tiles, 4)) : 1, std::min(tiles / 40, per(2304, wgs)));
+    if (!many) splits = std::max(tiles * (256 - wgs) > 11 * 256 ? std::min(per(512, wgs), per(tiles, 4)) : 1, std::min(tiles / 40, per(2304, wgs)));
     p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(splits, 64));
     p.chunk = (int) per(tiles, p.splits);
     if (p.splits > 1) {
