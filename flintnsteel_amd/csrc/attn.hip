@@ -66,6 +66,11 @@ template <class T> __device__ __forceinline__ void store4(T *p, f4 v) {  // any 
     __builtin_memcpy(p, t, sizeof t);
 }
 
+// The position before the first one that a token at pos sees, -1 if that is 0 (pos may be negative, where a sequence has fewer
+// positions than new tokens, and a window any width: their difference does not fit 32 bits).
+__device__ __forceinline__ int before_window(int pos, int window) {
+    return window ? max(max(pos, 0) - window, -1) : -1;
+}
 // A workgroup's rows (row = token of the sequence * group + head of the group) row0 .. row0 + rows - 1, and the tiles of
 // keys [t0, t1) that any of them sees.
 struct RowTiles {
@@ -78,7 +83,7 @@ __device__ __forceinline__ RowTiles row_tiles(const AttnArgs &a, const SeqRange 
     const int64_t cap = a.b.table_stride << a.c.shift;  // positions behind the table have no page
     RowTiles t;
     t.hi = (int) min((int64_t) first + i1 + 1, cap);
-    t.lo = a.window ? max(first + i0 - a.window + 1, 0) : 0;
+    t.lo = before_window(first + i0, a.window) + 1;
     t.t0 = t.lo / kTile;
     t.t1 = t.hi > t.lo ? t.hi / kTile + (t.hi % kTile > 0) : t.t0;
     return t;
@@ -318,7 +323,7 @@ struct Sight {
     int from, to;
 };
 __device__ __forceinline__ Sight sight(bool there, int pos, int window) {
-    return {there && window ? max(pos - window, -1) : -1, there ? pos : INT32_MAX};
+    return {there ? before_window(pos, window) : -1, there ? pos : INT32_MAX};
 }
 // Bits of the lane's 16 keys (base + 16 g ..) that a row sees; there: the tile's keys that exist.
 __device__ __forceinline__ uint32_t seen(const Sight &w, int base, uint64_t there) {
@@ -865,7 +870,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     DigitScales<D, T> qsc[CT];
     const int w0 = row0 + wave * 32;  // the wave's rows, and the positions that they see at most and at least
     const int most = w0 < rows ? first + min(w0 + 31, rows - 1) / a.group : -1;
-    const int least = a.window ? first + w0 / a.group - a.window + 1 : 0;
+    const int least = before_window(first + w0 / a.group, a.window) + 1;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         const int row = w0 + 16 * c + r, i = row / a.group;
