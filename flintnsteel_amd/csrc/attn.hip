@@ -1049,7 +1049,8 @@ int attn_check(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
 
 // How a call is divided: rows of a workgroup, splits of the keys and tiles of a split, by the host's numbers.
 struct Plan {
-    int rows, row_tiles, splits, chunk;
+    int rows, splits, chunk;
+    int64_t row_tiles;  // (more than a grid has are attn's to refuse)
     size_t ml_off, bytes;
 };
 Plan attn_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
@@ -1063,7 +1064,7 @@ Plan attn_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
     const int64_t heads = (int64_t) b->n_seq * c->n_head_kv;
     const bool many = rows > kFewRows && heads * per(rows, kManyRows) >= 512;
     p.rows = many ? kManyRows : rows <= 16 || c->head_dim == 256 ? 16 : 32;
-    p.row_tiles = (int) ((rows + p.rows - 1) / p.rows);
+    p.row_tiles = per(rows, p.rows);
     const int64_t wgs = std::max<int64_t>(1, heads * p.row_tiles);
     const int64_t tiles = std::max<int64_t>(1, (b->max_kv + kTile - 1) / kTile);
     // A split costs its join and a second start, 4-6 us, about what 11 tiles cost a workgroup; what it saves is the tiles' time
@@ -1137,8 +1138,8 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
             else hipLaunchKernelGGL((k_attn_many<D, false, decltype(type)>), grid, dim3(256), 0, st, a);
             FNS_TRY(host::check_launch("attn"));
             const dim3 some(grid.x, std::min(grid.y, (512 + grid.x - 1) / grid.x));
-            if (small) hipLaunchKernelGGL((k_attn_redo<D, true, decltype(type)>), some, dim3(64 * kFewWaves), 0, st, a, p.row_tiles);
-            else hipLaunchKernelGGL((k_attn_redo<D, false, decltype(type)>), some, dim3(64 * kFewWaves), 0, st, a, p.row_tiles);
+            if (small) hipLaunchKernelGGL((k_attn_redo<D, true, decltype(type)>), some, dim3(64 * kFewWaves), 0, st, a, (int) p.row_tiles);
+            else hipLaunchKernelGGL((k_attn_redo<D, false, decltype(type)>), some, dim3(64 * kFewWaves), 0, st, a, (int) p.row_tiles);
         } else if constexpr (D == 256) few(dim, std::integral_constant<int, 1>{}, type);
         else if (p.rows == 16) few(dim, std::integral_constant<int, 1>{}, type);
         else few(dim, std::integral_constant<int, 2>{}, type);
