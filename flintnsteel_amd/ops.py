@@ -784,6 +784,8 @@ def attn(cache: KvCache, batch: KvBatch, q: torch.Tensor, scale: float | None = 
     desc.scale = D ** -0.5 if scale is None else scale
     if ws is None:
         ws = attn_workspace(cache, batch, q)
+    elif not ws.is_contiguous():
+        raise ValueError("attn: the workspace must be contiguous")
     st = _here("attn", cache.pages, batch.kv_len, q, out, sinks, ws)
     call("fns_hip_attn", cache.ref, batch._for(cache), ctypes.byref(desc), q.data_ptr(), out.data_ptr(), ws.data_ptr(),
          ws.numel() * ws.element_size(), st)

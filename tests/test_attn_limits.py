@@ -20,3 +20,20 @@ def test_calls_of_more_row_tiles_than_a_grid_has_are_refused(n_tok, n_head):
     L, r = _lib.lib(), ctypes.byref
     assert L.fns_hip_attn(r(cache), r(batch), r(att), P(BUF), P(2 * BUF), P(3 * BUF), 1 << 50, None) == -2
     assert b"too many" in L.fns_hip_last_error()
+
+
+def test_a_workspace_has_to_be_contiguous(monkeypatch):
+    """Its elements are counted, and the kernels write that many bytes from its address on."""
+    calls = []
+    monkeypatch.setattr(ops, "_here", lambda what, *ts: 0)
+    monkeypatch.setattr(ops, "call", lambda name, *args: calls.append(name))
+    cache = ops.KvCache(4, 16, 1, 64, pages=torch.zeros(4, ops.lib().fns_hip_kv_page_bytes(1, 64, 16), dtype=torch.uint8))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    batch = ops.KvBatch(i32(0, 1), i32(10), i32(0).view(1, 1), 1, 1)
+    q = torch.zeros(1, 2, 64)
+    for ws in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 20, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="contiguous"):
+            ops.attn(cache, batch, q, ws=ws)
+    assert not calls
+    ops.attn(cache, batch, q, ws=torch.zeros(1 << 10, dtype=torch.uint8))
+    assert calls == ["fns_hip_attn"]
