@@ -23,9 +23,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 64;     // keys of a step
 constexpr int kFewRows = 64, kManyRows = 128;  // rows that always take the few-row form; rows of a workgroup of the other
 constexpr int kFewWaves = 4;  // waves of a workgroup of few rows
-constexpr int kHead = 12;     // V expands to f16 with the largest block scale so far at 2^12 (codes to 6: 24576)
+constexpr int kHead = 12;     // V expands to f16 with the largest block scale so far, E, at 2^12 (codes to 6: 24576)
 constexpr int kBias = 127 + kHead;
 constexpr int kBand = 36;     // block scales from E down that f16 holds exactly
+// E starts at 2^-17 (V below that is exact too, down to 2^-53), and where it has grown by more than 2^100, sums from before
+// may be next to f32's subnormals: a row has at least 2^8 of p, times 2^(12 - 36) of a block, so 2^-16 before the growth.
+constexpr int kFloor = 110, kGrown = kFloor + 100;
 // p is carried times 2^8: its low half stays clear of f16's subnormals. Sums are rescaled only where a row's maximum has
 // grown by more than 2^7 since the last time, so p stays below 2^15.
 constexpr float kPShift = 8.0f, kLazy = 7.0f;
@@ -47,7 +50,7 @@ struct AttnArgs {
     int64_t q_stride, out_stride;
     int n_head, group, window, splits, chunk;
     float scale;
-    uint8_t *redo;  // many rows: [n_seq * n_kv][row tiles][4 waves], whether low blocks were left out
+    uint8_t *redo;  // many rows: [n_seq * n_kv][row tiles][4 waves], whether some row may have lost something of V
 };
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
@@ -111,9 +114,9 @@ struct TileInfo {
     bool low;  // there are blocks (of those that the wave expands) that f16 cannot hold beside the largest
 };
 // The block scales of V as the f32 operands of the expansion, in the wave's LDS, [NB][64 keys]: 2^(e - E + 12), E at least
-// every scale so far. Half of 2^(12 - kBand) is the last bit of f16: blocks of E - kBand and below become zeros here and are
-// low_blocks' work (they are nothing beside the largest, but there may be rows that do not see the largest). w: the scale
-// bytes of the lane's key.
+// every scale so far. Half of 2^(12 - kBand) is the last bit of f16: blocks of E - kBand and below become zeros here and send
+// the rows to v_in_bands (they are nothing beside the largest, but there may be rows that do not see the largest). w: the
+// scale bytes of the lane's key.
 template <int NB> struct ScaleBytes {
     std::conditional_t<NB == 2, uint16_t, uint32_t> w[(NB + 3) / 4];
 };
@@ -499,32 +502,68 @@ template <int D, bool SMALL> struct TileReader {
     }
 };
 
-// The second product of a tile's low blocks, in bands of kBand scales, each at a scale of its own and straight from the cache.
+// The second product of a tile whatever the blocks' sizes: V straight from the cache, in bands of kBand scales, each expanded
+// at a scale of its own and added at the row's, E[c] (a lane's, as its row is): the largest that the row has seen so far, of
+// kFloor at least. What a row gives depends on no block that it does not see.
 template <int D, bool SMALL, int CT, int SPLIT>
-__device__ __forceinline__ void low_blocks(const AttnArgs &a, TileReader<D, SMALL> rd, const int32_t *table, int tile, const RowTiles &rt, int ev,
-                                           const h8 (&p)[CT][SPLIT][2], RowState<D / 32> (&st)[CT]) {
+__device__ __forceinline__ void v_in_bands(const AttnArgs &a, TileReader<D, SMALL> rd, const int32_t *table, int tile, const TileInfo &ti,
+                                           const Sight (&see)[CT], const h8 (&p)[CT][SPLIT][2], RowState<D / 32> (&st)[CT], int (&E)[CT]) {
+    constexpr int NB = D / 32;
     rd.ask(a, table, tile);
     rd.take(a, tile);
-    const int at = SMALL ? (rd.row + 16 * rd.g) & (rd.P - 1) : rd.row + 16 * rd.g, key = tile * kTile + 16 * rd.g;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-        const u4 codes = rd.v_block(j);
-        const uint8_t *scale = rd.bv + KvParts<D>::v_scale(rd.P, at) + j;
+    const int at = SMALL ? (rd.row + 16 * rd.g) & (rd.P - 1) : rd.row + 16 * rd.g, base = tile * kTile;
+    const uint32_t keys = (uint32_t) (ti.there >> (16 * rd.g)) & 0xffffu;
+    const uint8_t *scale = rd.bv + KvParts<D>::v_scale(rd.P, at);
+    int most[CT] = {};
 #pragma unroll 1
-        for (int top = ev - kBand; top > 0 && ev - top < 4 * kBand; top -= kBand) {  // (below: nothing that f32 sums hold)
+    for (int i = 0; i < 16; ++i) {
+        int e = 0;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int x = scale[i * NB + j];
+            e = x == 255 ? e : max(e, x);  // (rows that see a NaN are NaN)
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) most[c] = max(most[c], seen(see[c], base, ti.there) >> i & 1 ? e : 0);
+    }
+    int from = 0;  // the largest scale that any row sees
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        most[c] = max(most[c], xor_lane_i<16>(most[c]));
+        most[c] = max(most[c], xor_lane_i<32>(most[c]));
+        const int to = max(E[c], most[c]);
+        const float keep = ldexpf(1.0f, E[c] - to);
+        E[c] = to;
+#pragma unroll
+        for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= keep;
+        from = max(from, most[c]);
+    }
+    from = max(from, xor_lane_i<1>(from));
+    from = max(from, xor_lane_i<2>(from));
+    from = max(from, xor_lane_i<4>(from));
+    from = __builtin_amdgcn_readfirstlane(max(from, xor_lane_i<8>(from)));
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const u4 codes = rd.v_block(j);
+#pragma unroll 1
+        for (int top = from; top > 0; top -= kBand) {
+            float w[16];
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int e = keys >> i & 1 ? scale[i * NB + j] : 0;
+                const bool in = e <= top && e > max(top - kBand, 0);
+                any |= in;
+                w[i] = in ? __builtin_bit_cast(float, (uint32_t) (e - top + kBias) << 23) : 0.0f;
+            }
+            if (!__any(any)) continue;
             f4 lo[CT], hi[CT];
 #pragma unroll
             for (int c = 0; c < CT; ++c) lo[c] = hi[c] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-                float w[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int k = key + 8 * v + i, e = rd.there && k >= rt.lo && k < rt.hi ? scale[(8 * v + i) * (D / 32)] : 0;
-                    w[i] = e <= top && e > max(top - kBand, 0) ? __builtin_bit_cast(float, (uint32_t) (e - top + kBias) << 23) : 0.0f;
-                }
                 h8 x, y;
-                expand_v(codes[2 * v], codes[2 * v + 1], w, x, y);
+                expand_v(codes[2 * v], codes[2 * v + 1], w + 8 * v, x, y);
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -533,9 +572,12 @@ __device__ __forceinline__ void low_blocks(const AttnArgs &a, TileReader<D, SMAL
                         hi[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, p[c][h][v], hi[c], 0, 0, 0);
                     }
             }
-            const float unit = ldexpf(1.0f, top - ev);
 #pragma unroll
-            for (int c = 0; c < CT; ++c) st[c].o[2 * j] += lo[c] * unit, st[c].o[2 * j + 1] += hi[c] * unit;
+            for (int c = 0; c < CT; ++c) {
+                // (a row that sees nothing of a band more than kBand above its scale has zeros there: any finite unit will do)
+                const float unit = ldexpf(1.0f, min(top - E[c], kBand));
+                st[c].o[2 * j] += lo[c] * unit, st[c].o[2 * j + 1] += hi[c] * unit;
+            }
         }
     }
 }
@@ -549,7 +591,7 @@ __device__ __forceinline__ void low_blocks(const AttnArgs &a, TileReader<D, SMAL
 // of 64 keys, at about 4.3 cycles a vector instruction with three waves a SIMD), by a few dependent loads for short ones (500
 // keys: 9 us). What pays is waves, so the queries lie in LDS and the next tile's K is asked for when this one's is used up;
 // workgroups of 8 waves, or four waves a SIMD at 128 registers, were slower (48 contexts: 84 and 76 us where this took 74).
-// REDO: low blocks are known to be there.
+// A wave whose blocks of V turn out to be too far apart walks once more, by v_in_bands. REDO: that is known.
 template <int D, int CT, bool SMALL, bool REDO, class T>
 __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split) {
     constexpr int NB = D / 32, SPLIT = sizeof(T) == 4 ? 2 : 1, NW = kFewWaves;
@@ -615,11 +657,11 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
 
     float *vsc = lds + wave * kScale;
     uint8_t *ksb = (uint8_t *) (vsc + 64 * NB);  // K's scale bytes, [64 keys][NB]
-    int ev = 1;
-    // Returns whether there were low blocks; with `all`, they are added.
+    int ev = kFloor, E[CT];
+    // Returns whether some row may have lost something of V; with `all`, none does, and E has the rows' scales.
     const auto walk = [&](auto all) {
         bool low = false;
-        ev = 1;
+        ev = kFloor;
 #pragma unroll
         for (int c = 0; c < CT; ++c) st[c].reset();
         for (int tile = t0 + wave; tile < t1; tile += NW) {
@@ -665,10 +707,16 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
             rd.take(a, min(tile + NW, t1 - 1));
             rd.ask(a, table, min(tile + 2 * NW, t1 - 1));
             rd.scales(swk, swv), rd.k(kraw);
-            const float vkeep = ldexpf(1.0f, ev - ti.ev);
+            const float vkeep = all ? 1.0f : ldexpf(1.0f, ev - ti.ev);
             ev = ti.ev;
             h8 p[CT][SPLIT][2];
             softmax_tile<NB, CT, SPLIT>(sc, see, base, ti, vkeep, st, p);
+            if constexpr (all) {
+                v_in_bands<D, SMALL>(a, rd, table, tile, ti, see, p, st, E);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                continue;
+            }
 #pragma unroll
             for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -687,11 +735,7 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
                         }
                     __builtin_amdgcn_sched_barrier(0);  // (one step's operands at a time: the registers are counted)
                 }
-            if constexpr (all) {
-                if (ti.low) low_blocks<D, SMALL>(a, rd, table, tile, rt, ev, p, st);
-            } else {
-                low |= ti.low;
-            }
+            low |= ti.low;
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -700,9 +744,12 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         }
-        return low;
+        return low || ev > kGrown;
     };
-    if (REDO || walk(std::false_type{})) {
+    const bool again = REDO || walk(std::false_type{});
+#pragma unroll
+    for (int c = 0; c < CT; ++c) E[c] = again ? kFloor : ev;
+    if (again) {
         if (!REDO) {
             // (so that nothing of its addresses is kept through the first walk)
             asm volatile("" : "+v"(lane), "+v"(r), "+v"(g));
@@ -733,7 +780,7 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
         sum[c] = sink ? __builtin_amdgcn_exp2f(sk - off + kPShift) : 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) sum[c] += join[w][1][row] * __builtin_amdgcn_exp2f(join[w][0][row] - off);
-        const float f = sum[c] == 0.0f ? 0.0f : ldexpf(__builtin_amdgcn_exp2f(st[c].m - off) / sum[c], ev - kBias);
+        const float f = sum[c] == 0.0f ? 0.0f : ldexpf(__builtin_amdgcn_exp2f(st[c].m - off) / sum[c], E[c] - kBias);
 #pragma unroll
         for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= f;
     }
@@ -769,7 +816,7 @@ template <int D, int CT, bool SMALL, class T>
 __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k_attn_few(AttnArgs a) {
     few_rows<D, CT, SMALL, false, T>(a, blockIdx.y * 16 * CT, blockIdx.z);
 }
-// The rows of k_attn_many's workgroups that met low blocks: none as a rule, which takes 4-5 us with the launch. In one
+// The rows of k_attn_many's workgroups that have to be done again: none as a rule, which takes 4-5 us with the launch. In one
 // workgroup with the pass that found them, their scalars cost the f32 form's loop its registers (29 spilled instead of 9).
 template <int D, bool SMALL, class T>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void k_attn_redo(AttnArgs a, int row_tiles) {
@@ -785,9 +832,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_attn_redo(AttnArgs a, int
 // Many rows (prompts): a workgroup takes 128 rows, 32 a wave, and walks over the keys; its waves expand a tile's V together,
 // a tile ahead, into LDS as the second product wants it, [channel][64 keys] (rows 16 bytes apart in banks: a lane's 16-byte
 // reads of 16 channels touch every bank once). K needs no expansion: each wave reads its codes, which the workgroup's first
-// reader brings into L1, and keeps them in registers with the digits of its queries. A workgroup that meets low blocks leaves
-// them out and says so: its rows are then done again by the form of few rows (with low blocks in this loop, 4096 tokens at
-// 4096 took 539 us instead of 423).
+// reader brings into L1, and keeps them in registers with the digits of its queries. A workgroup whose blocks of V turn out to
+// be too far apart says so: its rows are then done again by the form of few rows (with low blocks in this loop, 4096 tokens
+// at 4096 took 539 us instead of 423).
 // 4096 tokens at 4096 keys, 32 heads over 8 of 128, bf16: 398 us, 1.04 PFLOP/s (a library product of 8192^3: 1.22). A tile
 // costs a wave 60 matrix instructions (about 970 cycles) and 147 vector instructions with 32 exponentials (about 890), of
 // which two waves a SIMD overlap little: the matrix pipe is busy 38% of the time. More waves do not fit the registers; the
@@ -856,7 +903,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
-    int ev = 1;
+    int ev = kFloor;
     int low = 0;
     TileInfo ti{}, next{};
     if (t0 < t1) {
@@ -956,7 +1003,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         ti = next;
         tile_barrier();
     }
-    if (lane == 0) *redo = low;
+    if (lane == 0) *redo = low | (ev > kGrown);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         const int row = w0 + 16 * c + r;

@@ -32,3 +32,72 @@ def test_windows_of_any_width_where_a_sequence_has_fewer_positions_than_new_toke
     _, out = _check_attn(s, 1, dtype, window=window)
     assert (out[:15] == 0).all() and (out[15:20] != 0).any(-1).all()
     assert (out[20:23] == 0).all() and (out[23:90] != 0).any(-1).all()
+
+
+# ---- blocks of V of all sizes -----------------------------------------------------------------------------------------
+
+def _v_scales(h: kd.Pages, head: int) -> np.ndarray:
+    """View of V's scale bytes, [pages][positions][blocks]."""
+    o = head * h.head_bytes + h.page * (h.dim + h.dim // 32)
+    return h.raw[:, o: o + h.page * (h.dim // 32)].reshape(h.n_pages, h.page, h.dim // 32)
+
+
+def _check_relative(s: Setup, group: int, dtype: str, window: int = 0) -> None:
+    """As _check_attn, without its absolute part: 2^-145 is left, for sums of parts that f32 holds as subnormals."""
+    q, qh = _rand(s.rng, (s.n_tok, s.heads_kv * group, s.dim), dtype)
+    got = ops.attn(s.cache, s.batch, q, window=window)[: s.tok].double().cpu().numpy()
+    ref, ax, vm = kd.attention(s.host, s.table, s.q_lens, s.kv_lens, qh[: s.tok], s.dim ** -0.5, window)
+    far = np.abs(ref) >= 2.0 ** 128  # f32's infinity
+    assert np.array_equal(got[far], np.copysign(np.inf, ref[far]))
+    tol = kd.attn_tolerance(dtype, s.dim, max(s.kv_lens), ref, ax, vm) - 1e-37 + 2.0 ** -145
+    bad = ~far & ~(np.abs(got - ref) <= tol)
+    assert not bad.any(), f"{bad.sum()} of {bad.size} off, rows {np.unique(np.nonzero(bad)[0])}"
+
+
+FORMS = [(64, 32, 3, False), (128, 64, 20, False), (64, 16, 50, False), (256, 32, 12, False), (128, 16, 100, False),
+         (128, 64, 140, True), (64, 32, 150, True), (256, 128, 70, True)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,page,q,many", FORMS)
+@pytest.mark.parametrize("least", [104, 60, 20])
+def test_rows_keep_what_they_see_beside_a_huge_block_that_they_do_not_see(least, dim, page, q, many, dtype):
+    """Everything at 2^(least - 127) and a few blocks of the largest scales, which rows before them and windows behind them do
+    not see."""
+    s = Setup([q, 2], [q + 90, 200], page, 1, dim, seed=least + dim, pad=MANY_ROWS if many else 0)
+    s.batch.desc.max_q = s.n_tok if many else q
+    v = _v_scales(s.host, 0)
+    v[:] = s.rng.integers(least, least + 4, v.shape)
+    for seq, pos, block, e in ((0, q + 89 - q // 2, 0, 254), (0, 40, 1, 253), (1, 199, dim // 32 - 1, 250)):
+        v[s.table[seq, pos // page], pos % page, block] = e
+    _upload(s)
+    _check_relative(s, 2, dtype)
+    _check_relative(s, 2, dtype, window=q // 3 + 1)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,page,q,many", FORMS)
+@pytest.mark.parametrize("least,most", [(100, 250), (20, 200), (60, 175), (112, 213), (75, 111), (74, 110)])
+def test_rows_keep_what_they_saw_before_a_tile_of_huge_blocks(least, most, dim, page, q, many, dtype):
+    """All blocks of the last positions (from 65 tokens on a whole tile) far above all others; rows before them see the small
+    ones only."""
+    kv = (q + 70) // 64 * 64 + 384  # the last new token sits at the end of a tile; more tiles than waves
+    s = Setup([q], [kv], page, 1, dim, seed=least + dim, pad=MANY_ROWS if many else 0)
+    s.batch.desc.max_q = s.n_tok if many else q
+    v = _v_scales(s.host, 0)
+    first = kv - min(q - 1, 64)
+    for pos in range(kv):
+        v[s.table[0, pos // page], pos % page] = least if pos < first else most
+    _upload(s)
+    _check_relative(s, 2, dtype)
+
+
+@pytest.mark.parametrize("dim,page,q,many", FORMS)
+@pytest.mark.parametrize("least,dtype", [(1, "f32"), (5, "f32"), (30, "f32"), (72, "f32"), (108, "f32"), (30, "bf16"), (72, "bf16")])
+def test_small_values_keep_their_bits(least, dim, page, q, many, dtype):
+    s = Setup([q], [q + 90], page, 1, dim, seed=least + dim, pad=MANY_ROWS if many else 0)
+    s.batch.desc.max_q = s.n_tok if many else q
+    v = _v_scales(s.host, 0)
+    v[:] = s.rng.integers(least, least + 4, v.shape)
+    _upload(s)
+    _check_relative(s, 2, dtype)
