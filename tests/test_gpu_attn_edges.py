@@ -101,3 +101,49 @@ def test_small_values_keep_their_bits(least, dim, page, q, many, dtype):
     v[:] = s.rng.integers(least, least + 4, v.shape)
     _upload(s)
     _check_relative(s, 2, dtype)
+
+
+# ---- contexts divided among workgroups --------------------------------------------------------------------------------
+
+def _splits(s: Setup, group: int, dtype: str) -> int:
+    """From the size of the workspace: a row of f32 and two numbers a split, token and head."""
+    H = s.heads_kv * group
+    q = torch.empty(s.n_tok, H, s.dim, dtype=torch.float32 if dtype == "f32" else torch.bfloat16, device="cuda")
+    return ops.attn_workspace(s.cache, s.batch, q).numel() // (s.n_tok * H * (4 * s.dim + 8))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page,q_lens,kv_lens,window,sinks,least", [
+    (16, [1], [5003], 0, False, 17),          # joined a workgroup a row, 20 splits with keys
+    (64, [1], [16384], 0, True, 64),          # 64
+    (32, [1], [9000], 3000, False, 17),       # a window's edge inside a split, and splits without keys
+    (16, [4, 1, 0, 3], [900, 70, 5, 700], 0, True, 2),  # joined a wave a row, sequences of other lengths
+    (128, [3, 5], [2500, 1900], 1000, False, 2),
+    (32, [20], [3000], 0, False, 2),          # more than a tile of rows
+    (16, [2], [4100], 77, True, 2),           # the window in one split
+])
+def test_divided_contexts(page, q_lens, kv_lens, window, sinks, least, dim, dtype):
+    s = Setup(q_lens, kv_lens, page, 1 if max(kv_lens) > 9000 else 2, dim, seed=89 + dim, pad=1)
+    assert _splits(s, 4, dtype) >= least
+    _check_attn(s, 4, dtype, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 32)])
+@pytest.mark.parametrize("q,window", [(1, 0), (5, 0), (5, 2000), (40, 0)])
+def test_divided_contexts_with_odd_places(q, window, dim, page, dtype):
+    """Missing pages, a huge block of V and a tiny one in one split each; then a NaN in V and one in K."""
+    s = Setup([q, 1], [4000, 2600], page, 1, dim, seed=97 + dim)
+    assert _splits(s, 3, dtype) >= 4
+    v = _v_scales(s.host, 0)
+    for seq, pos, block, e in ((0, 3999 - q // 2, 0, 170), (0, 1000, 1, 60), (1, 2599, 1, 180), (1, 30, 0, 50)):
+        v[s.table[seq, pos // page], pos % page, block] = e
+    s.table[0, [3500 // page, 2222 // page]] = [-1, s.host.n_pages]
+    _upload(s)
+    _check_attn(s, 3, dtype, window)
+    v[s.table[0, 3100 // page], 3100 % page, 0] = 255
+    page_of = s.table[1, 77 // page]
+    s.host.raw[page_of, page * dim + 77 % page * (dim // 32)] = 255
+    _upload(s)
+    _check_attn(s, 3, dtype, window)
