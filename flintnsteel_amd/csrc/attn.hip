@@ -238,7 +238,7 @@ __device__ __forceinline__ int query_digits(Digits<D, T> &w, const T *row, bool 
     top = max(top, xor_lane_i<32>(top));
     const float in_log2 = scale * kLog2e, amax = __builtin_bit_cast(float, top) * fabsf(in_log2);
     const bool bad = !(amax < INFINITY);
-    // (below 2^-100 the row is smaller than any difference that a score can show)
+    // (the last digit's scale byte is 125 + k - 25 at least: a smaller row enters with digits of a row at 2^-100)
     const int k = amax < 7.8886090522101181e-31f ? -100 : (int) (__builtin_bit_cast(uint32_t, amax) >> 23) - 126;  // amax < 2^k
     const float f = in_log2 * ldexpf(1.0f, 2 - k);
 #pragma unroll
@@ -414,7 +414,7 @@ __device__ __forceinline__ void softmax_tile(f4 (&s)[CT][4], const Sight (&see)[
                 const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
                 w[0][i] = __builtin_bit_cast(uint32_t, hi);
                 if constexpr (SPLIT == 2) {
-                    float x1, y1;  // what hi leaves, exactly, without a conversion first (f32, 4096 tokens at 8192: 644 us to 620)
+                    float x1, y1;  // what hi leaves, exactly, without a conversion first (f32, 4096 tokens at 4096: 4% less time)
                     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(x1) : "v"(w[0][i]), "v"(x));
                     asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(y1) : "v"(w[0][i]), "v"(y));
                     w[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x1, y1));
@@ -586,10 +586,11 @@ __device__ __forceinline__ void v_in_bands(const AttnArgs &a, TileReader<D, SMAL
 // from the pages to registers and stays there: S^T = K Q^T with K's rows in an order that leaves every lane with the 16
 // consecutive keys 16 g .. 16 g + 15 of its query row, which is where the second product, O^T = V^T P^T, wants P, and where
 // V's bytes (16 consecutive positions of a channel pair) are. Bound by the cache's bytes for one long context (131072 keys of
-// 8 heads, bf16: 143 MB in 26 us, 5.5 TB/s; the pages' pattern of loads alone reaches 5.5), by the vector pipe's work on a
-// tile for f32 and many contexts (48 to 16000 keys: 272 MB in 60 us, 4.5 TB/s: 260 vector and 56 matrix instructions a tile
-// of 64 keys, at about 4.3 cycles a vector instruction with three waves a SIMD), by a few dependent loads for short ones (500
-// keys: 9 us). What pays is waves, so the queries lie in LDS and the next tile's K is asked for when this one's is used up;
+// 8 heads, bf16: 143 MB in 26 us, 5.5 TB/s; the pages' pattern of loads alone reaches 5.5), by uneven shares for many (48 of
+// up to 16000 keys, f32: 272 MB in 59 us, 4.6 TB/s: 920 workgroups have keys and 768 fit at once, so that the busiest place
+// does 17 tiles a wave where 10 would be its share; the 260 vector and 56 matrix instructions of a tile, one after another,
+// are 26 us), by the start and a few dependent loads for short ones (500 keys: 9 us; 8 sequences of 4096, 4 tokens: two tiles a
+// wave, 16 us). What pays is waves, so the queries lie in LDS and the next tile's K is asked for when this one's is used up;
 // workgroups of 8 waves, or four waves a SIMD at 128 registers, were slower (48 contexts: 84 and 76 us where this took 74).
 // A wave whose blocks of V turn out to be too far apart walks once more, by v_in_bands. REDO: that is known.
 template <int D, int CT, bool SMALL, bool REDO, class T>
@@ -835,7 +836,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void k_attn_redo(AttnArgs a, int
 // reader brings into L1, and keeps them in registers with the digits of its queries. A workgroup whose blocks of V turn out to
 // be too far apart says so: its rows are then done again by the form of few rows (with low blocks in this loop, 4096 tokens
 // at 4096 took 539 us instead of 423).
-// 4096 tokens at 4096 keys, 32 heads over 8 of 128, bf16: 398 us, 1.04 PFLOP/s (a library product of 8192^3: 1.22). A tile
+// 4096 tokens at 4096 keys, 32 heads over 8 of 128, bf16: 395 us, 1.04 PFLOP/s (a library product of 8192^3: 1.22; f32,
+// whose five digits and two halves of p are 112 matrix instructions instead of 60: 566 us). A tile
 // costs a wave 60 matrix instructions (about 970 cycles) and 147 vector instructions with 32 exponentials (about 890), of
 // which two waves a SIMD overlap little: the matrix pipe is busy 38% of the time. More waves do not fit the registers; the
 // expansion of V among the first product's instructions, which helps bf16 (by 3%), costs heads of 256 channels 6 to 18%.

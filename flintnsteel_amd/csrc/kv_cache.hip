@@ -132,8 +132,10 @@ template <class F> __device__ __forceinline__ uint32_t hold8(const F (&v)[8], in
 // channels a thread: 2 D threads hold the 16 rows of a head. K and V are asked for before the angles are computed, a query
 // before the last one is stored, and the queries of the group's tokens are dealt to all threads: in turns by the threads of
 // their rows, one token's took as long as everything else (one token, 8 kv heads of 4 queries: 8.0 us, now 5.9; 61 sequences:
-// 10.0, now 5.9). For many tokens bound by the bytes: 4001 tokens, 168 MB in 34 us (a copy of them: 35); there it is waves
-// that pay, and a query's loads before the angles' arithmetic cost more registers than they hide (38 us).
+// 10.0, now 5.9). Few tokens are bound by what waits for what: the range, the table entry, the row, V's columns through LDS
+// (replayed, one token: 4.0 us without queries or rotation; the angles add 0.7, the queries' turn 0.7). Many by the bytes: 4001
+// tokens, 168 MB in 34 us (a copy of them: 35; bf16, 86 MB: 34); there it is waves that pay, and a query's loads before the
+// angles' arithmetic cost more registers than they hide (38 us).
 template <int D, int ROPE, class T>
 __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_append(AppendArgs a) {
     constexpr int NT = 2 * D, NR = D / 8;
@@ -230,8 +232,9 @@ __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_ap
     }
 }
 
-// Values of the batch's tokens as the cache holds them; NaN where a position has no page. Bound by what it writes (4001 tokens
-// of 8 heads of 128, 33 MB of f32: 11 us).
+// Values of the batch's tokens as the cache holds them; NaN where a position has no page. 4001 tokens of 8 heads of 128: 11 us,
+// for 33 MB written and 19.5 read; the tokens hold 4.4, but a thread takes its byte out of each of V's columns, whose lines the
+// next tokens' workgroups read again. A copy of 37 MB takes 8.
 template <int D>
 __global__ __launch_bounds__(256) void k_kv_read(KvView c, BatchView b, float *k, float *v) {
     const int s = blockIdx.y / c.n_kv, head = blockIdx.y % c.n_kv;

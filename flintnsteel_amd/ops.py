@@ -651,8 +651,8 @@ class KvCache:
 class KvBatch:
     """New tokens of some sequences over a KvCache (FnsKvBatch): q_start [n_seq + 1], kv_len [n_seq] and page_table
     [n_seq][pages of a sequence] int32 device tensors, whose values a captured graph takes anew at each replay; n_tok rows of
-    the token arrays, max_q at least the new tokens of any sequence, max_kv about the longest sequence (None: what the table
-    has room for)."""
+    the token arrays, max_q at least the new tokens of any sequence, max_kv about the longest sequence, by which attn divides its
+    work (None: what the table has room for; results are right, but far shorter contexts than that are divided badly)."""
 
     def __init__(self, q_start: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, n_tok: int, max_q: int,
                  max_kv: int | None = None):

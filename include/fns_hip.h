@@ -326,7 +326,9 @@ size_t fns_hip_kv_page_bytes(int n_head_kv, int head_dim, int page_size);
  * memory (a captured graph takes their values at each replay); the numbers below are the host's:
  *   n_tok   rows of the token arrays: tokens from q_start[n_seq] on are padding and left alone
  *   max_q   at least the new tokens of any sequence (more than this many are not handled)
- *   max_kv  about the longest kv_len: work is split by it, results hold for any
+ *   max_kv  about the longest kv_len: work is divided by it, results hold for any. Far too large (or with a window far shorter)
+ *           it leaves fns_hip_attn few workgroups with keys: one token at 4096 keys takes 11 us, with a max_kv of 131072 or a
+ *           window of 4096 in 131072 keys 19-21
  * A q_start range outside 0..n_tok or descending is a sequence without tokens. A position whose table entry is outside the
  * table or the cache's pages is never read or written: append leaves it out, attention sees no key there, kv_read gives NaN. */
 typedef struct FnsKvBatch {
@@ -343,8 +345,8 @@ typedef struct FnsKvBatch {
 /* k, v [n_tok][n_head_kv][head_dim] (tokens k_stride / v_stride elements apart) into the cache; the first rope_dim channels
  * of k and of q are turned by position * inv_freq[i] on the way (in 64 bits; k is held from the unrounded result). q
  * [n_tok][n_head][head_dim] -> q_out of the same type, n_head a multiple of n_head_kv, or n_head = 0: no queries. q_out may
- * be q (with its stride). Heads are contiguous within a token; no alignment beyond an element's is needed. Positions that
- * two sequences share (a common page) must not be appended by both in one call. */
+ * be q (with its stride) and overlaps nothing else. Heads are contiguous within a token; no alignment beyond an element's is
+ * needed. Positions that two sequences share (a common page) must not be appended by both in one call. */
 typedef struct FnsKvAppend {
     int dtype; /* of k, v, q and q_out: FNS_TYPE_F32 or FNS_TYPE_BF16 */
     int rope;  /* FNS_ROPE_* */
@@ -362,13 +364,18 @@ int fns_hip_kv_read(const FnsKvCache *cache, const FnsKvBatch *batch, float *k, 
 /* Attention of the batch's tokens over the cache (their own keys included: append first). Query head h reads kv head
  * h / (n_head / n_head_kv). The token at position p sees positions 0..p, with window > 0 the last `window` of them.
  *   out = sum_j p_j V_j, p = softmax over the seen positions of scale * q . K_j; with sinks, exp(sinks[h]) joins the
- *   softmax's denominator. A row that sees nothing is zero; one that sees a token whose K or V holds a NaN block is NaN.
- * A row of q that holds a NaN or an infinity gives NaN (where it sees anything).
+ *   softmax's denominator (-infinity: nothing; +infinity or a NaN: NaNs). A row that sees nothing is zero; one that sees a token
+ *   whose K or V holds a NaN block is NaN.
+ * A row of q that holds a NaN or an infinity, or a scale * q beyond f32, gives NaN (where it sees anything); so does a score
+ * beyond f32.
  * q and out [n_tok][n_head][head_dim], heads contiguous within a token, no overlap, any element alignment. What q enters the
- * products with is within 2^-24 (FNS_TYPE_F32) or 2^-14 (FNS_TYPE_BF16) of its row's largest magnitude, p carries 22 or 11
- * bits, and the sum of p counts the same values; softmax statistics and sums are f32. workspace: fns_hip_attn_workspace bytes
- * (they depend on the numbers of the batch and on n_head, not on device memory; fewer tokens can need more), 16-byte
- * aligned, no initialisation; calls that overlap in time need one each. */
+ * products with is within 2^-24 (FNS_TYPE_F32) or 2^-14 (FNS_TYPE_BF16) of its row's largest magnitude (where all of
+ * scale * log2(e) * q is below 2^-100: that part of 2^-101), p carries 22 or 11 bits, cut toward zero, and the sum of p counts
+ * the same values; softmax statistics and sums are f32. Blocks of V of any size that a row does not see leave its precision alone.
+ * One call takes one form for all its sequences, by max_q: decode tokens over long contexts beside a long prompt go undivided
+ * (31 at 8000 keys beside a prompt of 512: 222 us, apart 53 and 20), and are better a call of their own.
+ * workspace: fns_hip_attn_workspace bytes (they depend on the numbers of the batch and on n_head, not on device memory; fewer
+ * tokens can need more), 16-byte aligned, no initialisation; calls that overlap in time need one each. */
 typedef struct FnsAttn {
     int dtype; /* of q and out: FNS_TYPE_F32 or FNS_TYPE_BF16 */
     int n_head;

@@ -103,6 +103,34 @@ def test_small_values_keep_their_bits(least, dim, page, q, many, dtype):
     _check_relative(s, 2, dtype)
 
 
+# ---- sizes of queries and keys ----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,page,q,many", FORMS)
+def test_powers_of_two_between_queries_and_keys(dim, page, q, many, dtype):
+    """q 2^-n and K 2^n give the bits of q and K, as long as scale * log2(e) * q reaches 2^-100; below, a score is off by up to
+    2^-125 sum |K| of log2 units."""
+    s = Setup([q], [q + 90], page, 1, dim, seed=101 + dim, pad=MANY_ROWS if many else 0)
+    s.batch.desc.max_q = s.n_tok if many else q
+    x, _ = _rand(s.rng, (s.n_tok, 2, dim), dtype)
+    want = ops.attn(s.cache, s.batch, x)[: s.tok]
+    k = s.host.raw[:, page * dim: page * dim + page * (dim // 32)]
+    keep = k.copy()
+    for n in (-100, 50, 95, 118):
+        k[:] = keep.astype(int) + n
+        _upload(s)
+        small = x * 2.0 ** -n
+        got = ops.attn(s.cache, s.batch, small)[: s.tok]
+        if n < 100:
+            assert torch.equal(got, want), n
+            continue
+        ref, ax, vm = kd.attention(s.host, s.table, s.q_lens, s.kv_lens, small.double().cpu().numpy()[: s.tok], dim ** -0.5)
+        most = np.abs(s.host.get(np.repeat(np.arange(s.host.n_pages), page), np.tile(np.arange(page), s.host.n_pages), 0)[0]).sum(-1).max()
+        tol = kd.attn_tolerance(dtype, dim, q + 90, ref, ax, vm)
+        tol = tol + 2 * np.log(2) * 2.0 ** -125 * most * vm[..., None] * (1 if dtype == "f32" else 2 ** 10)
+        assert (np.abs(got.double().cpu().numpy() - ref) <= tol).all()
+
+
 # ---- contexts divided among workgroups --------------------------------------------------------------------------------
 
 def _splits(s: Setup, group: int, dtype: str) -> int:
