@@ -366,8 +366,8 @@ int fns_hip_kv_read(const FnsKvCache *cache, const FnsKvBatch *batch, float *k, 
  *   out = sum_j p_j V_j, p = softmax over the seen positions of scale * q . K_j; with sinks, exp(sinks[h]) joins the
  *   softmax's denominator (-infinity: nothing; +infinity or a NaN: NaNs). A row that sees nothing is zero; one that sees a token
  *   whose K or V holds a NaN block is NaN.
- * A row of q that holds a NaN or an infinity, or a scale * q beyond f32, gives NaN (where it sees anything); so does a score
- * beyond f32.
+ * A row of q that holds a NaN or an infinity, or a scale * q beyond f32, gives NaN (where it sees anything); scores beyond f32
+ * may.
  * q and out [n_tok][n_head][head_dim], heads contiguous within a token, no overlap, any element alignment. What q enters the
  * products with is within 2^-24 (FNS_TYPE_F32) or 2^-14 (FNS_TYPE_BF16) of its row's largest magnitude (where all of
  * scale * log2(e) * q is below 2^-100: that part of 2^-101), p carries 22 or 11 bits, cut toward zero, and the sum of p counts

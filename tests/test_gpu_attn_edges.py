@@ -131,6 +131,29 @@ def test_powers_of_two_between_queries_and_keys(dim, page, q, many, dtype):
         assert (np.abs(got.double().cpu().numpy() - ref) <= tol).all()
 
 
+@pytest.mark.parametrize("dim,page,q,many", FORMS + [(128, 64, 1, False)])
+def test_sinks_and_queries_beyond_f32(dim, page, q, many):
+    """Sinks of +infinity and NaN make their heads NaN, of -infinity are none; a row whose scale * q is beyond f32 is NaN; the
+    other heads and rows keep their bits."""
+    kv = q + 90 if q > 1 else 3000  # (divided)
+    s = Setup([q], [kv], page, 1, dim, seed=103 + dim, pad=MANY_ROWS // 4 if many else 0)
+    s.batch.desc.max_q = s.n_tok if many else q
+    x, _ = _rand(s.rng, (s.n_tok, 4, dim))
+    inf, some = float("inf"), torch.tensor([0.5, -1.0, 2.0, 0.0], device="cuda")
+    want, none = (ops.attn(s.cache, s.batch, x, sinks=t)[: s.tok] for t in (some, None))
+    odd = some.clone()
+    odd[0], odd[2], odd[3] = inf, -inf, float("nan")
+    got = ops.attn(s.cache, s.batch, x, sinks=odd)[: s.tok]
+    assert torch.isnan(got[:, [0, 3]]).all() and torch.equal(got[:, 1], want[:, 1]) and torch.equal(got[:, 2], none[:, 2])
+    x[q // 2, 1, dim - 1] = 3e38
+    got = ops.attn(s.cache, s.batch, x, scale=2.0)[: s.tok]
+    assert torch.isnan(got[q // 2, 1]).all()
+    x[q // 2, 1, dim - 1] = 0.0
+    want = ops.attn(s.cache, s.batch, x, scale=2.0)[: s.tok]
+    got[q // 2, 1] = want[q // 2, 1]
+    assert torch.equal(got, want)
+
+
 # ---- contexts divided among workgroups --------------------------------------------------------------------------------
 
 def _splits(s: Setup, group: int, dtype: str) -> int:
