@@ -29,6 +29,9 @@ constexpr int kBand = 36;     // block scales from E down that f16 holds exactly
 // E starts at 2^-17 (V below that is exact too, down to 2^-53), and where it has grown by more than 2^100, sums from before
 // may be next to f32's subnormals: a row has at least 2^8 of p, times 2^(12 - 36) of a block, so 2^-16 before the growth.
 constexpr int kFloor = 110, kGrown = kFloor + 100;
+// A split's mean of V is kept 2^2 down: codes of the largest scale are 1.5 times 2^129, and where such a key weighs little in the
+// row it may be all of its split.
+constexpr int kPart = 2;
 // p is carried times 2^8: its low half stays clear of f16's subnormals. Sums are rescaled only where a row's maximum has
 // grown by more than 2^7 since the last time, so p stays below 2^15.
 constexpr float kPShift = 8.0f, kLazy = 7.0f;
@@ -45,7 +48,7 @@ struct AttnArgs {
     const void *q;
     void *out;
     const float *sinks;
-    float *part;      // [split][n_tok * n_head][D] partial results, each already a weighted mean
+    float *part;      // [split][n_tok * n_head][D] partial results, each already a weighted mean, 2^-kPart of it
     float2 *part_ml;  // [split][n_tok * n_head] their maximum (log2) and sum
     int64_t q_stride, out_stride;
     int n_head, group, window, splits, chunk;
@@ -781,7 +784,8 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
         sum[c] = sink ? __builtin_amdgcn_exp2f(sk - off + kPShift) : 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) sum[c] += join[w][1][row] * __builtin_amdgcn_exp2f(join[w][0][row] - off);
-        const float f = sum[c] == 0.0f ? 0.0f : ldexpf(__builtin_amdgcn_exp2f(st[c].m - off) / sum[c], E[c] - kBias);
+        const int unit = E[c] - kBias - (a.splits > 1 ? kPart : 0);
+        const float f = sum[c] == 0.0f ? 0.0f : ldexpf(__builtin_amdgcn_exp2f(st[c].m - off) / sum[c], unit);
 #pragma unroll
         for (int d = 0; d < 2 * NB; ++d) st[c].o[d] *= f;
     }
@@ -1071,6 +1075,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int rows_per_wg) 
     T t[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+        o[c] *= (float) (1 << kPart);
         if constexpr (sizeof(T) == 4) t[c] = o[c];
         else t[c] = to_bf16(o[c]);
     }

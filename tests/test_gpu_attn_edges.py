@@ -198,3 +198,17 @@ def test_divided_contexts_with_odd_places(q, window, dim, page, dtype):
     s.host.raw[page_of, page * dim + 77 % page * (dim // 32)] = 255
     _upload(s)
     _check_attn(s, 3, dtype, window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 32)])
+@pytest.mark.parametrize("q,kv", [(1, 300), (1, 5121), (3, 4097), (20, 3009)])  # (the last key in a split of its own)
+def test_values_of_v_beyond_f32_with_small_weights(q, kv, dim, page, dtype):
+    """Codes of the largest scales stand for up to 6 * 2^127; a weight of one in a thousand makes them ordinary f32 numbers, divided
+    or not."""
+    s = Setup([q], [kv], page, 1, dim, seed=107 + dim)
+    v = _v_scales(s.host, 0)
+    for pos in (kv // 2, kv // 2 + 1, kv - 1):
+        v[s.table[0, pos // page], pos % page] = 254
+    _upload(s)
+    _check_attn(s, 3, dtype, std=0.1)
