@@ -21,6 +21,7 @@ class FnsError(RuntimeError):
 
 
 _P, _I64, _I, _SZ, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
+_D = ctypes.c_double
 
 # argtypes of every exported entry point (all return int status unless listed in _RESTYPE).
 SIGNATURES: dict[str, list] = {
@@ -89,6 +90,14 @@ SIGNATURES: dict[str, list] = {
     "fns_hip_kv_append": [_P, _P, _P, _P],
     "fns_hip_kv_read": [_P, _P, _P, _P, _P],
     "fns_hip_attn_workspace": [_P, _P, _P, _P],
+    "fns_hip_rope_scaled": [_I, _D, _D, _D, _D, _D, _P, _P],
+    "fns_hip_kv_append_at": [_P, _P, _P, _P, _F, _P],
+    "fns_hip_tree_plan": [_P, _P, _P, _I, _P, _P, _P],
+    "fns_hip_attn_tree": [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "fns_hip_kv_weigh_workspace": [_P, _P, _P, _P],
+    "fns_hip_kv_weigh": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "fns_hip_kv_evict": [_P, _P, _P, _P],
+    "fns_hip_kv_keep": [_P, _P, _P, _P],
     "fns_hip_attn": [_P, _P, _P, _P, _P, _P, _SZ, _P],
     "fns_hip_dense_ffn_workspace": [_P, _I64, _P],
     "fns_hip_dense_ffn": [_P, _P, _P, _I64, _P, _SZ, _P],

@@ -248,6 +248,44 @@ int fns_hip_kv_append(const FnsKvCache *cache, const FnsKvBatch *batch, const Fn
     return impl::kv_append(cache, batch, x, S(stream));
 }
 
+int fns_hip_rope_scaled(int rope_dim, double base, double factor, double original, double fast, double slow, float *inv_freq,
+                        float *magnitude) {
+    return impl::rope_scaled(rope_dim, base, factor, original, fast, slow, inv_freq, magnitude);
+}
+
+int fns_hip_kv_append_at(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvAppend *x, const int32_t *pos,
+                         float magnitude, void *stream) {
+    return impl::kv_append_at(cache, batch, x, pos, magnitude, S(stream));
+}
+
+int fns_hip_tree_plan(const FnsKvBatch *batch, const int32_t *parents, const int32_t *base, int words, uint64_t *sees,
+                      int32_t *pos, void *stream) {
+    return impl::tree_plan(batch, parents, base, words, sees, pos, S(stream));
+}
+
+int fns_hip_attn_tree(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const FnsKvTree *tree, const void *q,
+                      void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+    return impl::attn_tree(cache, batch, x, tree, q, out, lse, workspace, workspace_bytes, S(stream));
+}
+
+int fns_hip_kv_weigh_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, size_t *bytes) {
+    return impl::kv_weigh_workspace(cache, batch, x, bytes);
+}
+
+int fns_hip_kv_weigh(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const FnsKvTree *tree, const void *q,
+                     const float *lse, const float *past, float *weights, void *workspace, size_t workspace_bytes,
+                     void *stream) {
+    return impl::kv_weigh(cache, batch, x, tree, q, lse, past, weights, workspace, workspace_bytes, S(stream));
+}
+
+int fns_hip_kv_evict(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvEvict *x, void *stream) {
+    return impl::kv_evict(cache, batch, x, S(stream));
+}
+
+int fns_hip_kv_keep(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvKeep *x, void *stream) {
+    return impl::kv_keep(cache, batch, x, S(stream));
+}
+
 int fns_hip_kv_read(const FnsKvCache *cache, const FnsKvBatch *batch, float *k, float *v, void *stream) {
     return impl::kv_read(cache, batch, k, v, S(stream));
 }

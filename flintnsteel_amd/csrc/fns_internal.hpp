@@ -111,10 +111,20 @@ int add_rms_norm_q8_1(const float *x, const float *y, const float *w, float *sum
 int dequantize_q8_1(const void *xq, int dtype, void *x, void *sums, int64_t ncols, int64_t nrows, hipStream_t st);
 size_t kv_page_bytes(int n_head_kv, int head_dim, int page_size);
 int kv_append(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, hipStream_t st);
+int kv_append_at(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, const int32_t *pos, float magnitude, hipStream_t st);
 int kv_read(const FnsKvCache *c, const FnsKvBatch *b, float *k, float *v, hipStream_t st);
 int attn_workspace(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, size_t *bytes);
 int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void *q, void *out, void *ws, size_t ws_bytes,
          hipStream_t st);
+int rope_scaled(int rope_dim, double base, double factor, double original, double fast, double slow, float *inv_freq, float *magnitude);
+int tree_plan(const FnsKvBatch *b, const int32_t *parents, const int32_t *base, int words, uint64_t *sees, int32_t *pos, hipStream_t st);
+int attn_tree(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const FnsKvTree *t, const void *q, void *out, float *lse,
+              void *ws, size_t ws_bytes, hipStream_t st);
+int kv_weigh_workspace(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, size_t *bytes);
+int kv_weigh(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const FnsKvTree *t, const void *q, const float *lse,
+             const float *past, float *weights, void *ws, size_t ws_bytes, hipStream_t st);
+int kv_evict(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvEvict *x, hipStream_t st);
+int kv_keep(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvKeep *x, hipStream_t st);
 
 int fill_normal(float *out, int64_t n, uint64_t seed, uint64_t offset, float mean, float std, hipStream_t st);
 int quantize_weights(int type, const float *x, void *out, int64_t nrows, int64_t ncols, hipStream_t st);

@@ -2,14 +2,15 @@
 //
 // Append. A token of a batch brings k and v of every kv head (and its queries); its position is the sequence's length
 // less the tokens after it. With a rotation, a pair of channels (a, b) of k and q becomes
-//   (a cos t - b sin t, a sin t + b cos t),  t = position * inv_freq[i],
-// and k and v go into the cache in 4 bits, k from the rotated value before any rounding. The rotation and the block
+//   m (a cos t - b sin t, a sin t + b cos t),  t = position * inv_freq[i],
+// (position: in the cache, or the token's own; m: 1, or the magnitude that goes with frequencies scaled for a long context) and k and v go into the cache in 4 bits, k from the rotated value before any rounding. The rotation and the block
 // arithmetic are done in 64 bits: an f32 angle of a far position is off by its spacing (4e-3 at position 65536), and a
 // 4-bit code next to a border would depend on the last bit of a 32-bit rotation. The pass moves the bytes of q, k and
 // v and is bound by them (and by its launch for a few tokens), not by this arithmetic.
 #include "fns_kv.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 #include "fns/kernels.h"
 #include "fns_common.hpp"
@@ -32,6 +33,8 @@ struct AppendArgs {
     const float *inv_freq;
     int64_t k_stride, v_stride, q_stride, qo_stride;
     int rope_dim, n_group;  // n_group: query heads of a kv head (0: no queries)
+    const int32_t *at;      // [n_tok] what the tokens are turned by, or null: their positions in the cache
+    double magnitude;
 };
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
@@ -169,12 +172,13 @@ __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_ap
         const int half = a.rope_dim / 2;
         for (int i = tid; i < (hi - lo) * half; i += NT) {
             const int p = lo + i / half, c = i % half;
+            const int by = a.at ? a.at[r.q0 + (p - first)] : p;
             // in turns: the product is exact to 53 bits, its whole part leaves no error
-            double turns = (double) p * (double) a.inv_freq[c] * 0.15915494309189533577;
+            double turns = (double) by * (double) a.inv_freq[c] * 0.15915494309189533577;
             turns -= rint(turns);
             double sn, cn;
             sincospi(2.0 * turns, &sn, &cn);
-            cs[(p - base) * (D / 2) + c] = make_double2(cn, sn);
+            cs[(p - base) * (D / 2) + c] = make_double2(cn * a.magnitude, sn * a.magnitude);
         }
         __syncthreads();
     }
@@ -300,7 +304,9 @@ size_t kv_page_bytes(int n_head_kv, int head_dim, int page_size) {
     return (size_t) n_head_kv * dev::kv_head_bytes(head_dim, page_size);
 }
 
-int kv_append(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, hipStream_t st) {
+int kv_append(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, hipStream_t st) { return kv_append_at(c, b, x, nullptr, 1.0f, st); }
+
+int kv_append_at(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, const int32_t *pos, float magnitude, hipStream_t st) {
     FNS_TRY(host::kv_check(c, b, "kv_append"));
     if (!x) return host::set_error(host::ERR_SHAPE, "kv_append: null arguments");
     if (x->dtype != FNS_TYPE_F32 && x->dtype != FNS_TYPE_BF16)
@@ -312,6 +318,8 @@ int kv_append(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, hi
     if (x->rope != FNS_ROPE_NONE && (!x->inv_freq || x->rope_dim <= 0 || x->rope_dim > D || x->rope_dim % 16))
         return host::set_error(host::ERR_SHAPE, "kv_append: a rotation needs inv_freq and a rope_dim that is a multiple of 16 up to head_dim (%d)",
                                x->rope_dim);
+    if (x->rope != FNS_ROPE_NONE && !(magnitude > 0.0f && magnitude < INFINITY))
+        return host::set_error(host::ERR_SHAPE, "kv_append: the rotation's magnitude must be positive and finite (%g)", magnitude);
     if (x->n_head < 0 || x->n_head % c->n_head_kv)
         return host::set_error(host::ERR_SHAPE, "kv_append: n_head %d is no multiple of n_head_kv %d", x->n_head, c->n_head_kv);
     if (b->n_seq == 0 || b->n_tok == 0 || b->max_q == 0) return host::OK;
@@ -322,7 +330,7 @@ int kv_append(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x, hi
     if (x->n_head > 0 && x->q == x->q_out && x->q_stride != x->q_out_stride)
         return host::set_error(host::ERR_SHAPE, "kv_append: queries rotated in place keep their stride");
     AppendArgs a{host::kv_view(c), host::kv_batch(b), x->k, x->v, x->q, x->q_out, x->inv_freq, x->k_stride, x->v_stride,
-                 x->q_stride, x->q_out_stride, x->rope_dim, x->n_head / c->n_head_kv};
+                 x->q_stride, x->q_out_stride, x->rope_dim, x->n_head / c->n_head_kv, pos, magnitude};
     // new tokens of a sequence start anywhere in a group
     const int64_t most = std::min<int64_t>(b->max_q, b->n_tok);
     const dim3 grid((unsigned) ((most + kGroup - 2) / kGroup + 1), (unsigned) (b->n_seq * c->n_head_kv));
@@ -363,6 +371,9 @@ int kv_read(const FnsKvCache *c, const FnsKvBatch *b, float *k, float *v, hipStr
 namespace k {
 void kv_append(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsKvAppend &x, hipStream_t st) {
     host::abort_on_error(impl::kv_append(&cache, &batch, &x, st), "kv_append");
+}
+void kv_append_at(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsKvAppend &x, const int32_t *pos, float magnitude, hipStream_t st) {
+    host::abort_on_error(impl::kv_append_at(&cache, &batch, &x, pos, magnitude, st), "kv_append_at");
 }
 void kv_read(const FnsKvCache &cache, const FnsKvBatch &batch, float *k, float *v, hipStream_t st) {
     host::abort_on_error(impl::kv_read(&cache, &batch, k, v, st), "kv_read");

@@ -1,0 +1,373 @@
+// kv_tree.hip - what changes a paged 4-bit cache (fns_kv.hpp) after its tokens were appended: the bits of a tree of drafted
+// tokens, the accepted path made the sequence's own, eviction by accumulated attention weight. For MI355X gfx950.
+#include "fns_kv.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+#include "fns/kernels.h"
+#include "fns_common.hpp"
+#include "fns_host.hpp"
+#include "fns_internal.hpp"
+
+namespace fns {
+
+using namespace fns::dev;
+
+namespace {
+
+constexpr int kMaxWords = 16, kMaxNew = 64 * kMaxWords;
+
+// A workgroup a sequence, a thread a token: up the parents, which get smaller at every step, once to see that they end at -1
+// and how many they are, once to set the bits, a word at a time. Bound by the longest path's LDS reads.
+__global__ __launch_bounds__(256) void k_tree_plan(BatchView b, const int32_t *parents, const int32_t *base, int words, uint64_t *sees,
+                                                   int32_t *pos) {
+    __shared__ int up[kMaxNew];
+    const int s = blockIdx.x;
+    const SeqRange r = seq_range(b, s);
+    const int n = min(r.n, 64 * words);
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int p = parents[r.q0 + i];
+        up[i] = p >= -1 && p < i ? p : -2;
+    }
+    __syncthreads();
+    const int from = base ? base[s] : r.len - r.n;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        int depth = 0, j = i;
+        while (up[j] >= 0) j = up[j], ++depth;
+        const bool in = up[j] == -1;
+        if (pos) pos[r.q0 + i] = from + (in ? depth : 0);
+        uint64_t *row = sees + (r.q0 + i) * words;
+        j = in ? i : -1;
+        for (int w = words - 1; w >= 0; --w) {
+            uint64_t bits = 0;
+            while (j >= 64 * w) bits |= 1ull << (j - 64 * w), j = up[j];  // (j < 0 ends it: the words are not below 0)
+            row[w] = bits;
+        }
+    }
+}
+
+// A weight as a number whose order is the weights': 0 is no position, the largest one that is kept in any case.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);  // (-0 + 0 is 0)
+    if ((u & 0x7fffffffu) > 0x7f800000u) return 0xfffffffeu;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct EvictArgs {
+    KvView c;
+    BatchView b;
+    const float *w;
+    int32_t *kept, *new_len;
+    int budget, first, recent;
+};
+
+__device__ __forceinline__ int seq_len(const KvView &c, const BatchView &b, int s) {
+    return (int) min((int64_t) max(b.kv_len[s], 0), b.table_stride << c.shift);
+}
+
+// Which positions a sequence's kv head keeps: a workgroup each. The budget-th largest key digit by digit (11, 11, 10 bits), the
+// counts of a digit's values in LDS; then the positions in order, those above it and as many equal ones as there is room for.
+constexpr int kSel = 1024, kBins = 2048;
+__global__ __launch_bounds__(kSel) void k_kv_select(EvictArgs a) {
+    __shared__ int bins[kBins], waves[kSel / 64], found[2];
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const int n = seq_len(a.c, a.b, s), P = 1 << a.c.shift;
+    int32_t *kept = a.kept + (int64_t) blockIdx.x * a.budget;
+    // keys of positions 4 i .. 4 i + 3, which lie in one page
+    const auto keys = [&](int i, uint32_t (&k)[4]) {
+        const int at = 4 * i, page = at < n ? page_of(a.c, a.b, s, at) : -1;
+        float4 w = {};
+        if (page >= 0) w = *(const float4 *) (a.w + (((int64_t) page * a.c.n_kv + head) << a.c.shift) + (at & (P - 1)));
+        const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = at + j;
+            k[j] = page < 0 || p >= n ? 0u : p < a.first || p >= n - a.recent ? 0xffffffffu : weight_key(v[j]);
+        }
+    };
+    const auto wave_scan = [&](int v) {  // inclusive, over the wave
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int u = __shfl_up(v, o, 64);
+            v += lane >= o ? u : 0;
+        }
+        return v;
+    };
+    const int quads = n / 4 + (n % 4 > 0);
+    int want = a.budget, total = 0;
+    uint32_t prefix = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, high = pass == 0 ? 32 : pass == 1 ? 21 : 10;
+        for (int i = tid; i < kBins; i += kSel) bins[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < quads; i += kSel) {
+            uint32_t k[4];
+            keys(i, k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (k[j] != 0 && (pass == 0 || k[j] >> high == prefix)) atomicAdd(&bins[(k[j] >> shift) & (pass == 2 ? 1023 : 2047)], 1);
+        }
+        __syncthreads();
+        // from the largest digit down: thread t holds digits 2047 - 2 t and 2046 - 2 t
+        const int hi = bins[kBins - 1 - 2 * tid], lo = bins[kBins - 2 - 2 * tid];
+        int sum = wave_scan(hi + lo);
+        if (lane == 63) waves[wave] = sum;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) sum += waves[w];
+        if (pass == 0) {
+            if (tid == kSel - 1) found[0] = sum;
+            __syncthreads();
+            total = found[0];
+            want = min(want, total);
+            __syncthreads();
+        }
+        const int above = sum - hi - lo;  // keys of larger digits
+        if (want > above && want <= sum) {
+            const bool second = want > above + hi;
+            found[0] = kBins - 1 - 2 * tid - (second ? 1 : 0);
+            found[1] = above + (second ? hi : 0);
+        }
+        __syncthreads();
+        if (want > 0) {
+            prefix = pass == 2 ? (prefix << 10) | (uint32_t) found[0] : (prefix << 11) | (uint32_t) found[0];
+            want -= found[1];
+        }
+        __syncthreads();
+    }
+    // `want` of the keys equal to `prefix` are kept: the first ones
+    const int keep = min(a.budget, total);
+    int before = 0, equal = 0;  // kept above, and equal, of the positions so far
+    if (keep > 0)
+        for (int i0 = 0; i0 < quads; i0 += kSel) {
+            uint32_t k[4] = {};
+            if (i0 + tid < quads) keys(i0 + tid, k);
+            int gt = 0, eq = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) gt += k[j] > prefix, eq += k[j] == prefix;
+            const int both = wave_scan(gt | (eq << 16));
+            if (lane == 63) waves[wave] = both;
+            __syncthreads();
+            int at = both - (gt | (eq << 16)), all = 0;
+#pragma unroll
+            for (int w = 0; w < kSel / 64; ++w) {
+                at += w < wave ? waves[w] : 0;
+                all += waves[w];
+            }
+            int g = before + (at & 0xffff), e = equal + (at >> 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool is = k[j] == prefix;
+                if (k[j] > prefix || (is && e < want)) kept[g + min(e, want)] = 4 * (i0 + tid) + j;
+                g += k[j] > prefix, e += is;
+            }
+            before += all & 0xffff, equal += all >> 16;
+            __syncthreads();
+        }
+    for (int i = keep + tid; i < a.budget; i += kSel) kept[i] = -1;
+    if (head == 0 && tid == 0) a.new_len[s] = keep;
+}
+
+struct MoveArgs {
+    KvView c;
+    BatchView b;
+    const int32_t *to;  // the table that positions go to
+    int64_t to_stride;
+    const int32_t *list, *count;  // list[row][list_stride], row: a sequence's kv head, or (NEW) the sequence; count: NEW, per sequence
+    int64_t list_stride;
+    const float *w;
+    float *w_out;
+    int32_t *new_len;  // NEW
+};
+
+// Positions list[0], list[1], ... of a sequence's kv head to positions 0, 1, ... (NEW: both counted from its first new token,
+// the list one of the sequence). A workgroup moves a part of a position: K's codes, 16 byte columns of V, or the scale bytes and
+// the weight, for 1024 positions at a time, all of which are read before the first is written. In place one workgroup goes over
+// all of them in order: what it writes lies before everything that it has yet to read, since the list ascends (a list of new
+// tokens, which need not, has at most 1024). Elsewhere (INTO) the steps are workgroups of their own.
+constexpr int kMove = 1024;
+template <int D, bool NEW>
+__global__ __launch_bounds__(kMove) void k_kv_move(MoveArgs a) {
+    constexpr int NB = D / 32, NP = D / 32;  // 16-byte pieces of a K row
+    const int s = blockIdx.y / a.c.n_kv, head = blockIdx.y % a.c.n_kv, part = blockIdx.z, tid = threadIdx.x, P = 1 << a.c.shift;
+    int64_t first = 0;
+    int n, fresh = 0;
+    const int32_t *list;
+    if constexpr (NEW) {
+        const SeqRange r = seq_range(a.b, s);
+        first = (int64_t) r.len - r.n, fresh = r.n;
+        n = (int) min((int64_t) min(max(a.count[s], 0), r.n), a.list_stride);
+        list = a.list + s * a.list_stride;
+        if (head == 0 && part == 0 && tid == 0) a.new_len[s] = (int) max(first + n, (int64_t) 0);
+    } else {
+        n = (int) a.list_stride;
+        list = a.list + (int64_t) blockIdx.y * a.list_stride;
+    }
+    using L = KvParts<D>;
+    const int64_t head_off = head * kv_head_bytes(D, P);
+    // where the i-th one comes from and goes to: pages (-1: not moved) and rows
+    struct Place {
+        int from, to, row_from, row_to;
+    };
+    const auto place = [&](int i) {
+        Place p{-1, -1, 0, 0};
+        if (i >= n) return p;
+        const int x = list[i];
+        if (x < 0 || (NEW && x >= fresh)) return p;
+        const int64_t src = first + x, dst = first + i;
+        if (src == dst && a.to == a.b.table) return p;
+        if (src < 0 || dst < 0 || src > INT32_MAX || dst > INT32_MAX) return p;
+        p.from = page_of(a.c, a.b, s, (int) src);
+        const int64_t e = dst >> a.c.shift;
+        const int q = e < a.to_stride ? a.to[s * a.to_stride + e] : -1;
+        p.to = p.from >= 0 && q >= 0 && q < a.c.n_pages ? q : -1;
+        p.row_from = (int) src & (P - 1), p.row_to = (int) dst & (P - 1);
+        return p;
+    };
+    for (int64_t i0 = (int64_t) blockIdx.x * kMove; i0 < n; i0 += (int64_t) gridDim.x * kMove) {
+        if (part == 0) {
+            Place p[NP];
+            uint4 x[NP];
+#pragma unroll
+            for (int u = 0; u < NP; ++u) {
+                p[u] = place((int) i0 + (u * kMove + tid) / NP);
+                if (p[u].to >= 0)
+                    x[u] = *(const uint4 *) (a.c.pages + p[u].from * a.c.page_bytes + head_off + L::k_row(P, p[u].row_from) + tid % NP * 16);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < NP; ++u)
+                if (p[u].to >= 0) *(uint4 *) (a.c.pages + p[u].to * a.c.page_bytes + head_off + L::k_row(P, p[u].row_to) + tid % NP * 16) = x[u];
+        } else if (part == 1) {
+            const Place p = place((int) i0 + tid);
+            uint8_t k[NB], v[NB];
+            float w = 0.0f;
+            const uint8_t *src = a.c.pages + p.from * a.c.page_bytes + head_off;
+            if (p.to >= 0) {
+                __builtin_memcpy(k, __builtin_assume_aligned(src + L::k_scale(P, p.row_from), NB), NB);
+                __builtin_memcpy(v, __builtin_assume_aligned(src + L::v_scale(P, p.row_from), NB), NB);
+                if (a.w) w = a.w[(((int64_t) p.from * a.c.n_kv + head) << a.c.shift) + p.row_from];
+            }
+            __syncthreads();
+            uint8_t *dst = a.c.pages + p.to * a.c.page_bytes + head_off;
+            if (p.to >= 0) {
+                __builtin_memcpy(__builtin_assume_aligned(dst + L::k_scale(P, p.row_to), NB), k, NB);
+                __builtin_memcpy(__builtin_assume_aligned(dst + L::v_scale(P, p.row_to), NB), v, NB);
+                if (a.w) a.w_out[(((int64_t) p.to * a.c.n_kv + head) << a.c.shift) + p.row_to] = w;
+            }
+        } else {
+            const Place p = place((int) i0 + tid);
+            const int j = 16 * (part - 2);
+            uint8_t x[16];
+            if (p.to >= 0) {
+                const uint8_t *src = a.c.pages + p.from * a.c.page_bytes + head_off + L::v_col(P, j) + p.row_from;
+#pragma unroll
+                for (int u = 0; u < 16; ++u) x[u] = src[(int64_t) u * P];
+            }
+            __syncthreads();
+            if (p.to >= 0) {
+                uint8_t *dst = a.c.pages + p.to * a.c.page_bytes + head_off + L::v_col(P, j) + p.row_to;
+#pragma unroll
+                for (int u = 0; u < 16; ++u) dst[(int64_t) u * P] = x[u];
+            }
+        }
+    }
+}
+
+template <bool NEW> int move(const MoveArgs &a, int D, int n_seq, int64_t steps, const char *what, hipStream_t st) {
+    const auto go = [&](auto dim) {
+        constexpr int DD = decltype(dim)::value;
+        hipLaunchKernelGGL((k_kv_move<DD, NEW>), dim3((unsigned) steps, (unsigned) (n_seq * a.c.n_kv), 2 + DD / 32), dim3(kMove), 0, st, a);
+        return host::check_launch(what);
+    };
+    if (D == 64) return go(std::integral_constant<int, 64>{});
+    if (D == 128) return go(std::integral_constant<int, 128>{});
+    return go(std::integral_constant<int, 256>{});
+}
+
+}  // namespace
+
+namespace impl {
+
+int rope_scaled(int rope_dim, double base, double factor, double original, double fast, double slow, float *inv_freq, float *magnitude) {
+    if (rope_dim <= 0 || rope_dim % 2 || !inv_freq || !magnitude)
+        return host::set_error(host::ERR_SHAPE, "rope_scaled: an even rope_dim and two outputs are needed (%d)", rope_dim);
+    if (!(base > 1.0) || !(factor >= 1.0) || !(original >= 1.0) || !(slow > 0.0) || !(fast > slow) || !std::isfinite(base) ||
+        !std::isfinite(factor) || !std::isfinite(original) || !std::isfinite(fast))
+        return host::set_error(host::ERR_SHAPE, "rope_scaled: base above 1, factor and original of at least 1, fast above slow above 0");
+    const double pi = 3.14159265358979323846;
+    // the pair (as a real number) that turns `turns` times over the original positions
+    const auto at = [&](double turns) { return rope_dim * std::log(original / (turns * 2.0 * pi)) / (2.0 * std::log(base)); };
+    const double lo = std::max(std::floor(at(fast)), 0.0), hi = std::min(std::ceil(at(slow)), rope_dim / 2 - 1.0);
+    for (int i = 0; i < rope_dim / 2; ++i) {
+        const double f = std::pow(base, -2.0 * i / rope_dim);
+        const double slowed = std::min(std::max((i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+        inv_freq[i] = (float) (f * (1.0 - slowed) + f / factor * slowed);
+    }
+    *magnitude = (float) (0.1 * std::log(factor) + 1.0);
+    return host::OK;
+}
+
+int tree_plan(const FnsKvBatch *b, const int32_t *parents, const int32_t *base, int words, uint64_t *sees, int32_t *pos, hipStream_t st) {
+    // (a batch is checked together with a cache; this call needs none)
+    const FnsKvCache none{1, 64, 16, 1, (void *) 16};
+    FNS_TRY(host::kv_check(&none, b, "tree_plan"));
+    if (words < 1 || words > kMaxWords || b->max_q > 64 * words)
+        return host::set_error(host::ERR_SHAPE, "tree_plan: words must be 1..16 and hold max_q tokens (%d for %d)", words, b->max_q);
+    if (b->n_seq == 0 || b->n_tok == 0 || b->max_q == 0) return host::OK;
+    if (!parents || !sees) return host::set_error(host::ERR_SHAPE, "tree_plan: null argument");
+    hipLaunchKernelGGL(k_tree_plan, dim3((unsigned) b->n_seq), dim3(256), 0, st, host::kv_batch(b), parents, base, words, sees, pos);
+    return host::check_launch("tree_plan");
+}
+
+int kv_evict(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvEvict *x, hipStream_t st) {
+    FNS_TRY(host::kv_check(c, b, "kv_evict"));
+    if (!x) return host::set_error(host::ERR_SHAPE, "kv_evict: null arguments");
+    if (x->budget < 1 || x->budget > (1 << 30) || x->first < 0 || x->recent < 0 || (int64_t) x->first + x->recent > x->budget)
+        return host::set_error(host::ERR_SHAPE, "kv_evict: budget must be 1..2^30 and hold first and recent (%d, %d, %d)", x->budget, x->first, x->recent);
+    if (x->to_stride < 0 || x->to_stride > INT32_MAX || (x->to_table && x->to_stride == 0))
+        return host::set_error(host::ERR_SHAPE, "kv_evict: a table needs its stride");
+    if (b->n_seq == 0) return host::OK;
+    if (!x->weights || !x->weights_out || !x->kept || !x->new_len || ((uintptr_t) x->weights & 15))
+        return host::set_error(host::ERR_SHAPE, "kv_evict: null argument, or weights that are not 16-byte aligned");
+    if (x->new_len == b->kv_len) return host::set_error(host::ERR_SHAPE, "kv_evict: new_len must not be kv_len");
+    if (x->to_table == b->page_table) return host::set_error(host::ERR_SHAPE, "kv_evict: to_table must not be the batch's (NULL: in place)");
+    if (!x->to_table && x->weights_out != x->weights)
+        return host::set_error(host::ERR_SHAPE, "kv_evict: in place the weights move in place too");
+    EvictArgs a{host::kv_view(c), host::kv_batch(b), x->weights, x->kept, x->new_len, x->budget, x->first, x->recent};
+    hipLaunchKernelGGL(k_kv_select, dim3((unsigned) (b->n_seq * c->n_head_kv)), dim3(kSel), 0, st, a);
+    FNS_TRY(host::check_launch("kv_evict"));
+    MoveArgs m{a.c, a.b, x->to_table ? x->to_table : b->page_table, x->to_table ? x->to_stride : b->table_stride, x->kept, nullptr,
+               x->budget, x->weights, x->weights_out, nullptr};
+    const int64_t steps = x->to_table ? std::min<int64_t>((x->budget + kMove - 1) / kMove, 1024) : 1;
+    return move<false>(m, c->head_dim, b->n_seq, steps, "kv_evict", st);
+}
+
+int kv_keep(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvKeep *x, hipStream_t st) {
+    FNS_TRY(host::kv_check(c, b, "kv_keep"));
+    if (!x) return host::set_error(host::ERR_SHAPE, "kv_keep: null arguments");
+    if (x->stride < 1 || x->stride > kMove)
+        return host::set_error(host::ERR_SHAPE, "kv_keep: lists of 1..%d new tokens (%lld)", kMove, (long long) x->stride);
+    if (b->n_seq == 0) return host::OK;
+    if (!x->kept || !x->n_kept || !x->new_len) return host::set_error(host::ERR_SHAPE, "kv_keep: null argument");
+    if (x->new_len == b->kv_len || x->new_len == x->n_kept) return host::set_error(host::ERR_SHAPE, "kv_keep: new_len must not be kv_len or n_kept");
+    MoveArgs m{host::kv_view(c), host::kv_batch(b), b->page_table, b->table_stride, x->kept, x->n_kept, x->stride, x->weights,
+               x->weights, x->new_len};
+    return move<true>(m, c->head_dim, b->n_seq, 1, "kv_keep", st);
+}
+
+}  // namespace impl
+
+namespace k {
+void tree_plan(const FnsKvBatch &batch, const int32_t *parents, const int32_t *base, int words, uint64_t *sees, int32_t *pos, hipStream_t st) {
+    host::abort_on_error(impl::tree_plan(&batch, parents, base, words, sees, pos, st), "tree_plan");
+}
+void kv_evict(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsKvEvict &x, hipStream_t st) {
+    host::abort_on_error(impl::kv_evict(&cache, &batch, &x, st), "kv_evict");
+}
+void kv_keep(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsKvKeep &x, hipStream_t st) {
+    host::abort_on_error(impl::kv_keep(&cache, &batch, &x, st), "kv_keep");
+}
+}  // namespace k
+
+}  // namespace fns

@@ -629,6 +629,24 @@ class AttnDesc(ctypes.Structure):
                 ("sinks", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64)]
 
 
+class KvTreeDesc(ctypes.Structure):
+    """Mirror of FnsKvTree."""
+    _fields_ = [("sees", ctypes.c_void_p), ("words", ctypes.c_int)]
+
+
+class KvEvictDesc(ctypes.Structure):
+    """Mirror of FnsKvEvict."""
+    _fields_ = [("budget", ctypes.c_int), ("first", ctypes.c_int), ("recent", ctypes.c_int), ("weights", ctypes.c_void_p),
+                ("weights_out", ctypes.c_void_p), ("to_table", ctypes.c_void_p), ("to_stride", ctypes.c_int64),
+                ("kept", ctypes.c_void_p), ("new_len", ctypes.c_void_p)]
+
+
+class KvKeepDesc(ctypes.Structure):
+    """Mirror of FnsKvKeep."""
+    _fields_ = [("kept", ctypes.c_void_p), ("n_kept", ctypes.c_void_p), ("stride", ctypes.c_int64),
+                ("weights", ctypes.c_void_p), ("new_len", ctypes.c_void_p)]
+
+
 class KvCache:
     """A paged key/value cache held in 4 bits (FnsKvCache): n_pages pages of page_size positions of every kv head, one
     layer's. pages: uint8 device memory of an earlier cache of this shape, or None: zeroed."""
@@ -695,6 +713,56 @@ def rope_freqs(rope_dim: int, base: float = 10000.0, factors=None) -> torch.Tens
     return f.float().cuda()
 
 
+def rope_scaled(rope_dim: int, base: float, factor: float, original: float, fast: float = 32.0, slow: float = 1.0):
+    """-> (inv_freq f32 on the current device, magnitude) of kv_append for contexts of factor * original positions: pairs that
+    turn `fast` times or more over the original ones keep their frequency, those that turn `slow` times or less have it divided
+    by factor (fns_hip_rope_scaled)."""
+    if rope_dim <= 0 or rope_dim % 2:
+        raise ValueError(f"rope_scaled: an even rope_dim is needed ({rope_dim})")
+    freq, magnitude = (ctypes.c_float * (rope_dim // 2))(), ctypes.c_float()
+    call("fns_hip_rope_scaled", rope_dim, base, factor, original, fast, slow, freq, ctypes.byref(magnitude))
+    return torch.tensor(list(freq), dtype=torch.float32).cuda(), magnitude.value
+
+
+class KvTree:
+    """What the new tokens of a batch see of their sequence's new tokens (FnsKvTree): sees int64 [n_tok][words], bit j % 64 of
+    word j / 64 for the j-th of them; pos int32 [n_tok] or None, the positions that kv_append may turn them by."""
+
+    def __init__(self, sees: torch.Tensor, pos: torch.Tensor | None = None):
+        if sees.dtype != torch.int64 or not sees.is_contiguous() or sees.dim() != 2:
+            raise ValueError("KvTree: sees must be contiguous int64 [n_tok][words]")
+        _here("KvTree", sees, pos)
+        self.sees, self.pos = sees, pos
+        self.desc = KvTreeDesc(sees.data_ptr(), sees.shape[1])
+        self.ref = ctypes.byref(self.desc)
+
+    def _for(self, what: str, batch: KvBatch):
+        if self.sees.shape[0] != batch.n_tok:
+            raise ValueError(f"{what}: the tree has {self.sees.shape[0]} tokens, the batch {batch.n_tok}")
+        return self.ref
+
+
+def _ints(what: str, name: str, t: torch.Tensor, *shape: int) -> int:
+    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} must be contiguous int32 {list(shape)}")
+    return t.data_ptr()
+
+
+def tree_plan(batch: KvBatch, parents: torch.Tensor, base: torch.Tensor | None = None, words: int | None = None) -> KvTree:
+    """The tree of the batch's new tokens from parents int32 [n_tok] (index among the sequence's new tokens, -1: none, anything
+    below: no token of the tree), with positions base[sequence] (None: the sequence's first new position) + number of
+    ancestors. words: 64-bit words a token (None: as max_q needs)."""
+    if words is None:
+        words = max(1, (batch.desc.max_q + 63) // 64)
+    p = _ints("tree_plan", "parents", parents, batch.n_tok)
+    b = None if base is None else _ints("tree_plan", "base", base, batch.desc.n_seq)
+    sees = torch.empty((batch.n_tok, max(words, 0)), dtype=torch.int64, device=parents.device)
+    pos = torch.empty(batch.n_tok, dtype=torch.int32, device=parents.device)
+    st = _here("tree_plan", batch.kv_len, parents, base)
+    call("fns_hip_tree_plan", batch.ref, p, b, words, sees.data_ptr(), pos.data_ptr(), st)
+    return KvTree(sees, pos)
+
+
 def _heads(what: str, t: torch.Tensor, n_tok: int, dim: int, dtype: torch.dtype) -> int:
     """Token stride of t [n_tok][heads][dim], heads contiguous within a token (a slice of a fused projection is)."""
     shape = t.shape
@@ -716,9 +784,11 @@ def _heads(what: str, t: torch.Tensor, n_tok: int, dim: int, dtype: torch.dtype)
 
 
 def kv_append(cache: KvCache, batch: KvBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
-              rope: int = ROPE_NONE, inv_freq: torch.Tensor | None = None, q_out: torch.Tensor | None = None):
+              rope: int = ROPE_NONE, inv_freq: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+              pos: torch.Tensor | None = None, magnitude: float = 1.0):
     """k, v [n_tok][n_head_kv][head_dim] into the cache, k (and q) rotated by position * inv_freq over the first
-    2 * len(inv_freq) channels. -> the rotated q (in q_out, which may be q; None without q)."""
+    2 * len(inv_freq) channels. pos int32 [n_tok]: positions to turn by (None: those in the cache); magnitude: of what is
+    rotated. -> the rotated q (in q_out, which may be q; None without q)."""
     D, Hk, n_tok, dt = cache.head_dim, cache.n_head_kv, batch.n_tok, k.dtype
     x = KvAppendDesc()
     x.k_stride, x.v_stride = _heads("kv_append", k, n_tok, D, dt), _heads("kv_append", v, n_tok, D, dt)
@@ -741,8 +811,12 @@ def kv_append(cache: KvCache, batch: KvBatch, k: torch.Tensor, v: torch.Tensor, 
     else:
         inv_freq = None
     x.dtype, x.k, x.v = F32 if dt is torch.float32 else BF16, k.data_ptr(), v.data_ptr()
-    st = _here("kv_append", cache.pages, batch.kv_len, k, v, q, q_out, inv_freq)
-    call("fns_hip_kv_append", cache.ref, batch._for(cache), ctypes.byref(x), st)
+    st = _here("kv_append", cache.pages, batch.kv_len, k, v, q, q_out, inv_freq, pos)
+    if pos is None and magnitude == 1.0:
+        call("fns_hip_kv_append", cache.ref, batch._for(cache), ctypes.byref(x), st)
+    else:
+        at = None if pos is None else _ints("kv_append", "pos", pos, n_tok)
+        call("fns_hip_kv_append_at", cache.ref, batch._for(cache), ctypes.byref(x), at, magnitude, st)
     return q_out
 
 
@@ -766,9 +840,11 @@ def attn_workspace(cache: KvCache, batch: KvBatch, q: torch.Tensor) -> torch.Ten
 
 
 def attn(cache: KvCache, batch: KvBatch, q: torch.Tensor, scale: float | None = None, window: int = 0,
-         sinks: torch.Tensor | None = None, out: torch.Tensor | None = None, ws: torch.Tensor | None = None) -> torch.Tensor:
+         sinks: torch.Tensor | None = None, out: torch.Tensor | None = None, ws: torch.Tensor | None = None,
+         tree: KvTree | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [n_tok][n_head][head_dim] over the cache -> out (rows of no sequence are left as they were). scale
-    None: head_dim^-0.5; window > 0: the last `window` positions only; sinks f32 [n_head] join the denominator."""
+    None: head_dim^-0.5; window > 0: the last `window` positions only; sinks f32 [n_head] join the denominator. tree: what the
+    new tokens see of each other; lse f32 [n_tok][n_head]: takes the logarithms of the denominators (kv_weigh's)."""
     D, dt = cache.head_dim, q.dtype
     if out is None:
         out = torch.empty(q.shape, dtype=dt, device=q.device)
@@ -786,10 +862,100 @@ def attn(cache: KvCache, batch: KvBatch, q: torch.Tensor, scale: float | None = 
         ws = attn_workspace(cache, batch, q)
     elif not ws.is_contiguous():
         raise ValueError("attn: the workspace must be contiguous")
-    st = _here("attn", cache.pages, batch.kv_len, q, out, sinks, ws)
+    st = _here("attn", cache.pages, batch.kv_len, q, out, sinks, ws, lse)
+    if tree is not None or lse is not None:
+        if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != q.shape[:2]):
+            raise ValueError("attn: lse must be contiguous f32 [n_tok][n_head]")
+        call("fns_hip_attn_tree", cache.ref, batch._for(cache), ctypes.byref(desc), None if tree is None else tree._for("attn", batch),
+             q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(), st)
+        return out
     call("fns_hip_attn", cache.ref, batch._for(cache), ctypes.byref(desc), q.data_ptr(), out.data_ptr(), ws.data_ptr(),
          ws.numel() * ws.element_size(), st)
     return out
+
+
+def kv_weights(cache: KvCache) -> torch.Tensor:
+    """Zeroed attention weights of a cache's positions: f32 [n_pages][n_head_kv][page_size]."""
+    return torch.zeros(cache.desc.n_pages, cache.n_head_kv, cache.page_size, dtype=torch.float32, device=cache.pages.device)
+
+
+def _weights(what: str, cache: KvCache, *ts: torch.Tensor | None) -> None:
+    shape = (cache.desc.n_pages, cache.n_head_kv, cache.page_size)
+    for t in ts:
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or tuple(t.shape) != shape):
+            raise ValueError(f"{what}: weights must be contiguous f32 {list(shape)}")
+
+
+def kv_weigh_workspace(cache: KvCache, batch: KvBatch, q: torch.Tensor) -> torch.Tensor:
+    """A workspace of kv_weigh for this batch's numbers and q's heads; it may serve every layer of a step in turn."""
+    width = _heads("kv_weigh", q, batch.n_tok, cache.head_dim, q.dtype)
+    desc = AttnDesc(_dtype_code(q), q.shape[1], 0, 1.0, None, width, 0)
+    size = ctypes.c_size_t()
+    call("fns_hip_kv_weigh_workspace", cache.ref, batch._for(cache), ctypes.byref(desc), ctypes.byref(size))
+    return torch.empty(size.value, dtype=torch.uint8, device=q.device)
+
+
+def kv_weigh(cache: KvCache, batch: KvBatch, q: torch.Tensor, lse: torch.Tensor, past: torch.Tensor | None,
+             scale: float | None = None, window: int = 0, tree: KvTree | None = None, out: torch.Tensor | None = None,
+             ws: torch.Tensor | None = None) -> torch.Tensor:
+    """What every cached position (of sequences with new tokens) gets of the new tokens' attention, exp(scale * q . K - lse)
+    summed over tokens and the heads of a group, on top of `past` (as kv_weights; None: zeros; new positions start at 0) -> out
+    (None: past, in place). lse as attn gives it; rows whose lse is not finite add nothing."""
+    if out is None:
+        out = kv_weights(cache) if past is None else past
+    _weights("kv_weigh", cache, past, out)
+    D, dt = cache.head_dim, q.dtype
+    desc = AttnDesc(F32 if dt is torch.float32 else BF16, q.shape[1], min(window, 2 ** 31 - 1), D ** -0.5 if scale is None else scale,
+                    None, _heads("kv_weigh", q, batch.n_tok, D, dt), 0)
+    if lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != q.shape[:2]:
+        raise ValueError("kv_weigh: lse must be contiguous f32 [n_tok][n_head]")
+    if ws is None:
+        ws = kv_weigh_workspace(cache, batch, q)
+    elif not ws.is_contiguous():
+        raise ValueError("kv_weigh: the workspace must be contiguous")
+    st = _here("kv_weigh", cache.pages, batch.kv_len, q, lse, past, out, ws)
+    call("fns_hip_kv_weigh", cache.ref, batch._for(cache), ctypes.byref(desc), None if tree is None else tree._for("kv_weigh", batch),
+         q.data_ptr(), lse.data_ptr(), None if past is None else past.data_ptr(), out.data_ptr(), ws.data_ptr(),
+         ws.numel() * ws.element_size(), st)
+    return out
+
+
+def kv_evict(cache: KvCache, batch: KvBatch, weights: torch.Tensor, budget: int, first: int = 0, recent: int = 0,
+             to_table: torch.Tensor | None = None, weights_out: torch.Tensor | None = None):
+    """Cuts every sequence to `budget` positions a kv head: the first `first`, the last `recent`, and of the others those of the
+    largest weights; K, V and weights of the kept ones move to the front of the sequence, in order: of its own pages, or of
+    to_table's int32 [n_seq][pages] (weights_out: None: weights). -> (kept int32 [n_seq][n_head_kv][budget], the kept positions and
+    then -1; new_len int32 [n_seq])."""
+    if weights_out is None:
+        weights_out = weights
+    _weights("kv_evict", cache, weights, weights_out)
+    n_seq = batch.desc.n_seq
+    kept = torch.empty((n_seq, cache.n_head_kv, max(budget, 0)), dtype=torch.int32, device=cache.pages.device)
+    new_len = torch.empty(n_seq, dtype=torch.int32, device=cache.pages.device)
+    x = KvEvictDesc(budget, first, recent, weights.data_ptr(), weights_out.data_ptr(), None, 0, kept.data_ptr(), new_len.data_ptr())
+    if to_table is not None:
+        if to_table.dim() != 2:
+            raise ValueError("kv_evict: to_table must be [n_seq][pages]")
+        x.to_table, x.to_stride = _ints("kv_evict", "to_table", to_table, n_seq, to_table.shape[1]), to_table.shape[1]
+    st = _here("kv_evict", cache.pages, batch.kv_len, weights, weights_out, to_table)
+    call("fns_hip_kv_evict", cache.ref, batch._for(cache), ctypes.byref(x), st)
+    return kept, new_len
+
+
+def kv_keep(cache: KvCache, batch: KvBatch, kept: torch.Tensor, n_kept: torch.Tensor, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """Of every sequence's new tokens the listed ones (kept int32 [n_seq][most], the first n_kept[s] of a row, indices among the
+    sequence's new tokens) become its next positions, in the list's order; weights (as kv_weights) move along.
+    -> new_len int32 [n_seq]."""
+    _weights("kv_keep", cache, weights)
+    n_seq = batch.desc.n_seq
+    if kept.dim() != 2:
+        raise ValueError("kv_keep: kept must be [n_seq][most]")
+    new_len = torch.empty(n_seq, dtype=torch.int32, device=cache.pages.device)
+    x = KvKeepDesc(_ints("kv_keep", "kept", kept, n_seq, kept.shape[1]), _ints("kv_keep", "n_kept", n_kept, n_seq), kept.shape[1],
+                   None if weights is None else weights.data_ptr(), new_len.data_ptr())
+    st = _here("kv_keep", cache.pages, batch.kv_len, kept, n_kept, weights)
+    call("fns_hip_kv_keep", cache.ref, batch._for(cache), ctypes.byref(x), st)
+    return new_len
 
 
 class DenseFfnDesc(ctypes.Structure):

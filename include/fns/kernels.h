@@ -76,4 +76,17 @@ void kv_read(const FnsKvCache &cache, const FnsKvBatch &batch, float *k, float *
 void attn(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsAttn &x, const void *q, void *out, void *workspace,
           size_t workspace_bytes, hipStream_t st);
 
+// Trees of drafted tokens, and caches of a bounded length; rules and descriptors as in fns_hip.h (no counterpart in the
+// reference, which drafts a line of tokens).
+void kv_append_at(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsKvAppend &x, const int32_t *pos, float magnitude,
+                  hipStream_t st);
+void tree_plan(const FnsKvBatch &batch, const int32_t *parents, const int32_t *base, int words, uint64_t *sees, int32_t *pos,
+               hipStream_t st);
+void attn_tree(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsAttn &x, const FnsKvTree *tree, const void *q,
+               void *out, float *lse, void *workspace, size_t workspace_bytes, hipStream_t st);
+void kv_weigh(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsAttn &x, const FnsKvTree *tree, const void *q,
+              const float *lse, const float *past, float *weights, void *workspace, size_t workspace_bytes, hipStream_t st);
+void kv_evict(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsKvEvict &x, hipStream_t st);
+void kv_keep(const FnsKvCache &cache, const FnsKvBatch &batch, const FnsKvKeep &x, hipStream_t st);
+
 }  // namespace fns::k

@@ -388,6 +388,93 @@ int fns_hip_attn_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, con
 int fns_hip_attn(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const void *q, void *out,
                  void *workspace, size_t workspace_bytes, void *stream);
 
+/* --- trees of drafted tokens, and caches of a bounded length ---
+ * A verify step of a tree:  fns_hip_tree_plan -> (projections) -> fns_hip_kv_append_at -> fns_hip_attn_tree -> ... -> the engine
+ * picks a path -> fns_hip_kv_keep. A cache kept to a number of positions: fns_hip_attn_tree (its lse) -> fns_hip_kv_weigh every
+ * step, fns_hip_kv_evict now and then; after that a token's place in the cache is not its position in the text any more, and
+ * fns_hip_kv_append_at takes the latter. No counterparts in the reference, which drafts a line of tokens
+ * (src/engine.cu:601-603) and keeps every position. */
+
+/* Host arithmetic: inv_freq [rope_dim / 2] (host memory, f32) of a rotation made for `original` positions with
+ * base^(-2 i / rope_dim), scaled to factor * original by the published rule of frequency parts: a pair that turns `fast` times
+ * (32, say) or more over the original positions keeps its frequency, one that turns `slow` times (1) or less has it divided by
+ * factor, the pairs between go over linearly in their index. *magnitude = 0.1 ln(factor) + 1, for fns_hip_kv_append_at. A factor
+ * of 1 gives the plain frequencies and 1. */
+int fns_hip_rope_scaled(int rope_dim, double base, double factor, double original, double fast, double slow, float *inv_freq,
+                        float *magnitude);
+/* fns_hip_kv_append with the tokens turned by positions of their own: pos int32 [n_tok] (device memory), or NULL: their
+ * positions in the cache. What turns is also multiplied by `magnitude` (positive, finite; k and q alike). Without a rotation
+ * both are ignored. */
+int fns_hip_kv_append_at(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvAppend *x, const int32_t *pos,
+                         float magnitude, void *stream);
+
+/* What every new token of a batch sees of the new tokens of its sequence: bit j % 64 of sees[t * words + j / 64] for the j-th of
+ * them (device memory, [n_tok][words]; bits behind the sequence's tokens are ignored, tokens from 64 * words on are seen by
+ * none). */
+typedef struct FnsKvTree {
+    const uint64_t *sees;
+    int words; /* 1..16 */
+} FnsKvTree;
+/* Those bits from parents, int32 [n_tok]: of a sequence's i-th new token the index j < i of its parent among them, or -1: it
+ * follows the sequence's earlier positions. It sees itself and its ancestors. Anything else is no token of the tree (a plan of
+ * fixed size is filled up with, say, -2): neither it nor what descends from it sees anything. pos int32 [n_tok] (or NULL) =
+ * base[sequence] + its number of ancestors (0 for no token of the tree); base int32 [n_seq], or NULL: the position of the
+ * sequence's first new token. 64 * words is at least max_q. Tokens of no sequence are left alone. */
+int fns_hip_tree_plan(const FnsKvBatch *batch, const int32_t *parents, const int32_t *base, int words, uint64_t *sees,
+                      int32_t *pos, void *stream);
+/* fns_hip_attn of a tree, and its denominators. tree: a token sees the positions before its sequence's new tokens and, of these,
+ * what its bits say (not the others, itself only with its bit); with a window of W and n bits the last W - n of the earlier
+ * positions (none if n >= W: the bits alone say which new tokens it sees). A token without bits sees nothing: its output is
+ * zero. NULL: as fns_hip_attn, in the same bits (bf16: unless the contexts are divided, when it is within the roundings).
+ * lse: NULL or f32 [n_tok][n_head], the logarithm of the softmax's denominator (sinks included) of every row, -infinity for one
+ * that sees nothing, within 2^-20 + 2^-22 |lse| and what q is off by (above). The workspace is fns_hip_attn_workspace's. */
+int fns_hip_attn_tree(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const FnsKvTree *tree, const void *q,
+                      void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Attention weights of cached positions: f32 [n_pages][n_head_kv][page_size]. For every position j of the sequences that have
+ * new tokens, and every kv head,
+ *   weights = past (of positions before the new tokens; the new ones start at 0)
+ *             + sum over the sequence's new tokens t and the query heads h of the kv head of exp(scale * q[t][h] . K_j - lse[t][h])
+ * over the rows that see j (causal or by the tree's bits, the window). past: NULL (zeros), `weights` itself, or another array.
+ * x: dtype, n_head, window, scale and q_stride count. A row whose lse is not finite, or whose q is not, adds nothing (so an lse
+ * set to infinity leaves a rejected token out); a position whose K holds a NaN block gets nothing. q enters as f32 does in
+ * fns_hip_attn, whatever its type; sums are f32, in a fixed order. A position without a page has no weight. Sequences of a call
+ * must not share pages. workspace: fns_hip_kv_weigh_workspace bytes, 16-byte aligned, as fns_hip_attn's. */
+int fns_hip_kv_weigh_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, size_t *bytes);
+int fns_hip_kv_weigh(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const FnsKvTree *tree, const void *q,
+                     const float *lse, const float *past, float *weights, void *workspace, size_t workspace_bytes,
+                     void *stream);
+
+/* Eviction: of every sequence (all its kv_len positions; q_start, n_tok and max_q do not matter) each kv head keeps `budget`
+ * positions, or all if there are no more: the first `first`, the last `recent`, and of the others those of the largest weights (a
+ * NaN is the largest, of equal ones the earlier is kept). Positions without a page are not there. What is kept moves, in order,
+ * to positions 0, 1, ...: K, V (their bytes) and weights; the heads' choices differ, their number does not.
+ * The table that the kept positions go to: the batch's own (in place: no page may be in it twice, and weights_out is weights), or `to_table` with pages none of which any of the call's sequences has. What follows the kept positions is undefined
+ * in place, left alone elsewhere. kept: int32 [n_seq][n_head_kv][budget], the kept positions in order, then -1. new_len:
+ * int32 [n_seq], how many they are; not the batch's kv_len (which the engine sets afterwards). */
+typedef struct FnsKvEvict {
+    int budget, first, recent; /* budget 1..2^30, first + recent at most that */
+    const float *weights;
+    float *weights_out;        /* may be weights */
+    const int32_t *to_table;   /* NULL: in place; else [n_seq][to_stride] */
+    int64_t to_stride;
+    int32_t *kept, *new_len;
+} FnsKvEvict;
+int fns_hip_kv_evict(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvEvict *x, void *stream);
+
+/* Of the new tokens of every sequence those listed become its next positions, in the list's order: new token kept[s][i] (its
+ * index among the sequence's new tokens) goes to position kv_len - n + i, i < n_kept[s] (at most n and `stride`). Entries that are no
+ * new token of the sequence leave that position as it was. weights: NULL, or moved along. new_len int32 [n_seq] =
+ * kv_len - n + n_kept (kv_len for a sequence without new tokens); not the batch's kv_len (which the engine sets afterwards). */
+typedef struct FnsKvKeep {
+    const int32_t *kept;   /* [n_seq][stride] */
+    const int32_t *n_kept; /* [n_seq] */
+    int64_t stride;        /* 1..1024 */
+    float *weights;
+    int32_t *new_len;
+} FnsKvKeep;
+int fns_hip_kv_keep(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvKeep *x, void *stream);
+
 /* --- GGUF checkpoints: reader and fully resident MoE layers ---
  * Replaces the reference's loader (src/model.cpp:30-136: gguf header and tensor table, the file mapped without copying)
  * and expert placement (src/engine.cu:375-471: slots [gate | up | down] 256-byte aligned with 4096 zero bytes after the

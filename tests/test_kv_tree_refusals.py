@@ -1,0 +1,169 @@
+"""Argument checks of the tree and eviction entry points, on the host before any launch; the scaled frequencies."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from flintnsteel_amd import _lib, ops
+from test_attn_half_refusals import BAD_BATCHES, BAD_CACHES, BUF, P, app, att, batch, cache
+
+r = ctypes.byref
+
+
+def L():
+    return _lib.lib()
+
+
+def tree(**kw):
+    return ops.KvTreeDesc(**{**dict(sees=BUF, words=1), **kw})
+
+
+def evict(**kw):
+    return ops.KvEvictDesc(**{**dict(budget=8, first=2, recent=3, weights=BUF, weights_out=BUF, to_table=None, to_stride=0,
+                                     kept=BUF, new_len=2 * BUF), **kw})
+
+
+def keep(**kw):
+    return ops.KvKeepDesc(**{**dict(kept=BUF, n_kept=BUF, stride=4, weights=None, new_len=2 * BUF), **kw})
+
+
+def _plan(b=None, parents=BUF, base=None, words=1, sees=BUF, pos=BUF):
+    b = b or batch()
+    return L().fns_hip_tree_plan(r(b), P(parents), P(base), words, P(sees), P(pos), None)
+
+
+def _attn(c=None, b=None, x=None, t=None, q=BUF, out=2 * BUF, lse=BUF, ws=BUF, size=1 << 40):
+    c, b, x, t = c or cache(), b or batch(), x or att(), t or tree()
+    return L().fns_hip_attn_tree(r(c), r(b), r(x), r(t), P(q), P(out), P(lse), P(ws), size, None)
+
+
+def _weigh(c=None, b=None, x=None, t=None, q=BUF, lse=BUF, w=BUF, ws=BUF, size=1 << 40):
+    c, b, x, t = c or cache(), b or batch(), x or att(), t or tree()
+    return L().fns_hip_kv_weigh(r(c), r(b), r(x), r(t), P(q), P(lse), None, P(w), P(ws), size, None)
+
+
+def _evict(c=None, b=None, x=None):
+    c, b, x = c or cache(), b or batch(), x or evict()
+    return L().fns_hip_kv_evict(r(c), r(b), r(x), None)
+
+
+def _keep(c=None, b=None, x=None):
+    c, b, x = c or cache(), b or batch(), x or keep()
+    return L().fns_hip_kv_keep(r(c), r(b), r(x), None)
+
+
+@pytest.mark.parametrize("kw", BAD_CACHES)
+def test_bad_caches(kw):
+    c = cache(**kw)
+    x = app()
+    assert _attn(c=c) == _weigh(c=c) == _evict(c=c) == _keep(c=c) == -2
+    assert L().fns_hip_kv_append_at(r(c), r(batch()), r(x), P(BUF), 1.0, None) == -2
+
+
+@pytest.mark.parametrize("kw", BAD_BATCHES)
+def test_bad_batches(kw):
+    if kw == dict(n_seq=40000):  # too many for two kv heads; a plan has none
+        kw = dict(n_seq=70000)
+    b = batch(**kw)
+    assert _attn(b=b) == _weigh(b=b) == _evict(b=b) == _keep(b=b) == _plan(b=b) == -2
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(dtype=1), -1), (dict(n_head=5), -2), (dict(n_head=0), -2), (dict(window=-1), -2), (dict(q_stride=511), -2)])
+def test_attention_arguments(kw, rc):
+    assert _attn(x=att(**kw)) == rc and _weigh(x=att(**kw)) == rc
+    size = ctypes.c_size_t()
+    assert L().fns_hip_kv_weigh_workspace(r(cache()), r(batch()), r(att(**kw)), r(size)) == rc
+
+
+@pytest.mark.parametrize("kw", [dict(words=0), dict(words=17), dict(sees=None)])
+def test_trees(kw):
+    assert _attn(t=tree(**kw)) == -2 and _weigh(t=tree(**kw)) == -2
+
+
+@pytest.mark.parametrize("kw", [dict(parents=None), dict(sees=None), dict(words=0), dict(words=17), dict(b=batch(n_tok=200, max_q=65))])
+def test_plan_arguments(kw):
+    assert _plan(**kw) == -2
+    assert b"tree_plan" in L().fns_hip_last_error()
+
+
+@pytest.mark.parametrize("magnitude", [0.0, -1.0, float("inf"), float("nan")])
+def test_magnitudes(magnitude):
+    x = app(rope=1, rope_dim=64, inv_freq=BUF)
+    assert L().fns_hip_kv_append_at(r(cache()), r(batch()), r(x), P(BUF), magnitude, None) == -2
+
+
+@pytest.mark.parametrize("kw", [dict(budget=0), dict(budget=(1 << 30) + 1), dict(first=-1), dict(recent=-1), dict(first=6), dict(weights=None),
+                                dict(weights_out=None), dict(kept=None), dict(new_len=None), dict(weights=BUF + 4, weights_out=BUF + 4),
+                                dict(weights_out=2 * BUF), dict(new_len=BUF), dict(to_table=BUF, to_stride=4),
+                                dict(to_table=2 * BUF), dict(to_table=2 * BUF, to_stride=-1)])
+def test_evict_arguments(kw):
+    assert _evict(x=evict(**kw)) == -2
+    assert b"kv_evict" in L().fns_hip_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(stride=0), dict(stride=1025), dict(kept=None), dict(n_kept=None), dict(new_len=None), dict(new_len=BUF)])
+def test_keep_arguments(kw):
+    assert _keep(x=keep(**kw)) == -2
+    assert b"kv_keep" in L().fns_hip_last_error()
+
+
+def test_null_arguments_overlap_and_workspaces():
+    assert _attn(q=None) == _attn(out=None) == _attn(out=BUF) == -2
+    assert _weigh(q=None) == _weigh(lse=None) == _weigh(w=None) == -2
+    assert L().fns_hip_attn_tree(None, r(batch()), r(att()), None, P(BUF), P(2 * BUF), None, P(BUF), 0, None) == -2
+    assert L().fns_hip_attn_tree(r(cache()), r(batch()), None, None, P(BUF), P(2 * BUF), None, P(BUF), 0, None) == -2
+    assert L().fns_hip_kv_weigh(r(cache()), None, r(att()), None, P(BUF), P(BUF), None, P(BUF), P(BUF), 0, None) == -2
+    assert L().fns_hip_kv_evict(r(cache()), r(batch()), None, None) == -2
+    assert L().fns_hip_kv_keep(r(cache()), r(batch()), None, None) == -2
+    assert L().fns_hip_kv_weigh_workspace(r(cache()), r(batch()), r(att()), None) == -2
+    assert L().fns_hip_kv_weigh_workspace(r(cache()), r(batch()), None, None) == -2
+    size = ctypes.c_size_t()
+    b = batch(n_tok=100, max_q=100)
+    assert L().fns_hip_kv_weigh_workspace(r(cache()), r(b), r(att()), r(size)) == 0 and size.value > 0
+    for ws, n in ((None, size.value), (BUF, size.value - 1), (BUF + 8, size.value), (BUF, 0)):
+        assert _weigh(b=b, ws=ws, size=n) == -4
+    long = batch(max_kv=100000, table_stride=2000)
+    assert L().fns_hip_attn_workspace(r(cache()), r(long), r(att()), r(size)) == 0 and size.value > 0
+    assert _attn(b=long, ws=BUF, size=size.value - 1) == -4
+    many = batch(n_tok=1 << 30, max_q=1 << 30)
+    assert _weigh(c=cache(n_head_kv=1), b=many, x=att(n_head=16, q_stride=1 << 14), size=1 << 62) == -2
+
+
+def test_empty_batches_are_noops():
+    for kw in (dict(n_tok=0), dict(max_q=0), dict(n_seq=0, q_start=None, kv_len=None, page_table=None)):
+        b = batch(**kw)
+        assert _attn(b=b, ws=None, size=0) == _weigh(b=b, ws=None, size=0) == _plan(b=b) == 0
+    b = batch(n_seq=0, q_start=None, kv_len=None, page_table=None)
+    assert _evict(b=b) == _keep(b=b) == 0
+
+
+@pytest.mark.parametrize("dim,base,factor,original,fast,slow", [(128, 500000.0, 16.0, 8192, 32.0, 1.0), (64, 10000.0, 4.0, 4096, 32.0, 1.0),
+                                                                (2, 10000.0, 2.0, 100, 32.0, 1.0), (96, 1e6, 40.0, 32768, 16.0, 2.0),
+                                                                (128, 10000.0, 1.0, 2048, 32.0, 1.0)])
+def test_scaled_frequencies(dim, base, factor, original, fast, slow):
+    out, m = (ctypes.c_float * (dim // 2))(), ctypes.c_float()
+    assert L().fns_hip_rope_scaled(dim, base, factor, original, fast, slow, out, r(m)) == 0
+    i = np.arange(dim // 2)
+    f = base ** (-2.0 * i / dim)
+    turns = original * f / (2 * np.pi)
+    at = lambda t: dim * np.log(original / (t * 2 * np.pi)) / (2 * np.log(base))  # noqa: E731
+    lo, hi = max(np.floor(at(fast)), 0), min(np.ceil(at(slow)), dim // 2 - 1)
+    ramp = np.clip((i - lo) / max(hi - lo, 0.001), 0, 1)
+    got = np.array(out, np.float64)
+    assert np.allclose(got, f * (1 - ramp) + f / factor * ramp, rtol=2.0 ** -23, atol=0)
+    assert abs(m.value - (0.1 * np.log(factor) + 1)) <= 2.0 ** -23
+    # what the rule is for: fast pairs as they were, slow ones divided (a pair beside either border belongs to the ramp)
+    assert np.allclose(got[(turns >= fast) & (i <= lo)], f[(turns >= fast) & (i <= lo)], rtol=2.0 ** -23)
+    assert np.allclose(got[i >= max(hi, lo + 1)], (f / factor)[i >= max(hi, lo + 1)], rtol=2.0 ** -23)
+
+
+@pytest.mark.parametrize("args", [(0, 1e4, 2.0, 100.0, 32.0, 1.0), (3, 1e4, 2.0, 100.0, 32.0, 1.0), (64, 1.0, 2.0, 100.0, 32.0, 1.0),
+                                  (64, 1e4, 0.5, 100.0, 32.0, 1.0), (64, 1e4, 2.0, 0.0, 32.0, 1.0), (64, 1e4, 2.0, 100.0, 1.0, 1.0),
+                                  (64, 1e4, 2.0, 100.0, 32.0, 0.0), (64, float("nan"), 2.0, 100.0, 32.0, 1.0),
+                                  (64, 1e4, float("inf"), 100.0, 32.0, 1.0)])
+def test_scaled_frequencies_refusals(args):
+    out, m = (ctypes.c_float * 64)(), ctypes.c_float()
+    assert L().fns_hip_rope_scaled(*args, out, r(m)) == -2
+    assert L().fns_hip_rope_scaled(64, 1e4, 2.0, 100.0, 32.0, 1.0, None, r(m)) == -2
