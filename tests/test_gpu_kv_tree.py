@@ -498,7 +498,9 @@ def test_python_checks():
     with pytest.raises(FnsError, match="budget"):
         ops.kv_evict(s.cache, s.batch, w, 0)
     with pytest.raises(FnsError, match="workspace"):
-        ops.kv_weigh(s.cache, s.batch, q, lse, w, ws=ops.kv_weigh_workspace(s.cache, s.batch, q)[:-16])
+        many = ops.KvBatch.from_lists([100], [100], [s.lists[0] * 4])
+        q, lse = torch.zeros(100, 4, 64, device="cuda"), torch.zeros(100, 4, device="cuda")
+        ops.kv_weigh(s.cache, many, q, lse, w, ws=ops.kv_weigh_workspace(s.cache, many, q)[:-16])
 
 
 class Step:
