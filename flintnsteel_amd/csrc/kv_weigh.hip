@@ -20,7 +20,8 @@ template <int D> struct RowImage {
     using Q = QueryShape<D, float>;
     uint4 low[Q::N][Q::kSteps][64];   // a lane's 32 digits: 16 bytes,
     uint2 high[Q::N][Q::kSteps][64];  // and 8
-    int scale[kRowTile];    // block scale of digit 0
+    static constexpr int kHalves = D == 64 ? 2 : 1;  // (of 64 channels lanes below 32 and the others have different digits)
+    int scale[DigitScales<D, float>::W][kHalves][kRowTile];  // block scales of the digits
     float start[kRowTile];  // -lse in log2 units; -infinity: the row adds nothing
     int from[kRowTile], to[kRowTile], tok[kRowTile];  // Sight
     int any[4];             // the largest `from`, the least `to`, the least `from`, the last position that any row sees
@@ -68,8 +69,13 @@ __device__ __forceinline__ void make_image(const WeighArgs &x, const SeqRange &s
     };
     join(std::integral_constant<int, 1>{}), join(std::integral_constant<int, 2>{});
     join(std::integral_constant<int, 4>{}), join(std::integral_constant<int, 8>{});
+    DigitScales<D, float> qsc;
+    qsc.set(on ? scale : 127);
+    if (g % 2 == 0 && g / 2 < RowImage<D>::kHalves)
+#pragma unroll
+        for (int i = 0; i < qsc.W; ++i) o.scale[i][g / 2][r] = qsc.w[i];
     if (g == 0) {
-        o.scale[r] = on ? scale : 127, o.start[r] = on ? -lse * kLog2e : -INFINITY;
+        o.start[r] = on ? -lse * kLog2e : -INFINITY;
         o.from[r] = see.from, o.to[r] = see.to, o.tok[r] = see.tok;
         if (r == 0) o.any[0] = hi, o.any[1] = lo, o.any[2] = least, o.any[3] = most;
     }
@@ -95,6 +101,12 @@ template <int D, int KT> struct Keys {
             scale[t][u] = p[L::k_scale(P, row) + block];
         }
     }
+    __device__ __forceinline__ void wait() {  // (what is used here has arrived)
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int u = 0; u < kKPieces<D>; ++u) asm volatile("" : "+v"(k[t][u]), "+v"(scale[t][u]));
+    }
     __device__ __forceinline__ bool nan(int t) const {  // of key 16 t + r
         int bad = 0;
 #pragma unroll
@@ -105,14 +117,25 @@ template <int D, int KT> struct Keys {
     }
 };
 
+// Bits off .. off + 63 of a token's: what it sees of the new tokens from the off-th on.
+__device__ __forceinline__ uint64_t new_bits(const NewTokens<true> &nt, int tok, int off) {
+    if (off <= -64 || off >= 64 * nt.words) return 0;
+    const uint64_t *row = nt.sees + (int64_t) tok * nt.words;
+    const int i = off >> 6, sh = off & 63;
+    const uint64_t lo = i >= 0 ? row[i] : 0, hi = sh && i + 1 < nt.words ? row[i + 1] : 0;
+    return (lo >> sh) | (sh ? hi << (64 - sh) : 0);
+}
+
 // What 16 rows add to KT tiles of keys from base on: a lane's key is base + 16 t + r, its rows 4 g .. 4 g + 3.
-template <int D, int KT>
+// TREE: of a tree (causal rows need no look at its bits, whose loads would be waited for with all the others).
+template <bool TREE, int D, int KT>
 __device__ __forceinline__ void add_rows(const RowImage<D> &im, const NewTokens<true> &nt, const Keys<D, KT> &keys, int base, float (&sum)[KT]) {
     using Q = QueryShape<D, float>;
     const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     if (im.any[3] < base || im.any[2] >= base + 16 * KT - 1) return;
-    DigitScales<D, float> qsc;
-    qsc.set(im.scale[r]);
+    int qsc[DigitScales<D, float>::W];
+#pragma unroll
+    for (int i = 0; i < DigitScales<D, float>::W; ++i) qsc[i] = im.scale[i][RowImage<D>::kHalves == 2 ? g / 2 : 0][r];
     const f4 start = *(const f4 *) (im.start + 4 * g);
     f4 acc[KT];
 #pragma unroll
@@ -124,7 +147,7 @@ __device__ __forceinline__ void add_rows(const RowImage<D> &im, const NewTokens<
             const uint4 lo = im.low[n][u][lane];
             const uint2 hi = im.high[n][u][lane];
             const i8v q = {(int) lo.x, (int) lo.y, (int) lo.z, (int) lo.w, (int) hi.x, (int) hi.y, 0, 0};
-            const int w = qsc.w[n / 4];
+            const int w = qsc[n / 4];
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
                 const i8v k = {(int) keys.k[t][u][0], (int) keys.k[t][u][1], (int) keys.k[t][u][2], (int) keys.k[t][u][3], 0, 0, 0, 0};
@@ -136,12 +159,17 @@ __device__ __forceinline__ void add_rows(const RowImage<D> &im, const NewTokens<
     if (im.any[0] >= base || im.any[1] < base + 16 * KT - 1) {  // some row does not see all of the keys
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-            const int from = im.from[4 * g + v], to = im.to[4 * g + v], tok = im.tok[4 * g + v];
+            const int from = im.from[4 * g + v], to = im.to[4 * g + v];
+            uint64_t bits[KT / 4] = {};
+            if (TREE && nt.sees) {
+                const int tok = im.tok[4 * g + v];
+#pragma unroll
+                for (int i = 0; i < KT / 4; ++i) bits[i] = tok >= 0 ? new_bits(nt, tok, base + 64 * i - nt.first) : 0;
+            }
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
-                const int pos = base + 16 * t + r, j = pos - nt.first;
-                bool on = pos > from && pos <= to;
-                if (tok >= 0 && j >= 0 && j / 64 < nt.words) on = nt.sees[(int64_t) tok * nt.words + j / 64] >> (j % 64) & 1;
+                const int pos = base + 16 * t + r;
+                const bool on = (pos > from && pos <= to) || (bits[t / 4] >> (16 * (t % 4) + r) & 1);
                 acc[t][v] = on ? acc[t][v] : -INFINITY;
             }
         }
@@ -164,10 +192,14 @@ template <int KT> __device__ __forceinline__ float one_a_lane(const float (&sum)
     }
     return mine;
 }
+__device__ __forceinline__ int64_t weight_at(const WeighArgs &x, int head, int page, int pos) {
+    return (((int64_t) page * x.a.c.n_kv + head) << x.a.c.shift) + (pos & ((1 << x.a.c.shift) - 1));
+}
+__device__ __forceinline__ float past_weight(const WeighArgs &x, int head, int page, int pos, int first) {
+    return page >= 0 && x.past && pos < first ? x.past[weight_at(x, head, page, pos)] : 0.0f;
+}
 __device__ __forceinline__ void put_weight(const WeighArgs &x, int head, int page, int pos, int first, float sum) {
-    if (page < 0) return;
-    const int64_t at = (((int64_t) page * x.a.c.n_kv + head) << x.a.c.shift) + (pos & ((1 << x.a.c.shift) - 1));
-    x.weights[at] = (x.past && pos < first ? x.past[at] : 0.0f) + sum;
+    if (page >= 0) x.weights[weight_at(x, head, page, pos)] = past_weight(x, head, page, pos, first) + sum;
 }
 __device__ __forceinline__ int key_len(const AttnArgs &a, const SeqRange &sr) {  // positions behind the table have no page
     return (int) min((int64_t) sr.len, a.b.table_stride << a.c.shift);
@@ -186,6 +218,7 @@ template <int D, int RT, class T> __global__ __launch_bounds__(256) void k_weigh
     const NewTokens<true> nt(a, sr);
     Keys<D, 4> keys, next;
     int page = -1, after = -1;  // of the lane's own key, of these 64 and of the next
+    float past = 0.0f, coming = 0.0f;
     const auto ask = [&](int64_t base) { return base + lane < len ? page_of(a.c, a.b, s, (int) base + lane) : -1; };
     const auto load = [&](Keys<D, 4> &k, int base, int own) {
 #pragma unroll
@@ -195,6 +228,7 @@ template <int D, int RT, class T> __global__ __launch_bounds__(256) void k_weigh
     if (b0 < len) {
         page = ask(b0);
         load(keys, (int) b0, page);
+        past = past_weight(x, head, page, (int) b0 + lane, first);
         after = ask(b0 + step);
     }
     for (int t = wave; t < RT; t += 4) make_image<D, T>(x, sr, nt, head, rows, t * kRowTile, im[t]);
@@ -202,16 +236,20 @@ template <int D, int RT, class T> __global__ __launch_bounds__(256) void k_weigh
     for (; b0 < len; b0 += step) {
         const int base = (int) b0;
         const bool more = b0 + step < len;
-        if (more) load(next, base + step, after);
+        if (more) {
+            load(next, base + step, after);
+            coming = past_weight(x, head, after, base + step + lane, first);
+        }
         const int then = ask(b0 + 2 * (int64_t) step);
         float sum[4] = {};
         bool good[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) good[t] = !keys.nan(t);
 #pragma unroll 1
-        for (int t = 0; t < RT; ++t) add_rows<D, 4>(im[t], nt, keys, base, sum);
-        put_weight(x, head, page, base + lane, first, one_a_lane(sum, good, 0));
-        keys = next, page = after, after = then;
+        for (int t = 0; t < RT; ++t) add_rows<true, D, 4>(im[t], nt, keys, base, sum);
+        const float sums = one_a_lane(sum, good, 0);
+        if (page >= 0) x.weights[weight_at(x, head, page, base + lane)] = past + sums;
+        keys = next, page = after, after = then, past = coming;
     }
 }
 
@@ -227,13 +265,14 @@ template <int D, class T> __global__ __launch_bounds__(64) void k_weigh_rows(Wei
 }
 
 // Many rows (prompts, large trees): a workgroup takes 512 keys, 128 a wave and in its registers, and walks over the images of a
-// part of the rows, which come through LDS, the next one on its way to registers meanwhile.
-template <int D> __global__ __launch_bounds__(256, 2) void k_weigh_many(WeighArgs x) {
+// part of the rows, which come through LDS, the next two on their way to registers meanwhile. Heads are the grid's first
+// dimension: workgroups of one go to one XCD (where their number is a multiple of 8), whose L2 then holds its images.
+template <bool TREE, int D> __global__ __launch_bounds__(256, 2) void k_weigh_many(WeighArgs x) {
     constexpr int KT = kKeyTiles, PIECES = sizeof(RowImage<D>) / 16, PER = (PIECES + 255) / 256;
     static_assert(sizeof(RowImage<D>) % 16 == 0, "images are copied in pieces of 16 bytes");
     const AttnArgs &a = x.a;
     __shared__ __align__(16) RowImage<D> im[2];
-    const int s = blockIdx.y / a.c.n_kv, head = blockIdx.y % a.c.n_kv, part = blockIdx.z, tid = threadIdx.x, lane = tid % 64, r = lane % 16;
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, part = blockIdx.z, tid = threadIdx.x, lane = tid % 64, r = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const SeqRange sr = seq_range(a.b, s);
     const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) INT32_MAX);
@@ -241,13 +280,13 @@ template <int D> __global__ __launch_bounds__(256, 2) void k_weigh_many(WeighArg
     const int tiles = (int) min((int64_t) (rows - 1) / kRowTile + 1, x.row_tiles);  // (rows behind max_q tokens have no image)
     const int first = sr.len - sr.n, len = key_len(a, sr);
     const NewTokens<true> nt(a, sr);
-    const RowImage<D> *images = (const RowImage<D> *) x.rows + blockIdx.y * x.row_tiles;
-    for (int64_t b0 = (int64_t) blockIdx.x * kBlock; b0 < len; b0 += (int64_t) gridDim.x * kBlock) {
+    const RowImage<D> *images = (const RowImage<D> *) x.rows + blockIdx.x * x.row_tiles;
+    for (int64_t b0 = (int64_t) blockIdx.y * kBlock; b0 < len; b0 += (int64_t) gridDim.y * kBlock) {
         const bool apart = x.parts > 1 && b0 < (int64_t) x.blocks * kBlock;  // (longer than the host's number: the first part does all)
         if (!apart && part > 0) break;
         // the row tiles of this part that see any of these keys
         int t0 = apart ? (int) ((int64_t) tiles * part / x.parts) : 0, t1 = apart ? (int) ((int64_t) tiles * (part + 1) / x.parts) : tiles;
-        if (!a.sees) {
+        if (!TREE) {
             const int64_t row0 = max(b0 - first, (int64_t) 0) * a.group;
             t0 = (int) max((int64_t) t0, row0 / kRowTile);
             if (a.window) {
@@ -259,14 +298,15 @@ template <int D> __global__ __launch_bounds__(256, 2) void k_weigh_many(WeighArg
         Keys<D, KT> keys;
         bool good[KT];
         float sum[KT] = {};
-        uint4 stage[PER];
-        const auto fetch = [&](int t) {
+        u4 stage[2][PER];
+        const auto fetch = [&](int t, u4 (&to)[PER]) {
 #pragma unroll
             for (int p = 0; p < PER; ++p)
-                if (tid + 256 * p < PIECES) stage[p] = ((const uint4 *) (images + t))[tid + 256 * p];
+                to[p] = ((const u4 *) (images + t))[min(tid + 256 * p, PIECES - 1)];
         };
         if (t0 < t1) {
-            fetch(t0);
+            fetch(t0, stage[0]);
+            fetch(min(t0 + 1, t1 - 1), stage[1]);
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
                 const int pos = base + 16 * t + r;
@@ -274,14 +314,22 @@ template <int D> __global__ __launch_bounds__(256, 2) void k_weigh_many(WeighArg
             }
 #pragma unroll
             for (int t = 0; t < KT; ++t) good[t] = !keys.nan(t);
-            for (int i = t0; i < t1; ++i) {
-                uint4 *to = (uint4 *) &im[(i - t0) & 1];
+            keys.wait();  // (here, or every step would wait for its own fetch)
+            const auto turn = [&](int i, auto which) {
+                constexpr int W = decltype(which)::value;
+                u4 *to = (u4 *) &im[W];
 #pragma unroll
                 for (int p = 0; p < PER; ++p)
-                    if (tid + 256 * p < PIECES) to[tid + 256 * p] = stage[p];
-                if (i + 1 < t1) fetch(i + 1);
+                    if (tid + 256 * p < PIECES) to[tid + 256 * p] = stage[W][p];
+                fetch(min(i + 2, t1 - 1), stage[W]);  // (no branch: it would be waited for)
                 tile_barrier();
-                add_rows<D, KT>(im[(i - t0) & 1], nt, keys, base, sum);
+                add_rows<TREE, D, KT>(im[W], nt, keys, base, sum);
+            };
+            for (int i = t0;;) {  // (the way back is from the second turn alone: what is on its way is then known, and not waited for)
+                turn(i, std::integral_constant<int, 0>{});
+                if (++i >= t1) break;
+                turn(i, std::integral_constant<int, 1>{});
+                if (++i >= t1) break;
             }
             tile_barrier();  // (the next block writes the images again)
         }
@@ -289,7 +337,7 @@ template <int D> __global__ __launch_bounds__(256, 2) void k_weigh_many(WeighArg
         for (int t = 0; t < KT; t += 4) {
             const int pos = base + 16 * t + lane;
             const float mine = t0 < t1 ? one_a_lane(sum, good, t) : 0.0f;
-            if (apart) x.part[((int64_t) blockIdx.y * x.parts + part) * x.blocks * kBlock + pos] = mine;
+            if (apart) x.part[((int64_t) blockIdx.x * x.parts + part) * x.blocks * kBlock + pos] = mine;
             else put_weight(x, head, pos >= 0 && pos < len ? page_of(a.c, a.b, s, pos) : -1, pos, first, mine);
         }
     }
@@ -298,11 +346,11 @@ template <int D> __global__ __launch_bounds__(256, 2) void k_weigh_many(WeighArg
 // The parts of a key's sum, in order.
 __global__ __launch_bounds__(256) void k_weigh_join(WeighArgs x) {
     const AttnArgs &a = x.a;
-    const int s = blockIdx.y / a.c.n_kv, head = blockIdx.y % a.c.n_kv, pos = blockIdx.x * 256 + threadIdx.x;
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, pos = blockIdx.y * 256 + threadIdx.x;
     const SeqRange sr = seq_range(a.b, s);
     if (sr.n == 0 || pos >= key_len(a, sr)) return;
     const int64_t step = (int64_t) x.blocks * kBlock;
-    const float *p = x.part + blockIdx.y * x.parts * step + pos;
+    const float *p = x.part + blockIdx.x * x.parts * step + pos;
     float sum = 0.0f;
 #pragma unroll 8
     for (int i = 0; i < x.parts; ++i) sum += p[i * step];
@@ -326,7 +374,7 @@ WeighPlan weigh_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x)
         p.blocks = std::min(per(std::max<int64_t>(b->max_kv, 1), 256), per(2048, heads));
         return p;
     }
-    p.blocks = per(std::max<int64_t>(b->max_kv, 1), kBlock);
+    p.blocks = std::min<int64_t>(per(std::max<int64_t>(b->max_kv, 1), kBlock), 65535 / (kBlock / 256));
     p.parts = std::max<int64_t>(1, std::min(std::min<int64_t>(per(1024, heads * p.blocks), p.row_tiles / 8), (int64_t) 64));
     p.part_off = (size_t) (heads * p.row_tiles) * image_bytes(c->head_dim);
     p.bytes = p.part_off + (p.parts > 1 ? (size_t) (heads * p.parts * p.blocks) * kBlock * 4 : 0);
@@ -378,9 +426,11 @@ int kv_weigh(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const F
         if (p.few) return host::check_launch("kv_weigh");
         hipLaunchKernelGGL((k_weigh_rows<D, T>), dim3(heads, (unsigned) p.row_tiles), dim3(64), 0, st, w);
         FNS_TRY(host::check_launch("kv_weigh"));
-        hipLaunchKernelGGL((k_weigh_many<D>), dim3(blocks, heads, (unsigned) p.parts), dim3(256), 0, st, w);
+        const auto many = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(heads, blocks, (unsigned) p.parts), dim3(256), 0, st, w); };
+        if (t) many(k_weigh_many<true, D>);
+        else many(k_weigh_many<false, D>);
         FNS_TRY(host::check_launch("kv_weigh"));
-        if (p.parts > 1) hipLaunchKernelGGL(k_weigh_join, dim3(blocks * (kBlock / 256), heads), dim3(256), 0, st, w);
+        if (p.parts > 1) hipLaunchKernelGGL(k_weigh_join, dim3(heads, blocks * (kBlock / 256)), dim3(256), 0, st, w);
         return host::check_launch("kv_weigh");
     };
     const auto by_dim = [&](auto dim) { return x->dtype == FNS_TYPE_F32 ? by_type(dim, float{}) : by_type(dim, uint16_t{}); };
