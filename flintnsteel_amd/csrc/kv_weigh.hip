@@ -6,14 +6,17 @@
 // so that they come as exponents.
 #include "fns_attn.hpp"
 
+#include <cmath>
+#include <cstddef>
+
 namespace fns {
 
 namespace {
 
 constexpr int kRowTile = 16;
 constexpr int kFewTiles = 4;    // row tiles that a workgroup of few rows holds
-constexpr int kKeyTiles = 8;    // 16-key tiles of a wave of many rows
-constexpr int kBlock = 4 * 16 * kKeyTiles;  // keys of its workgroup
+constexpr int key_tiles(int D) { return D == 256 ? 4 : 8; }     // 16-key tiles of a wave of many rows (the registers are counted)
+constexpr int key_block(int D) { return 4 * 16 * key_tiles(D); }  // keys of its workgroup
 
 // Sixteen rows as the product takes them.
 template <int D> struct RowImage {
@@ -32,9 +35,10 @@ struct WeighArgs {
     const float *lse, *past;
     float *weights;
     void *rows;         // many rows: RowImage [n_seq * n_kv][row_tiles]
-    float *part;        // many rows in parts: [n_seq * n_kv][parts][blocks * kBlock] their sums
     int64_t row_tiles;
-    int parts, blocks;
+    int32_t *plan;      // [n_seq * n_kv][blocks + 1] the (block, row tile) steps before a block
+    float *part;        // [n_seq * n_kv][shares][2][block] sums over some of a block's rows
+    int blocks, shares, block;  // blocks of keys by the host's number; workgroups of a kv head; key_block
 };
 
 // The image of rows row0 .. row0 + 15 of a sequence's kv head, by a wave.
@@ -51,7 +55,7 @@ __device__ __forceinline__ void make_image(const WeighArgs &x, const SeqRange &s
     bool on = fabsf(lse) < INFINITY;
     Digits<D, float> w;
     const int scale = query_digits<D, float>(w, (const T *) a.q + tok * a.q_stride + (int64_t) h * D, on, a.scale);
-    on = on && scale != 255;
+    on = on && scale != 255 && (!nt.sees || see.tok >= 0);  // (a token without bits sees nothing)
 #pragma unroll
     for (int n = 0; n < Q::N; ++n)
 #pragma unroll
@@ -126,58 +130,80 @@ __device__ __forceinline__ uint64_t new_bits(const NewTokens<true> &nt, int tok,
     return (lo >> sh) | (sh ? hi << (64 - sh) : 0);
 }
 
-// What 16 rows add to KT tiles of keys from base on: a lane's key is base + 16 t + r, its rows 4 g .. 4 g + 3.
-// TREE: of a tree (causal rows need no look at its bits, whose loads would be waited for with all the others).
-template <bool TREE, int D, int KT>
-__device__ __forceinline__ void add_rows(const RowImage<D> &im, const NewTokens<true> &nt, const Keys<D, KT> &keys, int base, float (&sum)[KT]) {
+// The rows of an image against 64 keys (tiles T0 .. T0 + 3 of a wave's, from base on), a lane's key being base + 16 t + r and its
+// rows 4 g .. 4 g + 3: exponents of what they add, in two steps.
+template <int D> struct RowDigits {
     using Q = QueryShape<D, float>;
-    const int lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
-    if (im.any[3] < base || im.any[2] >= base + 16 * KT - 1) return;
-    int qsc[DigitScales<D, float>::W];
+    i8v q[Q::N][Q::kSteps];
+    int scale[DigitScales<D, float>::W];
+    f4 start;
+    // (offsets in 32 bits that a lane keeps, from an image's place in scalar registers)
+    __device__ __forceinline__ void read(const RowImage<D> &im) {
+        using I = RowImage<D>;
+        const uint32_t lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
+        const char *p = (const char *) &im;
+        const uint32_t at_low = lane * 16, at_high = lane * 8 + (uint32_t) offsetof(I, high);
+        const uint32_t at_scale = (I::kHalves == 2 ? g / 2 * kRowTile + r : r) * 4 + (uint32_t) offsetof(I, scale);
 #pragma unroll
-    for (int i = 0; i < DigitScales<D, float>::W; ++i) qsc[i] = im.scale[i][RowImage<D>::kHalves == 2 ? g / 2 : 0][r];
-    const f4 start = *(const f4 *) (im.start + 4 * g);
-    f4 acc[KT];
+        for (int n = 0; n < Q::N; ++n)
 #pragma unroll
-    for (int t = 0; t < KT; ++t) acc[t] = start;
+            for (int u = 0; u < Q::kSteps; ++u) {
+                const u4 lo = *(const u4 *) (p + (at_low + (n * Q::kSteps + u) * 1024));
+                const uint2 hi = *(const uint2 *) (p + (at_high + (n * Q::kSteps + u) * 512));
+                q[n][u] = i8v{(int) lo[0], (int) lo[1], (int) lo[2], (int) lo[3], (int) hi.x, (int) hi.y, 0, 0};
+            }
+#pragma unroll
+        for (int i = 0; i < DigitScales<D, float>::W; ++i) scale[i] = *(const int *) (p + (at_scale + i * I::kHalves * kRowTile * 4));
+        start = *(const f4 *) (p + (g * 16 + (uint32_t) offsetof(I, start)));
+    }
+};
+template <int T0, int D, int KT>
+__device__ __forceinline__ void products(const RowDigits<D> &rows, const Keys<D, KT> &keys, f4 (&acc)[4]) {
+    using Q = QueryShape<D, float>;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] = rows.start;
 #pragma unroll
     for (int n = 0; n < Q::N; ++n)  // the largest digit first: the rest adds to small numbers
 #pragma unroll
-        for (int u = 0; u < Q::kSteps; ++u) {
-            const uint4 lo = im.low[n][u][lane];
-            const uint2 hi = im.high[n][u][lane];
-            const i8v q = {(int) lo.x, (int) lo.y, (int) lo.z, (int) lo.w, (int) hi.x, (int) hi.y, 0, 0};
-            const int w = qsc[n / 4];
+        for (int u = 0; u < Q::kSteps; ++u)
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const i8v k = {(int) keys.k[t][u][0], (int) keys.k[t][u][1], (int) keys.k[t][u][2], (int) keys.k[t][u][3], 0, 0, 0, 0};
-                const int e = keys.scale[t][u];
+            for (int t = 0; t < 4; ++t) {
+                const u4 x = keys.k[T0 + t][u];
+                const i8v k = {(int) x[0], (int) x[1], (int) x[2], (int) x[3], 0, 0, 0, 0}, q = rows.q[n][u];
+                const int e = keys.scale[T0 + t][u], w = rows.scale[n / 4];
                 acc[t] = n % 4 == 0 ? row_mfma<0>(q, k, acc[t], w, e) : n % 4 == 1 ? row_mfma<1>(q, k, acc[t], w, e) :
                          n % 4 == 2 ? row_mfma<2>(q, k, acc[t], w, e) : row_mfma<3>(q, k, acc[t], w, e);
             }
+}
+// TREE: of a tree (causal rows need no look at its bits, whose loads would be waited for with all the others).
+template <bool TREE, int D>
+__device__ __forceinline__ void hide(const RowImage<D> &im, const NewTokens<true> &nt, int base, f4 (&acc)[4]) {
+    const int r = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        const int from = im.from[4 * g + v], to = im.to[4 * g + v];
+        uint64_t bits = 0;
+        if (TREE && nt.sees) {
+            const int tok = im.tok[4 * g + v];
+            bits = tok >= 0 ? new_bits(nt, tok, base - nt.first) : 0;
         }
-    if (im.any[0] >= base || im.any[1] < base + 16 * KT - 1) {  // some row does not see all of the keys
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int from = im.from[4 * g + v], to = im.to[4 * g + v];
-            uint64_t bits[KT / 4] = {};
-            if (TREE && nt.sees) {
-                const int tok = im.tok[4 * g + v];
-#pragma unroll
-                for (int i = 0; i < KT / 4; ++i) bits[i] = tok >= 0 ? new_bits(nt, tok, base + 64 * i - nt.first) : 0;
-            }
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const int pos = base + 16 * t + r;
-                const bool on = (pos > from && pos <= to) || (bits[t / 4] >> (16 * (t % 4) + r) & 1);
-                acc[t][v] = on ? acc[t][v] : -INFINITY;
-            }
+        for (int t = 0; t < 4; ++t) {
+            const int pos = base + 16 * t + r;
+            const bool on = (pos > from && pos <= to) || (TREE && (bits >> (16 * t + r) & 1));
+            acc[t][v] = on ? acc[t][v] : -INFINITY;
         }
     }
+}
+__device__ __forceinline__ void add_exps(const f4 (&acc)[4], float *sum) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int v = 0; v < 4; ++v) sum[t] += __builtin_amdgcn_exp2f(acc[t][v]);
+}
+// (nothing of the image is seen of the 64 keys from base on)
+template <int D> __device__ __forceinline__ bool unseen(const RowImage<D> &im, int base, int keys) {
+    return im.any[3] < base || im.any[2] >= base + keys - 1;
 }
 
 // The sums of 64 keys (tiles t0 .. t0 + 3), one a lane; good: whether key 16 t + r takes any.
@@ -204,6 +230,29 @@ __device__ __forceinline__ void put_weight(const WeighArgs &x, int head, int pag
 __device__ __forceinline__ int key_len(const AttnArgs &a, const SeqRange &sr) {  // positions behind the table have no page
     return (int) min((int64_t) sr.len, a.b.table_stride << a.c.shift);
 }
+
+// The row tiles [t0, t1) of `tiles` that see any of the keys base .. base + keys - 1.
+struct TileRange {
+    int t0, t1;
+};
+template <bool TREE> __device__ __forceinline__ TileRange tiles_seeing(const AttnArgs &a, int first, int tiles, int64_t base, int keys) {
+    TileRange t{0, tiles};
+    if (!TREE) {
+        const int64_t row0 = max(base - first, (int64_t) 0) * a.group;
+        t.t0 = (int) min(row0 / kRowTile, (int64_t) tiles);
+        if (a.window) {
+            const int64_t row1 = (base + keys - 1 + a.window - first) * a.group;  // (the token at pos sees from pos - window + 1 on)
+            t.t1 = (int) max((int64_t) t.t0, min((int64_t) tiles, max(row1, (int64_t) 0) / kRowTile + 1));
+        }
+    }
+    return t;
+}
+// Row tiles that have images, and the blocks of keys of a sequence by the host's number.
+__device__ __forceinline__ int image_tiles(const WeighArgs &x, const SeqRange &sr) {
+    const int64_t rows = min((int64_t) sr.n * x.a.group, (int64_t) INT32_MAX);
+    return (int) min((rows + kRowTile - 1) / kRowTile, x.row_tiles);
+}
+__device__ __forceinline__ int planned_blocks(const WeighArgs &x, int len) { return (int) min(((int64_t) len + x.block - 1) / x.block, (int64_t) x.blocks); }
 
 // Few rows (decode, verify): their images are made by every workgroup, whose waves take 64 keys in turn, the next ones' K
 // asked for before this one's products.
@@ -246,121 +295,266 @@ template <int D, int RT, class T> __global__ __launch_bounds__(256) void k_weigh
 #pragma unroll
         for (int t = 0; t < 4; ++t) good[t] = !keys.nan(t);
 #pragma unroll 1
-        for (int t = 0; t < RT; ++t) add_rows<true, D, 4>(im[t], nt, keys, base, sum);
+        for (int t = 0; t < RT; ++t) {
+            if (unseen(im[t], base, 64)) continue;
+            RowDigits<D> rows_;
+            f4 acc[4];
+            rows_.read(im[t]);
+            products<0>(rows_, keys, acc);
+            if (!(im[t].any[0] < base && im[t].any[1] >= base + 63)) hide<true>(im[t], nt, base, acc);  // (some row does not see all)
+            add_exps(acc, sum);
+        }
         const float sums = one_a_lane(sum, good, 0);
         if (page >= 0) x.weights[weight_at(x, head, page, base + lane)] = past + sums;
         keys = next, page = after, after = then, past = coming;
     }
 }
 
+// `all` steps dealt to n workgroups: the first ones get one more where they do not come out even.
+struct Shares {
+    int each, more;
+    __device__ __forceinline__ Shares(int all, int n) : each(all / n), more(all % n) {}
+    __device__ __forceinline__ int from(int share) const { return share * each + min(share, more); }
+    __device__ __forceinline__ int of(int step) const {  // (there is one: all > 0)
+        const int larger = more * (each + 1);
+        return step < larger ? step / (each + 1) : more + (step - larger) / max(each, 1);
+    }
+};
+
+// The images of many rows; the first wave of a kv head also counts the steps of its blocks of keys.
 template <int D, class T> __global__ __launch_bounds__(64) void k_weigh_rows(WeighArgs x) {
     const AttnArgs &a = x.a;
-    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv;
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, lane = threadIdx.x;
     const SeqRange sr = seq_range(a.b, s);
     const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) INT32_MAX);
+    if (blockIdx.y == 0) {
+        const int blocks = planned_blocks(x, key_len(a, sr)), tiles = image_tiles(x, sr), first = sr.len - sr.n;
+        int32_t *plan = x.plan + (int64_t) blockIdx.x * (x.blocks + 1), before = 0;  // (65535 tiles of 32767 blocks fit)
+        for (int i0 = 0; i0 < blocks; i0 += 64) {
+            const int i = i0 + lane;
+            int n = 0;
+            if (i < blocks) {
+                const int64_t base = (int64_t) i * x.block;
+                const TileRange t = a.sees ? tiles_seeing<true>(a, first, tiles, base, x.block) : tiles_seeing<false>(a, first, tiles, base, x.block);
+                n = t.t1 - t.t0;
+            }
+            int sum = n;
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                const int u = __shfl_up(sum, o, 64);
+                sum += lane >= o ? u : 0;
+            }
+            if (i < blocks) plan[i] = before + sum - n;
+            before += __shfl(sum, 63, 64);
+        }
+        if (lane == 0) plan[blocks] = before;
+    }
     const int64_t row0 = (int64_t) blockIdx.y * kRowTile;
     if (row0 >= rows) return;
     const NewTokens<true> nt(a, sr);
     make_image<D, T>(x, sr, nt, head, rows, (int) row0, ((RowImage<D> *) x.rows)[blockIdx.x * x.row_tiles + blockIdx.y]);
 }
 
-// Many rows (prompts, large trees): a workgroup takes 512 keys, 128 a wave and in its registers, and walks over the images of a
-// part of the rows, which come through LDS, the next two on their way to registers meanwhile. Heads are the grid's first
-// dimension: workgroups of one go to one XCD (where their number is a multiple of 8), whose L2 then holds its images.
-template <bool TREE, int D> __global__ __launch_bounds__(256, 2) void k_weigh_many(WeighArgs x) {
-    constexpr int KT = kKeyTiles, PIECES = sizeof(RowImage<D>) / 16, PER = (PIECES + 255) / 256;
-    static_assert(sizeof(RowImage<D>) % 16 == 0, "images are copied in pieces of 16 bytes");
+// Many rows (prompts, large trees): a workgroup takes 512 keys at a time (256 of 256 channels), a quarter a wave and in its
+// registers, and walks over the images of the rows, each wave by itself, the next image on its way to registers meanwhile (its
+// four readers find it in L1). Products of 64 keys go with the exponentials of the 64 before: both pipes work for one wave. The
+// steps of a kv head (a block of keys and an image) are counted and dealt out evenly, so a workgroup may begin and end inside a
+// block; what it has of a block that others share goes to `part`. Heads are the grid's first dimension: workgroups of one go to
+// one XCD (where their number is a multiple of 8), whose L2 then holds its images.
+template <bool TREE, int D> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_weigh_many(WeighArgs x) {
+    constexpr int KT = key_tiles(D), kBlock = key_block(D);
     const AttnArgs &a = x.a;
-    __shared__ __align__(16) RowImage<D> im[2];
-    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, part = blockIdx.z, tid = threadIdx.x, lane = tid % 64, r = lane % 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, share = blockIdx.y, lane = threadIdx.x % 64, r = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const SeqRange sr = seq_range(a.b, s);
-    const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) INT32_MAX);
-    if (rows == 0) return;
-    const int tiles = (int) min((int64_t) (rows - 1) / kRowTile + 1, x.row_tiles);  // (rows behind max_q tokens have no image)
-    const int first = sr.len - sr.n, len = key_len(a, sr);
+    if (sr.n == 0) return;
+    const int tiles = image_tiles(x, sr), first = sr.len - sr.n, len = key_len(a, sr), blocks = planned_blocks(x, len);
     const NewTokens<true> nt(a, sr);
     const RowImage<D> *images = (const RowImage<D> *) x.rows + blockIdx.x * x.row_tiles;
-    for (int64_t b0 = (int64_t) blockIdx.y * kBlock; b0 < len; b0 += (int64_t) gridDim.y * kBlock) {
-        const bool apart = x.parts > 1 && b0 < (int64_t) x.blocks * kBlock;  // (longer than the host's number: the first part does all)
-        if (!apart && part > 0) break;
-        // the row tiles of this part that see any of these keys
-        int t0 = apart ? (int) ((int64_t) tiles * part / x.parts) : 0, t1 = apart ? (int) ((int64_t) tiles * (part + 1) / x.parts) : tiles;
-        if (!TREE) {
-            const int64_t row0 = max(b0 - first, (int64_t) 0) * a.group;
-            t0 = (int) max((int64_t) t0, row0 / kRowTile);
-            if (a.window) {
-                const int64_t row1 = (b0 + kBlock - 1 + a.window - first) * a.group;  // (the token at pos sees from pos - window + 1 on)
-                t1 = (int) min((int64_t) t1, max(row1, (int64_t) 0) / kRowTile + 1);
-            }
+    const int32_t *plan = x.plan + (int64_t) blockIdx.x * (x.blocks + 1);
+    const Shares sh(plan[blocks], x.shares);
+    const int from = sh.from(share), to = sh.from(share + 1);
+    int block = -1;  // the first one with a step of this share: the last that begins at `from` or before
+    for (int i = 0; i < blocks; i += 64) block += __popcll(__ballot(i + lane < blocks && plan[i + lane] <= from));
+    int at = from;
+    // then blocks behind the host's number (a sequence longer than it says), each whole
+    for (int64_t extra = (int64_t) x.blocks + share; at < to || extra * kBlock < len;) {
+        const bool planned = at < to;
+        const int64_t b0 = planned ? (int64_t) block * kBlock : extra * kBlock;
+        TileRange tr = tiles_seeing<TREE>(a, first, tiles, b0, kBlock);
+        bool whole = true, begins = true;
+        if (planned) {
+            const int p0 = plan[block], p1 = plan[block + 1], e = min(to, p1);
+            whole = at == p0 && e == p1, begins = at == p0;
+            const int t0 = tr.t0 + (at - p0);
+            tr.t1 = tr.t0 + (e - p0), tr.t0 = t0;
+            at = e;
+            ++block;
+        } else {
+            extra += x.shares;
         }
+        // of them, those that see any of the wave's keys
         const int base = (int) b0 + wave * 16 * KT;
+        const TileRange own = tiles_seeing<TREE>(a, first, tiles, base, 16 * KT);
+        const int t0 = max(tr.t0, own.t0), t1 = base < 0 || base >= len ? 0 : min(tr.t1, own.t1);
         Keys<D, KT> keys;
-        bool good[KT];
+        bool good[KT] = {};
         float sum[KT] = {};
-        u4 stage[2][PER];
-        const auto fetch = [&](int t, u4 (&to)[PER]) {
-#pragma unroll
-            for (int p = 0; p < PER; ++p)
-                to[p] = ((const u4 *) (images + t))[min(tid + 256 * p, PIECES - 1)];
-        };
         if (t0 < t1) {
-            fetch(t0, stage[0]);
-            fetch(min(t0 + 1, t1 - 1), stage[1]);
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
                 const int pos = base + 16 * t + r;
                 keys.load(x, head, base, t, pos >= 0 && pos < len ? page_of(a.c, a.b, s, pos) : -1);
             }
+            // Rows from c0 to c1 see all of the keys: no masks there.
+            int c0 = t0, c1 = t1;
+            if (TREE) {
+                if (a.window || base + 16 * KT > first) c0 = t1;
+            } else {
+                const int64_t past_last = ((int64_t) base + 16 * KT - 1 - first) * a.group;  // the first row at the last key
+                c0 = (int) min(max((int64_t) t0, (past_last + kRowTile - 1) / kRowTile), (int64_t) t1);
+                if (a.window) {
+                    const int64_t below = ((int64_t) base + a.window - first) * a.group;  // the first row that does not see the first key
+                    c1 = (int) min(max(below / kRowTile, (int64_t) c0), (int64_t) t1);
+                }
+            }
+            // Causal rows see the key at pos from row (pos - first) * group on, with a window up to row (pos + window - first) * group.
+            int lo[KT], hi[KT];
+            if (!TREE && (t0 < c0 || c1 < t1)) {
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    const int64_t row = ((int64_t) base + 16 * t + r - first) * a.group;
+                    lo[t] = (int) min(max(row, (int64_t) 0), (int64_t) INT32_MAX);
+                    hi[t] = a.window ? (int) min(max(row + (int64_t) a.window * a.group, (int64_t) 0), (int64_t) INT32_MAX) : INT32_MAX;
+                }
+            }
 #pragma unroll
             for (int t = 0; t < KT; ++t) good[t] = !keys.nan(t);
-            keys.wait();  // (here, or every step would wait for its own fetch)
-            const auto turn = [&](int i, auto which) {
-                constexpr int W = decltype(which)::value;
-                u4 *to = (u4 *) &im[W];
+            keys.wait();  // (here, or every step would wait for what it has asked for)
+            const auto walk = [&](int i0, int i1, auto masked) {
+                constexpr bool MASK = decltype(masked)::value;
+                if (i0 >= i1) return;
+                RowDigits<D> now, next;
+                now.read(images[i0]);
+                f4 acc[2][4];
 #pragma unroll
-                for (int p = 0; p < PER; ++p)
-                    if (tid + 256 * p < PIECES) to[tid + 256 * p] = stage[W][p];
-                fetch(min(i + 2, t1 - 1), stage[W]);  // (no branch: it would be waited for)
-                tile_barrier();
-                add_rows<TREE, D, KT>(im[W], nt, keys, base, sum);
+                for (int t = 0; t < 4; ++t) acc[1][t] = f4{1, 1, 1, 1} * -INFINITY;
+                const auto begin = [](f4 (&x)[4]) {  // (the exponentials stay below here)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(x[t]));
+                };
+                const auto end = [](float *x) {  // (and above here)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(x[t]));
+                };
+                const auto mix = [&] {  // some instructions of the matrix pipe, then an exponential in their shadow
+                    if (MASK) return;
+                    constexpr int M = QueryShape<D, float>::N * QueryShape<D, float>::kSteps;  // of four exponentials
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x8, (M + 3) / 4, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x8, (M + 1) / 4, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x8, (M + 2) / 4, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x8, M / 4, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
+                    }
+                };
+                const auto cut = [&](int i, int h, f4 (&x)[4]) {
+                    if constexpr (MASK && TREE) {
+                        hide<TREE>(images[i], nt, base + 64 * h, x);
+                    } else if constexpr (MASK) {
+#pragma unroll
+                        for (int t = 0; t < 4; ++t)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) {
+                                const int row = i * kRowTile + 4 * (lane / 16) + v;
+                                x[t][v] = row >= lo[4 * h + t] && row < hi[4 * h + t] ? x[t][v] : -INFINITY;
+                            }
+                    }
+                };
+                const auto turn = [&](int i, RowDigits<D> &rows_, RowDigits<D> &then, auto which) {
+                    constexpr int W = decltype(which)::value;
+                    then.read(images[min(i + 1, i1 - 1)]);  // (no branch: it would be waited for)
+                    if constexpr (KT == 8) {
+                        begin(acc[1]);
+                        products<0>(rows_, keys, acc[0]);
+                        add_exps(acc[1], sum + 4);
+                        mix();
+                        end(sum + 4);
+                        cut(i, 0, acc[0]);
+                        begin(acc[0]);
+                        products<4>(rows_, keys, acc[1]);
+                        add_exps(acc[0], sum);
+                        mix();
+                        end(sum);
+                        cut(i, 1, acc[1]);
+                    } else {
+                        begin(acc[W ^ 1]);
+                        products<0>(rows_, keys, acc[W]);
+                        add_exps(acc[W ^ 1], sum);
+                        mix();
+                        end(sum);
+                        cut(i, 0, acc[W]);
+                    }
+                };
+#pragma unroll 1
+                for (int i = i0;;) {  // (the way back is from the second turn alone: what is on its way is then known)
+                    turn(i, now, next, std::integral_constant<int, 0>{});
+                    if (++i >= i1) break;
+                    turn(i, next, now, std::integral_constant<int, 1>{});
+                    if (++i >= i1) break;
+                }
+                add_exps(acc[KT == 8 || (i1 - i0) % 2 == 0], sum + KT - 4);
             };
-            for (int i = t0;;) {  // (the way back is from the second turn alone: what is on its way is then known, and not waited for)
-                turn(i, std::integral_constant<int, 0>{});
-                if (++i >= t1) break;
-                turn(i, std::integral_constant<int, 1>{});
-                if (++i >= t1) break;
-            }
-            tile_barrier();  // (the next block writes the images again)
+            walk(t0, c0, std::true_type{});
+            walk(c0, c1, std::false_type{});
+            if (a.window) walk(c1, t1, std::true_type{});
         }
 #pragma unroll
         for (int t = 0; t < KT; t += 4) {
             const int pos = base + 16 * t + lane;
-            const float mine = t0 < t1 ? one_a_lane(sum, good, t) : 0.0f;
-            if (apart) x.part[((int64_t) blockIdx.x * x.parts + part) * x.blocks * kBlock + pos] = mine;
-            else put_weight(x, head, pos >= 0 && pos < len ? page_of(a.c, a.b, s, pos) : -1, pos, first, mine);
+            const float mine = one_a_lane(sum, good, t);
+            if (whole) put_weight(x, head, pos >= 0 && pos < len ? page_of(a.c, a.b, s, pos) : -1, pos, first, mine);
+            else x.part[(((int64_t) blockIdx.x * x.shares + share) * 2 + begins) * kBlock + wave * 16 * KT + 16 * t + lane] = mine;
         }
     }
 }
 
-// The parts of a key's sum, in order.
+// The sums of blocks that workgroups share, or that no row sees, in the rows' order.
 __global__ __launch_bounds__(256) void k_weigh_join(WeighArgs x) {
     const AttnArgs &a = x.a;
-    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, pos = blockIdx.y * 256 + threadIdx.x;
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, in = blockIdx.y % (x.block / 256) * 256 + threadIdx.x;
     const SeqRange sr = seq_range(a.b, s);
-    if (sr.n == 0 || pos >= key_len(a, sr)) return;
-    const int64_t step = (int64_t) x.blocks * kBlock;
-    const float *p = x.part + blockIdx.x * x.parts * step + pos;
+    const int len = key_len(a, sr), block = blockIdx.y / (x.block / 256), blocks = planned_blocks(x, len);
+    const int64_t pos = (int64_t) block * x.block + in;
+    if (sr.n == 0 || block >= blocks || pos >= len) return;
+    const int32_t *plan = x.plan + (int64_t) blockIdx.x * (x.blocks + 1);
+    const int p0 = plan[block], p1 = plan[block + 1];
     float sum = 0.0f;
+    if (p0 < p1) {
+        const Shares sh(plan[blocks], x.shares);
+        const int w0 = sh.of(p0), w1 = sh.of(p1 - 1);
+        if (w0 == w1) return;  // (written by that workgroup)
+        const float *part = x.part + (int64_t) blockIdx.x * x.shares * 2 * x.block + in;
+        sum = part[(w0 * 2 + 1) * x.block];
 #pragma unroll 8
-    for (int i = 0; i < x.parts; ++i) sum += p[i * step];
-    put_weight(x, head, page_of(a.c, a.b, s, pos), pos, sr.len - sr.n, sum);
+        for (int w = w0 + 1; w <= w1; ++w) sum += part[w * 2 * x.block];
+    }
+    put_weight(x, head, page_of(a.c, a.b, s, (int) pos), (int) pos, sr.len - sr.n, sum);
 }
 
 struct WeighPlan {
     int few;  // row tiles of the form of few rows (1, 2 or 4), or 0
-    int64_t row_tiles, blocks, parts;
-    size_t part_off, bytes;
+    int64_t row_tiles, blocks, shares;
+    int block;
+    size_t plan_off, part_off, bytes;
 };
 size_t image_bytes(int D) { return D == 64 ? sizeof(RowImage<64>) : D == 128 ? sizeof(RowImage<128>) : sizeof(RowImage<256>); }
 WeighPlan weigh_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
@@ -374,10 +568,17 @@ WeighPlan weigh_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x)
         p.blocks = std::min(per(std::max<int64_t>(b->max_kv, 1), 256), per(2048, heads));
         return p;
     }
-    p.blocks = std::min<int64_t>(per(std::max<int64_t>(b->max_kv, 1), kBlock), 65535 / (kBlock / 256));
-    p.parts = std::max<int64_t>(1, std::min(std::min<int64_t>(per(1024, heads * p.blocks), p.row_tiles / 8), (int64_t) 64));
-    p.part_off = (size_t) (heads * p.row_tiles) * image_bytes(c->head_dim);
-    p.bytes = p.part_off + (p.parts > 1 ? (size_t) (heads * p.parts * p.blocks) * kBlock * 4 : 0);
+    p.block = key_block(c->head_dim);
+    p.blocks = std::min<int64_t>(per(std::max<int64_t>(b->max_kv, 1), p.block), 65535 / (p.block / 256));
+    // Workgroups of a kv head: as many as there are places for all heads' at once (two a CU; one of 256 channels), or, of many
+    // heads, so many that the last round's empty places do not matter; no more than give a share of four steps.
+    const int64_t places = c->head_dim == 256 ? 256 : 512;
+    p.shares = heads <= places / 2 ? places / heads : per(4 * places, heads);
+    p.shares = std::max<int64_t>(1, std::min(p.shares, p.row_tiles * p.blocks / 4));
+    const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    p.plan_off = up((size_t) (heads * p.row_tiles) * image_bytes(c->head_dim));
+    p.part_off = p.plan_off + up((size_t) (heads * (p.blocks + 1)) * 4);
+    p.bytes = p.part_off + (size_t) (heads * p.shares) * 2 * p.block * 4;
     return p;
 }
 
@@ -414,7 +615,8 @@ int kv_weigh(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const F
     w.a.group = x->n_head / c->n_head_kv, w.a.window = x->window, w.a.scale = x->scale;
     w.a.sees = t ? t->sees : nullptr, w.a.words = t ? t->words : 0;
     w.lse = lse, w.past = past, w.weights = weights, w.rows = ws, w.row_tiles = p.row_tiles;
-    w.part = (float *) ((uint8_t *) ws + p.part_off), w.parts = (int) p.parts, w.blocks = (int) p.blocks;
+    w.plan = (int32_t *) ((uint8_t *) ws + p.plan_off), w.part = (float *) ((uint8_t *) ws + p.part_off);
+    w.blocks = (int) p.blocks, w.shares = (int) p.shares, w.block = p.block;
     const unsigned heads = (unsigned) (b->n_seq * c->n_head_kv), blocks = (unsigned) p.blocks;
     const auto by_type = [&](auto dim, auto type) {
         constexpr int D = decltype(dim)::value;
@@ -426,11 +628,11 @@ int kv_weigh(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const F
         if (p.few) return host::check_launch("kv_weigh");
         hipLaunchKernelGGL((k_weigh_rows<D, T>), dim3(heads, (unsigned) p.row_tiles), dim3(64), 0, st, w);
         FNS_TRY(host::check_launch("kv_weigh"));
-        const auto many = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(heads, blocks, (unsigned) p.parts), dim3(256), 0, st, w); };
+        const auto many = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(heads, (unsigned) p.shares), dim3(256), 0, st, w); };
         if (t) many(k_weigh_many<true, D>);
         else many(k_weigh_many<false, D>);
         FNS_TRY(host::check_launch("kv_weigh"));
-        if (p.parts > 1) hipLaunchKernelGGL(k_weigh_join, dim3(heads, blocks * (kBlock / 256)), dim3(256), 0, st, w);
+        hipLaunchKernelGGL(k_weigh_join, dim3(heads, blocks * (p.block / 256)), dim3(256), 0, st, w);
         return host::check_launch("kv_weigh");
     };
     const auto by_dim = [&](auto dim) { return x->dtype == FNS_TYPE_F32 ? by_type(dim, float{}) : by_type(dim, uint16_t{}); };
