@@ -93,6 +93,7 @@ SIGNATURES: dict[str, list] = {
     "fns_hip_rope_scaled": [_I, _D, _D, _D, _D, _D, _P, _P],
     "fns_hip_kv_append_at": [_P, _P, _P, _P, _F, _P],
     "fns_hip_tree_plan": [_P, _P, _P, _I, _P, _P, _P],
+    "fns_hip_attn_tree_workspace": [_P, _P, _P, _P],
     "fns_hip_attn_tree": [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
     "fns_hip_kv_weigh_workspace": [_P, _P, _P, _P],
     "fns_hip_kv_weigh": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],

@@ -6,7 +6,35 @@
 
 namespace fns {
 
+namespace {
+
+// A tree's rows all see the same tiles of keys, so that the form of many rows can be divided over them as the other is.
+host::AttnPlan division(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
+    host::AttnPlan p = host::attn_plan(c, b, x);
+    const auto per = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
+    const int64_t rows = std::min<int64_t>(b->max_q, b->n_tok) * (x->n_head / c->n_head_kv), heads = (int64_t) b->n_seq * c->n_head_kv;
+    if (rows <= kFewRows) return p;
+    p.rows = kManyRows, p.row_tiles = per(rows, kManyRows);
+    const int64_t wgs = std::max<int64_t>(1, heads * p.row_tiles), tiles = std::max<int64_t>(1, (b->max_kv + kTile - 1) / kTile);
+    p.splits = (int) std::max<int64_t>(1, std::min({per(512, wgs), per(tiles, 4), (int64_t) 64}));
+    p.chunk = (int) per(tiles, p.splits);
+    const size_t n = p.splits > 1 ? (size_t) p.splits * b->n_tok * x->n_head : 0;
+    p.ml_off = n * c->head_dim * 4;
+    p.redo_off = p.ml_off + n * 8;
+    p.bytes = p.redo_off + (size_t) (heads * p.row_tiles * p.splits) * 4;
+    return p;
+}
+
+}  // namespace
+
 namespace impl {
+
+int attn_tree_workspace(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, size_t *bytes) {
+    FNS_TRY(host::attn_check(c, b, x, "attn_tree"));
+    if (!bytes) return host::set_error(host::ERR_SHAPE, "attn_tree_workspace: null output");
+    *bytes = std::max(host::attn_plan(c, b, x).bytes, division(c, b, x).bytes);
+    return host::OK;
+}
 
 int attn_tree(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const FnsKvTree *t, const void *q, void *out, float *lse,
               void *ws, size_t ws_bytes, hipStream_t st) {
@@ -14,7 +42,7 @@ int attn_tree(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const 
     if (t && (t->words < 1 || t->words > 16)) return host::set_error(host::ERR_SHAPE, "attn_tree: words must be 1..16 (%d)", t->words);
     if (b->n_seq == 0 || b->n_tok == 0 || b->max_q == 0) return host::OK;
     if (t && !t->sees) return host::set_error(host::ERR_SHAPE, "attn_tree: a tree without bits");
-    const host::AttnPlan p = host::attn_plan(c, b, x);
+    const host::AttnPlan p = t ? division(c, b, x) : host::attn_plan(c, b, x);
     FNS_TRY(host::attn_check_buffers(p, b, q, out, ws, ws_bytes, "attn_tree"));
     AttnArgs a = attn_args(c, b, x, p, q, out, ws);
     a.sees = t ? t->sees : nullptr, a.words = t ? t->words : 0, a.lse = lse;

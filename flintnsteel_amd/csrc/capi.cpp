@@ -263,6 +263,10 @@ int fns_hip_tree_plan(const FnsKvBatch *batch, const int32_t *parents, const int
     return impl::tree_plan(batch, parents, base, words, sees, pos, S(stream));
 }
 
+int fns_hip_attn_tree_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, size_t *bytes) {
+    return impl::attn_tree_workspace(cache, batch, x, bytes);
+}
+
 int fns_hip_attn_tree(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const FnsKvTree *tree, const void *q,
                       void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
     return impl::attn_tree(cache, batch, x, tree, q, out, lse, workspace, workspace_bytes, S(stream));

@@ -118,6 +118,7 @@ int attn(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const void 
          hipStream_t st);
 int rope_scaled(int rope_dim, double base, double factor, double original, double fast, double slow, float *inv_freq, float *magnitude);
 int tree_plan(const FnsKvBatch *b, const int32_t *parents, const int32_t *base, int words, uint64_t *sees, int32_t *pos, hipStream_t st);
+int attn_tree_workspace(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, size_t *bytes);
 int attn_tree(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const FnsKvTree *t, const void *q, void *out, float *lse,
               void *ws, size_t ws_bytes, hipStream_t st);
 int kv_weigh_workspace(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, size_t *bytes);

@@ -831,11 +831,12 @@ def kv_read(cache: KvCache, batch: KvBatch):
 
 
 def attn_workspace(cache: KvCache, batch: KvBatch, q: torch.Tensor) -> torch.Tensor:
-    """A workspace of attn for this batch's numbers and q's heads; it may serve every layer of a step in turn."""
+    """A workspace of attn (with or without a tree) for this batch's numbers and q's heads; it may serve every layer of a step
+    in turn."""
     width = _heads("attn", q, batch.n_tok, cache.head_dim, q.dtype)
     desc = AttnDesc(_dtype_code(q), q.shape[1], 0, 1.0, None, width, q.shape[1] * cache.head_dim)
     size = ctypes.c_size_t()
-    call("fns_hip_attn_workspace", cache.ref, batch._for(cache), ctypes.byref(desc), ctypes.byref(size))
+    call("fns_hip_attn_tree_workspace", cache.ref, batch._for(cache), ctypes.byref(desc), ctypes.byref(size))
     return torch.empty(size.value, dtype=torch.uint8, device=q.device)
 
 

@@ -427,7 +427,9 @@ int fns_hip_tree_plan(const FnsKvBatch *batch, const int32_t *parents, const int
  * positions (none if n >= W: the bits alone say which new tokens it sees). A token without bits sees nothing: its output is
  * zero. NULL: as fns_hip_attn, in the same bits (bf16: unless the contexts are divided, when it is within the roundings).
  * lse: NULL or f32 [n_tok][n_head], the logarithm of the softmax's denominator (sinks included) of every row, -infinity for one
- * that sees nothing, within 2^-20 + 2^-22 |lse| and what q is off by (above). The workspace is fns_hip_attn_workspace's. */
+ * that sees nothing, within 2^-20 + 2^-22 |lse| and what q is off by (above). workspace: fns_hip_attn_tree_workspace bytes
+ * (with or without a tree; at least fns_hip_attn_workspace's), as fns_hip_attn's. */
+int fns_hip_attn_tree_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, size_t *bytes);
 int fns_hip_attn_tree(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const FnsKvTree *tree, const void *q,
                       void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 
