@@ -66,11 +66,26 @@ __device__ __forceinline__ int seq_len(const KvView &c, const BatchView &b, int 
     return (int) min((int64_t) max(b.kv_len[s], 0), b.table_stride << c.shift);
 }
 
+// Inclusive sum over the wave's lanes up to each, by moves within rows of 16 lanes and from the end of rows to later ones.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 // Which positions a sequence's kv head keeps: a workgroup each. The budget-th largest key digit by digit (11, 11, 10 bits), the
 // counts of a digit's values in LDS; then the positions in order, those above it and as many equal ones as there is room for.
-constexpr int kSel = 1024, kBins = 2048;
-__global__ __launch_bounds__(kSel) void k_kv_select(EvictArgs a) {
-    __shared__ int bins[kBins], waves[kSel / 64], found[2];
+// Up to 4096 Q positions a thread has its 4 Q keys in registers; Q = 0: any number, read anew by every pass. Bound by what waits
+// for what: the table, the weights, three times counting and the search among 2048 counts, the scan of the kept.
+constexpr int kSel = 1024, kBins = 2048, kSelWaves = kSel / 64;
+constexpr int kCopies = 4;  // of the counts: lanes with the same value wait for each other (many positions may have none at all)
+template <int Q> __global__ __launch_bounds__(kSel) void k_kv_select(EvictArgs a) {
+    __shared__ __align__(16) int bins[3][kCopies][kBins];
+    __shared__ int waves[Q > 0 ? Q : 1][kSelWaves], found[3][2];
     const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const int n = seq_len(a.c, a.b, s), P = 1 << a.c.shift;
     int32_t *kept = a.kept + (int64_t) blockIdx.x * a.budget;
@@ -86,84 +101,126 @@ __global__ __launch_bounds__(kSel) void k_kv_select(EvictArgs a) {
             k[j] = page < 0 || p >= n ? 0u : p < a.first || p >= n - a.recent ? 0xffffffffu : weight_key(v[j]);
         }
     };
-    const auto wave_scan = [&](int v) {  // inclusive, over the wave
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const int u = __shfl_up(v, o, 64);
-            v += lane >= o ? u : 0;
-        }
-        return v;
-    };
     const int quads = n / 4 + (n % 4 > 0);
+    uint32_t own[Q > 0 ? Q : 1][4];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) keys(min(tid + q * kSel, 0x1fffffff), own[q]);
+    // f(the number of the thread's quad, its keys) for all of them
+    const auto each = [&](auto f) {
+        if constexpr (Q > 0) {
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                if (q * kSel < quads) f(own[q]);
+        } else {
+            for (int i = tid; i < quads; i += kSel) {
+                uint32_t k[4];
+                keys(i, k);
+                f(k);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < 3 * kCopies * kBins / 4 / kSel; ++i) ((int4 *) bins)[tid + i * kSel] = make_int4(0, 0, 0, 0);
+    __syncthreads();
     int want = a.budget, total = 0;
     uint32_t prefix = 0;
+#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, high = pass == 0 ? 32 : pass == 1 ? 21 : 10;
-        for (int i = tid; i < kBins; i += kSel) bins[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < quads; i += kSel) {
-            uint32_t k[4];
-            keys(i, k);
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, high = pass == 1 ? 21 : 10;
+        each([&](const uint32_t (&k)[4]) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (k[j] != 0 && (pass == 0 || k[j] >> high == prefix)) atomicAdd(&bins[(k[j] >> shift) & (pass == 2 ? 1023 : 2047)], 1);
-        }
+                if (k[j] != 0 && (pass == 0 || k[j] >> high == prefix)) atomicAdd(&bins[pass][lane % kCopies][(k[j] >> shift) & (pass == 2 ? 1023 : 2047)], 1);
+        });
         __syncthreads();
         // from the largest digit down: thread t holds digits 2047 - 2 t and 2046 - 2 t
-        const int hi = bins[kBins - 1 - 2 * tid], lo = bins[kBins - 2 - 2 * tid];
-        int sum = wave_scan(hi + lo);
-        if (lane == 63) waves[wave] = sum;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) sum += waves[w];
-        if (pass == 0) {
-            if (tid == kSel - 1) found[0] = sum;
-            __syncthreads();
-            total = found[0];
-            want = min(want, total);
-            __syncthreads();
+        int hi = 0, lo = 0;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int2 two = *(const int2 *) &bins[pass][i][kBins - 2 - 2 * tid];
+            hi += two.y, lo += two.x;
         }
+        int sum = wave_scan(hi + lo);
+        if (lane == 63) waves[0][wave] = sum;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kSelWaves; ++w) {
+            const int x = waves[0][w];
+            sum += w < wave ? x : 0, all += x;
+        }
+        if (pass == 0) total = all, want = min(want, total);
         const int above = sum - hi - lo;  // keys of larger digits
         if (want > above && want <= sum) {
             const bool second = want > above + hi;
-            found[0] = kBins - 1 - 2 * tid - (second ? 1 : 0);
-            found[1] = above + (second ? hi : 0);
+            found[pass][0] = kBins - 1 - 2 * tid - (second ? 1 : 0);
+            found[pass][1] = above + (second ? hi : 0);
         }
         __syncthreads();
         if (want > 0) {
-            prefix = pass == 2 ? (prefix << 10) | (uint32_t) found[0] : (prefix << 11) | (uint32_t) found[0];
-            want -= found[1];
+            prefix = (prefix << (pass == 2 ? 10 : 11)) | (uint32_t) found[pass][0];
+            want -= found[pass][1];
         }
-        __syncthreads();
     }
     // `want` of the keys equal to `prefix` are kept: the first ones
     const int keep = min(a.budget, total);
-    int before = 0, equal = 0;  // kept above, and equal, of the positions so far
-    if (keep > 0)
-        for (int i0 = 0; i0 < quads; i0 += kSel) {
-            uint32_t k[4] = {};
-            if (i0 + tid < quads) keys(i0 + tid, k);
-            int gt = 0, eq = 0;
+    const auto counts = [&](const uint32_t (&k)[4]) {  // above in the low half, equal in the high one
+        int c = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) gt += k[j] > prefix, eq += k[j] == prefix;
-            const int both = wave_scan(gt | (eq << 16));
-            if (lane == 63) waves[wave] = both;
-            __syncthreads();
-            int at = both - (gt | (eq << 16)), all = 0;
+        for (int j = 0; j < 4; ++j) c += (k[j] > prefix ? 1 : 0) + (k[j] == prefix ? 1 << 16 : 0);
+        return c;
+    };
+    const auto put = [&](const uint32_t (&k)[4], int quad, int above, int equal) {  // (of the positions before these)
 #pragma unroll
-            for (int w = 0; w < kSel / 64; ++w) {
-                at += w < wave ? waves[w] : 0;
-                all += waves[w];
-            }
-            int g = before + (at & 0xffff), e = equal + (at >> 16);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool is = k[j] == prefix;
-                if (k[j] > prefix || (is && e < want)) kept[g + min(e, want)] = 4 * (i0 + tid) + j;
-                g += k[j] > prefix, e += is;
-            }
-            before += all & 0xffff, equal += all >> 16;
-            __syncthreads();
+        for (int j = 0; j < 4; ++j) {
+            const bool is = k[j] == prefix;
+            if (k[j] > prefix || (is && equal < want)) kept[above + min(equal, want)] = 4 * quad + j;
+            above += k[j] > prefix, equal += is;
         }
+    };
+    if (keep > 0) {
+        if constexpr (Q > 0) {
+            int before[Q];
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                if (q * kSel >= quads) break;
+                const int c = counts(own[q]), both = wave_scan(c);
+                if (lane == 63) waves[q][wave] = both;
+                before[q] = both - c;
+            }
+            __syncthreads();
+            int all = 0;  // (at most 32768 of either fit a half)
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                if (q * kSel >= quads) break;
+                int at = all + before[q];
+#pragma unroll
+                for (int w = 0; w < kSelWaves; ++w) {
+                    const int x = waves[q][w];
+                    at += w < wave ? x : 0, all += x;
+                }
+                put(own[q], tid + q * kSel, at & 0xffff, at >> 16);
+            }
+        } else {
+            int above = 0, equal = 0;
+            for (int i0 = 0; i0 < quads; i0 += kSel) {
+                uint32_t k[4] = {};
+                if (i0 + tid < quads) keys(i0 + tid, k);
+                const int c = counts(k), both = wave_scan(c);
+                __syncthreads();
+                if (lane == 63) waves[0][wave] = both;
+                __syncthreads();
+                int at = both - c, all = 0;
+#pragma unroll
+                for (int w = 0; w < kSelWaves; ++w) {
+                    const int x = waves[0][w];
+                    at += w < wave ? x : 0, all += x;
+                }
+                put(k, i0 + tid, above + (at & 0xffff), equal + (at >> 16));
+                above += all & 0xffff, equal += all >> 16;
+            }
+        }
+    }
     for (int i = keep + tid; i < a.budget; i += kSel) kept[i] = -1;
     if (head == 0 && tid == 0) a.new_len[s] = keep;
 }
@@ -180,36 +237,28 @@ struct MoveArgs {
     int32_t *new_len;  // NEW
 };
 
-// Positions list[0], list[1], ... of a sequence's kv head to positions 0, 1, ... (NEW: both counted from its first new token,
-// the list one of the sequence). A workgroup moves a part of a position: K's codes, 16 byte columns of V, or the scale bytes and
-// the weight, for 1024 positions at a time, all of which are read before the first is written. In place one workgroup goes over
-// all of them in order: what it writes lies before everything that it has yet to read, since the list ascends (a list of new
-// tokens, which need not, has at most 1024). Elsewhere (INTO) the steps are workgroups of their own.
-constexpr int kMove = 1024;
-template <int D, bool NEW>
-__global__ __launch_bounds__(kMove) void k_kv_move(MoveArgs a) {
-    constexpr int NB = D / 32, NP = D / 32;  // 16-byte pieces of a K row
-    const int s = blockIdx.y / a.c.n_kv, head = blockIdx.y % a.c.n_kv, part = blockIdx.z, tid = threadIdx.x, P = 1 << a.c.shift;
-    int64_t first = 0;
-    int n, fresh = 0;
+// Where the i-th position of a list comes from and goes to: pages (to = -1: it is not moved) and rows.
+struct Place {
+    int from, to, row_from, row_to;
+};
+// Positions list[0], list[1], ... of a sequence's kv head go to positions 0, 1, ... (NEW: both counted from its first new token,
+// the list one of the sequence).
+template <bool NEW> struct Places {
     const int32_t *list;
-    if constexpr (NEW) {
-        const SeqRange r = seq_range(a.b, s);
-        first = (int64_t) r.len - r.n, fresh = r.n;
-        n = (int) min((int64_t) min(max(a.count[s], 0), r.n), a.list_stride);
-        list = a.list + s * a.list_stride;
-        if (head == 0 && part == 0 && tid == 0) a.new_len[s] = (int) max(first + n, (int64_t) 0);
-    } else {
-        n = (int) a.list_stride;
-        list = a.list + (int64_t) blockIdx.y * a.list_stride;
+    int64_t first;
+    int n, fresh;
+    __device__ __forceinline__ Places(const MoveArgs &a, int s, int row) : first(0), fresh(0) {
+        if constexpr (NEW) {
+            const SeqRange r = seq_range(a.b, s);
+            first = (int64_t) r.len - r.n, fresh = r.n;
+            n = (int) min((int64_t) min(max(a.count[s], 0), r.n), a.list_stride);
+            list = a.list + s * a.list_stride;
+        } else {
+            n = (int) a.list_stride;
+            list = a.list + row * a.list_stride;
+        }
     }
-    using L = KvParts<D>;
-    const int64_t head_off = head * kv_head_bytes(D, P);
-    // where the i-th one comes from and goes to: pages (-1: not moved) and rows
-    struct Place {
-        int from, to, row_from, row_to;
-    };
-    const auto place = [&](int i) {
+    __device__ __forceinline__ Place at(const MoveArgs &a, int s, int64_t i) const {
         Place p{-1, -1, 0, 0};
         if (i >= n) return p;
         const int x = list[i];
@@ -217,20 +266,35 @@ __global__ __launch_bounds__(kMove) void k_kv_move(MoveArgs a) {
         const int64_t src = first + x, dst = first + i;
         if (src == dst && a.to == a.b.table) return p;
         if (src < 0 || dst < 0 || src > INT32_MAX || dst > INT32_MAX) return p;
-        p.from = page_of(a.c, a.b, s, (int) src);
+        const int P = 1 << a.c.shift;
         const int64_t e = dst >> a.c.shift;
         const int q = e < a.to_stride ? a.to[s * a.to_stride + e] : -1;
+        p.from = page_of(a.c, a.b, s, (int) src);
         p.to = p.from >= 0 && q >= 0 && q < a.c.n_pages ? q : -1;
         p.row_from = (int) src & (P - 1), p.row_to = (int) dst & (P - 1);
         return p;
-    };
-    for (int64_t i0 = (int64_t) blockIdx.x * kMove; i0 < n; i0 += (int64_t) gridDim.x * kMove) {
+    }
+};
+
+// In place, any number: a workgroup moves a part of a position (K's codes, 16 byte columns of V, or the scale bytes and the
+// weight) for 1024 positions at a time, all of which are read before the first is written, and goes over all of them in order:
+// what it writes lies before everything that it has yet to read, since the list ascends (a list of new tokens, which need not,
+// has at most 1024).
+constexpr int kMove = 1024;
+template <int D, bool NEW> __global__ __launch_bounds__(kMove) void k_kv_walk(MoveArgs a) {
+    constexpr int NB = D / 32, NP = D / 32;  // 16-byte pieces of a K row
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, part = blockIdx.y, tid = threadIdx.x, P = 1 << a.c.shift;
+    const Places<NEW> places(a, s, blockIdx.x);
+    if (NEW && head == 0 && part == 0 && tid == 0) a.new_len[s] = (int) max(places.first + places.n, (int64_t) 0);
+    using L = KvParts<D>;
+    const int64_t head_off = head * kv_head_bytes(D, P);
+    for (int64_t i0 = 0; i0 < places.n; i0 += kMove) {
         if (part == 0) {
             Place p[NP];
             uint4 x[NP];
 #pragma unroll
             for (int u = 0; u < NP; ++u) {
-                p[u] = place((int) i0 + (u * kMove + tid) / NP);
+                p[u] = places.at(a, s, i0 + (u * kMove + tid) / NP);
                 if (p[u].to >= 0)
                     x[u] = *(const uint4 *) (a.c.pages + p[u].from * a.c.page_bytes + head_off + L::k_row(P, p[u].row_from) + tid % NP * 16);
             }
@@ -239,7 +303,7 @@ __global__ __launch_bounds__(kMove) void k_kv_move(MoveArgs a) {
             for (int u = 0; u < NP; ++u)
                 if (p[u].to >= 0) *(uint4 *) (a.c.pages + p[u].to * a.c.page_bytes + head_off + L::k_row(P, p[u].row_to) + tid % NP * 16) = x[u];
         } else if (part == 1) {
-            const Place p = place((int) i0 + tid);
+            const Place p = places.at(a, s, i0 + tid);
             uint8_t k[NB], v[NB];
             float w = 0.0f;
             const uint8_t *src = a.c.pages + p.from * a.c.page_bytes + head_off;
@@ -256,7 +320,7 @@ __global__ __launch_bounds__(kMove) void k_kv_move(MoveArgs a) {
                 if (a.w) a.w_out[(((int64_t) p.to * a.c.n_kv + head) << a.c.shift) + p.row_to] = w;
             }
         } else {
-            const Place p = place((int) i0 + tid);
+            const Place p = places.at(a, s, i0 + tid);
             const int j = 16 * (part - 2);
             uint8_t x[16];
             if (p.to >= 0) {
@@ -274,15 +338,94 @@ __global__ __launch_bounds__(kMove) void k_kv_move(MoveArgs a) {
     }
 }
 
-template <bool NEW> int move(const MoveArgs &a, int D, int n_seq, int64_t steps, const char *what, hipStream_t st) {
-    const auto go = [&](auto dim) {
+// To other pages, or at most W positions in all: a workgroup W positions of a kv head, whose places are looked up once; all is read
+// before anything is written.
+template <int D, int W, bool NEW> __global__ __launch_bounds__(256) void k_kv_copy(MoveArgs a) {
+    constexpr int NB = D / 32, NP = D / 32, KR = (W * NP + 255) / 256, COLS = D / 2 * W / 256;  // a thread's pieces of K, bytes of V
+    static_assert(D / 2 * W % 256 == 0 && W <= 64, "columns are dealt out evenly, and scales and weights have a thread each");
+    __shared__ Place place[W];
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, tid = threadIdx.x, P = 1 << a.c.shift;
+    const Places<NEW> places(a, s, blockIdx.x);
+    const int64_t i0 = (int64_t) blockIdx.y * W;
+    if (NEW && head == 0 && tid == 0) a.new_len[s] = (int) max(places.first + places.n, (int64_t) 0);
+    if (i0 >= places.n) return;
+    if (tid < W) place[tid] = places.at(a, s, i0 + tid);
+    __syncthreads();
+    using L = KvParts<D>;
+    const int64_t head_off = head * kv_head_bytes(D, P);
+    const auto from = [&](const Place &p) { return a.c.pages + p.from * a.c.page_bytes + head_off; };
+    const auto to = [&](const Place &p) { return a.c.pages + p.to * a.c.page_bytes + head_off; };
+    uint4 k[KR];
+#pragma unroll
+    for (int u = 0; u < KR; ++u) {
+        const int i = tid + 256 * u;
+        if (i < W * NP && place[i / NP].to >= 0) k[u] = *(const uint4 *) (from(place[i / NP]) + L::k_row(P, place[i / NP].row_from) + i % NP * 16);
+    }
+    const Place own = place[tid % W];  // V, scales and the weight: a thread's position
+    uint8_t v[COLS] = {}, e[NB];
+    float w = 0.0f;
+    const int kind = tid / W, col = kind * COLS;  // its byte columns; the first W threads also K's scales, the next V's, then the weights
+    if (own.to >= 0) {
+        const uint8_t *src = from(own);
+#pragma unroll
+        for (int u = 0; u < COLS; ++u) v[u] = src[L::v_col(P, col + u) + own.row_from];
+        if (kind < 2)
+            __builtin_memcpy(e, __builtin_assume_aligned(src + (kind == 0 ? L::k_scale(P, own.row_from) : L::v_scale(P, own.row_from)), NB), NB);
+        else if (kind == 2 && a.w)
+            w = a.w[(((int64_t) own.from * a.c.n_kv + head) << a.c.shift) + own.row_from];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < KR; ++u) {
+        const int i = tid + 256 * u;
+        if (i < W * NP && place[i / NP].to >= 0) *(uint4 *) (to(place[i / NP]) + L::k_row(P, place[i / NP].row_to) + i % NP * 16) = k[u];
+    }
+    uint8_t *dst = to(own);
+    if constexpr (COLS % 4 == 0 && !NEW) {
+        // four lanes have four consecutive positions, aligned: turned, a lane has four positions of a column, one store
+        int all = own.to >= 0;
+        all &= xor_lane_i<1>(all);
+        all &= xor_lane_i<2>(all);
+        const uint32_t q = tid % 4, pick = q | (4 + q) << 8;
+#pragma unroll
+        for (int u = 0; u < COLS; u += 4) {
+            const uint32_t x = v[u] | (uint32_t) v[u + 1] << 8 | (uint32_t) v[u + 2] << 16 | (uint32_t) v[u + 3] << 24;
+            const uint32_t x0 = __builtin_amdgcn_update_dpp(0, x, 0x00, 0xf, 0xf, false), x1 = __builtin_amdgcn_update_dpp(0, x, 0x55, 0xf, 0xf, false);
+            const uint32_t x2 = __builtin_amdgcn_update_dpp(0, x, 0xaa, 0xf, 0xf, false), x3 = __builtin_amdgcn_update_dpp(0, x, 0xff, 0xf, 0xf, false);
+            const uint32_t y = __builtin_amdgcn_perm(x1, x0, pick | 0x0c0c0000u) | __builtin_amdgcn_perm(x3, x2, pick << 16 | 0x0c0cu);
+            if (all) *(uint32_t *) (dst + L::v_col(P, col + u + (int) q) + (own.row_to & ~3)) = y;
+        }
+        if (!all && own.to >= 0)
+#pragma unroll
+            for (int u = 0; u < COLS; ++u) dst[L::v_col(P, col + u) + own.row_to] = v[u];
+    } else if (own.to >= 0) {
+#pragma unroll
+        for (int u = 0; u < COLS; ++u) dst[L::v_col(P, col + u) + own.row_to] = v[u];
+    }
+    if (own.to >= 0) {
+        if (kind < 2)
+            __builtin_memcpy(__builtin_assume_aligned(dst + (kind == 0 ? L::k_scale(P, own.row_to) : L::v_scale(P, own.row_to)), NB), e, NB);
+        else if (kind == 2 && a.w)
+            a.w_out[(((int64_t) own.to * a.c.n_kv + head) << a.c.shift) + own.row_to] = w;
+    }
+}
+
+template <bool NEW> int move(const MoveArgs &a, int D, int n_seq, const char *what, hipStream_t st) {
+    const unsigned heads = (unsigned) (n_seq * a.c.n_kv);
+    const auto by_dim = [&](auto dim) {
         constexpr int DD = decltype(dim)::value;
-        hipLaunchKernelGGL((k_kv_move<DD, NEW>), dim3((unsigned) steps, (unsigned) (n_seq * a.c.n_kv), 2 + DD / 32), dim3(kMove), 0, st, a);
+        const auto copy = [&](auto width, unsigned steps) {
+            hipLaunchKernelGGL((k_kv_copy<DD, decltype(width)::value, NEW>), dim3(heads, steps), dim3(256), 0, st, a);
+        };
+        if (NEW && a.list_stride <= 16) copy(std::integral_constant<int, 16>{}, 1u);
+        else if (NEW && a.list_stride <= 64) copy(std::integral_constant<int, 64>{}, 1u);
+        else if (!NEW && a.to != a.b.table && a.list_stride <= 64 * 65535) copy(std::integral_constant<int, 64>{}, (unsigned) ((a.list_stride + 63) / 64));
+        else hipLaunchKernelGGL((k_kv_walk<DD, NEW>), dim3(heads, 2 + DD / 32), dim3(kMove), 0, st, a);
         return host::check_launch(what);
     };
-    if (D == 64) return go(std::integral_constant<int, 64>{});
-    if (D == 128) return go(std::integral_constant<int, 128>{});
-    return go(std::integral_constant<int, 256>{});
+    if (D == 64) return by_dim(std::integral_constant<int, 64>{});
+    if (D == 128) return by_dim(std::integral_constant<int, 128>{});
+    return by_dim(std::integral_constant<int, 256>{});
 }
 
 }  // namespace
@@ -335,12 +478,18 @@ int kv_evict(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvEvict *x, hipS
     if (!x->to_table && x->weights_out != x->weights)
         return host::set_error(host::ERR_SHAPE, "kv_evict: in place the weights move in place too");
     EvictArgs a{host::kv_view(c), host::kv_batch(b), x->weights, x->kept, x->new_len, x->budget, x->first, x->recent};
-    hipLaunchKernelGGL(k_kv_select, dim3((unsigned) (b->n_seq * c->n_head_kv)), dim3(kSel), 0, st, a);
+    const auto select = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned) (b->n_seq * c->n_head_kv)), dim3(kSel), 0, st, a); };
+    // positions that a sequence can have at all: of its table (the batch's max_kv is no bound)
+    const int64_t room = b->table_stride * c->page_size;
+    if (room <= 4 * kSel) select(k_kv_select<1>);
+    else if (room <= 8 * kSel) select(k_kv_select<2>);
+    else if (room <= 16 * kSel) select(k_kv_select<4>);
+    else if (room <= 32 * kSel) select(k_kv_select<8>);
+    else select(k_kv_select<0>);
     FNS_TRY(host::check_launch("kv_evict"));
     MoveArgs m{a.c, a.b, x->to_table ? x->to_table : b->page_table, x->to_table ? x->to_stride : b->table_stride, x->kept, nullptr,
                x->budget, x->weights, x->weights_out, nullptr};
-    const int64_t steps = x->to_table ? std::min<int64_t>((x->budget + kMove - 1) / kMove, 1024) : 1;
-    return move<false>(m, c->head_dim, b->n_seq, steps, "kv_evict", st);
+    return move<false>(m, c->head_dim, b->n_seq, "kv_evict", st);
 }
 
 int kv_keep(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvKeep *x, hipStream_t st) {
@@ -353,7 +502,7 @@ int kv_keep(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvKeep *x, hipStr
     if (x->new_len == b->kv_len || x->new_len == x->n_kept) return host::set_error(host::ERR_SHAPE, "kv_keep: new_len must not be kv_len or n_kept");
     MoveArgs m{host::kv_view(c), host::kv_batch(b), b->page_table, b->table_stride, x->kept, x->n_kept, x->stride, x->weights,
                x->weights, x->new_len};
-    return move<true>(m, c->head_dim, b->n_seq, 1, "kv_keep", st);
+    return move<true>(m, c->head_dim, b->n_seq, "kv_keep", st);
 }
 
 }  // namespace impl
