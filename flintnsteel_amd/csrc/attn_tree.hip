@@ -8,20 +8,28 @@ namespace fns {
 
 namespace {
 
-// A tree's rows all see the same tiles of keys, so that the form of many rows can be divided over them as the other is.
+// How a tree's call is divided: attn's form, but that of few rows otherwise than for causal rows, since a tree's rows all walk over
+// the same tiles. Sixteen rows a workgroup, until their steps (of 64 keys) are so many that reading K and V half as often
+// is ahead of having twice the workgroups (26 tokens of 4 heads over 726 positions: 12.6 us against 16.7 with 32; 60 tokens
+// over 100000: 194 against 167; 32 tokens of 8 heads over 24 contexts of up to 2900: both 49). Splits until 512 workgroups where they
+// outweigh their join (60 tokens over 100000: 167 us with 512 workgroups, 176 with 1024, 210 with 384); of unequal sequences beyond
+// that pieces of 40 tiles, up to 1024 (8 contexts of 16000, equal: 184 us with 512, 194 with 1024, 206 with 2048).
 host::AttnPlan division(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
     host::AttnPlan p = host::attn_plan(c, b, x);
+    if (p.rows == kManyRows) return p;
     const auto per = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
     const int64_t rows = std::min<int64_t>(b->max_q, b->n_tok) * (x->n_head / c->n_head_kv), heads = (int64_t) b->n_seq * c->n_head_kv;
-    if (rows <= kFewRows) return p;
-    p.rows = kManyRows, p.row_tiles = per(rows, kManyRows);
-    const int64_t wgs = std::max<int64_t>(1, heads * p.row_tiles), tiles = std::max<int64_t>(1, (b->max_kv + kTile - 1) / kTile);
-    p.splits = (int) std::max<int64_t>(1, std::min({per(512, wgs), per(tiles, 4), (int64_t) 64}));
+    const int64_t tiles = std::max<int64_t>(1, (b->max_kv + kTile - 1) / kTile);
+    p.rows = c->head_dim == 256 || rows <= 16 || heads * per(rows, 16) * tiles < 100000 ? 16 : 32;
+    p.row_tiles = per(rows, p.rows);
+    const int64_t wgs = std::max<int64_t>(1, heads * p.row_tiles);
+    int64_t splits = tiles * (256 - wgs) > 11 * 256 ? std::min(per(512, wgs), per(tiles, 4)) : 1;
+    if (b->n_seq > 1) splits = std::max(splits, std::min(tiles / 40, per(1024, wgs)));
+    p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(splits, 64));
     p.chunk = (int) per(tiles, p.splits);
     const size_t n = p.splits > 1 ? (size_t) p.splits * b->n_tok * x->n_head : 0;
     p.ml_off = n * c->head_dim * 4;
-    p.redo_off = p.ml_off + n * 8;
-    p.bytes = p.redo_off + (size_t) (heads * p.row_tiles * p.splits) * 4;
+    p.bytes = p.ml_off + n * 8;
     return p;
 }
 

@@ -27,7 +27,7 @@ namespace host {
 struct AttnPlan {
     int rows, splits, chunk;
     int64_t row_tiles;  // (more than a grid has are refused)
-    size_t ml_off, redo_off, bytes;
+    size_t ml_off, bytes;
 };
 // (attn.hip) Checks of a call's numbers, its plan, and checks of its pointers against the plan; `what` names the call.
 int attn_check(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const char *what);
@@ -919,11 +919,10 @@ __global__ __launch_bounds__(64 * kFewWaves, D == 256 || CT == 2 ? 2 : 3) void k
 // workgroup with the pass that found them, their scalars cost the f32 form's loop its registers (29 spilled instead of 9).
 template <bool MORE, int D, bool SMALL, class T>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void k_attn_redo(AttnArgs a, int row_tiles) {
-    const int splits = MORE ? a.splits : 1;
-    for (int i = blockIdx.y; i < row_tiles * splits; i += gridDim.y) {
-        if (!((const uint32_t *) a.redo)[(int64_t) blockIdx.x * row_tiles * splits + i]) continue;
+    for (int tile = blockIdx.y; tile < row_tiles; tile += gridDim.y) {
+        if (!((const uint32_t *) a.redo)[(int64_t) blockIdx.x * row_tiles + tile]) continue;
         for (int sub = 0; sub < kManyRows / 16; ++sub) {
-            few_rows<MORE, D, 1, SMALL, true, T>(a, i / splits * kManyRows + 16 * sub, i % splits);
+            few_rows<MORE, D, 1, SMALL, true, T>(a, tile * kManyRows + 16 * sub, 0);
             __syncthreads();
         }
     }
@@ -962,25 +961,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) INT32_MAX);
     // the last rows, which see the most keys, first
     const int row0 = ((int) gridDim.y - 1 - (int) blockIdx.y) * kManyRows;
-    const int split = MORE ? blockIdx.z : 0, splits = MORE ? a.splits : 1;  // (a tree's rows see the same tiles)
-    uint8_t *redo = a.redo + (((int64_t) blockIdx.x * gridDim.y + row0 / kManyRows) * splits + split) * NW + wave;
+    uint8_t *redo = a.redo + ((int64_t) blockIdx.x * gridDim.y + row0 / kManyRows) * NW + wave;
     if (row0 >= rows) {
         if (lane == 0) *redo = 0;
         return;
     }
     const RowTiles rt = row_tiles<MORE>(a, sr, row0, kManyRows);
     const NewTokens<MORE> nt(a, sr);
-    int t0 = rt.t0, t1 = rt.t1;
-    const int P = 1 << a.c.shift, first = sr.len - sr.n;
-    if (MORE && splits > 1) {
-        const int chunk = split_chunk(a, rt);
-        t0 = (int) min((int64_t) rt.t0 + (int64_t) split * chunk, (int64_t) rt.t1);
-        t1 = min(t0 + chunk, rt.t1);
-        if (split > 0 && t0 >= t1) {  // (split 0 of an empty range writes the zeros)
-            if (lane == 0) *redo = 0;
-            return;
-        }
-    }
+    const int t0 = rt.t0, t1 = rt.t1, P = 1 << a.c.shift, first = sr.len - sr.n;
     float *vsc = vsc_all[wave];
     uint8_t *ksb = ksb_all[wave];
 
@@ -1130,13 +1118,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         const int64_t tok = sr.q0 + row / a.group;
         const int h = head * a.group + row % a.group;
         float sum = st[c].l[0], off = st[c].m;
-        if (MORE && splits > 1) {
-            const float f = sum == 0.0f ? 0.0f : ldexpf(1.0f / sum, ev - kBias - kPart);
-#pragma unroll
-            for (int d = 0; d < 2 * NB; ++d) store_row<D, T>(a, tok, h, split, 16 * d + 4 * g, st[c].o[d] * f);
-            if (g == 0) a.part_ml[(split * a.b.n_tok + tok) * a.n_head + h] = make_float2(off, SPLIT == 1 ? lx[c] : sum);
-            continue;
-        }
         if constexpr (MORE) {
             float den = SPLIT == 1 ? lx[c] : sum, from = off;
             if (a.sinks) {
@@ -1221,7 +1202,7 @@ AttnArgs attn_args(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, c
     a.q_stride = x->q_stride, a.out_stride = x->out_stride;
     a.n_head = x->n_head, a.group = x->n_head / c->n_head_kv, a.window = x->window;
     a.splits = p.splits, a.chunk = p.chunk, a.scale = x->scale;
-    a.redo = (uint8_t *) ws + p.redo_off;
+    a.redo = (uint8_t *) ws;
     return a;
 }
 
@@ -1251,7 +1232,7 @@ int attn_launch(const AttnArgs &a, const host::AttnPlan &p, const FnsKvCache *c,
             if (small) hipLaunchKernelGGL((k_attn_many<MORE, D, true, decltype(type)>), grid, dim3(256), 0, st, a);
             else hipLaunchKernelGGL((k_attn_many<MORE, D, false, decltype(type)>), grid, dim3(256), 0, st, a);
             FNS_TRY(host::check_launch(what));
-            const dim3 some(grid.x, std::min(grid.y * grid.z, (512 + grid.x - 1) / grid.x));
+            const dim3 some(grid.x, std::min(grid.y, (512 + grid.x - 1) / grid.x));
             if (small) hipLaunchKernelGGL((k_attn_redo<MORE, D, true, decltype(type)>), some, dim3(64 * kFewWaves), 0, st, a, (int) p.row_tiles);
             else hipLaunchKernelGGL((k_attn_redo<MORE, D, false, decltype(type)>), some, dim3(64 * kFewWaves), 0, st, a, (int) p.row_tiles);
         } else if constexpr (D == 256) few(dim, std::integral_constant<int, 1>{}, type);

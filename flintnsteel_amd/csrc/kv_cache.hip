@@ -156,7 +156,8 @@ __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_ap
     const int64_t tok = r.q0 + (pos - first);
     const int page = page_of(a.c, a.b, s, base);  // 16 aligned positions lie in one page
     Row8<T> k8 = {}, v8 = {}, q8 = {};
-    if (have) {
+    const bool keys = blockIdx.z == 0;  // the others have queries only
+    if (have && keys) {
         k8.load((const T *) a.k + tok * a.k_stride + head * D + ch);
         v8.load((const T *) a.v + tok * a.v_stride + head * D + ch);
     }
@@ -164,7 +165,10 @@ __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_ap
     // threads of a row are lanes of one wave, whose loads all precede the stores they feed.
     const int n_group = a.n_group;
     int qp = hi, qh = 0, dp = 0, dh = 0;
-    if (n_group) qp = lo + row / n_group, qh = row % n_group, dp = kGroup / n_group, dh = kGroup % n_group;
+    if (n_group) {
+        const int item = row + kGroup * (int) blockIdx.z, step = kGroup * (int) gridDim.z;
+        qp = lo + item / n_group, qh = item % n_group, dp = step / n_group, dh = step % n_group;
+    }
     const auto ask = [&] {
         if (qp < hi) q8.load((const T *) a.q + (r.q0 + (qp - first)) * a.q_stride + (int64_t) (head * n_group + qh) * D + ch);
     };
@@ -184,45 +188,47 @@ __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_ap
     }
     ask();
     const auto angles = [&](int p) { return cs + (ROPE == FNS_ROPE_NONE ? 0 : (p - base) * (D / 2)); };
-    const int P = 1 << a.c.shift;
-    uint8_t *dst = a.c.pages + (int64_t) max(page, 0) * a.c.page_bytes + head * kv_head_bytes(D, P);
-    using L = KvParts<D>;
-    const bool put = have && page >= 0 && pos >= 0;
-    int e;
-    uint32_t w;
-    if constexpr (ROPE == FNS_ROPE_NONE) {
-        float k[8];
+    if (keys) {
+        const int P = 1 << a.c.shift;
+        uint8_t *dst = a.c.pages + (int64_t) max(page, 0) * a.c.page_bytes + head * kv_head_bytes(D, P);
+        using L = KvParts<D>;
+        const bool put = have && page >= 0 && pos >= 0;
+        int e;
+        uint32_t w;
+        if constexpr (ROPE == FNS_ROPE_NONE) {
+            float k[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) k[i] = to_f32(k8.x[i]);
-        w = hold8(k, e);
-    } else {
-        double k[8] = {};
-        if (have) rotated<ROPE>(k8, ch, a.rope_dim, angles(pos), k);
-        w = hold8(k, e);
-    }
-    if (put) {
-        *(uint32_t *) (dst + L::k_row(P, pos & (P - 1)) + ch / 2) = w;
-        if (ch % 32 == 0) dst[L::k_scale(P, pos & (P - 1)) + ch / 32] = (uint8_t) e;
-    }
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32(v8.x[i]);
-    w = hold8(v, e);
-    if (put && ch % 32 == 0) dst[L::v_scale(P, pos & (P - 1)) + ch / 32] = (uint8_t) e;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) code[ch + i][row] = (uint8_t) ((w >> (4 * i)) & 15u);
-    __syncthreads();
-    if (page >= 0 && base >= 0) {  // byte column tid / 4, positions 4 (tid % 4) .. + 3
-        const int j = tid / 4, p4 = base + tid % 4 * 4;
-        const int c0 = j / 16 * 32 + j % 16;
-        const uint32_t b = *(const uint32_t *) &code[c0][tid % 4 * 4] | (*(const uint32_t *) &code[c0 + 16][tid % 4 * 4] << 4);
-        uint8_t *o = dst + L::v_col(P, j) + (p4 & (P - 1));
-        if (p4 >= lo && p4 + 4 <= hi) {
-            *(uint32_t *) o = b;
+            for (int i = 0; i < 8; ++i) k[i] = to_f32(k8.x[i]);
+            w = hold8(k, e);
         } else {
+            double k[8] = {};
+            if (have) rotated<ROPE>(k8, ch, a.rope_dim, angles(pos), k);
+            w = hold8(k, e);
+        }
+        if (put) {
+            *(uint32_t *) (dst + L::k_row(P, pos & (P - 1)) + ch / 2) = w;
+            if (ch % 32 == 0) dst[L::k_scale(P, pos & (P - 1)) + ch / 32] = (uint8_t) e;
+        }
+        float v[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (p4 + i >= lo && p4 + i < hi) o[i] = (uint8_t) (b >> (8 * i));
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(v8.x[i]);
+        w = hold8(v, e);
+        if (put && ch % 32 == 0) dst[L::v_scale(P, pos & (P - 1)) + ch / 32] = (uint8_t) e;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[ch + i][row] = (uint8_t) ((w >> (4 * i)) & 15u);
+        __syncthreads();
+        if (page >= 0 && base >= 0) {  // byte column tid / 4, positions 4 (tid % 4) .. + 3
+            const int j = tid / 4, p4 = base + tid % 4 * 4;
+            const int c0 = j / 16 * 32 + j % 16;
+            const uint32_t b = *(const uint32_t *) &code[c0][tid % 4 * 4] | (*(const uint32_t *) &code[c0 + 16][tid % 4 * 4] << 4);
+            uint8_t *o = dst + L::v_col(P, j) + (p4 & (P - 1));
+            if (p4 >= lo && p4 + 4 <= hi) {
+                *(uint32_t *) o = b;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (p4 + i >= lo && p4 + i < hi) o[i] = (uint8_t) (b >> (8 * i));
+            }
         }
     }
     while (qp < hi) {
@@ -333,7 +339,12 @@ int kv_append_at(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x,
                  x->q_stride, x->q_out_stride, x->rope_dim, x->n_head / c->n_head_kv, pos, magnitude};
     // new tokens of a sequence start anywhere in a group
     const int64_t most = std::min<int64_t>(b->max_q, b->n_tok);
-    const dim3 grid((unsigned) ((most + kGroup - 2) / kGroup + 1), (unsigned) (b->n_seq * c->n_head_kv));
+    const int64_t groups = (most + kGroup - 2) / kGroup + 1, heads = (int64_t) b->n_seq * c->n_head_kv;
+    // A few tokens' queries are more rows than a workgroup's sixteen, one after another: workgroups of their own, while they
+    // have places (26 tokens, 32 heads over 8: 9.8 us in one, 8.2 in parts; 24 sequences of 32, 64 over 8 of 64: 16 and 11.5).
+    const int64_t turns = (std::min<int64_t>(most, kGroup) * a.n_group + kGroup - 1) / kGroup;
+    const int64_t parts = std::max<int64_t>(1, std::min(turns, 2048 / std::max<int64_t>(1, groups * heads)));
+    const dim3 grid((unsigned) groups, (unsigned) heads, (unsigned) parts);
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(2 * D), 0, st, a); };
     auto by_type = [&](auto dim, auto rope) {
         constexpr int DD = decltype(dim)::value, R = decltype(rope)::value;
