@@ -241,6 +241,8 @@ template <int D, class T> struct QueryShape {
     static constexpr int N = (kDigits + kPerStep - 1) / kPerStep;
 };
 typedef uint32_t u6 __attribute__((ext_vector_type(6)));
+// MORE: always as many digits as f32 has: a denominator's logarithm is f32, whatever the queries are (3 digits left it 1e-4 off).
+template <bool MORE, class T> using DigitType = std::conditional_t<MORE, float, T>;
 template <int D, class T> using Digits = u6[QueryShape<D, T>::N][QueryShape<D, T>::kSteps];
 // The row is first multiplied by scale * log2(e): scores are log2 units. Returns the block scale of digit 0 (255: the row has a
 // NaN or an infinity, and every score is NaN).
@@ -679,7 +681,8 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
     constexpr int NB = D / 32, SPLIT = sizeof(T) == 4 ? 2 : 1, NW = kFewWaves;
     constexpr int kScale = 64 * NB + 16 * NB, kJoin = NW / 2 * CT * 2 * NB * 256;
     __shared__ __align__(16) float lds[NW * kScale > kJoin ? NW * kScale : kJoin];
-    using Q = QueryShape<D, T>;
+    using Dt = DigitType<MORE, T>;
+    using Q = QueryShape<D, Dt>;
     __shared__ __align__(16) uint2 qs[CT][Q::N][Q::kSteps][64][3];
     __shared__ int qscale[CT][16];
     constexpr bool EXACT = MORE && SPLIT == 1;  // the denominator's logarithm takes a sum of its own
@@ -715,8 +718,8 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
 
     if (wave < CT) {  // a wave a column tile
         const int row = row0 + 16 * wave + r, i = row / a.group;
-        Digits<D, T> w;
-        const int scale = query_digits<D, T>(w, (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D,
+        Digits<D, Dt> w;
+        const int scale = query_digits<D, Dt>(w, (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D,
                                              row < rows, a.scale);
 #pragma unroll
         for (int n = 0; n < Q::N; ++n)
@@ -736,7 +739,7 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
         see[c] = sight(a, sr, nt, row < rows, row / a.group);
     }
     __syncthreads();
-    DigitScales<D, T> qsc[CT];
+    DigitScales<D, Dt> qsc[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) qsc[c].set(qscale[c][r]);
 
@@ -779,7 +782,7 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
                             q[u][2 * i] = w.x, q[u][2 * i + 1] = w.y;
                         }
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q, qsc[c], n, sc[c][t]);
+                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, Dt>(kraw[t], ksc[t], q, qsc[c], n, sc[c][t]);
                 }
             // K is used up here, before the next tile's is asked for: the products may not sink below the loads, which would
             // keep both tiles' registers
@@ -950,7 +953,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
     constexpr int NB = D / 32, SPLIT = sizeof(T) == 4 ? 2 : 1, NW = 4, CT = 2;
     constexpr int VS = 64 + 8;             // f16 values between V rows
     constexpr int MB = (NB + NW - 1) / NW; // blocks that a wave expands: wave, wave + 4
-    using Q = QueryShape<D, T>;
+    using Dt = DigitType<MORE, T>;
+    using Q = QueryShape<D, Dt>;
     __shared__ __align__(16) _Float16 vt[2][D * VS];
     __shared__ __align__(16) float vsc_all[NW][MB * 64];
     __shared__ __align__(16) uint8_t ksb_all[NW][64 * NB];
@@ -1013,9 +1017,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         rd.scales(swk, swv), rd.k(kraw), load_v();
         rd.ask(a, table, min(t0 + 1, t1 - 1));
     }
-    Digits<D, T> q[CT];
+    Digits<D, Dt> q[CT];
     RowState<NB> st[CT];
-    DigitScales<D, T> qsc[CT];
+    DigitScales<D, Dt> qsc[CT];
     const int w0 = row0 + wave * 32;  // the wave's rows, and the positions that they see at most and at least
     const bool tree = MORE && a.sees;
     const int most = w0 >= rows ? -1 : tree ? sr.len - 1 : first + min(w0 + 31, rows - 1) / a.group;
@@ -1026,7 +1030,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
         const int row = w0 + 16 * c + r, i = row / a.group;
         const bool there = row < rows;
         if (g == 0) sights[wave][c][r] = sight(a, sr, nt, there, i);
-        qsc[c].set(query_digits<D, T>(q[c], (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D, there, a.scale));
+        qsc[c].set(query_digits<D, Dt>(q[c], (const T *) a.q + (sr.q0 + i) * a.q_stride + (int64_t) (head * a.group + row % a.group) * D, there, a.scale));
         st[c].reset();
     }
     if (t0 < t1) {
@@ -1062,7 +1066,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_many(AttnArgs a)
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, T>(kraw[t], ksc[t], q[c][n], qsc[c], n, sc[c][t]);
+                    for (int t = 0; t < 4; ++t) sc[c][t] = scores<D, Dt>(kraw[t], ksc[t], q[c][n], qsc[c], n, sc[c][t]);
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll

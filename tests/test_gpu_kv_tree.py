@@ -207,7 +207,7 @@ def test_denominators_of_plain_attention(q, kv, many, dtype):
         x, out, _, sk = _check_tree(s, 4, dtype, window, sinks, rows=None)
         plain = torch.full_like(out, 7.0)
         ops.attn(s.cache, s.batch, x, window=window, sinks=sk, out=plain)
-        if dtype == "f32" or kv < 9000:
+        if dtype == "f32":  # (bf16 queries enter with more digits than attn takes)
             assert torch.equal(plain, out)
 
 

@@ -97,7 +97,7 @@ def lse_tolerance(dtype: str, D: int, n: int, lse: np.ndarray, ax: np.ndarray) -
     (of up to |lse| log2(e) and the running maximum, bounded by ax[0], plus log2 of a sum that is carried 2^8 up, below 64),
     each of its four operations within two half steps of what it handles."""
     h = kd.F32_STEP
-    x = ax[..., 0] * (D + 14) * h + ax[..., 1] * 2.0 ** (-14 if dtype == "bf16" else -24)
+    x = ax[..., 0] * (D + 14) * h + ax[..., 1] * 2.0 ** -24  # (queries of either type enter as f32 does)
     return x + 4 * h + n * h + 2.0 ** -21 + 8 * h * (np.abs(np.where(np.isfinite(lse), lse, 0)) + ax[..., 0] + 64)
 
 
