@@ -731,12 +731,14 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
     }
     RowState<NB> st[CT];
     const NewTokens<MORE> nt(a, sr);
+    __shared__ Sight<MORE> sights[MORE ? CT : 1][16];  // (a tree's: the registers are counted, 60 tokens at 100000: 177 -> 169 us)
     Sight<MORE> see[CT];
     float lx[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         const int row = row0 + 16 * c + r;
         see[c] = sight(a, sr, nt, row < rows, row / a.group);
+        if (MORE && wave == 0 && g == 0) sights[MORE ? c : 0][r] = see[c];
     }
     __syncthreads();
     DigitScales<D, Dt> qsc[CT];
@@ -798,6 +800,9 @@ __device__ __forceinline__ void few_rows(const AttnArgs &a, int row0, int split)
             const float vkeep = all ? 1.0f : ldexpf(1.0f, ev - ti.ev);
             ev = ti.ev;
             h8 p[CT][SPLIT][2];
+            if constexpr (MORE)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) see[c] = sights[c][r];
             softmax_tile<MORE, NB, CT, SPLIT>(sc, nt, see, base, ti, vkeep, st, p, lx);
             if constexpr (all) {
                 v_in_bands<MORE, D, SMALL>(a, rd, table, tile, ti, nt, see, p, st, E);
