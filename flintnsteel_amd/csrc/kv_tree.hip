@@ -254,7 +254,7 @@ template <bool NEW> struct Places {
             n = (int) min((int64_t) min(max(a.count[s], 0), r.n), a.list_stride);
             list = a.list + s * a.list_stride;
         } else {
-            n = (int) a.list_stride;
+            n = (int) min(a.list_stride, (int64_t) seq_len(a.c, a.b, s));  // (no more are kept)
             list = a.list + row * a.list_stride;
         }
     }

@@ -863,7 +863,7 @@ def attn(cache: KvCache, batch: KvBatch, q: torch.Tensor, scale: float | None = 
         ws = attn_workspace(cache, batch, q)
     elif not ws.is_contiguous():
         raise ValueError("attn: the workspace must be contiguous")
-    st = _here("attn", cache.pages, batch.kv_len, q, out, sinks, ws, lse)
+    st = _here("attn", cache.pages, batch.kv_len, q, out, sinks, ws, lse, None if tree is None else tree.sees)
     if tree is not None or lse is not None:
         if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or lse.shape != q.shape[:2]):
             raise ValueError("attn: lse must be contiguous f32 [n_tok][n_head]")
@@ -914,7 +914,7 @@ def kv_weigh(cache: KvCache, batch: KvBatch, q: torch.Tensor, lse: torch.Tensor,
         ws = kv_weigh_workspace(cache, batch, q)
     elif not ws.is_contiguous():
         raise ValueError("kv_weigh: the workspace must be contiguous")
-    st = _here("kv_weigh", cache.pages, batch.kv_len, q, lse, past, out, ws)
+    st = _here("kv_weigh", cache.pages, batch.kv_len, q, lse, past, out, ws, None if tree is None else tree.sees)
     call("fns_hip_kv_weigh", cache.ref, batch._for(cache), ctypes.byref(desc), None if tree is None else tree._for("kv_weigh", batch),
          q.data_ptr(), lse.data_ptr(), None if past is None else past.data_ptr(), out.data_ptr(), ws.data_ptr(),
          ws.numel() * ws.element_size(), st)

@@ -474,6 +474,60 @@ def test_keep_outside_the_cache():
     assert new_len.tolist() == [40, 3]
 
 
+# ---- anywhere -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("q_lens,kv_lens,many", [([9, 2], [300, 41], False), ([70, 40], [500, 90], True)])
+def test_strided_queries_and_outputs(q_lens, kv_lens, many, dtype):
+    """Queries and outputs as slices of wider rows at odd offsets: the bits of contiguous ones, and the same bits twice."""
+    s = Setup(q_lens, kv_lens, 32, 2, 128, seed=13, pad=MANY_ROWS // 4 if many else 0)
+    if many:
+        s.batch.desc.max_q = s.n_tok
+    rows = [td.seen_by(p) for p in trees_of(s, 5)]
+    t = kv_tree(s, rows)
+    q = _rand(s.rng, (s.n_tok, 8, 128), dtype)[0]
+    wide = torch.zeros(s.n_tok * (12 * 128 + 7) + 3, dtype=q.dtype, device="cuda")[3:].view(s.n_tok, 12 * 128 + 7)
+    qs, outs = wide[:, 128: 9 * 128].view(s.n_tok, 8, 128), torch.zeros_like(wide)[:, 5: 5 + 8 * 128].view(s.n_tok, 8, 128)
+    qs.copy_(q)
+    a, b = torch.zeros(2, s.n_tok, 8, device="cuda")
+    first = ops.attn(s.cache, s.batch, q, tree=t, lse=a)
+    ops.attn(s.cache, s.batch, qs, tree=t, lse=b, out=outs)
+    tok = slice(0, s.tok)
+    assert torch.equal(first[tok], outs[tok]) and torch.equal(a[tok], b[tok])
+    w = ops.kv_weigh(s.cache, s.batch, q, a, None, tree=t)
+    for x in (qs, q):
+        assert torch.equal(w, ops.kv_weigh(s.cache, s.batch, x, a, None, tree=t))
+
+
+def test_pages_behind_four_gigabytes():
+    """A cache of more bytes than 32 bits count, its sequences in the last pages: what a small cache gives."""
+    s = Setup([40, 3], [700, 90], 64, 8, 128, seed=3)
+    n = s.host.n_pages
+    far = (5 << 30) // s.cache.page_bytes
+    pages = torch.empty(far + n, s.cache.page_bytes, dtype=torch.uint8, device="cuda")
+    pages[far:] = s.cache.pages
+    big = ops.KvCache(far + n, 64, 8, 128, pages=pages)
+    there = ops.KvBatch(s.batch.q_start, s.batch.kv_len, torch.where(s.batch.page_table >= 0, s.batch.page_table + far, -1).int(),
+                        n_tok=s.tok, max_q=40, max_kv=700)
+    parents = dev([p for seq in trees_of(s, 3) for p in seq])
+    q, k, v = (_rand(s.rng, (s.tok, h, 128))[0] for h in (16, 8, 8))
+    kept, n_kept = dev([[0, 2, 9], [1, 2, 0]]), dev([3, 2])
+    freq = ops.rope_freqs(128)
+    got = []
+    for cache, batch in ((s.cache, s.batch), (big, there)):
+        t = ops.tree_plan(batch, parents)
+        x = ops.kv_append(cache, batch, k, v, q=q, rope=ops.ROPE_HALVES, inv_freq=freq, pos=t.pos)
+        lse = torch.empty(s.tok, 16, device="cuda")
+        out = ops.attn(cache, batch, x, tree=t, lse=lse)
+        w = ops.kv_weigh(cache, batch, x, lse, ops.kv_weights(cache), tree=t)
+        new_len = ops.kv_keep(cache, batch, kept, n_kept, weights=w)
+        after = ops.KvBatch(batch.q_start, new_len, batch.page_table, n_tok=s.tok, max_q=40, max_kv=700)
+        which, cut = ops.kv_evict(cache, after, w, 300, first=3, recent=50)
+        got.append([x, out, lse, new_len, which, cut, w[-n:], cache.pages[-n:]])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 # ---- together -------------------------------------------------------------------------------------------------------
 
 def test_python_checks():
