@@ -97,6 +97,7 @@ SIGNATURES: dict[str, list] = {
     "fns_hip_attn_tree": [_P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
     "fns_hip_kv_weigh_workspace": [_P, _P, _P, _P],
     "fns_hip_kv_weigh": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "fns_hip_kv_evict_workspace": [_P, _P, _P],
     "fns_hip_kv_evict": [_P, _P, _P, _P],
     "fns_hip_kv_keep": [_P, _P, _P, _P],
     "fns_hip_attn": [_P, _P, _P, _P, _P, _P, _SZ, _P],

@@ -282,6 +282,10 @@ int fns_hip_kv_weigh(const FnsKvCache *cache, const FnsKvBatch *batch, const Fns
     return impl::kv_weigh(cache, batch, x, tree, q, lse, past, weights, workspace, workspace_bytes, S(stream));
 }
 
+int fns_hip_kv_evict_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, size_t *bytes) {
+    return impl::kv_evict_workspace(cache, batch, bytes);
+}
+
 int fns_hip_kv_evict(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvEvict *x, void *stream) {
     return impl::kv_evict(cache, batch, x, S(stream));
 }

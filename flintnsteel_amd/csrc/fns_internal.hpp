@@ -124,6 +124,7 @@ int attn_tree(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const 
 int kv_weigh_workspace(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, size_t *bytes);
 int kv_weigh(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const FnsKvTree *t, const void *q, const float *lse,
              const float *past, float *weights, void *ws, size_t ws_bytes, hipStream_t st);
+int kv_evict_workspace(const FnsKvCache *c, const FnsKvBatch *b, size_t *bytes);
 int kv_evict(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvEvict *x, hipStream_t st);
 int kv_keep(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvKeep *x, hipStream_t st);
 

@@ -77,152 +77,246 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
-// Which positions a sequence's kv head keeps: a workgroup each. The budget-th largest key digit by digit (11, 11, 10 bits), the
-// counts of a digit's values in LDS; then the positions in order, those above it and as many equal ones as there is room for.
-// Up to 4096 Q positions a thread has its 4 Q keys in registers; Q = 0: any number, read anew by every pass. Bound by what waits
-// for what: the table, the weights, three times counting and the search among 2048 counts, the scan of the kept.
+// Which positions a sequence's kv head keeps. The budget-th largest key digit by digit (11, 11, 10 bits), the counts of a
+// digit's values in LDS; then the positions in order, those above it and as many equal ones as there is room for.
 constexpr int kSel = 1024, kBins = 2048, kSelWaves = kSel / 64;
 constexpr int kCopies = 4;  // of the counts: lanes with the same value wait for each other (many positions may have none at all)
+__device__ __forceinline__ int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ __forceinline__ bool digit_counts(int pass, uint32_t key, uint32_t prefix) {  // whether a key is counted in a pass
+    return key != 0 && (pass == 0 || key >> (pass == 1 ? 21 : 10) == prefix);
+}
+// Keys of positions 4 i .. 4 i + 3 (which lie in one page) of a sequence of n.
+__device__ __forceinline__ void weight_keys(const EvictArgs &a, int s, int head, int n, int i, uint32_t (&k)[4]) {
+    const int at = (int) (4u * i), page = (uint32_t) at < (uint32_t) n ? page_of(a.c, a.b, s, at) : -1;
+    float4 w = {};
+    if (page >= 0) w = *(const float4 *) (a.w + (((int64_t) page * a.c.n_kv + head) << a.c.shift) + (at & ((1 << a.c.shift) - 1)));
+    const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int p = at + j;
+        k[j] = page < 0 || p >= n ? 0u : p < a.first || p >= n - a.recent ? 0xffffffffu : weight_key(v[j]);
+    }
+}
+// What the counts of a digit's values say, by a workgroup: the digit of the want-th largest (thread t brings the counts of digits
+// 2047 - 2 t and 2046 - 2 t), how many are above it, and how many there are at all.
+struct Digit {
+    int digit, above, total;
+};
+__device__ __forceinline__ Digit find_digit(int hi, int lo, int want, bool clip, int *waves, int *found) {
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    int sum = wave_scan(hi + lo), all = 0;
+    if (lane == 63) waves[wave] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSelWaves; ++w) {
+        const int x = waves[w];
+        sum += w < wave ? x : 0, all += x;
+    }
+    if (clip) want = min(want, all);
+    const int above = sum - hi - lo;  // keys of larger digits
+    if (want > above && want <= sum) {
+        const bool second = want > above + hi;
+        found[0] = kBins - 1 - 2 * tid - (second ? 1 : 0);
+        found[1] = above + (second ? hi : 0);
+    }
+    __syncthreads();
+    return {found[0], found[1], all};
+}
+// Keys above the prefix in the low half, equal ones in the high half; and their places, after so many of either.
+__device__ __forceinline__ int above_and_equal(const uint32_t (&k)[4], uint32_t prefix) {
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c += (k[j] > prefix ? 1 : 0) + (k[j] == prefix ? 1 << 16 : 0);
+    return c;
+}
+__device__ __forceinline__ void put_kept(int32_t *kept, const uint32_t (&k)[4], uint32_t prefix, int want, int quad, int above, int equal) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const bool is = k[j] == prefix;
+        if (k[j] > prefix || (is && equal < want)) kept[above + min(equal, want)] = 4 * quad + j;
+        above += k[j] > prefix, equal += is;
+    }
+}
+
+// Up to 4096 Q positions: a workgroup, of which a thread has its 4 Q keys in registers. Bound by what waits for what: the table,
+// the weights, three times counting and the search among 2048 counts, the scan of the kept (4160 positions of 8 heads: 8.2 us,
+// 16 sequences of up to 20000: 16.7).
 template <int Q> __global__ __launch_bounds__(kSel) void k_kv_select(EvictArgs a) {
     __shared__ __align__(16) int bins[3][kCopies][kBins];
-    __shared__ int waves[Q > 0 ? Q : 1][kSelWaves], found[3][2];
+    __shared__ int waves[Q][kSelWaves], found[3][2];
     const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-    const int n = seq_len(a.c, a.b, s), P = 1 << a.c.shift;
+    const int n = seq_len(a.c, a.b, s), quads = n / 4 + (n % 4 > 0);
     int32_t *kept = a.kept + (int64_t) blockIdx.x * a.budget;
-    // keys of positions 4 i .. 4 i + 3, which lie in one page
-    const auto keys = [&](int i, uint32_t (&k)[4]) {
-        const int at = 4 * i, page = at < n ? page_of(a.c, a.b, s, at) : -1;
-        float4 w = {};
-        if (page >= 0) w = *(const float4 *) (a.w + (((int64_t) page * a.c.n_kv + head) << a.c.shift) + (at & (P - 1)));
-        const float v[4] = {w.x, w.y, w.z, w.w};
+    uint32_t own[Q][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int p = at + j;
-            k[j] = page < 0 || p >= n ? 0u : p < a.first || p >= n - a.recent ? 0xffffffffu : weight_key(v[j]);
-        }
-    };
-    const int quads = n / 4 + (n % 4 > 0);
-    uint32_t own[Q > 0 ? Q : 1][4];
-#pragma unroll
-    for (int q = 0; q < Q; ++q) keys(min(tid + q * kSel, 0x1fffffff), own[q]);
-    // f(the number of the thread's quad, its keys) for all of them
-    const auto each = [&](auto f) {
-        if constexpr (Q > 0) {
-#pragma unroll
-            for (int q = 0; q < Q; ++q)
-                if (q * kSel < quads) f(own[q]);
-        } else {
-            for (int i = tid; i < quads; i += kSel) {
-                uint32_t k[4];
-                keys(i, k);
-                f(k);
-            }
-        }
-    };
+    for (int q = 0; q < Q; ++q) weight_keys(a, s, head, n, tid + q * kSel, own[q]);
 #pragma unroll
     for (int i = 0; i < 3 * kCopies * kBins / 4 / kSel; ++i) ((int4 *) bins)[tid + i * kSel] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    int want = a.budget, total = 0;
+    int want = a.budget, keep = 0;
     uint32_t prefix = 0;
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, high = pass == 1 ? 21 : 10;
-        each([&](const uint32_t (&k)[4]) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (k[j] != 0 && (pass == 0 || k[j] >> high == prefix)) atomicAdd(&bins[pass][lane % kCopies][(k[j] >> shift) & (pass == 2 ? 1023 : 2047)], 1);
-        });
+        for (int q = 0; q < Q; ++q)
+            if (q * kSel < quads)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (digit_counts(pass, own[q][j], prefix))
+                        atomicAdd(&bins[pass][lane % kCopies][(own[q][j] >> digit_shift(pass)) & (pass == 2 ? 1023 : 2047)], 1);
         __syncthreads();
-        // from the largest digit down: thread t holds digits 2047 - 2 t and 2046 - 2 t
         int hi = 0, lo = 0;
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             const int2 two = *(const int2 *) &bins[pass][i][kBins - 2 - 2 * tid];
             hi += two.y, lo += two.x;
         }
-        int sum = wave_scan(hi + lo);
-        if (lane == 63) waves[0][wave] = sum;
-        __syncthreads();
-        int all = 0;
-#pragma unroll
-        for (int w = 0; w < kSelWaves; ++w) {
-            const int x = waves[0][w];
-            sum += w < wave ? x : 0, all += x;
-        }
-        if (pass == 0) total = all, want = min(want, total);
-        const int above = sum - hi - lo;  // keys of larger digits
-        if (want > above && want <= sum) {
-            const bool second = want > above + hi;
-            found[pass][0] = kBins - 1 - 2 * tid - (second ? 1 : 0);
-            found[pass][1] = above + (second ? hi : 0);
-        }
-        __syncthreads();
-        if (want > 0) {
-            prefix = (prefix << (pass == 2 ? 10 : 11)) | (uint32_t) found[pass][0];
-            want -= found[pass][1];
-        }
+        const Digit d = find_digit(hi, lo, want, pass == 0, waves[0], found[pass]);
+        if (pass == 0) keep = want = min(want, d.total);
+        if (want > 0) prefix = (prefix << (pass == 2 ? 10 : 11)) | (uint32_t) d.digit, want -= d.above;
     }
     // `want` of the keys equal to `prefix` are kept: the first ones
-    const int keep = min(a.budget, total);
-    const auto counts = [&](const uint32_t (&k)[4]) {  // above in the low half, equal in the high one
-        int c = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c += (k[j] > prefix ? 1 : 0) + (k[j] == prefix ? 1 << 16 : 0);
-        return c;
-    };
-    const auto put = [&](const uint32_t (&k)[4], int quad, int above, int equal) {  // (of the positions before these)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool is = k[j] == prefix;
-            if (k[j] > prefix || (is && equal < want)) kept[above + min(equal, want)] = 4 * quad + j;
-            above += k[j] > prefix, equal += is;
-        }
-    };
     if (keep > 0) {
-        if constexpr (Q > 0) {
-            int before[Q];
+        int before[Q];
 #pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                if (q * kSel >= quads) break;
-                const int c = counts(own[q]), both = wave_scan(c);
-                if (lane == 63) waves[q][wave] = both;
-                before[q] = both - c;
+        for (int q = 0; q < Q; ++q) {
+            if (q * kSel >= quads) break;
+            const int c = above_and_equal(own[q], prefix), both = wave_scan(c);
+            if (lane == 63) waves[q][wave] = both;
+            before[q] = both - c;
+        }
+        __syncthreads();
+        int all = 0;  // (at most 32768 of either fit a half)
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            if (q * kSel >= quads) break;
+            int at = all + before[q];
+#pragma unroll
+            for (int w = 0; w < kSelWaves; ++w) {
+                const int x = waves[q][w];
+                at += w < wave ? x : 0, all += x;
             }
-            __syncthreads();
-            int all = 0;  // (at most 32768 of either fit a half)
-#pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                if (q * kSel >= quads) break;
-                int at = all + before[q];
-#pragma unroll
-                for (int w = 0; w < kSelWaves; ++w) {
-                    const int x = waves[q][w];
-                    at += w < wave ? x : 0, all += x;
-                }
-                put(own[q], tid + q * kSel, at & 0xffff, at >> 16);
-            }
-        } else {
-            int above = 0, equal = 0;
-            for (int i0 = 0; i0 < quads; i0 += kSel) {
-                uint32_t k[4] = {};
-                if (i0 + tid < quads) keys(i0 + tid, k);
-                const int c = counts(k), both = wave_scan(c);
-                __syncthreads();
-                if (lane == 63) waves[0][wave] = both;
-                __syncthreads();
-                int at = both - c, all = 0;
-#pragma unroll
-                for (int w = 0; w < kSelWaves; ++w) {
-                    const int x = waves[0][w];
-                    at += w < wave ? x : 0, all += x;
-                }
-                put(k, i0 + tid, above + (at & 0xffff), equal + (at >> 16));
-                above += all & 0xffff, equal += all >> 16;
-            }
+            put_kept(kept, own[q], prefix, want, tid + q * kSel, at & 0xffff, at >> 16);
         }
     }
     for (int i = keep + tid; i < a.budget; i += kSel) kept[i] = -1;
     if (head == 0 && tid == 0) a.new_len[s] = keep;
+}
+
+// Longer sequences: chunks of 16384 positions, a workgroup each, which meet between launches: the counts of each digit in memory
+// (whole numbers, whose order of adding does not matter), then how many of each chunk are kept. 124729 positions of 2 heads: 38 us in
+// six launches, about 115 in one workgroup that reads its weights four times.
+constexpr int kChunkQuads = 4, kChunk = 4 * kSel * kChunkQuads;
+struct SelectState {
+    int bins[3][kBins];
+    int want[4], keep;  // want[p]: after p passes
+    uint32_t prefix[4];
+};
+template <int PHASE> __global__ __launch_bounds__(kSel) void k_kv_select_chunks(EvictArgs a, SelectState *states, int32_t *counts, int chunks) {
+    __shared__ __align__(16) int bins[kCopies][kBins];
+    __shared__ int waves[kChunkQuads][kSelWaves], found[2], sums[2];
+    const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const int n = seq_len(a.c, a.b, s), used = n / kChunk + (n % kChunk > 0);
+    SelectState &st = states[blockIdx.x];
+    if (PHASE == 0) {  // (one workgroup a kv head)
+        for (int i = tid; i < 3 * kBins; i += kSel) ((int *) st.bins)[i] = 0;
+        if (tid == 0) st.want[0] = a.budget, st.prefix[0] = 0;
+        return;
+    }
+    const bool lead = blockIdx.y == 0;  // (does what is there once, also for a sequence without positions)
+    if ((int) blockIdx.y >= used && !lead) return;
+    // after PHASE - 1 passes
+    int want = st.want[0];
+    uint32_t prefix = 0;
+    if (PHASE > 1) {
+        constexpr int P = PHASE == 5 ? 3 : PHASE - 1;
+        if (PHASE < 5) {
+            want = st.want[P - 1], prefix = st.prefix[P - 1];
+            const int2 two = *(const int2 *) &st.bins[P - 1][kBins - 2 - 2 * tid];
+            const Digit d = find_digit(two.y, two.x, want, P == 1, waves[0], found);
+            if (P == 1) want = min(want, d.total);
+            const int keep = want;
+            if (want > 0) prefix = (prefix << (P == 3 ? 10 : 11)) | (uint32_t) d.digit, want -= d.above;
+            if (lead && tid == 0) {
+                st.want[P] = want, st.prefix[P] = prefix;
+                if (P == 1) st.keep = keep;
+            }
+        } else {
+            want = st.want[3], prefix = st.prefix[3];
+        }
+    }
+    int32_t *kept = a.kept + (int64_t) blockIdx.x * a.budget;
+    const int keep = PHASE == 5 ? st.keep : 0;
+    int above = 0, equal = 0;  // of the chunks before this one
+    int done = 0;              // chunks counted in them
+    for (int chunk = blockIdx.y; chunk < used; chunk += gridDim.y) {
+        uint32_t own[kChunkQuads][4];
+#pragma unroll
+        for (int q = 0; q < kChunkQuads; ++q) weight_keys(a, s, head, n, chunk * (kChunk / 4) + tid + q * kSel, own[q]);
+        if (PHASE <= 3) {
+            constexpr int pass = PHASE - 1;
+#pragma unroll
+            for (int i = 0; i < kCopies * kBins / 4 / kSel; ++i) ((int4 *) bins)[tid + i * kSel] = make_int4(0, 0, 0, 0);
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < kChunkQuads; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (digit_counts(pass, own[q][j], prefix))
+                        atomicAdd(&bins[lane % kCopies][(own[q][j] >> digit_shift(pass)) & (pass == 2 ? 1023 : 2047)], 1);
+            __syncthreads();
+            for (int i = tid; i < kBins; i += kSel) {
+                const int c = bins[0][i] + bins[1][i] + bins[2][i] + bins[3][i];
+                if (c) atomicAdd(&st.bins[pass][i], c);
+            }
+            __syncthreads();
+        } else {
+            int before[kChunkQuads];
+#pragma unroll
+            for (int q = 0; q < kChunkQuads; ++q) {
+                const int c = above_and_equal(own[q], prefix), both = wave_scan(c);
+                if (lane == 63) waves[q][wave] = both;
+                before[q] = both - c;
+            }
+            __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int q = 0; q < kChunkQuads; ++q) {
+                before[q] += all;
+#pragma unroll
+                for (int w = 0; w < kSelWaves; ++w) {
+                    const int x = waves[q][w];
+                    before[q] += w < wave ? x : 0, all += x;
+                }
+            }
+            int32_t *mine = counts + ((int64_t) blockIdx.x * chunks + chunk) * 2;
+            if (PHASE == 4) {
+                if (tid == 0) mine[0] = all & 0xffff, mine[1] = all >> 16;
+            } else if (keep > 0) {
+                // what the chunks before have, by the first wave
+                if (wave == 0) {
+                    int x = 0, y = 0;
+                    for (int i = done + lane; i < chunk; i += 64) {
+                        const int32_t *c = counts + ((int64_t) blockIdx.x * chunks + i) * 2;
+                        x += c[0], y += c[1];
+                    }
+                    x = lanes_sum_i<64>(x), y = lanes_sum_i<64>(y);
+                    if (lane == 0) sums[0] = x, sums[1] = y;
+                }
+                __syncthreads();
+                above += sums[0], equal += sums[1], done = chunk;
+#pragma unroll
+                for (int q = 0; q < kChunkQuads; ++q)
+                    put_kept(kept, own[q], prefix, want, chunk * (kChunk / 4) + tid + q * kSel, above + (before[q] & 0xffff), equal + (before[q] >> 16));
+            }
+            __syncthreads();
+        }
+    }
+    if (PHASE == 5) {
+        const int64_t workers = min((int64_t) max(used, 1), (int64_t) gridDim.y);
+        for (int64_t i = keep + (int64_t) blockIdx.y * kSel + tid; i < a.budget; i += workers * kSel) kept[i] = -1;
+        if (head == 0 && lead && tid == 0) a.new_len[s] = keep;
+    }
 }
 
 struct MoveArgs {
@@ -463,6 +557,22 @@ int tree_plan(const FnsKvBatch *b, const int32_t *parents, const int32_t *base, 
     return host::check_launch("tree_plan");
 }
 
+namespace {
+
+// Positions that a sequence of a call can have at all, by its table (max_kv is no bound), and how they are gone over.
+constexpr int64_t kOneSelect = 32 * kSel;
+int select_chunks(int64_t room) { return (int) ((std::min<int64_t>(room, INT32_MAX) + kChunk - 1) / kChunk); }
+
+}  // namespace
+
+int kv_evict_workspace(const FnsKvCache *c, const FnsKvBatch *b, size_t *bytes) {
+    FNS_TRY(host::kv_check(c, b, "kv_evict"));
+    if (!bytes) return host::set_error(host::ERR_SHAPE, "kv_evict_workspace: null output");
+    const int64_t room = b->table_stride * c->page_size;
+    *bytes = room <= kOneSelect ? 0 : (size_t) b->n_seq * c->n_head_kv * (sizeof(SelectState) + (size_t) select_chunks(room) * 8);
+    return host::OK;
+}
+
 int kv_evict(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvEvict *x, hipStream_t st) {
     FNS_TRY(host::kv_check(c, b, "kv_evict"));
     if (!x) return host::set_error(host::ERR_SHAPE, "kv_evict: null arguments");
@@ -477,15 +587,31 @@ int kv_evict(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvEvict *x, hipS
     if (x->to_table == b->page_table) return host::set_error(host::ERR_SHAPE, "kv_evict: to_table must not be the batch's (NULL: in place)");
     if (!x->to_table && x->weights_out != x->weights)
         return host::set_error(host::ERR_SHAPE, "kv_evict: in place the weights move in place too");
+    size_t need = 0;
+    FNS_TRY(kv_evict_workspace(c, b, &need));
+    if (need && (!x->workspace || x->workspace_bytes < need || ((uintptr_t) x->workspace & 15)))
+        return host::set_error(host::ERR_NOMEM, "kv_evict: workspace of %zu bytes, %zu needed (16-byte aligned)", x->workspace ? x->workspace_bytes : 0, need);
     EvictArgs a{host::kv_view(c), host::kv_batch(b), x->weights, x->kept, x->new_len, x->budget, x->first, x->recent};
-    const auto select = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned) (b->n_seq * c->n_head_kv)), dim3(kSel), 0, st, a); };
-    // positions that a sequence can have at all: of its table (the batch's max_kv is no bound)
+    const unsigned heads = (unsigned) (b->n_seq * c->n_head_kv);
+    const auto select = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(heads), dim3(kSel), 0, st, a); };
     const int64_t room = b->table_stride * c->page_size;
     if (room <= 4 * kSel) select(k_kv_select<1>);
     else if (room <= 8 * kSel) select(k_kv_select<2>);
     else if (room <= 16 * kSel) select(k_kv_select<4>);
-    else if (room <= 32 * kSel) select(k_kv_select<8>);
-    else select(k_kv_select<0>);
+    else if (room <= kOneSelect) select(k_kv_select<8>);
+    else {
+        const int chunks = select_chunks(room);
+        SelectState *states = (SelectState *) x->workspace;
+        int32_t *counts = (int32_t *) (states + heads);
+        const auto phase = [&](auto kern, unsigned n) { hipLaunchKernelGGL(kern, dim3(heads, n), dim3(kSel), 0, st, a, states, counts, chunks); };
+        const unsigned wgs = (unsigned) std::min(chunks, 65535);
+        phase(k_kv_select_chunks<0>, 1u);
+        phase(k_kv_select_chunks<1>, wgs);
+        phase(k_kv_select_chunks<2>, wgs);
+        phase(k_kv_select_chunks<3>, wgs);
+        phase(k_kv_select_chunks<4>, wgs);
+        phase(k_kv_select_chunks<5>, wgs);
+    }
     FNS_TRY(host::check_launch("kv_evict"));
     MoveArgs m{a.c, a.b, x->to_table ? x->to_table : b->page_table, x->to_table ? x->to_stride : b->table_stride, x->kept, nullptr,
                x->budget, x->weights, x->weights_out, nullptr};

@@ -15,6 +15,9 @@ namespace {
 
 constexpr int kRowTile = 16;
 constexpr int kFewTiles = 4;    // row tiles that a workgroup of few rows holds
+constexpr int64_t kMidSteps = 4096;
+template <int D> constexpr int kMidPhases = D == 256 ? 2 : 4;
+template <int D> constexpr int kMidTiles = D == 256 ? 8 : 16;  // and of sixteen waves, in all of a CU's memory
 constexpr int key_tiles(int D) { return D == 256 ? 4 : 8; }     // 16-key tiles of a wave of many rows (the registers are counted)
 constexpr int key_block(int D) { return 4 * 16 * key_tiles(D); }  // keys of its workgroup
 
@@ -255,13 +258,16 @@ __device__ __forceinline__ int image_tiles(const WeighArgs &x, const SeqRange &s
 __device__ __forceinline__ int planned_blocks(const WeighArgs &x, int len) { return (int) min(((int64_t) len + x.block - 1) / x.block, (int64_t) x.blocks); }
 
 // Few rows (decode, verify): their images are made by every workgroup, whose waves take 64 keys in turn, the next ones' K
-// asked for before this one's products.
-template <int D, int RT, class T> __global__ __launch_bounds__(256, D == 256 ? 2 : 4) void k_weigh_few(WeighArgs x) {
+// asked for before this one's products. PH > 1 (up to sixteen tiles of rows): PH waves have the same keys and every PH-th tile
+// each, and the first adds up what they found.
+template <int D, int RT, int PH, class T> __global__ __launch_bounds__(256 * PH, D < 256 ? 4 : 2) void k_weigh_few(WeighArgs x) {
     const AttnArgs &a = x.a;
     __shared__ __align__(16) RowImage<D> im[RT];
-    const int s = blockIdx.y / a.c.n_kv, head = blockIdx.y % a.c.n_kv, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    __shared__ float found[PH > 1 ? PH - 1 : 1][256];
+    const int s = blockIdx.y / a.c.n_kv, head = blockIdx.y % a.c.n_kv, lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), phase = wave / 4, keys_of = wave % 4;
     const SeqRange sr = seq_range(a.b, s);
-    const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) RT * kRowTile);
+    const int rows = (int) min((int64_t) sr.n * a.group, x.row_tiles * kRowTile), tiles = PH > 1 ? (rows - 1) / kRowTile + 1 : RT;
     const int len = key_len(a, sr), first = sr.len - sr.n, step = (int) gridDim.x * 256;
     if (rows == 0 || (int) blockIdx.x * 256 >= len) return;
     const NewTokens<true> nt(a, sr);
@@ -273,39 +279,49 @@ template <int D, int RT, class T> __global__ __launch_bounds__(256, D == 256 ? 2
 #pragma unroll
         for (int t = 0; t < 4; ++t) k.load(x, head, base, t, __builtin_amdgcn_readlane(own, 16 * t));  // 16 aligned positions lie in one page
     };
-    int64_t b0 = (int64_t) blockIdx.x * 256 + wave * 64;
+    const auto before = [&](int base, int own) { return phase == 0 ? past_weight(x, head, own, base + lane, first) : 0.0f; };
+    int64_t b0 = (int64_t) blockIdx.x * 256 + keys_of * 64;
     if (b0 < len) {
         page = ask(b0);
         load(keys, (int) b0, page);
-        past = past_weight(x, head, page, (int) b0 + lane, first);
+        past = before((int) b0, page);
         after = ask(b0 + step);
     }
-    for (int t = wave; t < RT; t += 4) make_image<D, T>(x, sr, nt, head, rows, t * kRowTile, im[t]);
+    for (int t = wave; t < tiles; t += 4 * PH) make_image<D, T>(x, sr, nt, head, rows, t * kRowTile, im[t]);
     __syncthreads();
-    for (; b0 < len; b0 += step) {
+    for (; PH > 1 ? b0 - keys_of * 64 < len : b0 < len; b0 += step) {  // (PH > 1: of the whole workgroup)
         const int base = (int) b0;
-        const bool more = b0 + step < len;
-        if (more) {
+        if (b0 + step < len) {
             load(next, base + step, after);
-            coming = past_weight(x, head, after, base + step + lane, first);
+            coming = before(base + step, after);
         }
         const int then = ask(b0 + 2 * (int64_t) step);
         float sum[4] = {};
+        if (PH == 1 || b0 < len) {
+#pragma unroll 1
+            for (int t = phase; t < tiles; t += PH) {
+                if (unseen(im[t], base, 64)) continue;
+                RowDigits<D> rows_;
+                f4 acc[4];
+                rows_.read(im[t]);
+                products<0>(rows_, keys, acc);
+                if (!(im[t].any[0] < base && im[t].any[1] >= base + 63)) hide<true>(im[t], nt, base, acc);  // (some row does not see all)
+                add_exps(acc, sum);
+            }
+        }
         bool good[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) good[t] = !keys.nan(t);
-#pragma unroll 1
-        for (int t = 0; t < RT; ++t) {
-            if (unseen(im[t], base, 64)) continue;
-            RowDigits<D> rows_;
-            f4 acc[4];
-            rows_.read(im[t]);
-            products<0>(rows_, keys, acc);
-            if (!(im[t].any[0] < base && im[t].any[1] >= base + 63)) hide<true>(im[t], nt, base, acc);  // (some row does not see all)
-            add_exps(acc, sum);
+        float sums = one_a_lane(sum, good, 0);
+        if (PH > 1) {
+            if (phase > 0) found[phase - 1][keys_of * 64 + lane] = sums;
+            __syncthreads();
+            if (phase == 0)
+#pragma unroll
+                for (int i = 0; i < PH - 1; ++i) sums += found[i][keys_of * 64 + lane];
+            __syncthreads();
         }
-        const float sums = one_a_lane(sum, good, 0);
-        if (page >= 0) x.weights[weight_at(x, head, page, base + lane)] = past + sums;
+        if (phase == 0 && page >= 0) x.weights[weight_at(x, head, page, base + lane)] = past + sums;
         keys = next, page = after, after = then, past = coming;
     }
 }
@@ -551,7 +567,7 @@ __global__ __launch_bounds__(256) void k_weigh_join(WeighArgs x) {
 }
 
 struct WeighPlan {
-    int few;  // row tiles of the form of few rows (1, 2 or 4), or 0
+    int few;  // row tiles that a workgroup of few rows holds (1, 2, 4 or more), or 0
     int64_t row_tiles, blocks, shares;
     int block;
     size_t plan_off, part_off, bytes;
@@ -562,19 +578,28 @@ WeighPlan weigh_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x)
     const auto per = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
     const int64_t rows = std::min<int64_t>(b->max_q, b->n_tok) * (x->n_head / c->n_head_kv), heads = std::max<int64_t>(1, (int64_t) b->n_seq * c->n_head_kv);
     p.row_tiles = per(rows, kRowTile);
-    if (p.row_tiles <= kFewTiles) {
-        p.few = p.row_tiles <= 1 ? 1 : p.row_tiles == 2 ? 2 : 4;
+    const int64_t steps = per(std::max<int64_t>(b->max_kv, 1), 256);
+    // Up to 64 rows take the form of few rows; up to 256 (128 of 256 channels) too, in workgroups of sixteen waves (eight), unless
+    // there is so much to do that the many-row form's cheaper steps outweigh its two more launches (a tree of 20 tokens, 8 heads
+    // over 2 of 128, at 400 keys: 9.8 us against 25.9 in three launches; 4 sequences of 62 tokens at 56000: 59 against 81; 24 of 32
+    // tokens at 16000, 64 heads over 8: 208 against 174, but 256 channels 211 against 252).
+    const int mid = c->head_dim == 256 ? kMidTiles<256> : kMidTiles<128>;
+    const bool middle = p.row_tiles > kFewTiles && p.row_tiles <= mid && (c->head_dim == 256 || heads * steps <= kMidSteps);
+    if (p.row_tiles <= kFewTiles || middle) {
+        p.few = p.row_tiles <= 1 ? 1 : p.row_tiles == 2 ? 2 : middle ? mid : 4;
         // Workgroups of 256 keys at a time: of one sequence as many as run at once, of unequal ones twice that (one of 131072, f32:
         // 19.4 us with 1024, 21.4 with 2048; 24 of up to 16000, bf16: 27.4 and 25.1).
-        p.blocks = std::min(per(std::max<int64_t>(b->max_kv, 1), 256), per(b->n_seq == 1 ? 1024 : 2048, heads));
+        p.blocks = std::min(steps, per(middle ? 256 : b->n_seq == 1 ? 1024 : 2048, heads));
         return p;
     }
     p.block = key_block(c->head_dim);
     p.blocks = std::min<int64_t>(per(std::max<int64_t>(b->max_kv, 1), p.block), 65535 / (p.block / 256));
     // Workgroups of a kv head: as many as there are places for all heads' at once (two a CU; one of 256 channels), or, of many
-    // heads, so many that the last round's empty places do not matter; no more than give a share of four steps.
+    // heads, which may be of unequal sequences, so many that the longest, or the last round, does not run on alone; no more than
+    // give a share of four steps (24 sequences of up to 9000 keys, 64 tokens, 8 heads: 144 us against 229 in one round; 4 of 205
+    // tokens at 20000, 4 heads: 83 against 71).
     const int64_t places = c->head_dim == 256 ? 256 : 512;
-    p.shares = heads <= places / 2 ? places / heads : per(4 * places, heads);
+    p.shares = heads <= places / (b->n_seq == 1 ? 2 : 16) ? places / heads : per(4 * places, heads);
     p.shares = std::max<int64_t>(1, std::min(p.shares, p.row_tiles * p.blocks / 4));
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     p.plan_off = up((size_t) (heads * p.row_tiles) * image_bytes(c->head_dim));
@@ -622,10 +647,11 @@ int kv_weigh(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, const F
     const auto by_type = [&](auto dim, auto type) {
         constexpr int D = decltype(dim)::value;
         using T = decltype(type);
-        const auto few = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(blocks, heads), dim3(256), 0, st, w); };
-        if (p.few == 1) few(k_weigh_few<D, 1, T>);
-        else if (p.few == 2) few(k_weigh_few<D, 2, T>);
-        else if (p.few) few(k_weigh_few<D, 4, T>);
+        const auto few = [&](auto kern, unsigned waves) { hipLaunchKernelGGL(kern, dim3(blocks, heads), dim3(64 * waves), 0, st, w); };
+        if (p.few == 1) few(k_weigh_few<D, 1, 1, T>, 4);
+        else if (p.few == 2) few(k_weigh_few<D, 2, 1, T>, 4);
+        else if (p.few == kFewTiles) few(k_weigh_few<D, kFewTiles, 1, T>, 4);
+        else if (p.few) few(k_weigh_few<D, kMidTiles<D>, kMidPhases<D>, T>, 4 * kMidPhases<D>);
         if (p.few) return host::check_launch("kv_weigh");
         hipLaunchKernelGGL((k_weigh_rows<D, T>), dim3(heads, (unsigned) p.row_tiles), dim3(64), 0, st, w);
         FNS_TRY(host::check_launch("kv_weigh"));

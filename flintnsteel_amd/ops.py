@@ -638,7 +638,8 @@ class KvEvictDesc(ctypes.Structure):
     """Mirror of FnsKvEvict."""
     _fields_ = [("budget", ctypes.c_int), ("first", ctypes.c_int), ("recent", ctypes.c_int), ("weights", ctypes.c_void_p),
                 ("weights_out", ctypes.c_void_p), ("to_table", ctypes.c_void_p), ("to_stride", ctypes.c_int64),
-                ("kept", ctypes.c_void_p), ("new_len", ctypes.c_void_p)]
+                ("kept", ctypes.c_void_p), ("new_len", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_size_t)]
 
 
 class KvKeepDesc(ctypes.Structure):
@@ -921,8 +922,17 @@ def kv_weigh(cache: KvCache, batch: KvBatch, q: torch.Tensor, lse: torch.Tensor,
     return out
 
 
+def kv_evict_workspace(cache: KvCache, batch: KvBatch) -> torch.Tensor | None:
+    """A workspace of kv_evict for this batch's numbers; None where it needs none (tables of up to 32768 positions)."""
+    if batch.desc.table_stride * cache.page_size <= 32768:
+        return None
+    size = ctypes.c_size_t()
+    call("fns_hip_kv_evict_workspace", cache.ref, batch._for(cache), ctypes.byref(size))
+    return torch.empty(size.value, dtype=torch.uint8, device=cache.pages.device)
+
+
 def kv_evict(cache: KvCache, batch: KvBatch, weights: torch.Tensor, budget: int, first: int = 0, recent: int = 0,
-             to_table: torch.Tensor | None = None, weights_out: torch.Tensor | None = None):
+             to_table: torch.Tensor | None = None, weights_out: torch.Tensor | None = None, ws: torch.Tensor | None = None):
     """Cuts every sequence to `budget` positions a kv head: the first `first`, the last `recent`, and of the others those of the
     largest weights; K, V and weights of the kept ones move to the front of the sequence, in order: of its own pages, or of
     to_table's int32 [n_seq][pages] (weights_out: None: weights). -> (kept int32 [n_seq][n_head_kv][budget], the kept positions and
@@ -938,7 +948,13 @@ def kv_evict(cache: KvCache, batch: KvBatch, weights: torch.Tensor, budget: int,
         if to_table.dim() != 2:
             raise ValueError("kv_evict: to_table must be [n_seq][pages]")
         x.to_table, x.to_stride = _ints("kv_evict", "to_table", to_table, n_seq, to_table.shape[1]), to_table.shape[1]
-    st = _here("kv_evict", cache.pages, batch.kv_len, weights, weights_out, to_table)
+    if ws is None:
+        ws = kv_evict_workspace(cache, batch)
+    elif not ws.is_contiguous():
+        raise ValueError("kv_evict: the workspace must be contiguous")
+    if ws is not None:
+        x.workspace, x.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+    st = _here("kv_evict", cache.pages, batch.kv_len, weights, weights_out, to_table, ws)
     call("fns_hip_kv_evict", cache.ref, batch._for(cache), ctypes.byref(x), st)
     return kept, new_len
 

@@ -461,7 +461,11 @@ typedef struct FnsKvEvict {
     const int32_t *to_table;   /* NULL: in place; else [n_seq][to_stride] */
     int64_t to_stride;
     int32_t *kept, *new_len;
+    void *workspace;           /* fns_hip_kv_evict_workspace bytes, 16-byte aligned; calls that overlap in time need one each */
+    size_t workspace_bytes;
 } FnsKvEvict;
+/* Depends on the numbers of cache and batch alone: 0 where the table has room for at most 32768 positions of a sequence. */
+int fns_hip_kv_evict_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, size_t *bytes);
 int fns_hip_kv_evict(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsKvEvict *x, void *stream);
 
 /* Of the new tokens of every sequence those listed become its next positions, in the list's order: new token kept[s][i] (its

@@ -412,17 +412,33 @@ def test_evict_equal_weights_keeps_the_first(value):
     assert kept[0, 0].tolist() == [*range(2500), *range(4500, 5000)]
 
 
-def test_evict_long_sequences():
-    """Selection over more positions than one round of the workgroup holds, weights of all magnitudes."""
-    n, page = 70001, 64
-    s = Setup([1], [n], page, 1, 64, seed=4)
-    w = torch.exp(torch.randn(s.host.n_pages, 1, page, device="cuda") * 8)
-    budget = 33333
-    flat = w[dev(s.lists[0]).long(), 0].flatten()[:n].cpu().double()
-    kept, new_len = ops.kv_evict(s.cache, s.batch, w.clone(), budget, first=4, recent=1000)
-    flat[:4] = flat[n - 1000:] = float("inf")
-    want = torch.sort(flat, descending=True, stable=True).indices[:budget].sort().values
-    assert torch.equal(kept[0, 0].cpu().long(), want) and new_len.tolist() == [budget]
+@pytest.mark.parametrize("lens,page,heads,budget,first,recent", [
+    ([70001], 64, 1, 33333, 4, 1000), ([40000, 5, 0, 32768, 16384], 128, 2, 16000, 0, 0), ([33000], 16, 3, 32999, 1, 1), ([50000, 49152], 256, 1, 1, 0, 0),
+    ([36000], 64, 1, 70000, 5, 60)])
+@pytest.mark.parametrize("equal", [False, True])
+def test_evict_long_sequences(lens, page, heads, budget, first, recent, equal):
+    """Selection in chunks: weights of all magnitudes, or few different ones; the lists twice the same."""
+    s = Setup([1] * len(lens), lens, page, heads, 64, seed=4)
+    w = torch.exp(torch.randn(s.host.n_pages, heads, page, device="cuda") * 8)
+    if equal:
+        w = torch.randint(0, 3, w.shape, device="cuda").float()
+    assert ops.kv_evict_workspace(s.cache, s.batch) is not None
+    pages, w0 = s.cache.pages.clone(), w.clone()
+    kept, new_len = ops.kv_evict(s.cache, s.batch, w, budget, first=first, recent=recent)
+    for i, n in enumerate(lens):
+        assert new_len[i].item() == min(n, budget)
+        for h in range(heads if n else 0):
+            flat = w0[dev(s.lists[i]).long(), h].flatten()[:n].cpu().double()
+            flat[: min(first, n)] = float("inf")
+            flat[max(0, n - recent):] = float("inf")
+            want = torch.sort(flat, descending=True, stable=True).indices[:budget].sort().values
+            got = kept[i, h].cpu().long()
+            assert torch.equal(got[: len(want)], want) and (got[len(want):] == -1).all()
+            pg = dev(s.lists[i]).long()
+            assert torch.equal(w[pg, h].flatten()[: len(want)].cpu(), w0[pg, h].flatten()[:n].cpu()[want])
+    s.cache.pages.copy_(pages)
+    again, _ = ops.kv_evict(s.cache, s.batch, w0, budget, first=first, recent=recent)
+    assert torch.equal(kept, again)
 
 
 # ---- accepted paths -------------------------------------------------------------------------------------------------
@@ -552,8 +568,8 @@ def test_python_checks():
     with pytest.raises(FnsError, match="budget"):
         ops.kv_evict(s.cache, s.batch, w, 0)
     with pytest.raises(FnsError, match="workspace"):
-        many = ops.KvBatch.from_lists([100], [100], [s.lists[0] * 4])
-        q, lse = torch.zeros(100, 4, 64, device="cuda"), torch.zeros(100, 4, device="cuda")
+        many = ops.KvBatch.from_lists([200], [200], [s.lists[0] * 7])
+        q, lse = torch.zeros(200, 4, 64, device="cuda"), torch.zeros(200, 4, device="cuda")
         ops.kv_weigh(s.cache, many, q, lse, w, ws=ops.kv_weigh_workspace(s.cache, many, q)[:-16])
 
 

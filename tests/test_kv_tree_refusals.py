@@ -22,7 +22,7 @@ def tree(**kw):
 
 def evict(**kw):
     return ops.KvEvictDesc(**{**dict(budget=8, first=2, recent=3, weights=BUF, weights_out=BUF, to_table=None, to_stride=0,
-                                     kept=BUF, new_len=2 * BUF), **kw})
+                                     kept=BUF, new_len=2 * BUF, workspace=None, workspace_bytes=0), **kw})
 
 
 def keep(**kw):
@@ -120,7 +120,13 @@ def test_null_arguments_overlap_and_workspaces():
     assert L().fns_hip_kv_weigh_workspace(r(cache()), r(batch()), r(att()), None) == -2
     assert L().fns_hip_kv_weigh_workspace(r(cache()), r(batch()), None, None) == -2
     size = ctypes.c_size_t()
-    b = batch(n_tok=100, max_q=100)
+    assert L().fns_hip_kv_evict_workspace(r(cache()), r(batch()), None) == -2
+    assert L().fns_hip_kv_evict_workspace(r(cache()), r(batch(table_stride=512)), r(size)) == 0 and size.value == 0
+    wide = batch(table_stride=513)
+    assert L().fns_hip_kv_evict_workspace(r(cache()), r(wide), r(size)) == 0 and size.value > 0
+    for kw in (dict(), dict(workspace=BUF, workspace_bytes=size.value - 1), dict(workspace=BUF + 8, workspace_bytes=size.value)):
+        assert _evict(b=wide, x=evict(**kw)) == -4
+    b = batch(n_tok=1000, max_q=1000)
     assert L().fns_hip_kv_weigh_workspace(r(cache()), r(b), r(att()), r(size)) == 0 and size.value > 0
     for ws, n in ((None, size.value), (BUF, size.value - 1), (BUF + 8, size.value), (BUF, 0)):
         assert _weigh(b=b, ws=ws, size=n) == -4
