@@ -352,10 +352,9 @@ template <bool NEW> struct Places {
             list = a.list + row * a.list_stride;
         }
     }
-    __device__ __forceinline__ Place at(const MoveArgs &a, int s, int64_t i) const {
+    __device__ __forceinline__ int pick(int64_t i) const { return i < n ? list[i] : -1; }
+    __device__ __forceinline__ Place at(const MoveArgs &a, int s, int64_t i, int x) const {  // x = pick(i)
         Place p{-1, -1, 0, 0};
-        if (i >= n) return p;
-        const int x = list[i];
         if (x < 0 || (NEW && x >= fresh)) return p;
         const int64_t src = first + x, dst = first + i;
         if (src == dst && a.to == a.b.table) return p;
@@ -370,65 +369,80 @@ template <bool NEW> struct Places {
     }
 };
 
-// In place, any number: a workgroup moves a part of a position (K's codes, 16 byte columns of V, or the scale bytes and the
-// weight) for 1024 positions at a time, all of which are read before the first is written, and goes over all of them in order:
-// what it writes lies before everything that it has yet to read, since the list ascends (a list of new tokens, which need not,
-// has at most 1024).
+// In place, any number: a workgroup moves a part of a position (64 bytes of K's codes, 16 byte columns of V, or the scale bytes
+// and the weight) for 1024 positions at a time, all of which are read before the first is written, and goes over all of them in
+// order: what it writes lies before everything that it has yet to read, since the list ascends (a list of new tokens, which need
+// not, has at most 1024). Bound by what waits for what, a step at a time: a step's data, the next one's pages and the list of the
+// one after are asked for together (130000 positions of 8 heads cut to 100000: 354 us with the choice, 488 step by step; 9000 of 256
+// channels to 8192, 4 sequences of 2 heads: 39 and 106).
 constexpr int kMove = 1024;
+template <int N, bool NEW, class Pos, class Load, class Store>
+__device__ __forceinline__ void walk(const MoveArgs &a, const Places<NEW> &places, int s, Pos pos, Load load, Store store) {
+    Place p[N], then[N];
+    int x[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) p[u] = places.at(a, s, pos(u), places.pick(pos(u)));
+#pragma unroll
+    for (int u = 0; u < N; ++u) x[u] = places.pick(kMove + pos(u));
+    for (int64_t i0 = 0; i0 < places.n; i0 += kMove) {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (p[u].to >= 0) load(u, p[u]);
+#pragma unroll
+        for (int u = 0; u < N; ++u) then[u] = places.at(a, s, i0 + kMove + pos(u), x[u]), x[u] = places.pick(i0 + 2 * kMove + pos(u));
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            if (p[u].to >= 0) store(u, p[u]);
+            p[u] = then[u];
+        }
+    }
+}
+template <int D> constexpr int kMoveK = D == 64 ? 2 : 4;             // 16-byte pieces of K of a part
+template <int D> constexpr int kMoveParts = D / 32 / kMoveK<D> + 1 + D / 32;
 template <int D, bool NEW> __global__ __launch_bounds__(kMove) void k_kv_walk(MoveArgs a) {
-    constexpr int NB = D / 32, NP = D / 32;  // 16-byte pieces of a K row
+    constexpr int NB = D / 32, N = kMoveK<D>, KP = D / 32 / N;
     const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, part = blockIdx.y, tid = threadIdx.x, P = 1 << a.c.shift;
     const Places<NEW> places(a, s, blockIdx.x);
     if (NEW && head == 0 && part == 0 && tid == 0) a.new_len[s] = (int) max(places.first + places.n, (int64_t) 0);
     using L = KvParts<D>;
     const int64_t head_off = head * kv_head_bytes(D, P);
-    for (int64_t i0 = 0; i0 < places.n; i0 += kMove) {
-        if (part == 0) {
-            Place p[NP];
-            uint4 x[NP];
+    const auto at = [&](int page) { return a.c.pages + page * a.c.page_bytes + head_off; };
+    const auto one = [&](int) { return tid; };
+    if (part < KP) {
+        uint4 x[N];
+        const int piece = part * N + tid % N;
+        walk<N>(a, places, s, [&](int u) { return (u * kMove + tid) / N; },
+                [&](int u, const Place &p) { x[u] = *(const uint4 *) (at(p.from) + L::k_row(P, p.row_from) + piece * 16); },
+                [&](int u, const Place &p) { *(uint4 *) (at(p.to) + L::k_row(P, p.row_to) + piece * 16) = x[u]; });
+    } else if (part == KP) {
+        uint8_t k[NB], v[NB];
+        float w = 0.0f;
+        walk<1>(a, places, s, one,
+                [&](int, const Place &p) {
+                    __builtin_memcpy(k, __builtin_assume_aligned(at(p.from) + L::k_scale(P, p.row_from), NB), NB);
+                    __builtin_memcpy(v, __builtin_assume_aligned(at(p.from) + L::v_scale(P, p.row_from), NB), NB);
+                    if (a.w) w = a.w[(((int64_t) p.from * a.c.n_kv + head) << a.c.shift) + p.row_from];
+                },
+                [&](int, const Place &p) {
+                    __builtin_memcpy(__builtin_assume_aligned(at(p.to) + L::k_scale(P, p.row_to), NB), k, NB);
+                    __builtin_memcpy(__builtin_assume_aligned(at(p.to) + L::v_scale(P, p.row_to), NB), v, NB);
+                    if (a.w) a.w_out[(((int64_t) p.to * a.c.n_kv + head) << a.c.shift) + p.row_to] = w;
+                });
+    } else {
+        const int j = 16 * (part - KP - 1);
+        uint8_t x[16];
+        walk<1>(a, places, s, one,
+                [&](int, const Place &p) {
+                    const uint8_t *src = at(p.from) + L::v_col(P, j) + p.row_from;
 #pragma unroll
-            for (int u = 0; u < NP; ++u) {
-                p[u] = places.at(a, s, i0 + (u * kMove + tid) / NP);
-                if (p[u].to >= 0)
-                    x[u] = *(const uint4 *) (a.c.pages + p[u].from * a.c.page_bytes + head_off + L::k_row(P, p[u].row_from) + tid % NP * 16);
-            }
-            __syncthreads();
+                    for (int u = 0; u < 16; ++u) x[u] = src[(int64_t) u * P];
+                },
+                [&](int, const Place &p) {
+                    uint8_t *dst = at(p.to) + L::v_col(P, j) + p.row_to;
 #pragma unroll
-            for (int u = 0; u < NP; ++u)
-                if (p[u].to >= 0) *(uint4 *) (a.c.pages + p[u].to * a.c.page_bytes + head_off + L::k_row(P, p[u].row_to) + tid % NP * 16) = x[u];
-        } else if (part == 1) {
-            const Place p = places.at(a, s, i0 + tid);
-            uint8_t k[NB], v[NB];
-            float w = 0.0f;
-            const uint8_t *src = a.c.pages + p.from * a.c.page_bytes + head_off;
-            if (p.to >= 0) {
-                __builtin_memcpy(k, __builtin_assume_aligned(src + L::k_scale(P, p.row_from), NB), NB);
-                __builtin_memcpy(v, __builtin_assume_aligned(src + L::v_scale(P, p.row_from), NB), NB);
-                if (a.w) w = a.w[(((int64_t) p.from * a.c.n_kv + head) << a.c.shift) + p.row_from];
-            }
-            __syncthreads();
-            uint8_t *dst = a.c.pages + p.to * a.c.page_bytes + head_off;
-            if (p.to >= 0) {
-                __builtin_memcpy(__builtin_assume_aligned(dst + L::k_scale(P, p.row_to), NB), k, NB);
-                __builtin_memcpy(__builtin_assume_aligned(dst + L::v_scale(P, p.row_to), NB), v, NB);
-                if (a.w) a.w_out[(((int64_t) p.to * a.c.n_kv + head) << a.c.shift) + p.row_to] = w;
-            }
-        } else {
-            const Place p = places.at(a, s, i0 + tid);
-            const int j = 16 * (part - 2);
-            uint8_t x[16];
-            if (p.to >= 0) {
-                const uint8_t *src = a.c.pages + p.from * a.c.page_bytes + head_off + L::v_col(P, j) + p.row_from;
-#pragma unroll
-                for (int u = 0; u < 16; ++u) x[u] = src[(int64_t) u * P];
-            }
-            __syncthreads();
-            if (p.to >= 0) {
-                uint8_t *dst = a.c.pages + p.to * a.c.page_bytes + head_off + L::v_col(P, j) + p.row_to;
-#pragma unroll
-                for (int u = 0; u < 16; ++u) dst[(int64_t) u * P] = x[u];
-            }
-        }
+                    for (int u = 0; u < 16; ++u) dst[(int64_t) u * P] = x[u];
+                });
     }
 }
 
@@ -443,7 +457,7 @@ template <int D, int W, bool NEW> __global__ __launch_bounds__(256) void k_kv_co
     const int64_t i0 = (int64_t) blockIdx.y * W;
     if (NEW && head == 0 && tid == 0) a.new_len[s] = (int) max(places.first + places.n, (int64_t) 0);
     if (i0 >= places.n) return;
-    if (tid < W) place[tid] = places.at(a, s, i0 + tid);
+    if (tid < W) place[tid] = places.at(a, s, i0 + tid, places.pick(i0 + tid));
     __syncthreads();
     using L = KvParts<D>;
     const int64_t head_off = head * kv_head_bytes(D, P);
@@ -511,10 +525,15 @@ template <bool NEW> int move(const MoveArgs &a, int D, int n_seq, const char *wh
         const auto copy = [&](auto width, unsigned steps) {
             hipLaunchKernelGGL((k_kv_copy<DD, decltype(width)::value, NEW>), dim3(heads, steps), dim3(256), 0, st, a);
         };
-        if (NEW && a.list_stride <= 16) copy(std::integral_constant<int, 16>{}, 1u);
-        else if (NEW && a.list_stride <= 64) copy(std::integral_constant<int, 64>{}, 1u);
-        else if (!NEW && a.to != a.b.table && a.list_stride <= 64 * 65535) copy(std::integral_constant<int, 64>{}, (unsigned) ((a.list_stride + 63) / 64));
-        else hipLaunchKernelGGL((k_kv_walk<DD, NEW>), dim3(heads, 2 + DD / 32), dim3(kMove), 0, st, a);
+        const std::integral_constant<int, 64> most{};
+        bool done = false;
+        if constexpr (NEW) {
+            if ((done = a.list_stride <= 16)) copy(std::integral_constant<int, 16>{}, 1u);
+            else if ((done = a.list_stride <= 64)) copy(most, 1u);
+        } else if ((done = a.to != a.b.table && a.list_stride <= 64 * 65535)) {
+            copy(most, (unsigned) ((a.list_stride + 63) / 64));
+        }
+        if (!done) hipLaunchKernelGGL((k_kv_walk<DD, NEW>), dim3(heads, kMoveParts<DD>), dim3(kMove), 0, st, a);
         return host::check_launch(what);
     };
     if (D == 64) return by_dim(std::integral_constant<int, 64>{});

@@ -451,9 +451,11 @@ int fns_hip_kv_weigh(const FnsKvCache *cache, const FnsKvBatch *batch, const Fns
  * positions, or all if there are no more: the first `first`, the last `recent`, and of the others those of the largest weights (a
  * NaN is the largest, of equal ones the earlier is kept). Positions without a page are not there. What is kept moves, in order,
  * to positions 0, 1, ...: K, V (their bytes) and weights; the heads' choices differ, their number does not.
- * The table that the kept positions go to: the batch's own (in place: no page may be in it twice, and weights_out is weights), or `to_table` with pages none of which any of the call's sequences has. What follows the kept positions is undefined
- * in place, left alone elsewhere. kept: int32 [n_seq][n_head_kv][budget], the kept positions in order, then -1. new_len:
- * int32 [n_seq], how many they are; not the batch's kv_len (which the engine sets afterwards). */
+ * They go by the batch's own table (in place: no page may be in it twice, and weights_out is weights) or by `to_table`, with pages
+ * none of which any of the call's sequences has; what goes where that table has no page, or behind its end, is lost. What
+ * follows the kept positions is undefined in place, left alone elsewhere. kept: int32 [n_seq][n_head_kv][budget], the kept
+ * positions in order, then -1. new_len: int32 [n_seq], how many they are; not the batch's kv_len (which the engine sets
+ * afterwards). */
 typedef struct FnsKvEvict {
     int budget, first, recent; /* budget 1..2^30, first + recent at most that */
     const float *weights;

@@ -384,6 +384,8 @@ EVICT = [
     ([5000, 4097, 4096], 64, 1, 64, 2500, 3, 100),
     ([9000], 4096, 1, 64, 8999, 0, 5),
     ([3500, 100], 16, 2, 128, 1023, 4, 64),
+    ([4700, 1025], 64, 2, 128, 4300, 4, 64),
+    ([2600, 1500], 32, 2, 256, 2300, 1, 50),
 ]
 
 
