@@ -3,7 +3,8 @@
 // Append. A token of a batch brings k and v of every kv head (and its queries); its position is the sequence's length
 // less the tokens after it. With a rotation, a pair of channels (a, b) of k and q becomes
 //   m (a cos t - b sin t, a sin t + b cos t),  t = position * inv_freq[i],
-// (position: in the cache, or the token's own; m: 1, or the magnitude that goes with frequencies scaled for a long context) and k and v go into the cache in 4 bits, k from the rotated value before any rounding. The rotation and the block
+// (position: in the cache, or the token's own; m: 1, or the magnitude that goes with frequencies scaled for a long context)
+// and k and v go into the cache in 4 bits, k from the rotated value before any rounding. The rotation and the block
 // arithmetic are done in 64 bits: an f32 angle of a far position is off by its spacing (4e-3 at position 65536), and a
 // 4-bit code next to a border would depend on the last bit of a 32-bit rotation. The pass moves the bytes of q, k and
 // v and is bound by them (and by its launch for a few tokens), not by this arithmetic.
@@ -139,7 +140,9 @@ template <class F> __device__ __forceinline__ uint32_t hold8(const F (&v)[8], in
 // (replayed, one token: 4.0 us without queries or rotation; the angles add 0.7, the queries' turn 0.7). Many by the bytes: 4001
 // tokens, 168 MB in 34 us (a copy of them: 35; bf16, 86 MB: 34); there it is waves that pay, and a query's loads before the
 // angles' arithmetic cost more registers than they hide (38 us).
-template <int D, int ROPE, class T>
+// MORE: turned by positions of their own or with a magnitude, or queries in workgroups of their own: a form of its own, so that
+// the others keep their registers and their loads (one token: 8.2 us with kv_read, 8.4 in this one).
+template <int D, int ROPE, bool MORE, class T>
 __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_append(AppendArgs a) {
     constexpr int NT = 2 * D, NR = D / 8;
     __shared__ double2 cs[ROPE == FNS_ROPE_NONE ? 1 : kGroup * (D / 2)];
@@ -156,7 +159,8 @@ __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_ap
     const int64_t tok = r.q0 + (pos - first);
     const int page = page_of(a.c, a.b, s, base);  // 16 aligned positions lie in one page
     Row8<T> k8 = {}, v8 = {}, q8 = {};
-    const bool keys = blockIdx.z == 0;  // the others have queries only
+    const int part = MORE ? blockIdx.z : 0, parts = MORE ? gridDim.z : 1;
+    const bool keys = part == 0;  // the others have queries only
     if (have && keys) {
         k8.load((const T *) a.k + tok * a.k_stride + head * D + ch);
         v8.load((const T *) a.v + tok * a.v_stride + head * D + ch);
@@ -166,7 +170,7 @@ __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_ap
     const int n_group = a.n_group;
     int qp = hi, qh = 0, dp = 0, dh = 0;
     if (n_group) {
-        const int item = row + kGroup * (int) blockIdx.z, step = kGroup * (int) gridDim.z;
+        const int item = row + kGroup * part, step = kGroup * parts;
         qp = lo + item / n_group, qh = item % n_group, dp = step / n_group, dh = step % n_group;
     }
     const auto ask = [&] {
@@ -176,13 +180,13 @@ __global__ __launch_bounds__(2 * D, ROPE == FNS_ROPE_PAIRS ? 6 : 8) void k_kv_ap
         const int half = a.rope_dim / 2;
         for (int i = tid; i < (hi - lo) * half; i += NT) {
             const int p = lo + i / half, c = i % half;
-            const int by = a.at ? a.at[r.q0 + (p - first)] : p;
+            const int by = MORE && a.at ? a.at[r.q0 + (p - first)] : p;
             // in turns: the product is exact to 53 bits, its whole part leaves no error
             double turns = (double) by * (double) a.inv_freq[c] * 0.15915494309189533577;
             turns -= rint(turns);
             double sn, cn;
             sincospi(2.0 * turns, &sn, &cn);
-            cs[(p - base) * (D / 2) + c] = make_double2(cn * a.magnitude, sn * a.magnitude);
+            cs[(p - base) * (D / 2) + c] = MORE ? make_double2(cn * a.magnitude, sn * a.magnitude) : make_double2(cn, sn);
         }
         __syncthreads();
     }
@@ -348,8 +352,13 @@ int kv_append_at(const FnsKvCache *c, const FnsKvBatch *b, const FnsKvAppend *x,
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(2 * D), 0, st, a); };
     auto by_type = [&](auto dim, auto rope) {
         constexpr int DD = decltype(dim)::value, R = decltype(rope)::value;
-        if (x->dtype == FNS_TYPE_F32) go(k_kv_append<DD, R, float>);
-        else go(k_kv_append<DD, R, uint16_t>);
+        auto by_form = [&](auto more) {
+            constexpr bool MORE = decltype(more)::value;
+            if (x->dtype == FNS_TYPE_F32) go(k_kv_append<DD, R, MORE, float>);
+            else go(k_kv_append<DD, R, MORE, uint16_t>);
+        };
+        if (parts > 1 || (R != FNS_ROPE_NONE && (pos || magnitude != 1.0f))) by_form(std::true_type{});
+        else by_form(std::false_type{});
     };
     auto by_rope = [&](auto dim) {
         if (x->rope == FNS_ROPE_NONE) by_type(dim, std::integral_constant<int, FNS_ROPE_NONE>{});
