@@ -2,6 +2,9 @@
 // denominators: the kernels of fns_attn.hpp with what a token sees of its sequence's new tokens given as bits. Below the new
 // tokens a tile of keys is a causal one; the one or two tiles that hold them take the masked path, whose bits come from the
 // token's words. What a call costs beside attn's is that every row tile of a sequence walks over all of its new tokens.
+// 60 tokens of 32 heads over 8 of 128 at 100000 positions, f32: 167 us, 590 TFLOP/s of plain products (five digits and two halves of
+// p make 15 matrix instructions of 256 scores, 47 vector ones); vector instructions take 59% of the time, the matrix pipe is busy
+// 49%, two waves a SIMD. 26 tokens of 32 heads at 726: 12.4 us, a start, a walk of twelve tiles and the join of the waves.
 #include "fns_attn.hpp"
 
 namespace fns {
