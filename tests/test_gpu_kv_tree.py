@@ -270,6 +270,8 @@ def _check_weigh(s: Setup, group: int, dtype: str, window: int = 0, rows=None, p
     (64, 128, 2, 2, [130], [300], 40),
     (128, 32, 1, 17, [20], [400], 1),
     (64, 64, 1, 1, [257], [257], 0),
+    (256, 64, 1, 2, [130, 300], [700, 300], 0),
+    (256, 16, 2, 1, [150], [400], 90),
 ])
 def test_weigh(dim, page, heads_kv, group, q_lens, kv_lens, window, dtype):
     s = Setup(q_lens, kv_lens, page, heads_kv, dim, seed=dim + group, pad=2)
@@ -278,10 +280,15 @@ def test_weigh(dim, page, heads_kv, group, q_lens, kv_lens, window, dtype):
     _check_weigh(s, group, dtype, window, in_place=True)
 
 
-@pytest.mark.parametrize("dim,page,group,q_lens,kv_lens,window", [(128, 64, 4, [26, 0, 3], [200, 9, 3], 0), (64, 16, 2, [130, 70], [150, 400], 100),
-                                                                  (256, 32, 1, [64], [127], 9)])
-def test_weigh_of_a_tree(dim, page, group, q_lens, kv_lens, window):
+@pytest.mark.parametrize("longest", [None, 1 << 21])  # (work is divided by it: 65 to 256 rows in one launch, or by their images)
+@pytest.mark.parametrize("dim,page,group,q_lens,kv_lens,window", [
+    (128, 64, 4, [26, 0, 3], [200, 9, 3], 0), (64, 16, 2, [130, 70], [150, 400], 100), (256, 32, 1, [64], [127], 9),
+    (128, 128, 4, [60, 20, 1], [1500, 20, 777], 0), (256, 64, 2, [60, 33], [60, 1100], 0), (64, 32, 8, [32, 31, 5], [1030, 513, 300], 200),
+    (128, 16, 1, [256, 65], [700, 65], 0), (256, 16, 1, [128, 81], [128, 600], 60), (128, 64, 3, [170, 90], [300, 1400], 0)])
+def test_weigh_of_a_tree(dim, page, group, q_lens, kv_lens, window, longest):
     s = Setup(q_lens, kv_lens, page, 2, dim, seed=dim, pad=1)
+    if longest:
+        s.batch.desc.max_kv = longest
     rows = [td.seen_by(p) for p in trees_of(s, seed=group)]
     q, lse, out = _check_weigh(s, group, "f32", window, rows)
     # a rejected token's rows are left out by their lse
@@ -289,10 +296,19 @@ def test_weigh_of_a_tree(dim, page, group, q_lens, kv_lens, window):
     _check_weigh(s, group, "f32", window, rows, lse=lse, q=q)
 
 
-def test_weigh_odd_places():
+def test_weigh_of_many_heads():
+    """More heads than workgroups that run at once: each takes several steps of keys."""
+    n = 70
+    s = Setup([10 + i % 3 for i in range(n)], [1300 - 17 * i for i in range(n)], 64, 2, 64, seed=9)
+    _check_weigh(s, 8, "f32")
+    _check_weigh(s, 8, "bf16", in_place=True)
+
+
+@pytest.mark.parametrize("new,longest", [(60, 10), (60, 1 << 21), (150, 10), (150, 2000)])
+def test_weigh_odd_places(new, longest):
     """NaN blocks, missing pages, queries that are no numbers, lengths beyond the batch's longest and a prompt's many rows."""
-    s = Setup([60, 1], [300, 2000], 16, 2, 64, seed=61)
-    s.batch.desc.max_kv = 10
+    s = Setup([new, 1], [300, 2000], 16, 2, 64, seed=61)
+    s.batch.desc.max_kv = longest
     h = s.host
     s.table[0, 3], s.table[0, 5] = -1, h.n_pages
     for pos, off in ((300 - 7, 0), (300 - 12, 32), (20, 0)):
@@ -441,6 +457,27 @@ def test_evict_long_sequences(lens, page, heads, budget, first, recent, equal):
     s.cache.pages.copy_(pages)
     again, _ = ops.kv_evict(s.cache, s.batch, w0, budget, first=first, recent=recent)
     assert torch.equal(kept, again)
+
+
+@pytest.mark.parametrize("budget,first,recent", [(100, 40, 30), (390, 0, 0), (1, 0, 0), (5000, 3, 2)])
+def test_evict_in_chunks_picks_the_same(budget, first, recent):
+    """A table with room for more than is there: the same choice as without, of weights of all kinds and with pages missing."""
+    s = Setup([1, 1, 1], [400, 30, 0], 16, 2, 64, seed=12)
+    s.table[0, 2], s.table[0, 9], s.table[1, 1] = -1, s.host.n_pages, -5
+    w = np.round(np.exp(s.rng.standard_normal((s.host.n_pages, 2, 16))) * 4).astype(np.float32)
+    for v in (np.nan, np.inf, -np.inf, -0.0, -1.5, 1e-42, -np.nan):
+        w[s.rng.random(w.shape) < 0.03] = v
+    got = []
+    for columns in (s.table.shape[1], 2049):
+        table = np.full((3, columns), -1, np.int32)
+        table[:, : s.table.shape[1]] = s.table
+        batch = ops.KvBatch(s.batch.q_start, s.batch.kv_len, dev(table), 3, 1, 400)
+        assert (ops.kv_evict_workspace(s.cache, batch) is None) == (columns < 2049)
+        s.cache.pages.copy_(torch.from_numpy(s.host.raw.copy()).view(s.cache.pages.shape))
+        wd = torch.from_numpy(w.copy()).cuda()
+        got.append([*ops.kv_evict(s.cache, batch, wd, budget, first=first, recent=recent), wd.view(torch.int32), s.cache.pages.clone()])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
 
 
 # ---- accepted paths -------------------------------------------------------------------------------------------------
