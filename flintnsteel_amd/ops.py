@@ -733,9 +733,13 @@ class KvTree:
         if sees.dtype != torch.int64 or not sees.is_contiguous() or sees.dim() != 2:
             raise ValueError("KvTree: sees must be contiguous int64 [n_tok][words]")
         _here("KvTree", sees, pos)
+        self._set(sees, pos)
+
+    def _set(self, sees: torch.Tensor, pos: torch.Tensor | None) -> "KvTree":
         self.sees, self.pos = sees, pos
         self.desc = KvTreeDesc(sees.data_ptr(), sees.shape[1])
         self.ref = ctypes.byref(self.desc)
+        return self
 
     def _for(self, what: str, batch: KvBatch):
         if self.sees.shape[0] != batch.n_tok:
@@ -757,11 +761,11 @@ def tree_plan(batch: KvBatch, parents: torch.Tensor, base: torch.Tensor | None =
         words = max(1, (batch.desc.max_q + 63) // 64)
     p = _ints("tree_plan", "parents", parents, batch.n_tok)
     b = None if base is None else _ints("tree_plan", "base", base, batch.desc.n_seq)
-    sees = torch.empty((batch.n_tok, max(words, 0)), dtype=torch.int64, device=parents.device)
-    pos = torch.empty(batch.n_tok, dtype=torch.int32, device=parents.device)
+    sees = parents.new_empty((batch.n_tok, max(words, 0)), dtype=torch.int64)
+    pos = parents.new_empty(batch.n_tok)
     st = _here("tree_plan", batch.kv_len, parents, base)
     call("fns_hip_tree_plan", batch.ref, p, b, words, sees.data_ptr(), pos.data_ptr(), st)
-    return KvTree(sees, pos)
+    return KvTree.__new__(KvTree)._set(sees, pos)
 
 
 def _heads(what: str, t: torch.Tensor, n_tok: int, dim: int, dtype: torch.dtype) -> int:
@@ -797,7 +801,7 @@ def kv_append(cache: KvCache, batch: KvBatch, k: torch.Tensor, v: torch.Tensor, 
         raise ValueError(f"kv_append: expected {Hk} kv heads, got {k.shape[1]} and {v.shape[1]}")
     if q is not None:
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+            q_out = q.new_empty(q.shape, dtype=dt)
         x.q_stride = _heads("kv_append", q, n_tok, D, dt)
         x.q_out_stride = _heads("kv_append", q_out, n_tok, D, dt)
         if q_out.shape != q.shape:
@@ -825,8 +829,8 @@ def kv_read(cache: KvCache, batch: KvBatch):
     """-> (k, v) f32 [n_tok][n_head_kv][head_dim]: what the cache holds of the batch's tokens."""
     st = _here("kv_read", cache.pages, batch.kv_len)
     shape = (batch.n_tok, cache.n_head_kv, cache.head_dim)
-    k = torch.empty(shape, dtype=torch.float32, device=cache.pages.device)
-    v = torch.empty(shape, dtype=torch.float32, device=cache.pages.device)
+    k = cache.pages.new_empty(shape, dtype=torch.float32)
+    v = k.new_empty(shape)
     call("fns_hip_kv_read", cache.ref, batch._for(cache), k.data_ptr(), v.data_ptr(), st)
     return k, v
 
@@ -941,8 +945,8 @@ def kv_evict(cache: KvCache, batch: KvBatch, weights: torch.Tensor, budget: int,
         weights_out = weights
     _weights("kv_evict", cache, weights, weights_out)
     n_seq = batch.desc.n_seq
-    kept = torch.empty((n_seq, cache.n_head_kv, max(budget, 0)), dtype=torch.int32, device=cache.pages.device)
-    new_len = torch.empty(n_seq, dtype=torch.int32, device=cache.pages.device)
+    kept = batch.kv_len.new_empty((n_seq, cache.n_head_kv, max(budget, 0)))
+    new_len = batch.kv_len.new_empty(n_seq)
     x = KvEvictDesc(budget, first, recent, weights.data_ptr(), weights_out.data_ptr(), None, 0, kept.data_ptr(), new_len.data_ptr())
     if to_table is not None:
         if to_table.dim() != 2:
@@ -967,7 +971,7 @@ def kv_keep(cache: KvCache, batch: KvBatch, kept: torch.Tensor, n_kept: torch.Te
     n_seq = batch.desc.n_seq
     if kept.dim() != 2:
         raise ValueError("kv_keep: kept must be [n_seq][most]")
-    new_len = torch.empty(n_seq, dtype=torch.int32, device=cache.pages.device)
+    new_len = n_kept.new_empty(n_seq, dtype=torch.int32)
     x = KvKeepDesc(_ints("kv_keep", "kept", kept, n_seq, kept.shape[1]), _ints("kv_keep", "n_kept", n_kept, n_seq), kept.shape[1],
                    None if weights is None else weights.data_ptr(), new_len.data_ptr())
     st = _here("kv_keep", cache.pages, batch.kv_len, kept, n_kept, weights)
