@@ -81,7 +81,9 @@ __device__ __forceinline__ int wave_scan(int v) {
 // Which positions a sequence's kv head keeps. The budget-th largest key digit by digit (11, 11, 10 bits), the counts of a
 // digit's values in LDS; then the positions in order, those above it and as many equal ones as there is room for.
 constexpr int kSel = 1024, kBins = 2048, kSelWaves = kSel / 64;
-constexpr int kCopies = 4;  // of the counts: lanes with the same value wait for each other (many positions may have none at all)
+// Of the counts, in banks beside each other: lanes with the same value wait for each other (many positions may have no weight at
+// all: 16 sequences of 20000 without, 36 us and a move; copies in the same bank 48; with weights 27 both).
+constexpr int kCopies = 4;
 __device__ __forceinline__ int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 __device__ __forceinline__ bool digit_counts(int pass, uint32_t key, uint32_t prefix) {  // whether a key is counted in a pass
     return key != 0 && (pass == 0 || key >> (pass == 1 ? 21 : 10) == prefix);
@@ -143,7 +145,7 @@ __device__ __forceinline__ void put_kept(int32_t *kept, const uint32_t (&k)[4], 
 // the weights, three times counting and the search among 2048 counts, the scan of the kept (4160 positions of 8 heads: 8.2 us,
 // 16 sequences of up to 20000: 16.7).
 template <int Q> __global__ __launch_bounds__(kSel) void k_kv_select(EvictArgs a) {
-    __shared__ __align__(16) int bins[3][kCopies][kBins];
+    __shared__ __align__(16) int bins[3][kBins][kCopies];
     __shared__ int waves[Q][kSelWaves], found[3][2];
     const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const int n = seq_len(a.c, a.b, s), quads = n / 4 + (n % 4 > 0);
@@ -164,13 +166,13 @@ template <int Q> __global__ __launch_bounds__(kSel) void k_kv_select(EvictArgs a
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (digit_counts(pass, own[q][j], prefix))
-                        atomicAdd(&bins[pass][lane % kCopies][(own[q][j] >> digit_shift(pass)) & (pass == 2 ? 1023 : 2047)], 1);
+                        atomicAdd(&bins[pass][(own[q][j] >> digit_shift(pass)) & (pass == 2 ? 1023 : 2047)][lane % kCopies], 1);
         __syncthreads();
         int hi = 0, lo = 0;
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            const int2 two = *(const int2 *) &bins[pass][i][kBins - 2 - 2 * tid];
-            hi += two.y, lo += two.x;
+        for (int i = 0; i < kCopies; i += 4) {
+            const int4 x = *(const int4 *) &bins[pass][kBins - 2 - 2 * tid][i], y = *(const int4 *) &bins[pass][kBins - 1 - 2 * tid][i];
+            lo += (x.x + x.y) + (x.z + x.w), hi += (y.x + y.y) + (y.z + y.w);
         }
         const Digit d = find_digit(hi, lo, want, pass == 0, waves[0], found[pass]);
         if (pass == 0) keep = want = min(want, d.total);
@@ -214,7 +216,7 @@ struct SelectState {
     uint32_t prefix[4];
 };
 template <int PHASE> __global__ __launch_bounds__(kSel) void k_kv_select_chunks(EvictArgs a, SelectState *states, int32_t *counts, int chunks) {
-    __shared__ __align__(16) int bins[kCopies][kBins];
+    __shared__ __align__(16) int bins[kBins][kCopies];
     __shared__ int waves[kChunkQuads][kSelWaves], found[2], sums[2];
     const int s = blockIdx.x / a.c.n_kv, head = blockIdx.x % a.c.n_kv, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const int n = seq_len(a.c, a.b, s), used = n / kChunk + (n % kChunk > 0);
@@ -264,10 +266,12 @@ template <int PHASE> __global__ __launch_bounds__(kSel) void k_kv_select_chunks(
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (digit_counts(pass, own[q][j], prefix))
-                        atomicAdd(&bins[lane % kCopies][(own[q][j] >> digit_shift(pass)) & (pass == 2 ? 1023 : 2047)], 1);
+                        atomicAdd(&bins[(own[q][j] >> digit_shift(pass)) & (pass == 2 ? 1023 : 2047)][lane % kCopies], 1);
             __syncthreads();
             for (int i = tid; i < kBins; i += kSel) {
-                const int c = bins[0][i] + bins[1][i] + bins[2][i] + bins[3][i];
+                int c = 0;
+#pragma unroll
+                for (int j = 0; j < kCopies; ++j) c += bins[i][j];
                 if (c) atomicAdd(&st.bins[pass][i], c);
             }
             __syncthreads();
