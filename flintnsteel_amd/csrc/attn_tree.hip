@@ -11,13 +11,13 @@ namespace fns {
 
 namespace {
 
-// Into how many splits the tiles of one sequence's workgroups go: the least of what they are expected to take. Workgroups run in
+// Into how many splits the tiles of a call's workgroups go (of sequences of one length): the least of what they are expected to take. Workgroups run in
 // rounds of `places` a CU; with k of them on a CU a tile takes 1.5 + k units (of 0.1 to 0.25 us: 64 channels, 32 rows, 184 workgroups
 // over 40000 positions 235 us, twice as many 167), a round's starts and joins in LDS 25, the join of splits 30 and its bytes, a unit
 // 400000. So that neither a few workgroups are left for a round of their own (90 tokens of 64 heads over 8 of 64 at 40000: 184 us in
 // three splits, which are 552 workgroups for 512 places, 144 in five) nor half the places stay empty (146 of 32 over 4 of 256 at
 // 14320: 195 us whole, 160 in three; 33 of 16 over 2 of 256 at 60000: 102 in 16, 544 workgroups, 80 in 15).
-int64_t splits_of_one(int64_t wgs, int64_t tiles, int places, int64_t row_bytes) {
+int64_t splits_of(int64_t wgs, int64_t tiles, int places, int64_t row_bytes) {
     const auto per = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
     int64_t best = 1, least = INT64_MAX;
     for (int64_t s = 1; s <= 64 && (s == 1 || s * 4 < tiles + 4); ++s) {
@@ -32,9 +32,10 @@ int64_t splits_of_one(int64_t wgs, int64_t tiles, int places, int64_t row_bytes)
 // How a tree's call is divided: attn's form, but that of few rows otherwise than for causal rows, since a tree's rows all walk over
 // the same tiles. Sixteen rows a workgroup, until their steps (of 64 keys) are so many that reading K and V half as often
 // is ahead of having twice the workgroups (26 tokens of 4 heads over 726 positions: 12.6 us against 16.7 with 32; 60 tokens
-// over 100000: 194 against 167; 32 tokens of 8 heads over 24 contexts of up to 2900: both 49). Splits of one sequence as above; of
-// unequal ones until 512 workgroups where they outweigh their join, beyond that pieces of 40 tiles, up to 1024 (8 contexts of 16000,
-// equal: 184 us with 512, 194 with 1024, 206 with 2048).
+// over 100000: 194 against 167; 32 tokens of 8 heads over 24 contexts of up to 2900: both 49). Splits as above, but
+// long contexts of unequal sequences in pieces of 40 tiles up to 1024 workgroups, so that the longest do not run on alone (16 of up
+// to 9000 positions, 24 tokens of 32 heads over 8 of 128: 64 us in three, 130 whole; 8 of up to 4200, 63 tokens: 63 whole, 75 in
+// two).
 host::AttnPlan division(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x) {
     host::AttnPlan p = host::attn_plan(c, b, x);
     if (p.rows == kManyRows) return p;
@@ -44,15 +45,10 @@ host::AttnPlan division(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn 
     p.rows = c->head_dim == 256 || rows <= 16 || heads * per(rows, 16) * tiles < 100000 ? 16 : 32;
     p.row_tiles = per(rows, p.rows);
     const int64_t wgs = std::max<int64_t>(1, heads * p.row_tiles);
-    int64_t splits;
-    if (b->n_seq == 1) {
-        const int places = c->head_dim == 256 || p.rows == 32 ? 2 : 3;  // (by the registers)
-        splits = splits_of_one(wgs, tiles, places, (int64_t) b->n_tok * x->n_head * c->head_dim * 8);
-    } else {
-        splits = tiles * (256 - wgs) > 11 * 256 ? std::min(per(512, wgs), per(tiles, 4)) : 1;
-        splits = std::max(splits, std::min(tiles / 40, per(1024, wgs)));
-    }
-    p.splits = (int) std::max<int64_t>(1, std::min<int64_t>(splits, 64));
+    const int places = c->head_dim == 256 || p.rows == 32 ? 2 : 3;  // (by the registers)
+    int64_t splits = splits_of(wgs, tiles, places, (int64_t) b->n_tok * x->n_head * c->head_dim * 8);
+    if (b->n_seq > 1 && wgs >= 256) splits = std::max(splits, std::min(tiles / 40, per(1024, wgs)));
+    p.splits = (int) splits;
     p.chunk = (int) per(tiles, p.splits);
     const size_t n = p.splits > 1 ? (size_t) p.splits * b->n_tok * x->n_head : 0;
     p.ml_off = n * c->head_dim * 4;
