@@ -52,7 +52,7 @@ host::AttnPlan division(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn 
     p.chunk = (int) per(tiles, p.splits);
     const size_t n = p.splits > 1 ? (size_t) p.splits * b->n_tok * x->n_head : 0;
     p.ml_off = n * c->head_dim * 4;
-    p.bytes = p.ml_off + n * 8;
+    p.bytes = std::max(p.bytes, p.ml_off + n * 8);  // (one size, with a tree or without)
     return p;
 }
 
@@ -63,7 +63,7 @@ namespace impl {
 int attn_tree_workspace(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x, size_t *bytes) {
     FNS_TRY(host::attn_check(c, b, x, "attn_tree"));
     if (!bytes) return host::set_error(host::ERR_SHAPE, "attn_tree_workspace: null output");
-    *bytes = std::max(host::attn_plan(c, b, x).bytes, division(c, b, x).bytes);
+    *bytes = division(c, b, x).bytes;
     return host::OK;
 }
 
