@@ -561,10 +561,12 @@ int rope_scaled(int rope_dim, double base, double factor, double original, doubl
     const double pi = 3.14159265358979323846;
     // the pair (as a real number) that turns `turns` times over the original positions
     const auto at = [&](double turns) { return rope_dim * std::log(original / (turns * 2.0 * pi)) / (2.0 * std::log(base)); };
-    const double lo = std::max(std::floor(at(fast)), 0.0), hi = std::min(std::ceil(at(slow)), rope_dim / 2 - 1.0);
+    // The ramp starts at a pair and, as the published rule has it, ends at an index below rope_dim, which may lie behind the last
+    // pair: then none is divided fully. It is empty where the first pair is slow already (all are divided), or the last one fast.
+    const double lo = std::max(std::floor(at(fast)), 0.0), hi = std::min(std::ceil(at(slow)), rope_dim - 1.0);
     for (int i = 0; i < rope_dim / 2; ++i) {
         const double f = std::pow(base, -2.0 * i / rope_dim);
-        const double slowed = std::min(std::max((i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+        const double slowed = i >= hi ? 1.0 : i <= lo ? 0.0 : (i - lo) / (hi - lo);
         inv_freq[i] = (float) (f * (1.0 - slowed) + f / factor * slowed);
     }
     *magnitude = (float) (0.1 * std::log(factor) + 1.0);

@@ -398,8 +398,9 @@ int fns_hip_attn(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn
 /* Host arithmetic: inv_freq [rope_dim / 2] (host memory, f32) of a rotation made for `original` positions with
  * base^(-2 i / rope_dim), scaled to factor * original by the published rule of frequency parts: a pair that turns `fast` times
  * (32, say) or more over the original positions keeps its frequency, one that turns `slow` times (1) or less has it divided by
- * factor, the pairs between go over linearly in their index. *magnitude = 0.1 ln(factor) + 1, for fns_hip_kv_append_at. A factor
- * of 1 gives the plain frequencies and 1. */
+ * factor, the pairs between go over linearly in their index: from the last pair that keeps it (the first of all where none turns
+ * so often) to the first index that would turn `slow` times or less, behind the last pair too, but at most rope_dim - 1.
+ * *magnitude = 0.1 ln(factor) + 1, for fns_hip_kv_append_at. A factor of 1 gives the plain frequencies and 1. */
 int fns_hip_rope_scaled(int rope_dim, double base, double factor, double original, double fast, double slow, float *inv_freq,
                         float *magnitude);
 /* fns_hip_kv_append with the tokens turned by positions of their own: pos int32 [n_tok] (device memory), or NULL: their

@@ -173,3 +173,41 @@ def test_scaled_frequencies_refusals(args):
     out, m = (ctypes.c_float * 64)(), ctypes.c_float()
     assert L().fns_hip_rope_scaled(*args, out, r(m)) == -2
     assert L().fns_hip_rope_scaled(64, 1e4, 2.0, 100.0, 32.0, 1.0, None, r(m)) == -2
+
+
+@pytest.mark.parametrize("dim,base,factor,original,fast,slow", [
+    (128, 1e4, 4.0, 65536, 32.0, 1.0), (128, 1e4, 4.0, 131072, 32.0, 1.0), (64, 1e4, 16.0, 262144, 32.0, 1.0),  # no pair is slow
+    (16, 100.0, 4.0, 500, 32.0, 1.0), (128, 1e4, 4.0, 1e12, 32.0, 1.0), (64, 1e4, 4.0, 1e9, 32.0, 1.0),
+    (64, 1e4, 2.0, 6, 32.0, 1.0), (64, 1e4, 16.0, 1, 32.0, 1.0), (2, 1e4, 8.0, 2, 32.0, 1.0),                      # every pair is
+    (2, 1e4, 2.0, 100, 32.0, 1.0), (64, 1e4, 8.0, 100, 32.0, 1.0), (128, 5e5, 16.0, 8192, 32.0, 1.0), (96, 1e6, 40.0, 32768, 16.0, 2.0)])
+def test_scaled_frequencies_by_turns(dim, base, factor, original, fast, slow):
+    """From the pairs' turns over the original positions: kept, divided, or strictly between and linear in the index."""
+    out, m = (ctypes.c_float * (dim // 2))(), ctypes.c_float()
+    assert L().fns_hip_rope_scaled(dim, base, factor, original, fast, slow, out, r(m)) == 0
+    i = np.arange(dim // 2)
+    f = base ** (-2.0 * i / dim)
+    turns = original * f / (2 * np.pi)
+    kept, cut = turns >= fast, turns <= slow
+    if not kept.any() and not cut[0]:
+        kept[0] = True  # then the ramp starts at the first pair
+    part = np.array(out, np.float64) / f  # (f32: off by half a step, 2^-24, and f by less)
+    assert np.all(np.abs(part[kept] - 1) <= 2.0 ** -23)
+    assert np.all(np.abs(part[cut] * factor - 1) <= 2.0 ** -23)
+    between = part[~kept & ~cut]
+    assert np.all((between > 1 / factor + 2.0 ** -23) & (between < 1 - 2.0 ** -23))
+    # from the last kept pair to the first divided one (indices go on behind the last pair, up to dim - 1), in equal steps
+    first, last = kept.sum() - 1, int(cut.argmax()) if cut.any() else 0
+    while not cut.any() and last < dim - 1 and original * base ** (-2.0 * last / dim) / (2 * np.pi) > slow:
+        last += 1
+    for j in np.flatnonzero(~kept & ~cut):
+        assert abs(part[j] - (1 + (1 / factor - 1) * (j - first) / (last - first))) <= 2.0 ** -23
+
+
+@pytest.mark.parametrize("args,part", [((128, 1e4, 4.0, 65536.0), 1 - 3 / 4 * 23 / 25),
+                                       ((128, 1e4, 4.0, 131072.0), 1 - 3 / 4 * 18 / 25), ((64, 1e4, 16.0, 262144.0), 1 - 15 / 16 * 7 / 13)])
+def test_scaled_frequencies_where_no_pair_is_slow(args, part):
+    """The last pair's share by hand: the ramp ends at index 65, 70 and 37 and starts at 40, 45 and 24."""
+    n = args[0] // 2
+    out, m = (ctypes.c_float * n)(), ctypes.c_float()
+    assert L().fns_hip_rope_scaled(*args, 32.0, 1.0, out, r(m)) == 0
+    assert abs(out[n - 1] / args[1] ** (-2.0 * (n - 1) / args[0]) - part) <= 2.0 ** -23
