@@ -348,7 +348,7 @@ template <int D, class T> __global__ __launch_bounds__(64) void k_weigh_rows(Wei
     const int rows = (int) min((int64_t) sr.n * a.group, (int64_t) INT32_MAX);
     if (blockIdx.y == 0) {
         const int blocks = planned_blocks(x, key_len(a, sr)), tiles = image_tiles(x, sr), first = sr.len - sr.n;
-        int32_t *plan = x.plan + (int64_t) blockIdx.x * (x.blocks + 1), before = 0;  // (65535 tiles of 32767 blocks fit)
+        int32_t *plan = x.plan + (int64_t) blockIdx.x * (x.blocks + 1), before = 0;  // (weigh_plan sees that all steps fit)
         for (int i0 = 0; i0 < blocks; i0 += 64) {
             const int i = i0 + lane;
             int n = 0;
@@ -598,7 +598,10 @@ WeighPlan weigh_plan(const FnsKvCache *c, const FnsKvBatch *b, const FnsAttn *x)
         return p;
     }
     p.block = key_block(c->head_dim);
+    // Blocks that are planned: what the join's grid has, and their steps are counted in 32 bits (65535 tiles of the 32767 blocks of
+    // 512 keys fit; of 256 keys there may be 65535). Those behind are gone over whole.
     p.blocks = std::min<int64_t>(per(std::max<int64_t>(b->max_kv, 1), p.block), 65535 / (p.block / 256));
+    p.blocks = std::max<int64_t>(1, std::min(p.blocks, INT32_MAX / p.row_tiles));
     // Workgroups of a kv head: as many as there are places for all heads' at once (two a CU; one of 256 channels), or, of many
     // heads, which may be of unequal sequences, so many that the longest, or the last round, does not run on alone; no more than
     // give a share of four steps (24 sequences of up to 9000 keys, 64 tokens, 8 heads: 144 us against 229 in one round; 4 of 205

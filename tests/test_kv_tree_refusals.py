@@ -211,3 +211,17 @@ def test_scaled_frequencies_where_no_pair_is_slow(args, part):
     out, m = (ctypes.c_float * n)(), ctypes.c_float()
     assert L().fns_hip_rope_scaled(*args, 32.0, 1.0, out, r(m)) == 0
     assert abs(out[n - 1] / args[1] ** (-2.0 * (n - 1) / args[0]) - part) <= 2.0 ** -23
+
+
+@pytest.mark.parametrize("dim,tiles", [(256, 65535), (256, 40000), (256, 4000), (128, 65535), (64, 65535), (64, 4000)])
+def test_steps_of_many_rows_fit_their_plan(dim, tiles):
+    """kv_weigh counts the steps (16 rows, a block of keys) of a kv head in int32: row tiles times planned blocks stay below 2^31
+    at the longest context. What a plan of `blocks` takes is read off the workspace: 4 (blocks + 1) bytes, up to 256's multiple."""
+    def size(kv):
+        n, b = ctypes.c_size_t(), batch(n_tok=16 * tiles, max_q=16 * tiles, max_kv=kv, table_stride=1 << 20)
+        x = att(n_head=1, q_stride=dim)
+        assert L().fns_hip_kv_weigh_workspace(r(cache(n_head_kv=1, head_dim=dim)), r(b), r(x), r(n)) == 0
+        return n.value
+
+    most = (size(2 ** 31 - 1) - size(1) + 256) // 4 - 1  # (images and partial sums are as many; one block's plan takes 256 bytes)
+    assert most > 1000 and tiles * (most - 63) <= 2 ** 31 - 1
