@@ -210,7 +210,7 @@ template <int Q> __global__ __launch_bounds__(kSel) void k_kv_select(EvictArgs a
 // (whole numbers, whose order of adding does not matter), then how many of each chunk are kept. 124729 positions of 2 heads: 38 us in
 // six launches, about 115 in one workgroup that reads its weights four times.
 constexpr int kChunkQuads = 4, kChunk = 4 * kSel * kChunkQuads;
-struct SelectState {
+struct alignas(16) SelectState {  // (counts are read two at a time)
     int bins[3][kBins];
     int want[4], keep;  // want[p]: after p passes
     uint32_t prefix[4];

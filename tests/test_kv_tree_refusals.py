@@ -225,3 +225,16 @@ def test_steps_of_many_rows_fit_their_plan(dim, tiles):
 
     most = (size(2 ** 31 - 1) - size(1) + 256) // 4 - 1  # (images and partial sums are as many; one block's plan takes 256 bytes)
     assert most > 1000 and tiles * (most - 63) <= 2 ** 31 - 1
+
+
+def test_eviction_states_are_aligned():
+    """kv_evict's states of the kv heads lie beside each other in the 16-byte aligned workspace, before 8 bytes a chunk: of a kv
+    head's bytes at room for 65536 and 131072 positions, twice the first less the second is a state."""
+    def size(heads, room):
+        n = ctypes.c_size_t()
+        assert L().fns_hip_kv_evict_workspace(r(cache(n_head_kv=heads)), r(batch(table_stride=room // 64)), r(n)) == 0
+        return n.value
+
+    for heads in (1, 2, 3):
+        state = 2 * size(heads, 65536) - size(heads, 131072)
+        assert state % heads == 0 and state // heads % 16 == 0
