@@ -944,6 +944,8 @@ def kv_evict(cache: KvCache, batch: KvBatch, weights: torch.Tensor, budget: int,
     if weights_out is None:
         weights_out = weights
     _weights("kv_evict", cache, weights, weights_out)
+    if max(abs(budget), abs(first), abs(recent)) > 1 << 30:  # (they would wrap in the descriptor)
+        raise ValueError(f"kv_evict: budget must be 1..2^30 and hold first and recent ({budget}, {first}, {recent})")
     n_seq = batch.desc.n_seq
     kept = batch.kv_len.new_empty((n_seq, cache.n_head_kv, max(budget, 0)))
     new_len = batch.kv_len.new_empty(n_seq)

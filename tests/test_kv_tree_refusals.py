@@ -2,9 +2,11 @@
 from __future__ import annotations
 
 import ctypes
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
+import torch
 
 from flintnsteel_amd import _lib, ops
 from test_attn_half_refusals import BAD_BATCHES, BAD_CACHES, BUF, P, app, att, batch, cache
@@ -238,3 +240,13 @@ def test_eviction_states_are_aligned():
     for heads in (1, 2, 3):
         state = 2 * size(heads, 65536) - size(heads, 131072)
         assert state % heads == 0 and state // heads % 16 == 0
+
+
+@pytest.mark.parametrize("kw", [dict(first=1 << 32), dict(recent=(1 << 32) + 2), dict(first=-(1 << 32)), dict(budget=(1 << 32) + 5)])
+def test_eviction_numbers_beyond_32_bits(kw):
+    """Refused before they become others in the call's ints."""
+    c = SimpleNamespace(desc=cache(), n_head_kv=2, page_size=64, pages=torch.empty(0, dtype=torch.uint8))
+    b = SimpleNamespace(desc=batch(n_seq=0), kv_len=torch.zeros(0, dtype=torch.int32))
+    w = torch.zeros(4, 2, 64)
+    with pytest.raises(ValueError, match="budget"):
+        ops.kv_evict(c, b, w, **{**dict(budget=8), **kw})
