@@ -850,7 +850,8 @@ def attn(cache: KvCache, batch: KvBatch, q: torch.Tensor, scale: float | None = 
          tree: KvTree | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [n_tok][n_head][head_dim] over the cache -> out (rows of no sequence are left as they were). scale
     None: head_dim^-0.5; window > 0: the last `window` positions only; sinks f32 [n_head] join the denominator. tree: what the
-    new tokens see of each other; lse f32 [n_tok][n_head]: takes the logarithms of the denominators (kv_weigh's)."""
+    new tokens see of each other; lse f32 [n_tok][n_head]: takes the logarithms of the denominators (kv_weigh's; of a row
+    that sees nothing the sink, or -infinity)."""
     D, dt = cache.head_dim, q.dtype
     if out is None:
         out = torch.empty(q.shape, dtype=dt, device=q.device)

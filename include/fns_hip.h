@@ -427,9 +427,9 @@ int fns_hip_tree_plan(const FnsKvBatch *batch, const int32_t *parents, const int
  * what its bits say (not the others, itself only with its bit); with a window of W and n bits the last W - n of the earlier
  * positions (none if n >= W: the bits alone say which new tokens it sees). A token without bits sees nothing: its output is
  * zero. NULL: as fns_hip_attn (FNS_TYPE_F32: in the same bits). q enters as f32 does there, whatever its type.
- * lse: NULL or f32 [n_tok][n_head], the logarithm of the softmax's denominator (sinks included) of every row, -infinity for one
- * that sees nothing. workspace: fns_hip_attn_tree_workspace bytes
- * (with or without a tree; at least fns_hip_attn_workspace's), as fns_hip_attn's. */
+ * lse: NULL or f32 [n_tok][n_head], the logarithm of the softmax's denominator (sinks included) of every row; of one that sees
+ * nothing the head's sink, -infinity without sinks. workspace: fns_hip_attn_tree_workspace bytes (with or without a tree; at
+ * least fns_hip_attn_workspace's), as fns_hip_attn's. */
 int fns_hip_attn_tree_workspace(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, size_t *bytes);
 int fns_hip_attn_tree(const FnsKvCache *cache, const FnsKvBatch *batch, const FnsAttn *x, const FnsKvTree *tree, const void *q,
                       void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);

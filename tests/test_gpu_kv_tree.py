@@ -745,3 +745,54 @@ def test_two_streams():
     torch.cuda.synchronize()
     for t, o, w in zip((a, b), outs, want):
         assert all(torch.equal(x, y) for x, y in zip(t.results(o), w))
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_denominators_of_rows_that_see_nothing(many):
+    """The head's sink, minus infinity without sinks: of tokens without bits, and of causal ones in front of the context."""
+    s = Setup([70 if many else 5, 3], [200, 2], 16, 1, 64, seed=12)
+    q, sinks = _rand(s.rng, (s.n_tok, 4, 64))[0], torch.tensor([0.5, -3.0, 40.0, -200.0], device="cuda")
+    rows = [td.seen_by(p) for p in trees_of(s, 2)]
+    rows[0][1], rows[0][-1] = [], []
+    blind = [1, s.q_lens[0] - 1]
+    for tree, dark in ((kv_tree(s, rows), blind), (None, [s.q_lens[0]])):  # (a token at position -1 sees nothing)
+        for sink in (sinks, None):
+            lse = torch.zeros(s.n_tok, 4, device="cuda")
+            out = ops.attn(s.cache, s.batch, q, sinks=sink, tree=tree, lse=lse)
+            for t in dark:
+                assert not out[t].any()
+                want = sinks if sink is not None else torch.full_like(sinks, float("-inf"))
+                # to log2 units and back: two half steps each, and one step of the log of a sum that is held 2^8 up
+                assert torch.allclose(lse[t], want, rtol=2.0 ** -22, atol=2.0 ** -20)
+
+
+def test_weigh_behind_the_planned_blocks_of_256_channels():
+    """A prompt's rows over a context that is longer than the batch says: blocks behind the plan are gone over whole."""
+    for kv in (900, 2100):
+        s = Setup([280, 5], [kv, 700], 32, 1, 256, seed=kv)
+        s.batch.desc.max_kv = 300
+        _check_weigh(s, 2, "f32")
+        _check_weigh(s, 2, "bf16", window=77, in_place=True)
+
+
+def test_plan_of_a_line_of_1024():
+    """The deepest plan: every token's path is all tokens before it."""
+    s = Setup([1024, 700], [1024, 900], 64, 1, 64)
+    plan = ops.tree_plan(s.batch, dev([i - 1 for n in s.q_lens for i in range(n)]), base=dev([5, 7]))
+    bits = np.tril(np.ones((1024, 1024), np.uint8))
+    want = np.concatenate([np.packbits(bits[:n], axis=1, bitorder="little").view(np.int64) for n in s.q_lens])
+    assert np.array_equal(plan.sees.cpu().numpy(), want)
+    assert np.array_equal(plan.pos.cpu().numpy(), np.concatenate([5 + np.arange(1024), 7 + np.arange(700)]))
+
+
+def test_eviction_of_many_heads_in_chunks():
+    """States of several kv heads beside each other: the same choice as that of one head at a time."""
+    s = Setup([1, 1], [40000, 300], 64, 3, 64, seed=4)
+    w = torch.rand(s.host.n_pages, 3, 64, device="cuda")
+    kept, new_len = ops.kv_evict(s.cache, s.batch, w.clone(), 500, 3, 7)
+    assert new_len.tolist() == [500, 300]
+    for i, n in enumerate(s.kv_lens):
+        for h in range(3):
+            of = w[dev(s.lists[i]).long(), h].reshape(-1)[:n].cpu().numpy()
+            want = td.evicted(of, np.ones(n, bool), 500, 3, 7)
+            assert kept[i, h].tolist() == want + [-1] * (500 - len(want))

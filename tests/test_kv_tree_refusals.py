@@ -250,3 +250,16 @@ def test_eviction_numbers_beyond_32_bits(kw):
     w = torch.zeros(4, 2, 64)
     with pytest.raises(ValueError, match="budget"):
         ops.kv_evict(c, b, w, **{**dict(budget=8), **kw})
+
+
+def test_eviction_workspace_of_the_wrapper_is_the_librarys():
+    """ops asks the library only where it expects a workspace: the same tables."""
+    n = ctypes.c_size_t()
+    for page in (16, 64, 4096):
+        c = cache(page_size=page)
+        for pages in (1, 32768 // page, 32768 // page + 1, 5 * 32768 // page):
+            d = batch(table_stride=pages)
+            b = SimpleNamespace(desc=d, _for=lambda _, d=d: r(d))
+            got = ops.kv_evict_workspace(SimpleNamespace(ref=r(c), page_size=page, pages=torch.empty(0)), b)
+            assert L().fns_hip_kv_evict_workspace(r(c), r(d), r(n)) == 0
+            assert (0 if got is None else got.numel()) == n.value
