@@ -242,6 +242,8 @@ template <int D, class T> struct QueryShape {
 };
 typedef uint32_t u6 __attribute__((ext_vector_type(6)));
 // MORE: always as many digits as f32 has: a denominator's logarithm is f32, whatever the queries are (3 digits left it 1e-4 off).
+// Calls that ask for none pay too: bf16, 32 heads over 8 of 128, without a tree 8 x 30 tokens at 4000 take 43.1 us (36.8 with
+// attn's three digits), a prompt of 2801 105 (86), one token at 1500 or 100000 about 1 us more.
 template <bool MORE, class T> using DigitType = std::conditional_t<MORE, float, T>;
 template <int D, class T> using Digits = u6[QueryShape<D, T>::N][QueryShape<D, T>::kSteps];
 // The row is first multiplied by scale * log2(e): scores are log2 units. Returns the block scale of digit 0 (255: the row has a
@@ -488,7 +490,9 @@ __device__ __forceinline__ void softmax_tile(f4 (&s)[CT][4], const NewTokens<MOR
             for (int i = 0; i < 4; ++i) {
                 const float x = __builtin_amdgcn_exp2f(s[c][2 * v + i / 2][i % 2 * 2]), y = __builtin_amdgcn_exp2f(s[c][2 * v + i / 2][i % 2 * 2 + 1]);
                 if constexpr (MORE && SPLIT == 1) lx[c] += x + y;
-                // toward zero: a second part has the rest, and without one the sum of p counts the same values
+                // toward zero: a second part has the rest, and without one (bf16) the sum of p counts the same values. What is
+                // cut, up to 2^-10 of a p, is lost in the output's own rounding: 8 trees of 63 tokens with 64 channels are 1.675e-3
+                // (of the norm) from the exact values, 1.659e-3 with f32 all through; a part of them rounds the other way.
                 const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
                 w[0][i] = __builtin_bit_cast(uint32_t, hi);
                 if constexpr (SPLIT == 2) {

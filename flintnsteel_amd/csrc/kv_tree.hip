@@ -19,8 +19,9 @@ namespace {
 constexpr int kMaxWords = 16, kMaxNew = 64 * kMaxWords;
 
 // A workgroup a sequence, a thread a token: up the parents, which get smaller at every step, once to see that they end at -1
-// and how many they are, once to set the bits, a word at a time. Bound by the longest path's LDS reads (26
-// tokens: 2.7 us; 24 sequences of 32: 3.7).
+// and how many they are, once to set the bits, a word at a time. Bound by the longest path's LDS reads, one after another (26
+// tokens: 2.7 us; 24 sequences of 32: 3.7; 1000 tokens of a tree with two children each 10.9): a tree that is a line is the
+// worst there is, with work that grows by its square (lines of 26, 200 and 1000 tokens: 4.5, 22 and 257 us).
 __global__ __launch_bounds__(256) void k_tree_plan(BatchView b, const int32_t *parents, const int32_t *base, int words, uint64_t *sees,
                                                    int32_t *pos) {
     __shared__ int up[kMaxNew];
@@ -379,7 +380,8 @@ template <bool NEW> struct Places {
 // order: what it writes lies before everything that it has yet to read, since the list ascends (a list of new tokens, which need
 // not, has at most 1024). Bound by what waits for what, a step at a time: a step's data, the next one's pages and the list of the
 // one after are asked for together (130000 positions of 8 heads cut to 100000: 354 us with the choice, 488 step by step; 9000 of 256
-// channels to 8192, 4 sequences of 2 heads: 39 and 106).
+// channels to 8192, 4 sequences of 2 heads: 39 and 106). The bytes alone would be about 49 us of the 354: a head and part is one
+// workgroup, 48 of them for 8 heads of 128 on 256 CUs.
 constexpr int kMove = 1024;
 template <int N, bool NEW, class Pos, class Load, class Store>
 __device__ __forceinline__ void walk(const MoveArgs &a, const Places<NEW> &places, int s, Pos pos, Load load, Store store) {
@@ -587,7 +589,9 @@ int tree_plan(const FnsKvBatch *b, const int32_t *parents, const int32_t *base, 
 
 namespace {
 
-// Positions that a sequence of a call can have at all, by its table (max_kv is no bound), and how they are gone over.
+// Positions that a sequence of a call can have at all, by its table (max_kv is no bound), and how they are gone over: the table's
+// width decides, not the lengths, so that results hold for any. A wide table costs a short sequence its one launch (4160 positions
+// of 8 heads in place: 22.2 us, behind a table of 32768 positions 23.7, of 131072 42.4; 300 positions: 10.1, 11.6, 30.1).
 constexpr int64_t kOneSelect = 32 * kSel;
 int select_chunks(int64_t room) { return (int) ((std::min<int64_t>(room, INT32_MAX) + kChunk - 1) / kChunk); }
 
